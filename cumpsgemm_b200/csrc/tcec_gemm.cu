@@ -435,42 +435,53 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+// Three dimensions, one element between neighbours, no interleaving, zeros outside.  A thread that has made
+// no runtime call yet (autograd's, say) has no current context, which the driver call needs and a
+// cudaSetDevice binds.
+static bool encode_map(CUtensorMap *map, CUtensorMapDataType type, const void *base,
+                       const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+                       const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint32_t estr[3] = {1, 1, 1};
+  for (int attempt = 0;; ++attempt) {
+    const CUresult r = fn(map, type, 3, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    int dev = 0;
+    if (attempt > 0 || r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess ||
+        cudaSetDevice(dev) != cudaSuccess)
+      return false;
+  }
+}
+
 // Tensor map over a K-blocked panel (layout: split_kernels.cu); see gemm_common.cuh.
 bool make_panel_map(CUtensorMap *map, SplitKind kind, const void *panel, uint32_t k_pad,
                     uint32_t rows_pad, uint32_t planes, uint32_t box_rows) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return false;
   const uint32_t es = (kind == SplitKind::fp16) ? 2u : 4u;
   // K-blocked panel: 128-byte K slices of all rows of one K block are contiguous.
   const uint32_t kbe = ROW_BYTES / es;
   const uint32_t k_blocks = k_pad / kbe;
-  const cuuint64_t dims[3] = {kbe, rows_pad, static_cast<cuuint64_t>(planes) * k_blocks};
-  const cuuint64_t strides[2] = {ROW_BYTES, static_cast<cuuint64_t>(ROW_BYTES) * rows_pad};
-  const cuuint32_t box[3] = {kbe, box_rows, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUtensorMapDataType dt =
-      (kind == SplitKind::fp16) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-  const CUresult r =
-      fn(map, dt, 3, const_cast<void *>(panel), dims, strides, box, estr,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_map(
+      map, kind == SplitKind::fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+      panel, {kbe, rows_pad, static_cast<cuuint64_t>(planes) * k_blocks},
+      {ROW_BYTES, static_cast<cuuint64_t>(ROW_BYTES) * rows_pad}, {kbe, box_rows, 1},
+      CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool make_float_map(CUtensorMap *map, const float *base, const uint64_t (&dims)[3],
                     const uint64_t (&strides)[2], const uint32_t (&box)[3], bool swizzle) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
-  const cuuint64_t st[2] = {strides[0], strides[1]};
-  const cuuint32_t bx[3] = {box[0], box[1], box[2]};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(base), d, st, bx, estr,
-         CU_TENSOR_MAP_INTERLEAVE_NONE,
-         swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, {dims[0], dims[1], dims[2]},
+                    {strides[0], strides[1]}, {box[0], box[1], box[2]},
+                    swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+bool make_swizzled_map(CUtensorMap *map, int elem_bytes, const void *base, const uint64_t (&dims)[3],
+                       const uint64_t (&strides)[2], const uint32_t (&box)[3]) {
+  return encode_map(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                    base, {dims[0], dims[1], dims[2]}, {strides[0], strides[1]}, {box[0], box[1], box[2]},
+                    CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 namespace {
