@@ -130,6 +130,13 @@ PROTOTYPES = {
     "cuMpSGEMM_cgemm_Mx2x2": (i32, _TINY_ARGS),
     "cuMpSGEMM_sgemm_2xNx2": (i32, _TINY_ARGS),
     "cuMpSGEMM_cgemm_2xNx2": (i32, _TINY_ARGS),
+    "cuMpSGEMM_grouped_gemm": (i32, [vp, i32, u64, u64, u64, u32, vp, vp, vp, u64, vp, u64, u64, vp, vp,
+                                     u64, i32, i32]),
+    "cuMpSGEMM_grouped_gemm_wgrad": (i32, [vp, i32, u64, u64, u64, u32, vp, vp, vp, u64, vp, u64, vp, vp,
+                                           u64, u64, i32, i32]),
+    "cuMpSGEMM_i8_grouped_gemm": (i32, [vp, u64, u64, u64, u32, vp, vp, u64, vp, vp, u64, u64, vp, vp, vp,
+                                        u64, i32]),
+    "cuMpSGEMM_quantize_rows_i8": (i32, [vp, u64, u64, vp, u64, i32, vp, u64, vp, u64, vp]),
     # intercepted cuBLAS symbols (prototypes of cublas_api.h)
     "cublasSgemm_v2": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, vp, i32]),
     "cublasCgemm_v2": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, vp, i32]),

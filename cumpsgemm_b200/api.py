@@ -20,6 +20,11 @@ CUBLAS_OP_N = 0
 CUBLAS_OP_T = 1
 CUBLAS_OP_C = 2
 
+# cudaDataType_t
+CUDA_R_32F = 0
+CUDA_R_16F = 2
+CUDA_R_16BF = 14
+
 CUBLAS_STATUS_SUCCESS = 0
 CUBLAS_STATUS_NOT_INITIALIZED = 1
 CUBLAS_STATUS_ALLOC_FAILED = 3
@@ -73,6 +78,10 @@ def _ptr(x: DevPtr) -> int:
             raise ValueError("matrix operands must live in device memory")
         return x.data_ptr()
     raise TypeError(f"expected a CUDA tensor or a device address, got {type(x)}")
+
+
+def _ptr_or_null(x) -> Optional[int]:
+    return None if x is None else _ptr(x)
 
 
 def _is_complex(x: DevPtr, hint: Optional[bool]) -> bool:
@@ -218,6 +227,53 @@ class Handle:
                                               b, _ptr(Cmat), ldc, int(mode),
                                               C.byref(mod))
         return st, mod.value
+
+    # ------------------------------------------------------------------ rows grouped by expert
+    # Row-major, unlike the rest; cumpsgemm_b200.experts has them on torch tensors.
+    def grouped_gemm(self, op_W: int, rows: int, n: int, k: int, num_groups: int, group_ends, alpha,
+                     X: DevPtr, ldx: int, W: DevPtr, ldw: int, stridew: int, beta, Y: DevPtr, ldy: int,
+                     data_type: int, mode: int = ComputeMode.FP16TCEC, check: bool = True) -> int:
+        """cuMpSGEMM_grouped_gemm.  data_type is CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F."""
+        st = self._lib.cuMpSGEMM_grouped_gemm(
+            self._h, op_W, rows, n, k, num_groups, _ptr_or_null(group_ends), _scalar(alpha, False),
+            _ptr(X), ldx, _ptr(W), ldw, stridew, _scalar(beta, False), _ptr(Y), ldy, data_type, int(mode))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_grouped_gemm")
+        return st
+
+    def grouped_gemm_wgrad(self, op_W: int, rows: int, n: int, k: int, num_groups: int, group_ends,
+                           alpha, X: DevPtr, ldx: int, dY: DevPtr, lddy: int, beta, dW: DevPtr,
+                           lddw: int, stridedw: int, data_type: int,
+                           mode: int = ComputeMode.FP16TCEC, check: bool = True) -> int:
+        """cuMpSGEMM_grouped_gemm_wgrad."""
+        st = self._lib.cuMpSGEMM_grouped_gemm_wgrad(
+            self._h, op_W, rows, n, k, num_groups, _ptr_or_null(group_ends), _scalar(alpha, False),
+            _ptr(X), ldx, _ptr(dY), lddy, _scalar(beta, False), _ptr(dW), lddw, stridedw, data_type,
+            int(mode))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_grouped_gemm_wgrad")
+        return st
+
+    def i8_grouped_gemm(self, rows: int, n: int, k: int, num_groups: int, group_ends, Xq: DevPtr,
+                        ldx: int, x_scale: DevPtr, Wq: DevPtr, ldw: int, stridew: int, w_scale: DevPtr,
+                        bias, Y: DevPtr, ldy: int, y_type: int, check: bool = True) -> int:
+        """cuMpSGEMM_i8_grouped_gemm."""
+        st = self._lib.cuMpSGEMM_i8_grouped_gemm(
+            self._h, rows, n, k, num_groups, _ptr_or_null(group_ends), _ptr(Xq), ldx, _ptr(x_scale),
+            _ptr(Wq), ldw, stridew, _ptr(w_scale), _ptr_or_null(bias), _ptr(Y), ldy, y_type)
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_i8_grouped_gemm")
+        return st
+
+    def quantize_rows_i8(self, rows: int, k: int, X: DevPtr, ldx: int, data_type: int, row_index,
+                         src_rows: int, Q: DevPtr, ldq: int, scale: DevPtr, check: bool = True) -> int:
+        """cuMpSGEMM_quantize_rows_i8."""
+        st = self._lib.cuMpSGEMM_quantize_rows_i8(self._h, rows, k, _ptr(X), ldx, data_type,
+                                                  _ptr_or_null(row_index), src_rows, _ptr(Q), ldq,
+                                                  _ptr(scale))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_quantize_rows_i8")
+        return st
 
     def kernel_status(self) -> int:
         """Synchronise and return (then clear) the GEMM kernel's bounded-wait status word."""

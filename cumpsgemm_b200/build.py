@@ -41,6 +41,9 @@ CUDA_SOURCES = [
     "ext_api.cu",
     "static_scratch_gemm.cu",
     "tiny_gemm.cu",
+    "grouped_gemm.cu",
+    "row_kernels.cu",
+    "grouped_api.cu",
 ]
 CPP_SOURCES = ["cublas_shim.cpp", "default_rule.cpp"]
 

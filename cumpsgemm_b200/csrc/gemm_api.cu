@@ -39,8 +39,8 @@ bool may_allocate(const cuMpSGEMM_handle *h) {
   return cap == cudaStreamCaptureStatusNone;
 }
 
-// Makes the workspace hold `bytes`.  Returns false, with the old workspace untouched, while the
-// stream is being captured, and false without a workspace if there is no memory.
+} // namespace
+
 bool ensure_workspace(cuMpSGEMM_handle *h, std::size_t bytes) {
   if (h->workspace_bytes >= bytes) return true;
   if (!may_allocate(h)) return false;
@@ -58,6 +58,12 @@ bool ensure_workspace(cuMpSGEMM_handle *h, std::size_t bytes) {
   h->workspace_bytes = bytes;
   return true;
 }
+
+std::size_t workspace_limit(const cuMpSGEMM_handle *h) {
+  return h->workspace_limit_bytes ? h->workspace_limit_bytes : kDefaultWorkspaceLimit;
+}
+
+namespace {
 
 __global__ void dyn_params_from_flag_kernel(DynParams *out, const int *flag) {
   CUMPSGEMM_CHAINED_KERNEL_ENTRY();

@@ -1,0 +1,717 @@
+// Products of rows grouped by expert, on CTA pairs (tcgen05 cta_group::2).
+//
+//   product  y[r, :] = alpha * x[r, :] op(w_e) + beta * y[r, :]     for the rows r of group e
+//   wgrad    dw_e    = alpha * x_e^T dy_e + beta * dw_e             over the rows of group e
+//   8 bits   y[r, c] = sx[r] * sw[e][c] * sum_k xq[r, k] wq_e[c, k] (+ bias[e][c])
+//
+// The sizes of the groups are known on the device only (`ends`, the running total of rows), so the
+// grid is one persistent CTA pair per SM pair, and every pair walks the tiles of all groups, which it
+// finds from the running totals in shared memory.
+//
+// Which side is which.  The weights' output features are the M side of the tensor core's product
+// (lanes of tensor memory, 256 per pair) and the rows of a group its N side (columns): N goes by
+// steps of 32 to 256, so a group whose rows fill no tile costs what its rows cost, and a step of
+// decoding with four rows per expert multiplies 32 columns, not 256.  It also lets a warp's lanes
+// hold neighbouring features, which are neighbours in the row-major output.  For wgrad both
+// sides are weight dimensions, and lanes are the one that is contiguous in the output.
+//
+// Operands come by TMA as they lie in memory.  A 16-bit operand whose lanes (or columns) are the
+// contiguous dimension is read as such (make_mnmajor_desc): no transposed copies.  FP32
+// operands have been split into hi and lo FP16 planes of the same layout (row_kernels.cu), hi*hi is
+// drained from tensor memory every two stages and added in registers and the corrections have an
+// accumulator of their own, as in tcec_gemm_pair.cu.
+//
+// wgrad reduces over a group's rows, which end inside a 64-row block.  The next group's rows must not
+// count, not even multiplied by zero, since they may be NaN: the warp that issues the loads waits
+// for such a last block, zeroes the rows up to the next multiple of 16 in both operands, and the
+// tensor core gets only as many steps of 16.  That wait is hidden behind the blocks in front of it.
+//
+// Barriers ("leader" = cluster rank 0):
+//   full[s]       leader's only: 2 arrivals, one from each CTA's producer (the leader's with the
+//                 bytes of both CTAs' loads; for a last block each once its rows are zeroed)
+//   empty[s]      in both CTAs: commit multicast from the leader
+//   acc_full[b]   in both CTAs: commit multicast.  b: one of two accumulators (f16, i8), or hi*hi (0)
+//                 and the corrections (1)
+//   acc_empty[b]  leader's only: 16 arrivals, one from each epilogue warp of both CTAs
+//   tail          own: a last block's loads
+// Every wait is bounded; no TMA multicast is used.
+#include "epilogue.cuh"
+#include "gemm_common.cuh"
+#include "grouped.hpp"
+#include "ptx.cuh"
+#include "split_math.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <mutex>
+
+namespace cumpsgemm_b200 {
+namespace {
+
+constexpr int BM_CTA = 128;            // lanes per CTA
+constexpr uint32_t LANES = 2 * BM_CTA; // per pair
+constexpr uint32_t COLS = 256;         // most columns of a tile
+constexpr uint32_t ROW_BYTES = kGemmRowBytes;
+constexpr uint32_t TILE_BYTES = 128 * ROW_BYTES; // an operand's part of a stage in one CTA
+constexpr uint32_t ATOM_BYTES = 64 * ROW_BYTES;  // lanes (columns) contiguous: 64 of them by 64 of K
+constexpr uint32_t FEW_ROWS = 32;                // rows of the smaller box
+constexpr int NUM_THREADS = 384;
+constexpr int NUM_EPI_WARPS = 8;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t DRAIN_STAGES = 2; // tcec: 128 k values per drain (tcec_gemm_pair.cu has the figures)
+constexpr uint32_t BAND = 8;         // column tiles that are walked together
+
+constexpr int kF16 = static_cast<int>(GroupedKind::f16), kTcec = static_cast<int>(GroupedKind::tcec),
+              kI8 = static_cast<int>(GroupedKind::i8);
+
+template <int KIND> struct Cfg {
+  static constexpr uint32_t PLANES = KIND == kTcec ? 2 : 1;
+  static constexpr uint32_t STAGE_BYTES = 2 * PLANES * TILE_BYTES;
+  static constexpr uint32_t STAGES = KIND == kTcec ? 3 : 6;
+  static constexpr uint32_t K_ELEMS = KIND == kI8 ? 128 : 64; // of K in a stage
+  static constexpr uint32_t BARS = STAGES * STAGE_BYTES;      // offsets in shared memory
+  static constexpr uint32_t FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
+                            ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, TMEM_PTR = TAIL + 8,
+                            ABORT = TMEM_PTR + 4, START = BARS + 256,
+                            FIRST_TILE = START + 4 * (kMaxGroups + 2),
+                            BYTES = FIRST_TILE + 4 * (kMaxGroups + 2);
+  static_assert(ABORT + 4 <= START, "barriers and flags");
+  static constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
+};
+
+struct GroupedParams {
+  const int32_t *ends;
+  void *out;
+  uint64_t ldo, stride_o;
+  const float *lane_scale; // i8; tcec: the two factors of `unscale`, or null
+  const float *col_scale, *bias;
+  int *status;
+  uint32_t rows, groups, lane_dim, col_dim, k_blocks, idesc;
+  float alpha, beta;
+  uint32_t out_type;
+};
+static_assert(sizeof(GroupedParams) <= 128, "read from the constant bank (gemm_common.cuh)");
+
+// A tile: `cols` columns from col0 on (of the rows of x, or wgrad: of a weight dimension), 256 lanes
+// from lane0 on, `blocks` steps of K.  Without any, its product is zero.
+struct Tile {
+  uint32_t group, lane0, col0, cols, blocks;
+  uint32_t row0, rows;                                           // wgrad: the group's
+  __device__ __forceinline__ uint32_t width() const { return (cols + 31u) & ~31u; } // N of the product
+};
+
+// The tiles this pair takes.  Groups in turn; within one, bands of column tiles that all lane tiles
+// pass over, so that what runs at the same time shares operands in L2.
+template <int KIND, bool WGRAD> struct Walk {
+  const uint32_t *start, *first_tile; // shared memory
+  uint32_t tile, step, group, total;
+  __device__ __forceinline__ Walk(const uint8_t *smem, const GroupedParams &p, uint32_t cluster,
+                                  uint32_t clusters) {
+    start = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::START);
+    first_tile = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
+    tile = cluster;
+    step = clusters;
+    group = 0;
+    total = first_tile[p.groups + 1];
+  }
+  __device__ __forceinline__ bool next(const GroupedParams &p, Tile &x) {
+    if (tile >= total) return false;
+    while (tile >= first_tile[group + 1]) ++group;
+    const uint32_t local = tile - first_tile[group];
+    tile += step;
+    x.group = group;
+    const uint32_t r0 = start[group], r = start[group + 1] - r0;
+    const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
+    const uint32_t col_dim = WGRAD ? p.col_dim : r;
+    const uint32_t col_tiles = (col_dim + COLS - 1) / COLS;
+    const uint32_t band = local / (BAND * lane_tiles), in_band = local - band * BAND * lane_tiles;
+    const uint32_t width = min(BAND, col_tiles - band * BAND);
+    const uint32_t lt = in_band / width, ct = band * BAND + (in_band - lt * width);
+    x.lane0 = lt * LANES;
+    x.cols = min(COLS, col_dim - ct * COLS);
+    x.col0 = ct * COLS + (WGRAD ? 0u : r0);
+    x.blocks = WGRAD ? (r + 63u) / 64u : (group < p.groups ? p.k_blocks : 0u);
+    x.row0 = r0;
+    x.rows = r;
+    return true;
+  }
+};
+
+// First row and first tile of each group, by one warp.  What `ends` holds is never trusted: a total
+// that falls back or passes the number of rows is taken as the one in front of it, or as that number.
+// The rows behind the last group are a group of their own (product: its tiles have no blocks; wgrad:
+// it has no tiles).
+template <int KIND, bool WGRAD>
+__device__ __forceinline__ void find_groups(uint8_t *smem, const GroupedParams &p) {
+  uint32_t *start = reinterpret_cast<uint32_t *>(smem + Cfg<KIND>::START);
+  uint32_t *first_tile = reinterpret_cast<uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
+  uint32_t end_before = 0, tiles_before = 0;
+  for (uint32_t g0 = 0; g0 < p.groups + 1; g0 += 32) {
+    const uint32_t g = g0 + lane;
+    uint32_t end = 0;
+    if (g < p.groups)
+      end = p.ends == nullptr ? p.rows
+                              : static_cast<uint32_t>(min(max(__ldg(p.ends + g), 0),
+                                                          static_cast<int32_t>(p.rows)));
+    else if (g == p.groups) end = p.rows;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, end, d);
+      if (static_cast<int>(lane) >= d) end = max(end, o);
+    }
+    end = max(end, end_before);
+    uint32_t begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = end_before;
+    uint32_t tiles = 0;
+    if constexpr (WGRAD) {
+      if (g < p.groups) tiles = lane_tiles * ((p.col_dim + COLS - 1) / COLS);
+    } else {
+      if (g <= p.groups) tiles = lane_tiles * ((end - begin + COLS - 1) / COLS);
+    }
+    uint32_t upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (static_cast<int>(lane) >= d) upto += o;
+    }
+    if (g <= p.groups) {
+      start[g] = begin;
+      first_tile[g] = tiles_before + upto - tiles;
+      if (g == p.groups) {
+        start[g + 1] = end;
+        first_tile[g + 1] = tiles_before + upto;
+      }
+    }
+    end_before = __shfl_sync(0xffffffffu, end, 31);
+    tiles_before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (KIND == kI8) ptx::mma_i8_ss_pair(d, a, b, idesc, acc);
+  else ptx::mma_f16_ss_pair(d, a, b, idesc, acc);
+}
+
+__device__ __forceinline__ float load_as_float(const __half *p) { return __half2float(*p); }
+__device__ __forceinline__ float load_as_float(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_as_float(const float *p) { return *p; }
+// the one rounding of a result to its type
+__device__ __forceinline__ void store_from_float(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store_from_float(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_from_float(float *p, float v) { *p = v; }
+
+// drain_sums and add_corrections_in_tmem (epilogue.cuh) for the first `cols` columns, a multiple of 16.
+// A warp's columns end where its neighbour's begin, and in a narrow tile that is short of COLS / 2.
+__device__ __forceinline__ void drain_columns(uint32_t taddr, float (&sums)[COLS / 2], uint32_t cols) {
+#pragma unroll
+  for (uint32_t c = 0; c < COLS / 2; c += 16) {
+    if (c >= cols) break;
+    uint32_t v[16];
+    ptx::tmem_ld_32x32b_x16(taddr + c, v);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      sums[c + i] += __uint_as_float(v[i]);
+      asm volatile("" : "+f"(sums[c + i])); // added here and now, not where the sum is next used
+    }
+  }
+}
+__device__ __forceinline__ void add_corrections(uint32_t taddr, const float (&sums)[COLS / 2],
+                                                uint32_t cols) {
+#pragma unroll
+  for (uint32_t c = 0; c < COLS / 2; c += 16) {
+    if (c >= cols) break;
+    uint32_t v[16];
+    ptx::tmem_ld_32x32b_x16(taddr + c, v);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i)
+      v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), 1.f / 2048.f, sums[c + i]));
+    ptx::tmem_st_32x32b_x16(taddr + c, v);
+  }
+  ptx::tmem_st_wait();
+}
+
+// What turns a sum into a result, for one lane.
+struct Finish {
+  float f0, f1, add; // sum * f0 * f1 + add  (i8: f0 the lane's scale, f1 the column's)
+  float beta;
+};
+
+// `cols` columns of one lane from tensor memory (zero: there is no sum, the product is 0) to global
+// memory, column c at out + c * ldo.  A warp's lanes hold neighbouring elements.
+template <int KIND, class T>
+__device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out, uint64_t ldo,
+                                              uint32_t cols, bool lane_ok, const Finish &f,
+                                              const float *col_scale) {
+  constexpr uint32_t G = kEpiGroup;
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += G) {
+    float cs = 1.f;
+    if constexpr (KIND == kI8) {
+      if (lane < G && c + lane < cols) cs = __ldg(col_scale + c + lane);
+    }
+    uint32_t v[G];
+    if (!zero) {
+      ptx::tmem_ld_32x32b_x16(taddr + c, v);
+      ptx::tmem_ld_wait();
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < G; ++j) {
+      float x;
+      if constexpr (KIND == kI8) {
+        const float s = __shfl_sync(0xffffffffu, cs, j);
+        x = fmaf(__int2float_rn(static_cast<int>(v[j])) * f.f0, s, f.add);
+      } else {
+        x = __uint_as_float(v[j]) * f.f0 * f.f1;
+      }
+      if (zero) x = 0.f;
+      if (lane_ok && c + j < cols) {
+        T *at = out + static_cast<uint64_t>(c + j) * ldo;
+        if (f.beta != 0.f) x = fmaf(f.beta, load_as_float(at), x);
+        store_from_float(at, x);
+      }
+    }
+  }
+}
+
+template <int KIND, bool A_LANES, bool WGRAD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+    grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                        const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ CUtensorMap map_b_few, const GroupedParams p) {
+  using C = Cfg<KIND>;
+  constexpr uint32_t PLANES = C::PLANES, STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *const smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  volatile int *const abort_flag = reinterpret_cast<volatile int *>(smem + C::ABORT);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+  const uint32_t cluster_id = blockIdx.x >> 1;
+  const uint32_t clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(sbase + C::FULL + 8 * s, 2);
+      ptx::mbar_init(sbase + C::EMPTY + 8 * s, 1);
+    }
+    for (uint32_t b = 0; b < 2; ++b) {
+      ptx::mbar_init(sbase + C::ACC_FULL + 8 * b, 1);
+      ptx::mbar_init(sbase + C::ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
+    }
+    ptx::mbar_init(sbase + C::TAIL, 1);
+    *abort_flag = 0;
+    ptx::mbar_init_fence();
+    ptx::prefetch_tensormap(&map_a);
+    ptx::prefetch_tensormap(&map_b);
+    if (!WGRAD) ptx::prefetch_tensormap(&map_b_few);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(sbase + C::TMEM_PTR, TMEM_COLS);
+    ptx::tmem_relinquish_pair();
+  }
+  // everything above needs nothing of the kernel in front, everything below may
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  if (warp == 2) find_groups<KIND, WGRAD>(smem, p);
+  ptx::tc_fence_before();
+  __syncthreads();
+  // both CTAs' barriers must exist before any remote arrive / remote TMA completion
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<const uint32_t *>(smem + C::TMEM_PTR);
+
+  if (warp == 0) {
+    // ================================================================ TMA producer (both CTAs)
+    // One thread; for wgrad the whole warp, which has rows to zero.
+    if (WGRAD || ptx::elect_one()) {
+      uint32_t s = 0, ph = 1, tail_ph = 0;
+      bool ok = true;
+      Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+      Tile x;
+      while (ok && walk.next(p, x)) {
+        const int a_lane = static_cast<int>(x.lane0 + rank * BM_CTA);
+        const uint32_t half = x.width() / 2;
+        const int b_col = static_cast<int>(x.col0 + rank * half);
+        // boxes of the column operand: of 64 columns (wgrad), one of 128 rows, or as many of 32 as it takes
+        const bool whole_box = !WGRAD && half > 128 - FEW_ROWS;
+        const uint32_t boxes = WGRAD ? (half + 63u) / 64u
+                                     : (whole_box ? 1u : (half + FEW_ROWS - 1u) / FEW_ROWS);
+        const uint32_t bytes =
+            PLANES * (TILE_BYTES + boxes * (WGRAD ? ATOM_BYTES : whole_box ? TILE_BYTES : FEW_ROWS * ROW_BYTES));
+        for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+          ok = ptx::mbar_wait(sbase + C::EMPTY + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitEmpty);
+          if (WGRAD) ok = ptx::warp_agrees(ok);
+          if (!ok) break;
+          const uint32_t st = sbase + s * STAGE_BYTES;
+          const uint32_t full = ptx::map_to_cta(sbase + C::FULL + 8 * s, 0); // the leader's barrier
+          const uint32_t rows_here = WGRAD ? min(64u, x.rows - kb * 64u) : 64u;
+          const bool tail = WGRAD && rows_here < 64u;
+          if (!WGRAD || ptx::elect_one()) {
+            if (tail) ptx::mbar_arrive_expect_tx(sbase + C::TAIL, bytes);
+            else if (leader) ptx::mbar_arrive_expect_tx(sbase + C::FULL + 8 * s, 2 * bytes);
+            else ptx::mbar_arrive_cluster(full);
+            auto load = [&](uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2) {
+              if (tail) ptx::tma_load_3d(dst, m, sbase + C::TAIL, c0, c1, c2);
+              else ptx::tma_load_3d_pair(dst, m, full, c0, c1, c2);
+            };
+            const int red = static_cast<int>(WGRAD ? x.row0 + kb * 64u : kb * C::K_ELEMS);
+#pragma unroll
+            for (uint32_t pl = 0; pl < PLANES; ++pl) {
+              const uint32_t a_dst = st + pl * TILE_BYTES, b_dst = st + (PLANES + pl) * TILE_BYTES;
+              const int za = static_cast<int>(WGRAD ? pl : pl * p.groups + x.group);
+              if constexpr (A_LANES) {
+                load(a_dst, &map_a, a_lane, red, za);
+                load(a_dst + ATOM_BYTES, &map_a, a_lane + 64, red, za);
+              } else {
+                load(a_dst, &map_a, red, a_lane, za);
+              }
+              if constexpr (WGRAD) {
+                for (uint32_t b = 0; b < boxes; ++b)
+                  load(b_dst + b * ATOM_BYTES, &map_b, b_col + static_cast<int>(64 * b), red,
+                       static_cast<int>(pl));
+              } else if (whole_box) {
+                load(b_dst, &map_b, red, b_col, static_cast<int>(pl));
+              } else {
+                for (uint32_t b = 0; b < boxes; ++b)
+                  load(b_dst + b * FEW_ROWS * ROW_BYTES, &map_b_few, red,
+                       b_col + static_cast<int>(FEW_ROWS * b), static_cast<int>(pl));
+              }
+            }
+          }
+          if (tail) {
+            // (a row of 128 bytes is a row of 128 bytes under the swizzle too)
+            ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::TAIL, tail_ph, abort_flag, p.status,
+                                                 ptx::kErrWaitFull));
+            if (!ok) break;
+            tail_ph ^= 1u;
+            const uint32_t upto = (rows_here + 15u) & ~15u;
+            for (uint32_t pl = 0; pl < PLANES; ++pl)
+              for (uint32_t at = 0; at < 2 + boxes; ++at) {
+                const uint32_t atom = st + (at < 2 ? pl : PLANES + pl) * TILE_BYTES +
+                                      (at < 2 ? at : at - 2) * ATOM_BYTES;
+                for (uint32_t i = rows_here * ROW_BYTES + 16u * lane; i < upto * ROW_BYTES; i += 512u)
+                  st_shared_v4(atom + i, 0u, 0u, 0u, 0u);
+              }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(full);
+          }
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ================================================================ MMA issuer (leader only)
+    if (leader && ptx::elect_one()) {
+      constexpr uint16_t BOTH = 0x3;
+      constexpr uint64_t kStage = STAGE_BYTES >> 4, kTile = TILE_BYTES >> 4;
+      constexpr uint32_t A_STEP = A_LANES ? 2048 >> 4 : 2, B_STEP = WGRAD ? 2048 >> 4 : 2;
+      const uint64_t a0 = A_LANES ? ptx::make_mnmajor_desc(sbase, ATOM_BYTES)
+                                  : ptx::make_kmajor_desc<ROW_BYTES>(sbase);
+      const uint32_t b_addr = sbase + PLANES * TILE_BYTES;
+      const uint64_t b0 = WGRAD ? ptx::make_mnmajor_desc(b_addr, ATOM_BYTES)
+                                : ptx::make_kmajor_desc<ROW_BYTES>(b_addr);
+      uint32_t s = 0, ph = 0;
+      uint32_t acc = 0, e_ph = 1;          // accumulator in turn (f16, i8) and the phase of its barrier
+      uint32_t d0_ph = 1, d1_ph = 1;       // tcec
+      bool ok = true;
+      Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+      Tile x;
+      while (ok && walk.next(p, x)) {
+        if (x.blocks == 0) continue;
+        const uint32_t idesc = p.idesc | ((x.width() >> 3) << 17);
+        if constexpr (KIND != kTcec) {
+          ok = ptx::mbar_wait(sbase + C::ACC_EMPTY + 8 * acc, e_ph, abort_flag, p.status,
+                              ptx::kErrWaitD0Empty);
+          if (!ok) break;
+          ptx::tc_fence_after();
+        }
+        const uint32_t d = tmem_base + acc * COLS;
+        for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+          ok = ptx::mbar_wait(sbase + C::FULL + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitFull);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          const uint64_t a = a0 + s * kStage, b = b0 + s * kStage;
+          const uint32_t steps = WGRAD ? (min(64u, x.rows - kb * 64u) + 15u) / 16u : 4u;
+          if constexpr (KIND != kTcec) {
+#pragma unroll
+            for (uint32_t ks = 0; ks < 4; ++ks)
+              if (!WGRAD || ks < steps)
+                mma<KIND>(d, a + A_STEP * ks, b + B_STEP * ks, idesc, (kb | ks) != 0);
+          } else {
+            const bool first = kb % DRAIN_STAGES == 0;
+            auto corrections = [&](uint32_t acc_first) {
+#pragma unroll
+              for (uint32_t ks = 0; ks < 4; ++ks)
+                if (!WGRAD || ks < steps)
+                  mma<KIND>(tmem_base + COLS, a + kTile + A_STEP * ks, b + B_STEP * ks, idesc,
+                            ks > 0 ? 1u : acc_first);
+#pragma unroll
+              for (uint32_t ks = 0; ks < 4; ++ks)
+                if (!WGRAD || ks < steps)
+                  mma<KIND>(tmem_base + COLS, a + A_STEP * ks, b + kTile + B_STEP * ks, idesc, 1u);
+            };
+            // The corrections of a chunk's first stage come before its hi*hi products: the drain of
+            // the previous chunk hides behind them.  In a tile's first stage they wait for the
+            // epilogue to give their accumulator back, so they come last.
+            if (first && kb > 0) corrections(1u);
+            if (first) {
+              ok = ptx::mbar_wait(sbase + C::ACC_EMPTY, d0_ph, abort_flag, p.status,
+                                  ptx::kErrWaitD0Empty);
+              if (!ok) break;
+              d0_ph ^= 1u;
+              ptx::tc_fence_after();
+            }
+#pragma unroll
+            for (uint32_t ks = 0; ks < 4; ++ks)
+              if (!WGRAD || ks < steps)
+                mma<KIND>(tmem_base, a + A_STEP * ks, b + B_STEP * ks, idesc, !first || ks > 0);
+            if (kb % DRAIN_STAGES == DRAIN_STAGES - 1 || kb + 1 == x.blocks)
+              ptx::tc_commit_pair(sbase + C::ACC_FULL, BOTH);
+            if (!(first && kb > 0)) {
+              if (kb == 0) {
+                ok = ptx::mbar_wait(sbase + C::ACC_EMPTY + 8, d1_ph, abort_flag, p.status,
+                                    ptx::kErrWaitD1Empty);
+                if (!ok) break;
+                d1_ph ^= 1u;
+                ptx::tc_fence_after();
+              }
+              corrections(kb > 0 ? 1u : 0u);
+            }
+          }
+          ptx::tc_commit_pair(sbase + C::EMPTY + 8 * s, BOTH);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if constexpr (KIND == kTcec) {
+          ptx::tc_commit_pair(sbase + C::ACC_FULL + 8, BOTH);
+        } else {
+          ptx::tc_commit_pair(sbase + C::ACC_FULL + 8 * acc, BOTH);
+          acc ^= 1u;
+          if (acc == 0) e_ph ^= 1u;
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ================================================================ epilogue (both CTAs)
+    const uint32_t quarter = static_cast<uint32_t>(warp & 3), second = static_cast<uint32_t>(warp - 4) >> 2;
+    const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16);
+    const uint32_t acc_empty = ptx::map_to_cta(sbase + C::ACC_EMPTY, 0);
+    uint32_t acc = 0, f_ph = 0, d0_ph = 0, d1_ph = 0;
+    bool ok = true;
+    Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+    Tile x;
+    auto release = [&](uint32_t b) {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(acc_empty + 8 * b);
+    };
+    while (ok && walk.next(p, x)) {
+      const uint32_t half = x.width() / 2;
+      uint32_t t_sums = t_lanes + second * half;
+      const bool zero = x.blocks == 0;
+      if constexpr (KIND == kTcec) {
+        if (!zero) {
+          float sums[COLS / 2];
+#pragma unroll
+          for (uint32_t i = 0; i < COLS / 2; ++i) sums[i] = 0.f;
+          const uint32_t chunks = (x.blocks + DRAIN_STAGES - 1) / DRAIN_STAGES;
+#pragma unroll 1
+          for (uint32_t c = 0; c < chunks; ++c) {
+            ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::ACC_FULL, d0_ph, abort_flag, p.status,
+                                                 ptx::kErrWaitD0Full));
+            if (!ok) break;
+            d0_ph ^= 1u;
+            ptx::tc_fence_after();
+            drain_columns(t_sums, sums, half);
+            release(0);
+          }
+          if (!ok) break;
+          ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::ACC_FULL + 8, d1_ph, abort_flag, p.status,
+                                               ptx::kErrWaitD1Full));
+          if (!ok) break;
+          d1_ph ^= 1u;
+          ptx::tc_fence_after();
+          t_sums += COLS;
+          add_corrections(t_sums, sums, half);
+        }
+      } else if (!zero) {
+        ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::ACC_FULL + 8 * acc, f_ph, abort_flag, p.status,
+                                             ptx::kErrWaitD0Full));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        t_sums += acc * COLS;
+      }
+      const uint32_t lane_at = x.lane0 + rank * BM_CTA + quarter * 32u + static_cast<uint32_t>(lane);
+      const bool lane_ok = lane_at < p.lane_dim;
+      const uint32_t col = second * half;
+      const uint32_t cols = x.cols > col ? min(half, x.cols - col) : 0u;
+      const uint64_t at = (WGRAD ? x.group * p.stride_o : 0ull) +
+                          static_cast<uint64_t>(x.col0 + col) * p.ldo + lane_at;
+      Finish f = {p.alpha, 1.f, 0.f, p.beta};
+      const float *col_scale = nullptr;
+      if constexpr (KIND == kI8) {
+        f.f0 = 0.f;
+        if (!zero && lane_ok) {
+          const uint64_t feature = static_cast<uint64_t>(x.group) * p.lane_dim + lane_at;
+          f.f0 = __ldg(p.lane_scale + feature);
+          if (p.bias != nullptr) f.add = __ldg(p.bias + feature);
+        }
+        col_scale = p.col_scale + x.col0 + col;
+      } else if (KIND == kTcec && p.lane_scale != nullptr) {
+        f.f0 = p.alpha * __ldg(p.lane_scale);
+        f.f1 = __ldg(p.lane_scale + 1);
+      }
+      if (p.out_type == static_cast<uint32_t>(GroupedOut::f32))
+        store_columns<KIND>(t_sums, zero, static_cast<float *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
+      else if (KIND != kTcec && p.out_type == static_cast<uint32_t>(GroupedOut::bf16))
+        store_columns<KIND>(t_sums, zero, static_cast<__nv_bfloat16 *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
+      else if (KIND != kTcec)
+        store_columns<KIND>(t_sums, zero, static_cast<__half *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
+      if (!zero) {
+        if constexpr (KIND == kTcec) {
+          release(1);
+        } else {
+          release(acc);
+          acc ^= 1u;
+          if (acc == 0) f_ph ^= 1u;
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  // The peer's shared memory and TMEM are in use by the leader's MMAs until the last accumulator has
+  // been announced in both CTAs; neither CTA leaves before the other has finished its epilogue.
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (*abort_flag) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// Per device and kernel, once (any thread): shared-memory attribute and the pairs the device keeps
+// resident.  (A kernel of each instance has a type of its own here: its statics are its own.)
+template <int KIND, bool A_LANES, bool WGRAD> cudaError_t set_up(int *clusters_out) {
+  static std::once_flag once[64];
+  static cudaError_t setup_error[64];
+  static int max_clusters[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&]() {
+    const auto kernel = grouped_gemm_kernel<KIND, A_LANES, WGRAD>;
+    setup_error[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            Cfg<KIND>::SMEM);
+    int sms = 0;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int clusters = sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = Cfg<KIND>::SMEM;
+    int active = 0;
+    if (setup_error[dev] == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&active, kernel, &cfg) == cudaSuccess) {
+      if (active > 0 && active < clusters) clusters = active;
+    } else {
+      cudaGetLastError();
+    }
+    max_clusters[dev] = clusters > 0 ? clusters : 1;
+  });
+  *clusters_out = max_clusters[dev];
+  return setup_error[dev];
+}
+
+// `inner_box` by `outer_box` elements; with nothing in it (no rows at all) the map is of one row, which
+// no load asks for.
+bool operand_map(CUtensorMap *map, const GroupedOperand &o, int elem_bytes, const void *fallback,
+                 uint32_t inner_box, uint32_t outer_box) {
+  const uint64_t es = static_cast<uint64_t>(elem_bytes), planes = static_cast<uint64_t>(o.batch) * o.planes;
+  const uint64_t matrix = o.batch > 1 ? o.stride : (o.planes > 1 ? o.plane_stride : o.ld);
+  return make_swizzled_map(map, elem_bytes, o.outer > 0 ? o.ptr : fallback,
+                           {o.inner, o.outer > 0 ? o.outer : 1, planes}, {o.ld * es, matrix * es},
+                           {inner_box, outer_box, 1});
+}
+
+template <int KIND, bool A_LANES, bool WGRAD>
+cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
+  int clusters = 1;
+  const cudaError_t se = set_up<KIND, A_LANES, WGRAD>(&clusters);
+  if (se != cudaSuccess) return se;
+  constexpr int ES = KIND == kI8 ? 1 : 2;
+  CUtensorMap map_a, map_b, map_b_few;
+  // (any address does for an operand without rows; this one is 16-byte aligned)
+  const void *fallback = a.dev_status;
+  if (!operand_map(&map_a, a.a, ES, fallback, Cfg<KIND>::K_ELEMS, A_LANES ? 64 : BM_CTA) ||
+      !operand_map(&map_b, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, WGRAD ? 64 : BM_CTA) ||
+      !operand_map(&map_b_few, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, WGRAD ? 64 : FEW_ROWS))
+    return cudaErrorInvalidValue;
+  GroupedParams p = {};
+  p.ends = a.ends;
+  p.out = a.out;
+  p.ldo = a.ldo;
+  p.stride_o = a.stride_o;
+  p.lane_scale = KIND == kTcec ? a.unscale : a.lane_scale;
+  p.col_scale = a.col_scale;
+  p.bias = a.bias;
+  p.status = a.dev_status;
+  p.rows = a.rows;
+  p.groups = a.groups;
+  p.lane_dim = a.lane_dim;
+  p.col_dim = a.col_dim;
+  p.k_blocks = (a.k + Cfg<KIND>::K_ELEMS - 1) / Cfg<KIND>::K_ELEMS;
+  // formats: F32 sums of F16 (0) or BF16 (1), or S32 sums of S8 (1); bits 15 and 16: A, B with their
+  // lanes, columns contiguous
+  const uint32_t sum_format = KIND == kI8 ? 2u : 1u, format = KIND == kI8 ? 1u : (a.bf16 ? 1u : 0u);
+  p.idesc = (sum_format << 4) | (format << 7) | (format << 10) | (A_LANES ? 1u << 15 : 0u) |
+            (WGRAD ? 1u << 16 : 0u) | ((LANES >> 4) << 24);
+  p.alpha = a.alpha;
+  p.beta = a.beta;
+  p.out_type = static_cast<uint32_t>(a.out_type);
+  return launch_chained(grouped_gemm_kernel<KIND, A_LANES, WGRAD>, static_cast<unsigned>(2 * clusters),
+                        NUM_THREADS, Cfg<KIND>::SMEM, stream, map_a, map_b, map_b_few, p);
+}
+
+} // namespace
+
+cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream) {
+  if (a.kind == GroupedKind::i8) {
+    if (a.wgrad || a.a_lane_contig) return cudaErrorInvalidValue;
+    return launch<kI8, false, false>(a, stream);
+  }
+  if (a.kind == GroupedKind::tcec)
+    return a.wgrad            ? launch<kTcec, true, true>(a, stream)
+           : a.a_lane_contig  ? launch<kTcec, true, false>(a, stream)
+                              : launch<kTcec, false, false>(a, stream);
+  return a.wgrad           ? launch<kF16, true, true>(a, stream)
+         : a.a_lane_contig ? launch<kF16, true, false>(a, stream)
+                           : launch<kF16, false, false>(a, stream);
+}
+
+} // namespace cumpsgemm_b200

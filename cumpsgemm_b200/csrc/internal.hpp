@@ -208,6 +208,12 @@ inline void mark_stream_work(cuMpSGEMM_handle *h) {
     cudaGetLastError();
 }
 
+// Makes the handle's workspace hold `bytes`.  Returns false, with the old workspace untouched, while the
+// stream is being captured, and false without a workspace if there is no memory.
+bool ensure_workspace(cuMpSGEMM_handle *h, std::size_t bytes);
+// The most that a call may ask of it.
+std::size_t workspace_limit(const cuMpSGEMM_handle *h);
+
 // RAII: make the handle's device current for the duration of a call.
 struct DeviceGuard {
   int prev = -1;

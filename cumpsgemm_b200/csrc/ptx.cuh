@@ -461,6 +461,20 @@ __device__ __forceinline__ void mma_tf32_ss_pair(uint32_t d_tmem, uint64_t a_des
       : "memory");
 }
 
+// kind::i8: signed 8-bit operands, 32-bit integer accumulation
+__device__ __forceinline__ void mma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // The same with A in tensor memory, for one CTA (CG = 1) or a pair (2): lane = row (each CTA holds its
 // own 128), a 32-bit column = two consecutive FP16 or one TF32 value of K.
 template <int CG>
@@ -506,6 +520,21 @@ __device__ __forceinline__ uint64_t make_kmajor_desc(uint32_t smem_addr) {
   d |= static_cast<uint64_t>((8 * SWIZZLE_BYTES) >> 4) << 32;
   d |= 1ull << 46;
   d |= layout << 61;
+  return d;
+}
+
+// The same for a 16-bit operand stored with its M (or N) dimension contiguous: blocks of 64 elements
+// (128 bytes, one swizzle atom) by any number of K rows, `atom_bytes` from one block of 64 to the
+// next, 8 K rows 1024 bytes apart, as written by a TMA load with the 128-byte swizzle.  Here the
+// leading byte offset is the step between blocks and the stride byte offset the step of 8 K rows;
+// 16 K values further on is 2048 bytes further on.
+__device__ __forceinline__ uint64_t make_mnmajor_desc(uint32_t smem_addr, uint32_t atom_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(atom_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
   return d;
 }
 

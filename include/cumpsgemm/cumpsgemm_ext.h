@@ -344,6 +344,66 @@ cublasStatus_t cuMpSGEMM_sgemm_static_scratch(
     uint64_t k, const float *alpha, const float *a, uint64_t lda, const float *b, uint64_t ldb,
     const float *beta, float *c, uint64_t ldc, cuMpSGEMM_compute_mode_t compute_mode);
 
+/* ---- products of rows grouped by expert ---------------------------------- */
+/* No counterpart in the reference.  The products of a mixture-of-experts layer: rows (tokens) sorted
+ * by the group (expert) they belong to, and a weight matrix for each group.  Unlike the rest of this
+ * interface, all matrices are ROW-MAJOR, as the frameworks that train and serve such models hold them;
+ * ld* is the distance of rows and stride* of matrices, in elements.
+ *   group_ends[num_groups], in device memory: the running total of rows after each group, so group e
+ *     has the rows [group_ends[e - 1], group_ends[e]) of x, from 0 for the first.  It is read on the
+ *     device: nothing waits for the sizes of the groups.  Groups may be empty.  A total below the one in
+ *     front of it or above `rows` is taken as that.  NULL, with one group: all rows are of that group.
+ *     Rows behind the last total belong to no group; what stands in them never counts.
+ *   num_groups <= 1024; rows, n, k < 2^31.  rows may be 0.
+ *   type: CUDA_R_16F or CUDA_R_16BF, summed in FP32 and rounded once, or CUDA_R_32F, which `mode`
+ *     multiplies with error correction as the other calls do: CUMPSGEMM_FP16TCEC, or
+ *     CUMPSGEMM_FP16TCEC_SCALING, which first brings the largest finite magnitude of each operand (of its
+ *     rows in groups) to 2^14.  Other modes return CUBLAS_STATUS_NOT_SUPPORTED; 16-bit types do not look
+ *     at it.
+ *   Any leading dimension, stride and alignment.  FP32 operands, and 8- and 16-bit ones whose address,
+ *     leading dimension or stride is not a multiple of 16 bytes, go through the handle's workspace
+ *     (CUBLAS_STATUS_ALLOC_FAILED where it cannot hold them).
+ *   Results are the same from run to run.  Outputs must not overlap inputs. */
+
+/* y[r, :] = alpha * x[r, :] op(w_e) + beta * y[r, :] for the rows r of each group e; rows of no group:
+ * beta * y.  x is rows x k, y rows x n; w_e is stored k x n (op_W = CUBLAS_OP_N) or n x k (CUBLAS_OP_T).
+ * The gradient of x is the same call with y's gradient as x, n and k exchanged and the other op_W.
+ * beta == 0 does not read y. */
+cublasStatus_t cuMpSGEMM_grouped_gemm(cuMpSGEMM_handle_t handle, cublasOperation_t op_W, uint64_t rows,
+                                      uint64_t n, uint64_t k, uint32_t num_groups,
+                                      const int32_t *group_ends, const float *alpha, const void *x,
+                                      uint64_t ldx, const void *w, uint64_t ldw, uint64_t stridew,
+                                      const float *beta, void *y, uint64_t ldy, cudaDataType_t type,
+                                      cuMpSGEMM_compute_mode_t mode);
+/* The gradient of the weights: dw_e = alpha * x_e^T dy_e + beta * dw_e over the rows of group e, stored
+ * k x n (CUBLAS_OP_N) or n x k (CUBLAS_OP_T, the transpose).  Groups without rows: beta * dw_e. */
+cublasStatus_t cuMpSGEMM_grouped_gemm_wgrad(cuMpSGEMM_handle_t handle, cublasOperation_t op_W,
+                                            uint64_t rows, uint64_t n, uint64_t k, uint32_t num_groups,
+                                            const int32_t *group_ends, const float *alpha, const void *x,
+                                            uint64_t ldx, const void *dy, uint64_t lddy,
+                                            const float *beta, void *dw, uint64_t lddw,
+                                            uint64_t stridedw, cudaDataType_t type,
+                                            cuMpSGEMM_compute_mode_t mode);
+/* Product of 8-bit integers with a scale for each row of x (token) and each column of y (channel):
+ *   y[r, c] = x_scale[r] * w_scale[e * n + c] * sum_i xq[r, i] wq_e[c, i] (+ bias[e * n + c])
+ * for the rows r of each group e; rows of no group: 0.  wq_e is stored n x k.  The sums are exact
+ * (k <= 131071), the scales are applied in FP32 and the result is rounded once to y_type (any of the
+ * three).  bias may be NULL.  One group with group_ends = NULL is a plain quantised linear layer. */
+cublasStatus_t cuMpSGEMM_i8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t n, uint64_t k,
+                                         uint32_t num_groups, const int32_t *group_ends,
+                                         const int8_t *xq, uint64_t ldx, const float *x_scale,
+                                         const int8_t *wq, uint64_t ldw, uint64_t stridew,
+                                         const float *w_scale, const float *bias, void *y, uint64_t ldy,
+                                         cudaDataType_t y_type);
+/* Rows to 8 bits: with top the largest magnitude of a row, scale = top / 127 and
+ * q[i] = rint(x[i] * (127 / top)), ties to even; a row of zeros has scale 0, a row with an infinity or
+ * NaN has scale NaN and q = 0 (its products are NaN).  Row r is taken from row row_index[r] of x
+ * (NULL: r); an index outside [0, src_rows) gives a row of zeros.  type: that of x, any of the three. */
+cublasStatus_t cuMpSGEMM_quantize_rows_i8(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t k,
+                                          const void *x, uint64_t ldx, cudaDataType_t type,
+                                          const int32_t *row_index, uint64_t src_rows, int8_t *q,
+                                          uint64_t ldq, float *scale);
+
 #ifdef __cplusplus
 }
 #endif
