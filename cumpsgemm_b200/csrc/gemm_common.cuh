@@ -61,9 +61,9 @@ bool make_float_map(CUtensorMap *map, const float *base, const uint64_t (&dims)[
                     const uint64_t (&strides)[2], const uint32_t (&box)[3], bool swizzle);
 
 // Tensor map over matrices of 8- or 16-bit elements: dims[0] contiguous, strides (bytes) of dims 1 and
-// 2, box[0] = 128 bytes, 128-byte swizzle; what lies outside reads as zero.
-bool make_swizzled_map(CUtensorMap *map, int elem_bytes, const void *base, const uint64_t (&dims)[3],
-                       const uint64_t (&strides)[2], const uint32_t (&box)[3]);
+// 2; 128-byte swizzle with box[0] = 128 bytes, or none.  What lies outside reads as zero.
+bool make_byte_map(CUtensorMap *map, int elem_bytes, const void *base, const uint64_t (&dims)[3],
+                   const uint64_t (&strides)[2], const uint32_t (&box)[3], bool swizzle);
 
 // How the pair kernel deals `total_tiles` tiles with `units` x 64 k values to at most
 // `max_clusters` CTA pairs (tcec_gemm_pair.cu).

@@ -477,11 +477,11 @@ bool make_float_map(CUtensorMap *map, const float *base, const uint64_t (&dims)[
                     swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-bool make_swizzled_map(CUtensorMap *map, int elem_bytes, const void *base, const uint64_t (&dims)[3],
-                       const uint64_t (&strides)[2], const uint32_t (&box)[3]) {
+bool make_byte_map(CUtensorMap *map, int elem_bytes, const void *base, const uint64_t (&dims)[3],
+                   const uint64_t (&strides)[2], const uint32_t (&box)[3], bool swizzle) {
   return encode_map(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
                     base, {dims[0], dims[1], dims[2]}, {strides[0], strides[1]}, {box[0], box[1], box[2]},
-                    CU_TENSOR_MAP_SWIZZLE_128B);
+                    swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 namespace {
