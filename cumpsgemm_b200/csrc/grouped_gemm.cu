@@ -22,18 +22,19 @@
 // accumulator of their own, as in tcec_gemm_pair.cu.
 //
 // wgrad reduces over a group's rows, which end inside a 64-row block.  The next group's rows must not
-// count, not even multiplied by zero, since they may be NaN: the warp that issues the loads waits
-// for such a last block, zeroes the rows up to the next multiple of 16 in both operands, and the
-// tensor core gets only as many steps of 16.  That wait is hidden behind the blocks in front of it.
+// count, not even multiplied by zero, since they may be NaN: a warp of its own waits for such a last
+// block, zeroes the rows up to the next multiple of 16 in both operands, and the tensor core gets only
+// as many steps of 16.  (With the warp that issues the loads doing it the next tile's loads waited too:
+// 32768 rows x 4096 x 4096 over 16 experts in bfloat16 took 984 us instead of 895.)
 //
 // Barriers ("leader" = cluster rank 0):
 //   full[s]       leader's only: 2 arrivals, one from each CTA's producer (the leader's with the
-//                 bytes of both CTAs' loads; for a last block each once its rows are zeroed)
+//                 bytes of both CTAs' loads), or for a last block from the warps that zero its rows
 //   empty[s]      in both CTAs: commit multicast from the leader
 //   acc_full[b]   in both CTAs: commit multicast.  b: one of two accumulators (f16, i8), or hi*hi (0)
 //                 and the corrections (1)
 //   acc_empty[b]  leader's only: 16 arrivals, one from each epilogue warp of both CTAs
-//   tail          own: a last block's loads
+//   tail[s]       own: a last block's loads
 // Every wait is bounded; no TMA multicast is used.
 #include "epilogue.cuh"
 #include "gemm_common.cuh"
@@ -73,12 +74,12 @@ template <int KIND> struct Cfg {
   static constexpr uint32_t K_ELEMS = KIND == kI8 ? 128 : 64; // of K in a stage
   static constexpr uint32_t BARS = STAGES * STAGE_BYTES;      // offsets in shared memory
   static constexpr uint32_t FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
-                            ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, TMEM_PTR = TAIL + 8,
+                            ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, TMEM_PTR = TAIL + 8 * STAGES,
                             ABORT = TMEM_PTR + 4, START = BARS + 256,
                             FIRST_TILE = START + 4 * (kMaxGroups + 2),
                             OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
                             BYTES = OUT + (KIND == kTcec ? 0 : NUM_EPI_WARPS * 2 * OUT_BYTES);
-  static_assert(ABORT + 4 <= START, "barriers and flags");
+  static_assert(ABORT + 4 <= START && STAGES <= 32, "barriers and flags; phases are bits");
   static constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 };
 
@@ -102,6 +103,7 @@ struct Tile {
   uint32_t group, lane0, col0, cols, blocks;
   uint32_t row0, rows;                                           // wgrad: the group's
   __device__ __forceinline__ uint32_t width() const { return (cols + 31u) & ~31u; } // N of the product
+  __device__ __forceinline__ uint32_t tail_rows(uint32_t kb) const { return min(64u, rows - kb * 64u); }
 };
 
 // The tiles this pair takes.  Groups in turn; within one, bands of column tiles that all lane tiles
@@ -375,12 +377,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t s = 0; s < STAGES; ++s) {
       ptx::mbar_init(sbase + C::FULL + 8 * s, 2);
       ptx::mbar_init(sbase + C::EMPTY + 8 * s, 1);
+      ptx::mbar_init(sbase + C::TAIL + 8 * s, 1);
     }
     for (uint32_t b = 0; b < 2; ++b) {
       ptx::mbar_init(sbase + C::ACC_FULL + 8 * b, 1);
       ptx::mbar_init(sbase + C::ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
     }
-    ptx::mbar_init(sbase + C::TAIL, 1);
     *abort_flag = 0;
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_a);
@@ -405,9 +407,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 
   if (warp == 0) {
     // ================================================================ TMA producer (both CTAs)
-    // One thread; for wgrad the whole warp, which has rows to zero.
-    if (WGRAD || ptx::elect_one()) {
-      uint32_t s = 0, ph = 1, tail_ph = 0;
+    if (ptx::elect_one()) {
+      uint32_t s = 0, ph = 1;
       bool ok = true;
       Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
       Tile x;
@@ -423,61 +424,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             PLANES * (TILE_BYTES + boxes * (WGRAD ? ATOM_BYTES : whole_box ? TILE_BYTES : FEW_ROWS * ROW_BYTES));
         for (uint32_t kb = 0; kb < x.blocks; ++kb) {
           ok = ptx::mbar_wait(sbase + C::EMPTY + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitEmpty);
-          if (WGRAD) ok = ptx::warp_agrees(ok);
           if (!ok) break;
           const uint32_t st = sbase + s * STAGE_BYTES;
           const uint32_t full = ptx::map_to_cta(sbase + C::FULL + 8 * s, 0); // the leader's barrier
-          const uint32_t rows_here = WGRAD ? min(64u, x.rows - kb * 64u) : 64u;
-          const bool tail = WGRAD && rows_here < 64u;
-          if (!WGRAD || ptx::elect_one()) {
-            if (tail) ptx::mbar_arrive_expect_tx(sbase + C::TAIL, bytes);
-            else if (leader) ptx::mbar_arrive_expect_tx(sbase + C::FULL + 8 * s, 2 * bytes);
-            else ptx::mbar_arrive_cluster(full);
-            auto load = [&](uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2) {
-              if (tail) ptx::tma_load_3d(dst, m, sbase + C::TAIL, c0, c1, c2);
-              else ptx::tma_load_3d_pair(dst, m, full, c0, c1, c2);
-            };
-            const int red = static_cast<int>(WGRAD ? x.row0 + kb * 64u : kb * C::K_ELEMS);
+          const bool tail = WGRAD && x.tail_rows(kb) < 64u;
+          if (tail) ptx::mbar_arrive_expect_tx(sbase + C::TAIL + 8 * s, bytes);
+          else if (leader) ptx::mbar_arrive_expect_tx(sbase + C::FULL + 8 * s, 2 * bytes);
+          else ptx::mbar_arrive_cluster(full);
+          auto load = [&](uint32_t dst, const CUtensorMap *m, int c0, int c1, int c2) {
+            if (tail) ptx::tma_load_3d(dst, m, sbase + C::TAIL + 8 * s, c0, c1, c2);
+            else ptx::tma_load_3d_pair(dst, m, full, c0, c1, c2);
+          };
+          const int red = static_cast<int>(WGRAD ? x.row0 + kb * 64u : kb * C::K_ELEMS);
 #pragma unroll
-            for (uint32_t pl = 0; pl < PLANES; ++pl) {
-              const uint32_t a_dst = st + pl * TILE_BYTES, b_dst = st + (PLANES + pl) * TILE_BYTES;
-              const int za = static_cast<int>(WGRAD ? pl : pl * p.groups + x.group);
-              if constexpr (A_LANES) {
-                load(a_dst, &map_a, a_lane, red, za);
-                load(a_dst + ATOM_BYTES, &map_a, a_lane + 64, red, za);
-              } else {
-                load(a_dst, &map_a, red, a_lane, za);
-              }
-              if constexpr (WGRAD) {
-                for (uint32_t b = 0; b < boxes; ++b)
-                  load(b_dst + b * ATOM_BYTES, &map_b, b_col + static_cast<int>(64 * b), red,
-                       static_cast<int>(pl));
-              } else if (whole_box) {
-                load(b_dst, &map_b, red, b_col, static_cast<int>(pl));
-              } else {
-                for (uint32_t b = 0; b < boxes; ++b)
-                  load(b_dst + b * FEW_ROWS * ROW_BYTES, &map_b_few, red,
-                       b_col + static_cast<int>(FEW_ROWS * b), static_cast<int>(pl));
-              }
+          for (uint32_t pl = 0; pl < PLANES; ++pl) {
+            const uint32_t a_dst = st + pl * TILE_BYTES, b_dst = st + (PLANES + pl) * TILE_BYTES;
+            const int za = static_cast<int>(WGRAD ? pl : pl * p.groups + x.group);
+            if constexpr (A_LANES) {
+              load(a_dst, &map_a, a_lane, red, za);
+              load(a_dst + ATOM_BYTES, &map_a, a_lane + 64, red, za);
+            } else {
+              load(a_dst, &map_a, red, a_lane, za);
             }
-          }
-          if (tail) {
-            // (a row of 128 bytes is a row of 128 bytes under the swizzle too)
-            ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::TAIL, tail_ph, abort_flag, p.status,
-                                                 ptx::kErrWaitFull));
-            if (!ok) break;
-            tail_ph ^= 1u;
-            const uint32_t upto = (rows_here + 15u) & ~15u;
-            for (uint32_t pl = 0; pl < PLANES; ++pl)
-              for (uint32_t at = 0; at < 2 + boxes; ++at) {
-                const uint32_t atom = st + (at < 2 ? pl : PLANES + pl) * TILE_BYTES +
-                                      (at < 2 ? at : at - 2) * ATOM_BYTES;
-                for (uint32_t i = rows_here * ROW_BYTES + 16u * lane; i < upto * ROW_BYTES; i += 512u)
-                  st_shared_v4(atom + i, 0u, 0u, 0u, 0u);
-              }
-            fence_proxy_async_shared();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_cluster(full);
+            if constexpr (WGRAD) {
+              for (uint32_t b = 0; b < boxes; ++b)
+                load(b_dst + b * ATOM_BYTES, &map_b, b_col + static_cast<int>(64 * b), red,
+                     static_cast<int>(pl));
+            } else if (whole_box) {
+              load(b_dst, &map_b, red, b_col, static_cast<int>(pl));
+            } else {
+              for (uint32_t b = 0; b < boxes; ++b)
+                load(b_dst + b * FEW_ROWS * ROW_BYTES, &map_b_few, red,
+                     b_col + static_cast<int>(FEW_ROWS * b), static_cast<int>(pl));
+            }
           }
           if (++s == STAGES) {
             s = 0;
@@ -485,6 +464,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           }
         }
       }
+    }
+  } else if (WGRAD && warp == 2) {
+    // ================================================================ last blocks of groups (both CTAs)
+    uint32_t at = 0;    // stage uses in front of this tile's
+    uint32_t phases = 0; // bit s: the phase of TAIL[s]
+    bool ok = true;
+    Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+    Tile x;
+    while (ok && walk.next(p, x)) {
+      at += x.blocks;
+      if (x.blocks == 0 || x.tail_rows(x.blocks - 1) == 64u) continue;
+      const uint32_t s = (at - 1) % STAGES, st = sbase + s * STAGE_BYTES;
+      ok = ptx::warp_agrees(ptx::mbar_wait_backoff(sbase + C::TAIL + 8 * s, (phases >> s) & 1u, abort_flag,
+                                                   p.status, ptx::kErrWaitFull, 32));
+      if (!ok) break;
+      phases ^= 1u << s;
+      // (a row of 128 bytes is a row of 128 bytes under the swizzle too)
+      const uint32_t rows_here = x.tail_rows(x.blocks - 1), upto = (rows_here + 15u) & ~15u;
+      const uint32_t boxes = (x.width() / 2 + 63u) / 64u;
+      for (uint32_t pl = 0; pl < PLANES; ++pl)
+        for (uint32_t i = 0; i < 2 + boxes; ++i) {
+          const uint32_t atom = st + (i < 2 ? pl : PLANES + pl) * TILE_BYTES + (i < 2 ? i : i - 2) * ATOM_BYTES;
+          for (uint32_t b = rows_here * ROW_BYTES + 16u * lane; b < upto * ROW_BYTES; b += 512u)
+            st_shared_v4(atom + b, 0u, 0u, 0u, 0u);
+        }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(sbase + C::FULL + 8 * s, 0));
     }
   } else if (warp == 1) {
     // ================================================================ MMA issuer (leader only)
@@ -518,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           if (!ok) break;
           ptx::tc_fence_after();
           const uint64_t a = a0 + s * kStage, b = b0 + s * kStage;
-          const uint32_t steps = WGRAD ? (min(64u, x.rows - kb * 64u) + 15u) / 16u : 4u;
+          const uint32_t steps = WGRAD ? (x.tail_rows(kb) + 15u) / 16u : 4u;
           if constexpr (KIND != kTcec) {
 #pragma unroll
             for (uint32_t ks = 0; ks < 4; ++ks)
