@@ -61,8 +61,8 @@ constexpr int NUM_EPI_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t DRAIN_STAGES = 2; // tcec: 128 k values per drain (tcec_gemm_pair.cu has the figures)
 constexpr uint32_t BAND = 8;         // column tiles that are walked together
-constexpr uint32_t OUT_ROWS = 16;    // columns of D, rows of the output, that a warp stores by TMA at once
-constexpr uint32_t OUT_BYTES = OUT_ROWS * 32 * 2; // 32 lanes of 16-bit elements
+constexpr uint32_t OUT_COLS = 32;    // columns that a warp stores at a time
+constexpr uint32_t OUT_BYTES = OUT_COLS * 32 * 2; // 32 lanes of 16-bit elements
 
 constexpr int kF16 = static_cast<int>(GroupedKind::f16), kTcec = static_cast<int>(GroupedKind::tcec),
               kI8 = static_cast<int>(GroupedKind::i8);
@@ -78,7 +78,7 @@ template <int KIND> struct Cfg {
                             ABORT = TMEM_PTR + 4, START = BARS + 256,
                             FIRST_TILE = START + 4 * (kMaxGroups + 2),
                             OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                            BYTES = OUT + (KIND == kTcec ? 0 : NUM_EPI_WARPS * 2 * OUT_BYTES);
+                            BYTES = OUT + (KIND == kTcec ? 0 : NUM_EPI_WARPS * OUT_BYTES);
   static_assert(ABORT + 4 <= START && STAGES <= 32, "barriers and flags; phases are bits");
   static constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 };
@@ -93,7 +93,7 @@ struct GroupedParams {
   uint32_t rows, groups, lane_dim, col_dim, k_blocks, idesc;
   float alpha, beta;
   uint32_t out_type;
-  uint32_t tma_out; // 16-bit results that TMA can write, and beta is 0
+  uint32_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0
 };
 static_assert(sizeof(GroupedParams) <= 128, "read from the constant bank (gemm_common.cuh)");
 
@@ -263,16 +263,16 @@ __device__ __forceinline__ void st_shared_u16(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
 
-// Columns [first, cols) of one lane from tensor memory (zero: there is no sum, the product is 0) to global
+// `cols` columns of one lane from tensor memory (zero: there is no sum, the product is 0) to global
 // memory, column c at out + c * ldo.  A warp's lanes hold neighbouring elements.
 template <int KIND, class T>
 __device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out, uint64_t ldo,
-                                              uint32_t first, uint32_t cols, bool lane_ok,
-                                              const Finish &f, const float *col_scale) {
+                                              uint32_t cols, bool lane_ok, const Finish &f,
+                                              const float *col_scale) {
   constexpr uint32_t G = kEpiGroup;
   const uint32_t lane = threadIdx.x & 31u;
 #pragma unroll 1
-  for (uint32_t c = first; c < cols; c += G) {
+  for (uint32_t c = 0; c < cols; c += G) {
     float cs = 1.f;
     if constexpr (KIND == kI8) {
       if (lane < G && c + lane < cols) cs = __ldg(col_scale + c + lane);
@@ -295,61 +295,58 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out,
   }
 }
 
-// The whole groups of 16 columns of a warp, by TMA: 16-bit results to the warp's own buffers in shared
-// memory (two, in turn), 64 bytes for each column, and from there as 16 rows of 32 elements.  Stored
-// from the registers, 2 bytes a lane, a 256 x 256 tile took 7 to 11 us, of which the tensor core needs 2.4
-// with k = 2048 in 8 bits.  Returns the columns stored; the others are fewer than 16, of a group's last
-// tile, where a box of 16 rows would reach into the next group.
+// The same for 16-bit results in rows that allow 16-byte accesses: through the warp's own buffer in shared
+// memory, 32 columns at a time, 64 bytes for each column, and from there 16 bytes a lane.
 template <int KIND>
-__device__ __forceinline__ uint32_t store_by_tma(uint32_t taddr, bool zero, const CUtensorMap *map,
-                                                 uint32_t buffers, uint32_t &turn, int lane0, int row0,
-                                                 int matrix, uint32_t cols, const Finish &f,
-                                                 const float *col_scale, bool bf16) {
+__device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, uint16_t *out, uint64_t ldo,
+                                              uint32_t buf, uint32_t cols, uint32_t lanes,
+                                              const Finish &f, const float *col_scale, bool bf16) {
   const uint32_t lane = threadIdx.x & 31u;
-  const uint32_t whole = cols & ~(OUT_ROWS - 1u);
-  uint32_t v[OUT_ROWS];
+  uint32_t v[OUT_COLS];
   float cs = 0.f;
-  if (whole > 0) {
-    if (!zero) ptx::tmem_ld_32x32b_x16(taddr, v);
-    if (KIND == kI8 && !zero && lane < OUT_ROWS) cs = __ldg(col_scale + lane);
-  }
+  const uint32_t chunk = lane & 3u; // of 8 elements
+  out += 8 * chunk;
 #pragma unroll 1
-  for (uint32_t c = 0; c < whole; c += OUT_ROWS) {
-    // the buffer's store before last has read it
-    if (lane == 0) ptx::bulk_wait_read<1>();
-    __syncwarp();
-    const uint32_t buf = buffers + turn * OUT_BYTES;
-    turn ^= 1u;
-    uint32_t w[OUT_ROWS / 2];
+  for (uint32_t c = 0; c < cols; c += OUT_COLS) {
+    uint32_t w[OUT_COLS / 2];
     if (!zero) {
+      ptx::tmem_ld_32x32b_x32(taddr + c, v);
+      if (KIND == kI8 && c + lane < cols) cs = __ldg(col_scale + c + lane);
       ptx::tmem_ld_wait();
 #pragma unroll
-      for (uint32_t j = 0; j < OUT_ROWS; j += 2) {
+      for (uint32_t j = 0; j < OUT_COLS; j += 2) {
         const float s0 = KIND == kI8 ? __shfl_sync(0xffffffffu, cs, j) : 1.f,
                     s1 = KIND == kI8 ? __shfl_sync(0xffffffffu, cs, j + 1) : 1.f;
         w[j / 2] = pack_results(result<KIND>(v[j], s0, f), result<KIND>(v[j + 1], s1, f), bf16);
       }
-      if (c + OUT_ROWS < whole) { // the next columns come while these are stored
-        ptx::tmem_ld_32x32b_x16(taddr + c + OUT_ROWS, v);
-        if (KIND == kI8 && lane < OUT_ROWS) cs = __ldg(col_scale + c + OUT_ROWS + lane);
-      }
     } else {
 #pragma unroll
-      for (uint32_t j = 0; j < OUT_ROWS / 2; ++j) w[j] = 0;
+      for (uint32_t j = 0; j < OUT_COLS / 2; ++j) w[j] = 0;
     }
+    __syncwarp();
 #pragma unroll
-    for (uint32_t j = 0; j < OUT_ROWS; j += 2) {
+    for (uint32_t j = 0; j < OUT_COLS; j += 2) {
       st_shared_u16(buf + j * 64 + 2 * lane, w[j / 2]);
       st_shared_u16(buf + j * 64 + 64 + 2 * lane, w[j / 2] >> 16);
     }
-    fence_proxy_async_shared();
     __syncwarp();
-    if (lane == 0) {
-      ptx::tma_store_3d(map, buf, lane0, row0 + static_cast<int>(c), matrix);
-      ptx::bulk_commit();
+#pragma unroll
+    for (uint32_t j = 0; j < OUT_COLS; j += 8) {
+      const uint32_t col = j + (lane >> 2);
+      uint4 x;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                   : "r"(buf + col * 64 + chunk * 16));
+      uint16_t *at = out + static_cast<uint64_t>(c + col) * ldo;
+      if (c + col < cols && 8 * chunk + 8 <= lanes) *reinterpret_cast<uint4 *>(at) = x;
+      else if (c + col < cols) {
+        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (8 * chunk + i < lanes) at[i] = static_cast<uint16_t>(e[i / 2] >> (16 * (i & 1)));
+      }
     }
   }
-  return whole;
 }
 
 template <int KIND, bool A_LANES, bool WGRAD>
@@ -357,7 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                         const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ CUtensorMap map_b_few,
-                        const __grid_constant__ CUtensorMap map_out, const GroupedParams p) {
+                        const GroupedParams p) {
   using C = Cfg<KIND>;
   constexpr uint32_t PLANES = C::PLANES, STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
@@ -593,8 +590,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     const uint32_t quarter = static_cast<uint32_t>(warp & 3), second = static_cast<uint32_t>(warp - 4) >> 2;
     const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16);
     const uint32_t acc_empty = ptx::map_to_cta(sbase + C::ACC_EMPTY, 0);
-    const uint32_t buffers = sbase + C::OUT + static_cast<uint32_t>(warp - 4) * 2 * OUT_BYTES;
-    uint32_t acc = 0, f_ph = 0, d0_ph = 0, d1_ph = 0, turn = 0;
+    const uint32_t buf = sbase + C::OUT + static_cast<uint32_t>(warp - 4) * OUT_BYTES;
+    uint32_t acc = 0, f_ph = 0, d0_ph = 0, d1_ph = 0;
     bool ok = true;
     Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
     Tile x;
@@ -659,23 +656,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         f.f0 = p.alpha * __ldg(p.lane_scale);
         f.f1 = __ldg(p.lane_scale + 1);
       }
-      uint32_t stored = 0;
-      if constexpr (KIND != kTcec) {
-        if (p.tma_out != 0) {
-          const uint32_t lane0 = lane_at - static_cast<uint32_t>(lane);
-          if (lane0 < p.lane_dim)
-            stored = store_by_tma<KIND>(t_sums, zero, &map_out, buffers, turn, static_cast<int>(lane0),
-                                        static_cast<int>(x.col0 + col),
-                                        WGRAD ? static_cast<int>(x.group) : 0, cols, f, col_scale,
-                                        p.out_type == static_cast<uint32_t>(GroupedOut::bf16));
-        }
-      }
-      if (p.out_type == static_cast<uint32_t>(GroupedOut::f32))
-        store_columns<KIND>(t_sums, zero, static_cast<float *>(p.out) + at, p.ldo, stored, cols, lane_ok, f, col_scale);
+      if (KIND != kTcec && p.vector_out != 0) {
+        const uint32_t lane0 = lane_at - static_cast<uint32_t>(lane);
+        if (lane0 < p.lane_dim)
+          store_by_rows<KIND>(t_sums, zero, static_cast<uint16_t *>(p.out) + (at - lane), p.ldo, buf, cols,
+                              p.lane_dim - lane0, f, col_scale,
+                              p.out_type == static_cast<uint32_t>(GroupedOut::bf16));
+      } else if (p.out_type == static_cast<uint32_t>(GroupedOut::f32))
+        store_columns<KIND>(t_sums, zero, static_cast<float *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
       else if (KIND != kTcec && p.out_type == static_cast<uint32_t>(GroupedOut::bf16))
-        store_columns<KIND>(t_sums, zero, static_cast<__nv_bfloat16 *>(p.out) + at, p.ldo, stored, cols, lane_ok, f, col_scale);
+        store_columns<KIND>(t_sums, zero, static_cast<__nv_bfloat16 *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
       else if (KIND != kTcec)
-        store_columns<KIND>(t_sums, zero, static_cast<__half *>(p.out) + at, p.ldo, stored, cols, lane_ok, f, col_scale);
+        store_columns<KIND>(t_sums, zero, static_cast<__half *>(p.out) + at, p.ldo, cols, lane_ok, f, col_scale);
       if (!zero) {
         if constexpr (KIND == kTcec) {
           release(1);
@@ -686,8 +678,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         }
       }
     }
-    // (the buffers have been read and the results written before this CTA ends)
-    if (KIND != kTcec && lane == 0) ptx::bulk_wait<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -758,7 +748,7 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   const cudaError_t se = set_up<KIND, A_LANES, WGRAD>(&clusters);
   if (se != cudaSuccess) return se;
   constexpr int ES = KIND == kI8 ? 1 : 2;
-  CUtensorMap map_a, map_b, map_b_few, map_out = {};
+  CUtensorMap map_a, map_b, map_b_few;
   // (any address does for an operand without rows; this one is 16-byte aligned)
   const void *fallback = a.dev_status;
   if (!operand_map(&map_a, a.a, ES, fallback, Cfg<KIND>::K_ELEMS, A_LANES ? 64 : BM_CTA) ||
@@ -787,15 +777,11 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   p.alpha = a.alpha;
   p.beta = a.beta;
   p.out_type = static_cast<uint32_t>(a.out_type);
-  if (a.out_type != GroupedOut::f32 && a.beta == 0.f && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 &&
-      a.ldo % 8 == 0 && (!a.wgrad || a.groups == 1 || a.stride_o % 8 == 0)) {
-    const uint64_t out_rows = a.wgrad ? a.col_dim : a.rows, matrices = a.wgrad ? a.groups : 1;
-    p.tma_out = make_byte_map(&map_out, 2, a.out, {a.lane_dim, out_rows, matrices},
-                              {a.ldo * 2, (matrices > 1 ? a.stride_o : a.ldo) * 2}, {32, OUT_ROWS, 1},
-                              false);
-  }
+  p.vector_out = a.out_type != GroupedOut::f32 && a.beta == 0.f &&
+                 (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo % 8 == 0 &&
+                 (!a.wgrad || a.groups == 1 || a.stride_o % 8 == 0);
   return launch_chained(grouped_gemm_kernel<KIND, A_LANES, WGRAD>, static_cast<unsigned>(2 * clusters),
-                        NUM_THREADS, Cfg<KIND>::SMEM, stream, map_a, map_b, map_b_few, map_out, p);
+                        NUM_THREADS, Cfg<KIND>::SMEM, stream, map_a, map_b, map_b_few, p);
 }
 
 } // namespace
