@@ -193,7 +193,12 @@ int cuMpSGEMM_get_kernel_status(cuMpSGEMM_handle_t h) {
       cudaSuccess)
     return -2;
   if (cudaStreamSynchronize(h->cuda_stream) != cudaSuccess) return -3;
-  if (v != 0) cudaMemsetAsync(h->dev_status, 0, sizeof(int), h->cuda_stream);
+  if (v != 0) {
+    cudaMemsetAsync(h->dev_status, 0, sizeof(int), h->cuda_stream);
+    // a kernel that gave up may have left tiles uncounted
+    cudaMemsetAsync(h->dev_grouped_counters, 0, grouped_counters(h->num_sms) * sizeof(unsigned),
+                    h->cuda_stream);
+  }
   return v;
 }
 

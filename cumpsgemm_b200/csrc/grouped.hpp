@@ -42,8 +42,12 @@ struct GroupedArgs {
   const float *lane_scale; // i8: [groups][lane_dim]
   const float *col_scale;  // i8: [rows]
   const float *bias;       // i8, nullable: [groups][lane_dim]
+  float *parts; // nullable: grouped_parts_bytes() of workspace for the sums of slices
+  unsigned *counters; // grouped_counters() words, zero between calls
   int *dev_status;
 };
+// Memory with which a call may cut tiles into slices of K; 0 where it will not.
+std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms);
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream);
 
 // An operand brought into the form above: 8- or 16-bit elements copied to rows that TMA can address,

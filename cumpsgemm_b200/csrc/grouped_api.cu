@@ -70,15 +70,20 @@ cublasStatus_t stage(cuMpSGEMM_handle *h, const char *where, GroupedArgs &g, int
     bytes += round_up(o.planes * o.plane_stride * dst_elem, 1024);
     moved[s.count++] = &o;
   }
-  if (s.count == 0) return CUBLAS_STATUS_SUCCESS;
   const uint64_t records_at = bytes;
-  if (scale) bytes += (2 * kScaleRecords + 2) * sizeof(float);
-  if (bytes > workspace_limit(h) || !ensure_workspace(h, bytes)) {
+  if (scale && s.count > 0) bytes += round_up((2 * kScaleRecords + 2) * sizeof(float), 1024);
+  // the sums of slices are a matter of speed: without room for them tiles stay whole
+  const uint64_t parts_at = bytes, parts = grouped_parts_bytes(g, h->num_sms);
+  const bool with_parts = parts > 0 && bytes + parts <= workspace_limit(h) && ensure_workspace(h, bytes + parts);
+  if (!with_parts && bytes > 0 && (bytes > workspace_limit(h) || !ensure_workspace(h, bytes))) {
     log_error(std::string(where) + ": no workspace of " + std::to_string(bytes >> 20) +
               " MB for the operands");
     return CUBLAS_STATUS_ALLOC_FAILED;
   }
   char *ws = static_cast<char *>(h->workspace);
+  if (with_parts) g.parts = reinterpret_cast<float *>(ws + parts_at);
+  g.counters = h->dev_grouped_counters;
+  if (s.count == 0) return CUBLAS_STATUS_SUCCESS;
   for (int i = 0; i < s.count; ++i) {
     s.op[i].dst = ws + offset[i];
     moved[i]->ptr = ws + offset[i];

@@ -35,6 +35,9 @@
 //                 and the corrections (1)
 //   acc_empty[b]  leader's only: 16 arrivals, one from each epilogue warp of both CTAs
 //   tail[s]       own: a last block's loads
+//   next_full[i]  in both CTAs: 1 arrival, from the leader's warp that fetches the tiles, and their bytes
+//   next_empty[i] leader's only: one arrival from each role that took the tile
+//   want          leader's only: 1 arrival, from its producer towards the end of each tile
 // Every wait is bounded; no TMA multicast is used.
 #include "epilogue.cuh"
 #include "gemm_common.cuh"
@@ -45,6 +48,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <mutex>
+#include <type_traits>
 
 namespace cumpsgemm_b200 {
 namespace {
@@ -61,6 +65,13 @@ constexpr int NUM_EPI_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t DRAIN_STAGES = 2; // tcec: 128 k values per drain (tcec_gemm_pair.cu has the figures)
 constexpr uint32_t BAND = 8;         // column tiles that are walked together
+constexpr uint32_t AHEAD = 3;        // tiles that the roles may be apart
+constexpr uint32_t WANT_BLOCKS = 4;  // blocks of a tile that are left to load when the next one is fetched
+constexpr uint32_t TILE_WORDS = 12;  // of a Tile
+constexpr uint32_t MIN_SLICE = 4;    // least blocks of K in a slice
+constexpr uint32_t MAX_SLICES = 16;
+constexpr uint32_t SLICED_WAVES = 6; // fewer tiles than this many per pair: the last ones are sliced
+constexpr uint32_t PART = COLS * BM_CTA; // elements of a parked sum of one CTA
 constexpr uint32_t OUT_COLS = 32;    // columns that a warp stores at a time
 constexpr uint32_t OUT_BYTES = OUT_COLS * 32 * 2; // 32 lanes of 16-bit elements
 
@@ -74,12 +85,13 @@ template <int KIND> struct Cfg {
   static constexpr uint32_t K_ELEMS = KIND == kI8 ? 128 : 64; // of K in a stage
   static constexpr uint32_t BARS = STAGES * STAGE_BYTES;      // offsets in shared memory
   static constexpr uint32_t FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
-                            ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, TMEM_PTR = TAIL + 8 * STAGES,
-                            ABORT = TMEM_PTR + 4, START = BARS + 256,
+                            ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, NEXT_FULL = TAIL + 8 * STAGES,
+                            NEXT_EMPTY = NEXT_FULL + 8 * AHEAD, WANT = NEXT_EMPTY + 8 * AHEAD, TMEM_PTR = WANT + 8,
+                            ABORT = TMEM_PTR + 4, NEXT = BARS + 256, START = NEXT + AHEAD * TILE_WORDS * 4,
                             FIRST_TILE = START + 4 * (kMaxGroups + 2),
                             OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
                             BYTES = OUT + (KIND == kTcec ? 0 : NUM_EPI_WARPS * OUT_BYTES);
-  static_assert(ABORT + 4 <= START && STAGES <= 32, "barriers and flags; phases are bits");
+  static_assert(ABORT + 4 <= NEXT && STAGES <= 32, "barriers and flags; phases are bits");
   static constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 };
 
@@ -89,57 +101,140 @@ struct GroupedParams {
   uint64_t ldo, stride_o;
   const float *lane_scale; // i8; tcec: the two factors of `unscale`, or null
   const float *col_scale, *bias;
+  float *parts;       // nullable: sums of slices, [slot][CTA rank][COLS][BM_CTA]
+  unsigned *counters; // next tile, pairs that are through, then arrivals for each sliced tile, CTA and warp
   int *status;
-  uint32_t rows, groups, lane_dim, col_dim, k_blocks, idesc;
+  uint32_t rows, groups, lane_dim;
+  uint32_t col_dim; // wgrad; product: steps of K
+  uint32_t idesc;
   float alpha, beta;
-  uint32_t out_type;
-  uint32_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0
+  uint16_t out_type;
+  uint16_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0
 };
 static_assert(sizeof(GroupedParams) <= 128, "read from the constant bank (gemm_common.cuh)");
 
-// A tile: `cols` columns from col0 on (of the rows of x, or wgrad: of a weight dimension), 256 lanes
-// from lane0 on, `blocks` steps of K.  Without any, its product is zero.
-struct Tile {
-  uint32_t group, lane0, col0, cols, blocks;
-  uint32_t row0, rows;                                           // wgrad: the group's
+// A tile, or a slice of one: `cols` columns from col0 on (of the rows of x, or wgrad: of a weight
+// dimension), 256 lanes from lane0 on, steps [k0, k0 + blocks) of K.  Without any, its product is zero.
+struct alignas(16) Tile {
+  uint32_t group, lane0, col0, cols; // cols == 0: there are no more tiles
+  uint32_t k0, blocks;
+  uint32_t row0, rows;          // wgrad: the group's
+  uint32_t slices, slice, slot; // slot: of the slice's sum; the tile's others follow or precede it
+  uint32_t sliced;              // which of the sliced tiles
   __device__ __forceinline__ uint32_t width() const { return (cols + 31u) & ~31u; } // N of the product
-  __device__ __forceinline__ uint32_t tail_rows(uint32_t kb) const { return min(64u, rows - kb * 64u); }
+  // wgrad: rows of the group in step kb of the slice
+  __device__ __forceinline__ uint32_t rows_at(uint32_t kb) const { return min(64u, rows - (k0 + kb) * 64u); }
 };
+static_assert(sizeof(Tile) == TILE_WORDS * 4, "three times 16 bytes");
 
-// The tiles this pair takes.  Groups in turn; within one, bands of column tiles that all lane tiles
-// pass over, so that what runs at the same time shares operands in L2.
-template <int KIND, bool WGRAD> struct Walk {
-  const uint32_t *start, *first_tile; // shared memory
-  uint32_t tile, step, group, total;
-  __device__ __forceinline__ Walk(const uint8_t *smem, const GroupedParams &p, uint32_t cluster,
-                                  uint32_t clusters) {
+// The items of a launch, which are tiles or slices of tiles, by their numbers: groups in turn; within one,
+// bands of column tiles that all lane tiles pass over, so that what runs at the same time shares
+// operands in L2.  With few tiles they are cut into slices of K, whose sums are parked and added in the
+// order of the slices by the warp that comes last: all of them if they are at most half as many as
+// pairs, else the last ones, half as many as pairs, into two.
+template <int KIND, bool WGRAD> struct Items {
+  const uint32_t *start, *first_tile;
+  uint32_t group, total, whole, slices;
+  __device__ __forceinline__ Items(const uint8_t *smem, const GroupedParams &p, uint32_t clusters) {
     start = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::START);
     first_tile = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
-    tile = cluster;
-    step = clusters;
     group = 0;
-    total = first_tile[p.groups + 1];
+    const uint32_t tiles = first_tile[p.groups + 1];
+    whole = tiles;
+    slices = 1;
+    if (p.parts != nullptr && tiles > 0) {
+      if (tiles <= clusters / 2) {
+        slices = min(clusters / tiles, MAX_SLICES);
+        whole = 0;
+      } else if (tiles < SLICED_WAVES * clusters) {
+        slices = 2;
+        whole = tiles - clusters / 2;
+      }
+    }
+    total = whole + (tiles - whole) * slices;
   }
-  __device__ __forceinline__ bool next(const GroupedParams &p, Tile &x) {
-    if (tile >= total) return false;
+  // item < total, and not below that of an earlier call; false: it is none (a tile of few blocks has
+  // fewer slices than others)
+  __device__ __forceinline__ bool get(const GroupedParams &p, uint32_t item, Tile &x) {
+    x.slices = 1;
+    x.slice = x.slot = x.sliced = 0;
+    uint32_t tile = item;
+    if (item >= whole) {
+      x.slot = item - whole;
+      x.sliced = x.slot / slices;
+      tile = whole + x.sliced;
+    }
     while (tile >= first_tile[group + 1]) ++group;
-    const uint32_t local = tile - first_tile[group];
-    tile += step;
-    x.group = group;
     const uint32_t r0 = start[group], r = start[group + 1] - r0;
     const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
     const uint32_t col_dim = WGRAD ? p.col_dim : r;
     const uint32_t col_tiles = (col_dim + COLS - 1) / COLS;
+    const uint32_t local = tile - first_tile[group];
     const uint32_t band = local / (BAND * lane_tiles), in_band = local - band * BAND * lane_tiles;
     const uint32_t width = min(BAND, col_tiles - band * BAND);
     const uint32_t lt = in_band / width, ct = band * BAND + (in_band - lt * width);
+    x.group = group;
     x.lane0 = lt * LANES;
     x.cols = min(COLS, col_dim - ct * COLS);
     x.col0 = ct * COLS + (WGRAD ? 0u : r0);
-    x.blocks = WGRAD ? (r + 63u) / 64u : (group < p.groups ? p.k_blocks : 0u);
     x.row0 = r0;
     x.rows = r;
+    x.k0 = 0;
+    x.blocks = WGRAD ? (r + 63u) / 64u : (group < p.groups ? p.col_dim : 0u);
+    if (item >= whole) {
+      const uint32_t all = x.blocks;
+      x.slices = max(1u, min(slices, all / MIN_SLICE));
+      x.slice = x.slot - x.sliced * slices;
+      if (x.slice >= x.slices) return false;
+      x.k0 = all * x.slice / x.slices;
+      x.blocks = all * (x.slice + 1) / x.slices - x.k0;
+    }
     return true;
+  }
+};
+
+__device__ __forceinline__ void ld_shared_v4(uint32_t addr, uint32_t &x, uint32_t &y, uint32_t &z, uint32_t &w) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(addr));
+}
+
+// The tiles a role takes.  Their numbers come from a counter that all pairs share, as they get through:
+// tiles differ in width (product) and depth (wgrad), and dealt in turn the slowest pair of the cases
+// measured was up to a quarter behind the mean.  A warp of the leader fetches one when the producer has
+// WANT_BLOCKS blocks of the last to load (a tile that is taken earlier waits where another pair may be
+// idle), works it out, a handful of divisions, and sends it to both CTAs.
+template <int KIND, bool WARP> struct Tiles { // taken by a warp, or by one thread
+  uint32_t sbase, turn, phase;
+  __device__ __forceinline__ explicit Tiles(uint32_t sbase_) : sbase(sbase_), turn(0), phase(0) {}
+  // false at the end, or where the wait gave up
+  __device__ __forceinline__ bool next(const GroupedParams &p, volatile int *abort_flag, Tile &x) {
+    if (!look(p, abort_flag, x)) return false;
+    take(x);
+    return x.cols != 0;
+  }
+  // The same in two steps: the tile can be read again until it is taken.
+  __device__ __forceinline__ bool look(const GroupedParams &p, volatile int *abort_flag, Tile &x) {
+    bool ok = ptx::mbar_wait(sbase + Cfg<KIND>::NEXT_FULL + 8 * turn, phase, abort_flag, p.status,
+                             ptx::kErrWaitTile);
+    if (WARP) ok = ptx::warp_agrees(ok);
+    if (ok) read(x);
+    return ok;
+  }
+  __device__ __forceinline__ void read(Tile &x) const {
+    const uint32_t at = sbase + Cfg<KIND>::NEXT + turn * sizeof(Tile);
+    ld_shared_v4(at, x.group, x.lane0, x.col0, x.cols);
+    ld_shared_v4(at + 16, x.k0, x.blocks, x.row0, x.rows);
+    ld_shared_v4(at + 32, x.slices, x.slice, x.slot, x.sliced);
+  }
+  __device__ __forceinline__ void take(const Tile &x) {
+    using C = Cfg<KIND>;
+    if (WARP) __syncwarp();
+    // the tile has been read when a word of it is compared (no group is ~0)
+    if (x.group != ~0u && (!WARP || (threadIdx.x & 31) == 0))
+      ptx::mbar_arrive_cluster_relaxed(ptx::map_to_cta(sbase + C::NEXT_EMPTY + 8 * turn, 0));
+    if (++turn == AHEAD) {
+      turn = 0;
+      phase ^= 1u;
+    }
   }
 };
 
@@ -253,16 +348,65 @@ __device__ __forceinline__ float result(uint32_t sum, float col_scale, const Fin
   else return __uint_as_float(sum) * f.f0 * f.f1;
 }
 // two results to 16 bits, x in the low half
-__device__ __forceinline__ uint32_t pack_results(float x, float y, bool bf16) {
+template <class T> __device__ __forceinline__ uint32_t pack_results(float x, float y) {
   uint32_t w;
-  if (bf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
   return w;
 }
 
+// A slice of a tile: its sums are parked, and the warp that is the last of the tile's slices to park the
+// same lanes and columns adds them all, in the order of the slices, and leaves the total in tensor
+// memory in place of its own.  Returns whether it was that warp.  Nothing waits.
+template <int KIND>
+__device__ __forceinline__ bool join_slices(const GroupedParams &p, const Tile &x, uint32_t rank,
+                                            uint32_t warp, uint32_t col, uint32_t quarter,
+                                            uint32_t taddr, uint32_t cols) {
+  const uint32_t lane = threadIdx.x & 31u;
+  const uint64_t at = static_cast<uint64_t>(col) * BM_CTA + quarter * 32u + lane;
+  uint32_t *parts = reinterpret_cast<uint32_t *>(p.parts) + rank * static_cast<uint64_t>(PART) + at;
+  uint32_t *mine = parts + static_cast<uint64_t>(x.slot) * 2 * PART;
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+    ptx::tmem_ld_32x32b_x16(taddr + c, v);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) __stcg(mine + (c + j) * BM_CTA, v[j]);
+  }
+  __threadfence();
+  __syncwarp();
+  uint32_t before = 0;
+  if (lane == 0)
+    before = atomicInc(p.counters + 2 + (x.sliced * 2 + rank) * NUM_EPI_WARPS + warp, x.slices - 1);
+  if (__shfl_sync(0xffffffffu, before, 0) != x.slices - 1) return false;
+  __threadfence();
+  const uint32_t *first = parts + static_cast<uint64_t>(x.slot - x.slice) * 2 * PART;
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) v[j] = __ldcg(first + (c + j) * BM_CTA);
+    for (uint32_t s = 1; s < x.slices; ++s) {
+      const uint32_t *part = first + static_cast<uint64_t>(s) * 2 * PART;
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j) {
+        const uint32_t y = __ldcg(part + (c + j) * BM_CTA);
+        v[j] = KIND == kI8 ? v[j] + y : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(y));
+      }
+    }
+    ptx::tmem_st_32x32b_x16(taddr + c, v);
+  }
+  ptx::tmem_st_wait();
+  return true;
+}
+
 // `cols` columns of one lane from tensor memory (zero: there is no sum, the product is 0) to global
-// memory, column c at out + c * ldo.  A warp's lanes hold neighbouring elements.
-template <int KIND, class T>
+// memory, column c at out + c * ldo.  A warp's lanes hold neighbouring elements.  The loop body has no
+// branches but the one for its own group: with one for each element's bounds and beta 16 columns took
+// 1500 cycles.
+template <int KIND, class T, bool BETA>
 __device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out, uint64_t ldo,
                                               uint32_t cols, bool lane_ok, const Finish &f,
                                               const float *col_scale) {
@@ -275,21 +419,37 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out,
       if (lane < G && c + lane < cols) cs = __ldg(col_scale + c + lane);
     }
     uint32_t v[G];
+    float old[G], x[G];
+    const uint32_t here = lane_ok ? cols - c : 0u; // columns that this lane stores
+    T *at = out;
+    if constexpr (BETA) {
+#pragma unroll
+      for (uint32_t j = 0; j < G; ++j, at += ldo) old[j] = j < here ? load_as_float(at) : 0.f;
+      at = out;
+    }
     if (!zero) {
       ptx::tmem_ld_32x32b_x16(taddr + c, v);
       ptx::tmem_ld_wait();
     }
 #pragma unroll
     for (uint32_t j = 0; j < G; ++j) {
-      float x = result<KIND>(v[j], KIND == kI8 ? __shfl_sync(0xffffffffu, cs, j) : 1.f, f);
-      if (zero) x = 0.f;
-      if (lane_ok && c + j < cols) {
-        T *at = out + static_cast<uint64_t>(c + j) * ldo;
-        if (f.beta != 0.f) x = fmaf(f.beta, load_as_float(at), x);
-        store_from_float(at, x);
-      }
+      x[j] = result<KIND>(v[j], KIND == kI8 ? __shfl_sync(0xffffffffu, cs, j) : 1.f, f);
+      if (zero) x[j] = 0.f;
+      if constexpr (BETA) x[j] = fmaf(f.beta, old[j], x[j]);
     }
+#pragma unroll
+    for (uint32_t j = 0; j < G; ++j, at += ldo)
+      if (j < here) store_from_float(at, x[j]);
+    out = at;
   }
+}
+template <int KIND, class T>
+__device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out, uint64_t ldo,
+                                              uint32_t cols, bool lane_ok, const Finish &f,
+                                              const float *col_scale) {
+  if (KIND != kI8 && f.beta != 0.f)
+    store_columns<KIND, T, true>(taddr, zero, out, ldo, cols, lane_ok, f, col_scale);
+  else store_columns<KIND, T, false>(taddr, zero, out, ldo, cols, lane_ok, f, col_scale);
 }
 
 // The same for 16-bit results in rows that allow 16-byte accesses, 32 columns at a time: read as fragments,
@@ -297,21 +457,24 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, bool zero, T *out,
 // chunks of two columns side by side XORed so that neither side meets a bank twice), and from there 16 bytes
 // a lane.  Stored from the registers, 2 bytes a lane, a 256 x 256 tile took 7 to 11 us; 2 bytes a lane
 // into shared memory the gradient of 64 experts of 2000 x 1000 took 98 us, and this way 93.
-template <int KIND>
-__device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, uint16_t *out, uint64_t ldo,
+template <int KIND, class T>
+__device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, T *out, uint64_t ldo,
                                               uint32_t buf, uint32_t cols, uint32_t lanes,
-                                              const Finish (&f)[4], const float *col_scale, bool bf16) {
+                                              const Finish (&f)[4], const float *col_scale) {
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t chunk = lane & 3u; // of 8 elements
+  const uint32_t elems = lanes > 8 * chunk ? min(lanes - 8 * chunk, 8u) : 0u; // of it, that there are
   // this thread's matrix row on the way in, and its 16 bytes of every 8 columns on the way out
   const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
   const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
-  out += 8 * chunk;
+  const uint64_t step = 8 * ldo;
+  T *at = out + (lane >> 2) * ldo + 8 * chunk;
 #pragma unroll 1
   for (uint32_t c = 0; c < cols; c += OUT_COLS) {
-    uint32_t lo[16], hi[16];
-    float cs[8];
+    uint32_t w[4][4];
     if (!zero) {
+      uint32_t lo[16], hi[16];
+      float cs[8];
       ptx::tmem_ld_16x256b_x4(taddr + c, lo);
       ptx::tmem_ld_16x256b_x4(taddr + c + (16u << 16), hi);
       if constexpr (KIND == kI8) {
@@ -322,39 +485,43 @@ __device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, uint16_
         }
       }
       ptx::tmem_ld_wait();
-    }
-    __syncwarp(); // the buffer has been read
 #pragma unroll
-    for (uint32_t g = 0; g < 4; ++g) {
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (!zero) {
+      for (uint32_t g = 0; g < 4; ++g) {
         const float s0 = KIND == kI8 ? cs[2 * g] : 1.f, s1 = KIND == kI8 ? cs[2 * g + 1] : 1.f;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
           const uint32_t x = i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4],
                          y = i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3];
-          w[i] = pack_results(result<KIND>(x, s0, f[i]), result<KIND>(y, s1, f[i]), bf16);
+          w[g][i] = pack_results<T>(result<KIND>(x, s0, f[i]), result<KIND>(y, s1, f[i]));
         }
       }
-      ptx::stmatrix_x4_trans(in + g * 512u, w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g) w[g][0] = w[g][1] = w[g][2] = w[g][3] = 0;
     }
+    __syncwarp(); // the buffer has been read
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g)
+      ptx::stmatrix_x4_trans(in + g * 512u, w[g][0], w[g][1], w[g][2], w[g][3]);
     __syncwarp();
+    const uint32_t first = c + (lane >> 2);
 #pragma unroll
-    for (uint32_t g = 0; g < 4; ++g) {
-      const uint32_t col = c + 8 * g + (lane >> 2);
-      uint4 x;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                   : "r"(back + g * 512u));
-      uint16_t *at = out + static_cast<uint64_t>(col) * ldo;
-      if (col < cols && 8 * chunk + 8 <= lanes) *reinterpret_cast<uint4 *>(at) = x;
-      else if (col < cols) {
-        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+    for (uint32_t g = 0; g < 4; ++g)
+      ld_shared_v4(back + g * 512u, w[g][0], w[g][1], w[g][2], w[g][3]);
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i)
-          if (8 * chunk + i < lanes) at[i] = static_cast<uint16_t>(e[i / 2] >> (16 * (i & 1)));
-      }
+    for (uint32_t g = 0; g < 4; ++g)
+      if (first + 8 * g < cols && elems == 8)
+        *reinterpret_cast<uint4 *>(at + g * step) = make_uint4(w[g][0], w[g][1], w[g][2], w[g][3]);
+    if (elems > 0 && elems < 8) { // the last lanes of a width that is no multiple of 8
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g)
+        if (first + 8 * g < cols)
+          for (uint32_t i = 0; i < elems; ++i) {
+            const uint32_t e = i < 4 ? (i < 2 ? w[g][0] : w[g][1]) : (i < 6 ? w[g][2] : w[g][3]);
+            reinterpret_cast<uint16_t *>(at + g * step)[i] = static_cast<uint16_t>(e >> (16 * (i & 1)));
+          }
     }
+    at += 4 * step;
   }
 }
 
@@ -390,6 +557,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       ptx::mbar_init(sbase + C::ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
     }
     *abort_flag = 0;
+    for (uint32_t i = 0; i < AHEAD; ++i) {
+      ptx::mbar_init(sbase + C::NEXT_FULL + 8 * i, 1);
+      // taken by the issuer, and in both CTAs by producer, epilogue warps and (wgrad) the warp for last blocks
+      ptx::mbar_init(sbase + C::NEXT_EMPTY + 8 * i, 1 + 2 * (1 + NUM_EPI_WARPS + (WGRAD ? 1 : 0)));
+    }
+    ptx::mbar_init(sbase + C::WANT, 1);
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_a);
     ptx::prefetch_tensormap(&map_b);
@@ -416,9 +589,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     if (ptx::elect_one()) {
       uint32_t s = 0, ph = 1;
       bool ok = true;
-      Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+      Tiles<KIND, false> tiles(sbase);
       Tile x;
-      while (ok && walk.next(p, x)) {
+      while (ok && tiles.next(p, abort_flag, x)) {
         const int a_lane = static_cast<int>(x.lane0 + rank * BM_CTA);
         const uint32_t half = x.width() / 2;
         const int b_col = static_cast<int>(x.col0 + rank * half);
@@ -428,12 +601,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
                                      : (whole_box ? 1u : (half + FEW_ROWS - 1u) / FEW_ROWS);
         const uint32_t bytes =
             PLANES * (TILE_BYTES + boxes * (WGRAD ? ATOM_BYTES : whole_box ? TILE_BYTES : FEW_ROWS * ROW_BYTES));
+        const uint32_t want = x.blocks > WANT_BLOCKS ? x.blocks - WANT_BLOCKS : 0u;
+        if (leader && x.blocks == 0) ptx::mbar_arrive(sbase + C::WANT);
         for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+          if (leader && kb == want) ptx::mbar_arrive(sbase + C::WANT);
           ok = ptx::mbar_wait(sbase + C::EMPTY + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitEmpty);
           if (!ok) break;
           const uint32_t st = sbase + s * STAGE_BYTES;
           const uint32_t full = ptx::map_to_cta(sbase + C::FULL + 8 * s, 0); // the leader's barrier
-          const bool tail = WGRAD && x.tail_rows(kb) < 64u;
+          const bool tail = WGRAD && x.rows_at(kb) < 64u;
           if (tail) ptx::mbar_arrive_expect_tx(sbase + C::TAIL + 8 * s, bytes);
           else if (leader) ptx::mbar_arrive_expect_tx(sbase + C::FULL + 8 * s, 2 * bytes);
           else ptx::mbar_arrive_cluster(full);
@@ -441,7 +617,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             if (tail) ptx::tma_load_3d(dst, m, sbase + C::TAIL + 8 * s, c0, c1, c2);
             else ptx::tma_load_3d_pair(dst, m, full, c0, c1, c2);
           };
-          const int red = static_cast<int>(WGRAD ? x.row0 + kb * 64u : kb * C::K_ELEMS);
+          const int red = static_cast<int>(WGRAD ? x.row0 + (x.k0 + kb) * 64u : (x.k0 + kb) * C::K_ELEMS);
 #pragma unroll
           for (uint32_t pl = 0; pl < PLANES; ++pl) {
             const uint32_t a_dst = st + pl * TILE_BYTES, b_dst = st + (PLANES + pl) * TILE_BYTES;
@@ -476,18 +652,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     uint32_t at = 0;    // stage uses in front of this tile's
     uint32_t phases = 0; // bit s: the phase of TAIL[s]
     bool ok = true;
-    Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+    Tiles<KIND, true> tiles(sbase);
     Tile x;
-    while (ok && walk.next(p, x)) {
+    while (ok && tiles.next(p, abort_flag, x)) {
       at += x.blocks;
-      if (x.blocks == 0 || x.tail_rows(x.blocks - 1) == 64u) continue;
+      if (x.blocks == 0 || x.rows_at(x.blocks - 1) == 64u) continue;
       const uint32_t s = (at - 1) % STAGES, st = sbase + s * STAGE_BYTES;
       ok = ptx::warp_agrees(ptx::mbar_wait_backoff(sbase + C::TAIL + 8 * s, (phases >> s) & 1u, abort_flag,
                                                    p.status, ptx::kErrWaitFull, 32));
       if (!ok) break;
       phases ^= 1u << s;
       // (a row of 128 bytes is a row of 128 bytes under the swizzle too)
-      const uint32_t rows_here = x.tail_rows(x.blocks - 1), upto = (rows_here + 15u) & ~15u;
+      const uint32_t rows_here = x.rows_at(x.blocks - 1), upto = (rows_here + 15u) & ~15u;
       const uint32_t boxes = (x.width() / 2 + 63u) / 64u;
       for (uint32_t pl = 0; pl < PLANES; ++pl)
         for (uint32_t i = 0; i < 2 + boxes; ++i) {
@@ -514,9 +690,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       uint32_t acc = 0, e_ph = 1;          // accumulator in turn (f16, i8) and the phase of its barrier
       uint32_t d0_ph = 1, d1_ph = 1;       // tcec
       bool ok = true;
-      Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+      Tiles<KIND, false> tiles(sbase);
       Tile x;
-      while (ok && walk.next(p, x)) {
+      while (ok && tiles.next(p, abort_flag, x)) {
         if (x.blocks == 0) continue;
         const uint32_t idesc = p.idesc | ((x.width() >> 3) << 17);
         if constexpr (KIND != kTcec) {
@@ -531,7 +707,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           if (!ok) break;
           ptx::tc_fence_after();
           const uint64_t a = a0 + s * kStage, b = b0 + s * kStage;
-          const uint32_t steps = WGRAD ? (x.tail_rows(kb) + 15u) / 16u : 4u;
+          const uint32_t steps = WGRAD ? (x.rows_at(kb) + 15u) / 16u : 4u;
           if constexpr (KIND != kTcec) {
 #pragma unroll
             for (uint32_t ks = 0; ks < 4; ++ks)
@@ -594,6 +770,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         }
       }
     }
+  } else if (warp == 3) {
+    // ================================================================ the next tiles (leader only)
+    if (leader && ptx::elect_one()) {
+      Items<KIND, WGRAD> items(smem, p, clusters);
+      Tile x;
+      uint32_t turn = 0, ph = 1, want = 0, item = cluster_id; // the first is the pair's own
+      bool more = true;
+      while (more) {
+        while (item < items.total && !items.get(p, item, x)) item = clusters + atomicAdd(p.counters, 1u);
+        more = item < items.total;
+        if (!more) x.group = x.cols = 0;
+        if (!ptx::mbar_wait(sbase + C::NEXT_EMPTY + 8 * turn, ph, abort_flag, p.status, ptx::kErrWaitTile))
+          break;
+#pragma unroll
+        for (uint32_t r = 0; r < 2; ++r) {
+          const uint32_t to = ptx::map_to_cta(sbase + C::NEXT + turn * sizeof(Tile), r),
+                         bar = ptx::map_to_cta(sbase + C::NEXT_FULL + 8 * turn, r);
+          ptx::mbar_arrive_expect_tx_cluster(bar, sizeof(Tile));
+          ptx::send_words(to, make_uint4(x.group, x.lane0, x.col0, x.cols), bar);
+          ptx::send_words(to + 16, make_uint4(x.k0, x.blocks, x.row0, x.rows), bar);
+          ptx::send_words(to + 32, make_uint4(x.slices, x.slice, x.slot, x.sliced), bar);
+        }
+        if (++turn == AHEAD) {
+          turn = 0;
+          ph ^= 1u;
+        }
+        if (more) {
+          if (!ptx::mbar_wait(sbase + C::WANT, want, abort_flag, p.status, ptx::kErrWaitTile)) break;
+          want ^= 1u;
+          item = clusters + atomicAdd(p.counters, 1u);
+        }
+      }
+      // the last pair to get here leaves the counter as it was found; the other wraps by itself
+      if (atomicInc(p.counters + 1, clusters - 1) == clusters - 1) atomicExch(p.counters, 0u);
+    }
   } else if (warp >= 4) {
     // ================================================================ epilogue (both CTAs)
     const uint32_t quarter = static_cast<uint32_t>(warp & 3), second = static_cast<uint32_t>(warp - 4) >> 2;
@@ -602,18 +813,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     const uint32_t buf = sbase + C::OUT + static_cast<uint32_t>(warp - 4) * OUT_BYTES;
     uint32_t acc = 0, f_ph = 0, d0_ph = 0, d1_ph = 0;
     bool ok = true;
-    Walk<KIND, WGRAD> walk(smem, p, cluster_id, clusters);
+    Tiles<KIND, true> tiles(sbase);
     Tile x;
+    // The reads of tensor memory are complete (wait::ld): that is all there is to order.  (As a release
+    // it also waited for the results to be written, 1 to 2 us a tile.)
     auto release = [&](uint32_t b) {
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(acc_empty + 8 * b);
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(acc_empty + 8 * b);
     };
-    while (ok && walk.next(p, x)) {
-      const uint32_t half = x.width() / 2;
-      uint32_t t_sums = t_lanes + second * half;
-      const bool zero = x.blocks == 0;
+    auto give_back = [&]() { // the accumulator that held the sums
       if constexpr (KIND == kTcec) {
+        release(1);
+      } else {
+        release(acc);
+        acc ^= 1u;
+        if (acc == 0) f_ph ^= 1u;
+      }
+    };
+    while (true) {
+      if constexpr (KIND == kTcec) ok = tiles.look(p, abort_flag, x) && x.cols != 0;
+      else ok = tiles.next(p, abort_flag, x);
+      if (!ok) break;
+      uint32_t t_sums = t_lanes + second * (x.width() / 2);
+      if constexpr (KIND == kTcec) {
+        // (the sums take the registers that the tile was in: it is read again behind them)
+        const uint32_t half = x.width() / 2;
+        const bool zero = x.blocks == 0;
         if (!zero) {
           float sums[COLS / 2];
 #pragma unroll
@@ -635,15 +861,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           if (!ok) break;
           d1_ph ^= 1u;
           ptx::tc_fence_after();
-          t_sums += COLS;
-          add_corrections(t_sums, sums, half);
+          add_corrections(t_sums + COLS, sums, half);
         }
-      } else if (!zero) {
+        tiles.read(x);
+        tiles.take(x);
+        t_sums = t_lanes + second * (x.width() / 2) + COLS;
+      } else if (x.blocks != 0) {
         ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::ACC_FULL + 8 * acc, f_ph, abort_flag, p.status,
                                              ptx::kErrWaitD0Full));
         if (!ok) break;
         ptx::tc_fence_after();
         t_sums += acc * COLS;
+      }
+      const uint32_t half = x.width() / 2;
+      const bool zero = x.blocks == 0;
+      if (x.slices > 1 && !join_slices<KIND>(p, x, rank, static_cast<uint32_t>(warp - 4), second * half,
+                                             quarter, t_sums, min(half, x.width() - second * half))) {
+        give_back();
+        continue;
       }
       const uint32_t lane0 = x.lane0 + rank * BM_CTA + quarter * 32u; // the warp's first
       const uint32_t col = second * half;
@@ -666,32 +901,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         }
         return f;
       };
-      const bool bf16 = p.out_type == static_cast<uint32_t>(GroupedOut::bf16);
+      const auto type = static_cast<GroupedOut>(p.out_type);
       if (KIND != kTcec && p.vector_out != 0) {
         const uint32_t l = static_cast<uint32_t>(lane) >> 2;
         const Finish f[4] = {finish_of(l), finish_of(l + 8), finish_of(l + 16), finish_of(l + 24)};
-        store_by_rows<KIND>(t_sums, zero, static_cast<uint16_t *>(p.out) + at, p.ldo, buf, cols,
-                            p.lane_dim - lane0, f, col_scale, bf16);
+        const uint32_t lanes = p.lane_dim > lane0 ? p.lane_dim - lane0 : 0u;
+        if (type == GroupedOut::bf16)
+          store_by_rows<KIND>(t_sums, zero, static_cast<__nv_bfloat16 *>(p.out) + at, p.ldo, buf, cols, lanes, f, col_scale);
+        else
+          store_by_rows<KIND>(t_sums, zero, static_cast<__half *>(p.out) + at, p.ldo, buf, cols, lanes, f, col_scale);
       } else {
         const Finish f = finish_of(static_cast<uint32_t>(lane));
         const bool lane_ok = lane0 + static_cast<uint32_t>(lane) < p.lane_dim;
         const uint64_t mine = at + static_cast<uint32_t>(lane);
-        if (p.out_type == static_cast<uint32_t>(GroupedOut::f32))
+        if (KIND != kF16 && type == GroupedOut::f32)
           store_columns<KIND>(t_sums, zero, static_cast<float *>(p.out) + mine, p.ldo, cols, lane_ok, f, col_scale);
-        else if (KIND != kTcec && bf16)
+        else if (KIND != kTcec && type == GroupedOut::bf16)
           store_columns<KIND>(t_sums, zero, static_cast<__nv_bfloat16 *>(p.out) + mine, p.ldo, cols, lane_ok, f, col_scale);
         else if (KIND != kTcec)
           store_columns<KIND>(t_sums, zero, static_cast<__half *>(p.out) + mine, p.ldo, cols, lane_ok, f, col_scale);
       }
-      if (!zero) {
-        if constexpr (KIND == kTcec) {
-          release(1);
-        } else {
-          release(acc);
-          acc ^= 1u;
-          if (acc == 0) f_ph ^= 1u;
-        }
-      }
+      if (!zero) give_back();
     }
   }
 
@@ -778,12 +1008,13 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   p.lane_scale = KIND == kTcec ? a.unscale : a.lane_scale;
   p.col_scale = a.col_scale;
   p.bias = a.bias;
+  p.parts = a.parts;
+  p.counters = a.counters;
   p.status = a.dev_status;
   p.rows = a.rows;
   p.groups = a.groups;
   p.lane_dim = a.lane_dim;
-  p.col_dim = a.col_dim;
-  p.k_blocks = (a.k + Cfg<KIND>::K_ELEMS - 1) / Cfg<KIND>::K_ELEMS;
+  p.col_dim = WGRAD ? a.col_dim : (a.k + Cfg<KIND>::K_ELEMS - 1) / Cfg<KIND>::K_ELEMS;
   // formats: F32 sums of F16 (0) or BF16 (1), or S32 sums of S8 (1); bits 15 and 16: A, B with their
   // lanes, columns contiguous
   const uint32_t sum_format = KIND == kI8 ? 2u : 1u, format = KIND == kI8 ? 1u : (a.bf16 ? 1u : 0u);
@@ -791,7 +1022,7 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
             (WGRAD ? 1u << 16 : 0u) | ((LANES >> 4) << 24);
   p.alpha = a.alpha;
   p.beta = a.beta;
-  p.out_type = static_cast<uint32_t>(a.out_type);
+  p.out_type = static_cast<uint16_t>(a.out_type);
   p.vector_out = a.out_type != GroupedOut::f32 && a.beta == 0.f &&
                  (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo % 8 == 0 &&
                  (!a.wgrad || a.groups == 1 || a.stride_o % 8 == 0);
@@ -800,6 +1031,14 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
 }
 
 } // namespace
+
+std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
+  const uint64_t pairs = num_sms / 2, lane_tiles = (a.lane_dim + LANES - 1) / LANES;
+  // tiles there are at least: the groups of a product may leave some unfilled
+  const uint64_t least = lane_tiles * (a.wgrad ? a.groups * static_cast<uint64_t>((a.col_dim + COLS - 1) / COLS)
+                                               : (a.rows + COLS - 1) / COLS);
+  return least < SLICED_WAVES * pairs ? pairs * 2 * PART * sizeof(float) : 0;
+}
 
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream) {
   if (a.kind == GroupedKind::i8) {

@@ -93,6 +93,8 @@ extern "C" cublasStatus_t cuMpSGEMM_create(cuMpSGEMM_handle_t *const handle) {
         cudaSuccess;
   ok &= cudaMalloc(&h->dev_dyn_params, sizeof(DynParams) * h->dyn_params_length) == cudaSuccess;
   ok &= cudaMalloc(&h->dev_status, 2 * sizeof(int)) == cudaSuccess;
+  const size_t counters_bytes = grouped_counters(h->num_sms) * sizeof(unsigned);
+  ok &= cudaMalloc(&h->dev_grouped_counters, counters_bytes) == cudaSuccess;
   ok &= cudaEventCreateWithFlags(&h->order_event, cudaEventDisableTiming) == cudaSuccess;
   const size_t scan_scratch_bytes = static_cast<size_t>(h->num_sms) * 8 * 24 * 2 + 16;
   ok &= cudaMalloc(&es.dev_scan_scratch, scan_scratch_bytes) == cudaSuccess;
@@ -108,6 +110,7 @@ extern "C" cublasStatus_t cuMpSGEMM_create(cuMpSGEMM_handle_t *const handle) {
   cudaMemsetAsync(h->dyn_launch.flag_buffer, 0, sizeof(int) * h->dyn_launch.flag_buffer_length,
                   h->cuda_stream);
   cudaMemsetAsync(h->dev_status, 0, 2 * sizeof(int), h->cuda_stream);
+  cudaMemsetAsync(h->dev_grouped_counters, 0, counters_bytes, h->cuda_stream);
   cudaMemsetAsync(es.dev_scan_scratch, 0, scan_scratch_bytes, h->cuda_stream);
   configure_mode_buffer(h);
   init_flag_buffer(h);
@@ -134,6 +137,7 @@ extern "C" cublasStatus_t cuMpSGEMM_destroy(cuMpSGEMM_handle_t handle) {
   cudaFree(handle->dyn_launch.flag_buffer);
   cudaFree(handle->dev_dyn_params);
   cudaFree(handle->dev_status);
+  cudaFree(handle->dev_grouped_counters);
   cudaFree(handle->workspace);
   for (void *w : handle->graph_workspaces) cudaFree(w);
   if (handle->order_event != nullptr) cudaEventDestroy(handle->order_event);

@@ -163,6 +163,10 @@ struct cuMpSGEMM_handle {
   // Device status word the GEMM kernel writes when a bounded wait gives up.
   int *dev_status = nullptr; // [0] kernel status word, [1] wave counter of the pair kernel
 
+  // Words the kernel of grouped products counts tiles and slices with (grouped_gemm.cu); zero between
+  // calls, and set to zero again when the status word is found raised.
+  unsigned *dev_grouped_counters = nullptr;
+
   // Optional per-launch timing: events recorded on the launching stream before the split
   // pass, between split pass and GEMM kernel, and after the GEMM kernel.
   struct TimingTriple {
@@ -207,6 +211,9 @@ inline void mark_stream_work(cuMpSGEMM_handle *h) {
   else
     cudaGetLastError();
 }
+
+// Words of dev_grouped_counters: two, and for each pair of CTAs one for each of their 16 epilogue warps.
+inline std::size_t grouped_counters(unsigned num_sms) { return 2 + num_sms / 2 * 16; }
 
 // Makes the handle's workspace hold `bytes`.  Returns false, with the old workspace untouched, while the
 // stream is being captured, and false without a workspace if there is no memory.

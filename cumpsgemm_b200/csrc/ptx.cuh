@@ -103,7 +103,8 @@ enum : int {
   kErrWaitD0Full = 4,  // epilogue waited for a chunk's main accumulator
   kErrWaitD1Full = 5,  // epilogue waited for the correction accumulator
   kErrBadLaunch = 6,
-  kErrWaitD1Empty = 7  // MMA issuer waited for the epilogue to give the correction accumulator back
+  kErrWaitD1Empty = 7, // MMA issuer waited for the epilogue to give the correction accumulator back
+  kErrWaitTile = 8     // a role waited for the number of its next tile, or for it to be taken
 };
 
 constexpr uint64_t kWaitLimitNs = 1000ull * 1000ull * 1000ull; // 1 s
@@ -420,6 +421,25 @@ __device__ __forceinline__ void cluster_wait() {
 // arrive on an mbarrier that may live in the other CTA of the cluster
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+// The same where nothing but tensor memory or a word already read is handed over.  The plain form is a release,
+// which waits until the thread's stores to global memory are visible.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+// Sixteen bytes for a CTA of the cluster (addresses: shared::cluster): stored asynchronously to its shared
+// memory and counted on a barrier there that expects them.  Who waits for that barrier in the ordinary
+// way, at CTA scope, sees them.
+__device__ __forceinline__ void send_words(uint32_t addr, uint4 v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.u32 [%0], {%1, %2, %3, %4}, [%5];"
+               :
+               : "r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr), "r"(bytes)
                : "memory");
 }
 // TMA load into this CTA's shared memory whose completion bytes are counted on an mbarrier

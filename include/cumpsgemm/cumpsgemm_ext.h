@@ -125,7 +125,7 @@ cublasStatus_t cuMpSGEMM_sgemm_module(
  * code in a device word.  This call synchronises the handle's stream, returns the word and
  * clears it.  0 = no error; 1 = a producer / converter waited for a free stage, 2 = the MMA
  * issuer for operands, 3 / 7 = the MMA issuer for the drain of an accumulator, 4 / 5 = the
- * epilogue for an accumulator, 6 = bad launch. */
+ * epilogue for an accumulator, 6 = bad launch, 8 = a role of the grouped products for its next tile. */
 int cuMpSGEMM_get_kernel_status(cuMpSGEMM_handle_t handle);
 /* Which kernels the handle's last GEMM call launched, and in *cut_along_k (nullable) whether any of
  * its tiles was cut along K; host state only, nothing is synchronised.  CUMPSGEMM_ROUTE_NONE: no call
