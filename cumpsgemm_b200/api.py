@@ -97,8 +97,15 @@ def _is_complex(x: DevPtr, hint: Optional[bool]) -> bool:
 _ComplexScalar = C.c_float * 2
 
 
+_ONE, _ZERO = C.byref(C.c_float(1.0)), C.byref(C.c_float(0.0))
+
+
 def _scalar(value, is_complex: bool):
     """alpha / beta as a pointer argument (the argument keeps its storage alive)."""
+    if not is_complex and value == 1.0:  # the usual ones are there already
+        return _ONE
+    if not is_complex and value == 0.0:
+        return _ZERO
     if is_complex:
         z = complex(value)
         return C.byref(_ComplexScalar(z.real, z.imag))

@@ -32,59 +32,68 @@ def _data_type(dtype) -> int:
         raise ValueError(f"expected float16, bfloat16 or float32, got {dtype}") from None
 
 
+# A call with few rows takes as long as its checks: they ask a tensor for each thing once.
 def _rows_of(t, what: str, cols: Optional[int] = None):
     """(rows, columns, leading dimension) of a matrix whose rows are contiguous."""
-    if t.dim() != 2:
-        raise ValueError(f"{what} must have two dimensions, got {tuple(t.shape)}")
-    rows, n = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{what} must have two dimensions, got {tuple(shape)}")
+    rows, n = shape
+    ld, step = t.stride()
     if cols is not None and n != cols:
         raise ValueError(f"{what} has {n} columns where {cols} are needed")
-    if n > 1 and t.stride(1) != 1:
+    if step != 1 and n > 1:
         raise ValueError(f"the rows of {what} must be contiguous")
-    if rows > 1 and t.stride(0) < n:
+    if rows <= 1:
+        return rows, n, n
+    if ld < n:
         raise ValueError(f"the rows of {what} overlap")
-    return rows, n, t.stride(0) if rows > 1 else n
+    return rows, n, ld
 
 
 def _matrices_of(t, what: str):
     """(matrices, rows, columns, leading dimension, stride) of a stack of such matrices."""
-    if t.dim() != 3:
-        raise ValueError(f"{what} must have three dimensions, got {tuple(t.shape)}")
-    e, rows, n = t.shape
-    if n > 1 and t.stride(2) != 1:
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what} must have three dimensions, got {tuple(shape)}")
+    e, rows, n = shape
+    stride, ld, step = t.stride()
+    if step != 1 and n > 1:
         raise ValueError(f"the rows of {what} must be contiguous")
-    ld = t.stride(1) if rows > 1 else n
-    if ld < n or (e > 1 and t.stride(0) < (rows - 1) * ld + n):
+    if rows <= 1:
+        ld = n
+    if e <= 1:
+        stride = rows * ld
+    if ld < n or stride < (rows - 1) * ld + n:
         raise ValueError(f"the matrices of {what} overlap")
-    return e, rows, n, ld, t.stride(0) if e > 1 else rows * ld
+    return e, rows, n, ld, stride
 
 
-def _check(tensors, group_ends, groups: int) -> None:
-    device = tensors[0].device
-    for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("operands must live in device memory")
-        if t.device != device:
+def _check(device: int, others, group_ends, groups: int) -> None:
+    if device < 0:
+        raise ValueError("operands must live in device memory")
+    for t in others:
+        if t.get_device() != device:
             raise ValueError("operands are on different devices")
     if group_ends is None:
         if groups != 1:
             raise ValueError("group_ends is needed for more than one expert")
         return
-    if group_ends.dtype != torch.int32 or group_ends.dim() != 1 or not group_ends.is_contiguous():
+    if group_ends.dtype is not torch.int32 or group_ends.dim() != 1 or not group_ends.is_contiguous():
         raise ValueError("group_ends must be a contiguous int32 vector")
-    if group_ends.device != device:
+    if group_ends.get_device() != device:
         raise ValueError("group_ends is on another device")
-    if group_ends.numel() != groups:
-        raise ValueError(f"{group_ends.numel()} group_ends for {groups} experts")
+    if len(group_ends) != groups:
+        raise ValueError(f"{len(group_ends)} group_ends for {groups} experts")
 
 
-def _output(out, beta, shape, dtype, device):
+def _output(out, beta, shape, dtype, like):
     if out is None:
         if beta != 0.0:
             raise ValueError("beta needs an out to read")
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out must be {dtype} of shape {tuple(shape)} on {device}")
+        return like.new_empty(shape, dtype=dtype)
+    if tuple(out.shape) != shape or out.dtype is not dtype or out.get_device() != like.get_device():
+        raise ValueError(f"out must be {dtype} of shape {shape} on {like.device}")
     return out
 
 
@@ -100,14 +109,17 @@ def grouped_matmul(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
     groups, w_rows, w_cols, ldw, stridew = _matrices_of(w, "w")
     k, n = (w_cols, w_rows) if transpose_w else (w_rows, w_cols)
     rows, _, ldx = _rows_of(x, "x", k)
-    _check((x, w), group_ends, groups)
-    if x.dtype != w.dtype:
-        raise ValueError(f"x is {x.dtype}, w is {w.dtype}")
-    out = _output(out, beta, (rows, n), x.dtype, x.device)
-    _, _, ldy = _rows_of(out, "out")
+    _check(x.get_device(), (w,), group_ends, groups)
+    dtype = x.dtype
+    if dtype is not w.dtype:
+        raise ValueError(f"x is {dtype}, w is {w.dtype}")
+    data_type = _data_type(dtype)
+    ldy = n
+    if out is not None:
+        _, _, ldy = _rows_of(out, "out")
+    out = _output(out, beta, (rows, n), dtype, x)
     handle.grouped_gemm(api.CUBLAS_OP_T if transpose_w else api.CUBLAS_OP_N, rows, n, k, groups,
-                        group_ends, alpha, x, ldx, w, ldw, stridew, beta, out, ldy,
-                        _data_type(x.dtype), mode)
+                        group_ends, alpha, x, ldx, w, ldw, stridew, beta, out, ldy, data_type, mode)
     return out
 
 
@@ -120,16 +132,20 @@ def grouped_matmul_wgrad(handle: api.Handle, x, dy, group_ends=None, transpose_w
     dy_rows, n, lddy = _rows_of(dy, "dy")
     if dy_rows != rows:
         raise ValueError(f"x has {rows} rows, dy {dy_rows}")
-    groups = 1 if group_ends is None else group_ends.numel()
-    _check((x, dy), group_ends, groups)
-    if x.dtype != dy.dtype:
-        raise ValueError(f"x is {x.dtype}, dy is {dy.dtype}")
+    groups = 1 if group_ends is None else len(group_ends)
+    _check(x.get_device(), (dy,), group_ends, groups)
+    dtype = x.dtype
+    if dtype is not dy.dtype:
+        raise ValueError(f"x is {dtype}, dy is {dy.dtype}")
+    data_type = _data_type(dtype)
     shape = (groups, n, k) if transpose_w else (groups, k, n)
-    out = _output(out, beta, shape, x.dtype, x.device)
-    _, _, _, lddw, stridedw = _matrices_of(out, "out")
+    lddw, stridedw = shape[2], n * k
+    if out is not None:
+        _, _, _, lddw, stridedw = _matrices_of(out, "out")
+    out = _output(out, beta, shape, dtype, x)
     handle.grouped_gemm_wgrad(api.CUBLAS_OP_T if transpose_w else api.CUBLAS_OP_N, rows, n, k, groups,
                               group_ends, alpha, x, ldx, dy, lddy, beta, out, lddw, stridedw,
-                              _data_type(x.dtype), mode)
+                              data_type, mode)
     return out
 
 
@@ -140,19 +156,21 @@ def quantize_rows(handle: api.Handle, x, row_index=None) -> Tuple[torch.Tensor, 
     q's rows start at multiples of 16 bytes, so that ``i8_matmul`` reads them in place; a weight of
     (experts, n, k) is quantised as (experts * n, k) rows."""
     src_rows, k, ldx = _rows_of(x, "x")
-    if not x.is_cuda:
+    device = x.get_device()
+    if device < 0:
         raise ValueError("operands must live in device memory")
+    data_type = _data_type(x.dtype)
     rows = src_rows
     if row_index is not None:
-        if row_index.dtype != torch.int32 or row_index.dim() != 1 or not row_index.is_contiguous():
+        if row_index.dtype is not torch.int32 or row_index.dim() != 1 or not row_index.is_contiguous():
             raise ValueError("row_index must be a contiguous int32 vector")
-        if row_index.device != x.device:
+        if row_index.get_device() != device:
             raise ValueError("row_index is on another device")
-        rows = row_index.numel()
+        rows = len(row_index)
     ldq = (k + 15) // 16 * 16
-    q = torch.empty((rows, ldq), dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    handle.quantize_rows_i8(rows, k, x, ldx, _data_type(x.dtype), row_index, src_rows, q, ldq, scale)
+    q = x.new_empty((rows, ldq), dtype=torch.int8)
+    scale = x.new_empty(rows, dtype=torch.float32)
+    handle.quantize_rows_i8(rows, k, x, ldx, data_type, row_index, src_rows, q, ldq, scale)
     return (q if ldq == k else q[:, :k]), scale
 
 
@@ -166,17 +184,22 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
         wq = wq.unsqueeze(0)
     groups, n, k, ldw, stridew = _matrices_of(wq, "wq")
     rows, _, ldx = _rows_of(xq, "xq", k)
-    _check((xq, x_scale, wq, w_scale) + (() if bias is None else (bias,)), group_ends, groups)
-    if xq.dtype != torch.int8 or wq.dtype != torch.int8:
+    _check(xq.get_device(), (x_scale, wq, w_scale) if bias is None else (x_scale, wq, w_scale, bias),
+           group_ends, groups)
+    if xq.dtype is not torch.int8 or wq.dtype is not torch.int8:
         raise ValueError(f"xq is {xq.dtype}, wq is {wq.dtype}: both must be int8")
     for t, what, count in ((x_scale, "x_scale", rows), (w_scale, "w_scale", groups * n),
                            (bias, "bias", groups * n)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous()):
             raise ValueError(f"{what} must be {count} contiguous float32 values")
-    out = _output(out, 0.0, (rows, n), out_dtype if out is None else out.dtype, xq.device)
-    _, _, ldy = _rows_of(out, "out")
+    ldy = n
+    if out is not None:
+        out_dtype = out.dtype
+        _, _, ldy = _rows_of(out, "out")
+    data_type = _data_type(out_dtype)
+    out = _output(out, 0.0, (rows, n), out_dtype, xq)
     handle.i8_grouped_gemm(rows, n, k, groups, group_ends, xq, ldx, x_scale, wq, ldw, stridew, w_scale,
-                           bias, out, ldy, _data_type(out.dtype))
+                           bias, out, ldy, data_type)
     return out
 
 
