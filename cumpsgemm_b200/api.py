@@ -66,6 +66,8 @@ DevPtr = Union[int, "torch.Tensor"]  # noqa: F821
 
 
 def _ptr(x: DevPtr) -> int:
+    if type(x) is int:
+        return x
     try:  # a CUDA tensor, the usual case: three operands per call come through here
         if x.is_cuda:
             return x.data_ptr()

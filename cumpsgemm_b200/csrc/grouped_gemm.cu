@@ -68,9 +68,10 @@ constexpr uint32_t BAND = 8;         // column tiles that are walked together
 constexpr uint32_t AHEAD = 3;        // tiles that the roles may be apart
 constexpr uint32_t WANT_BLOCKS = 4;  // blocks of a tile that are left to load when the next one is fetched
 constexpr uint32_t TILE_WORDS = 12;  // of a Tile
-constexpr uint32_t MIN_SLICE = 4;    // least blocks of K in a slice
+constexpr uint32_t MIN_SLICED = 32;  // least blocks of K in a tile that is sliced, and in a slice of it
+constexpr uint32_t MIN_SLICE = 8;
 constexpr uint32_t MAX_SLICES = 16;
-constexpr uint32_t SLICED_WAVES = 6; // fewer tiles than this many per pair: the last ones are sliced
+constexpr uint32_t JOIN_AHEAD = 4;   // slices whose sums are fetched together
 constexpr uint32_t PART = COLS * BM_CTA; // elements of a parked sum of one CTA
 constexpr uint32_t OUT_COLS = 32;    // columns that a warp stores at a time
 constexpr uint32_t OUT_BYTES = OUT_COLS * 32 * 2; // 32 lanes of 16-bit elements
@@ -120,7 +121,7 @@ struct alignas(16) Tile {
   uint32_t k0, blocks;
   uint32_t row0, rows;          // wgrad: the group's
   uint32_t slices, slice, slot; // slot: of the slice's sum; the tile's others follow or precede it
-  uint32_t sliced;              // which of the sliced tiles
+  uint32_t sliced;              // the tile's number
   __device__ __forceinline__ uint32_t width() const { return (cols + 31u) & ~31u; } // N of the product
   // wgrad: rows of the group in step kb of the slice
   __device__ __forceinline__ uint32_t rows_at(uint32_t kb) const { return min(64u, rows - (k0 + kb) * 64u); }
@@ -129,41 +130,31 @@ static_assert(sizeof(Tile) == TILE_WORDS * 4, "three times 16 bytes");
 
 // The items of a launch, which are tiles or slices of tiles, by their numbers: groups in turn; within one,
 // bands of column tiles that all lane tiles pass over, so that what runs at the same time shares
-// operands in L2.  With few tiles they are cut into slices of K, whose sums are parked and added in the
-// order of the slices by the warp that comes last: all of them if they are at most half as many as
-// pairs, else the last ones, half as many as pairs, into two.
+// operands in L2.
+// Tiles that are at most half as many as pairs are cut into slices of K, whose sums are parked and added in
+// the order of the slices by the warp that comes last.  A block of K takes 0.3 us (256 columns), and a
+// slice adds 1.6 us for the SM that fetches its sums, so the sum of both is least with the square root
+// of 50 * blocks / columns slices, and below 32 blocks with one (256 rows of 4096, one expert of 1024: 25 us
+// whole, 21 so; 54 with 16 slices).  Slicing the last tiles of longer launches was no gain.
 template <int KIND, bool WGRAD> struct Items {
   const uint32_t *start, *first_tile;
-  uint32_t group, total, whole, slices;
+  uint32_t group, total, slices; // slices: item numbers of a tile
   __device__ __forceinline__ Items(const uint8_t *smem, const GroupedParams &p, uint32_t clusters) {
     start = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::START);
     first_tile = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
     group = 0;
     const uint32_t tiles = first_tile[p.groups + 1];
-    whole = tiles;
-    slices = 1;
-    if (p.parts != nullptr && tiles > 0) {
-      if (tiles <= clusters / 2) {
-        slices = min(clusters / tiles, MAX_SLICES);
-        whole = 0;
-      } else if (tiles < SLICED_WAVES * clusters) {
-        slices = 2;
-        whole = tiles - clusters / 2;
-      }
-    }
-    total = whole + (tiles - whole) * slices;
+    slices = p.parts != nullptr && tiles > 0 && tiles <= clusters / 2 ? min(clusters / tiles, MAX_SLICES) : 1u;
+    total = tiles * slices;
   }
   // item < total, and not below that of an earlier call; false: it is none (a tile of few blocks has
   // fewer slices than others)
   __device__ __forceinline__ bool get(const GroupedParams &p, uint32_t item, Tile &x) {
+    const uint32_t tile = slices > 1 ? item / slices : item;
     x.slices = 1;
-    x.slice = x.slot = x.sliced = 0;
-    uint32_t tile = item;
-    if (item >= whole) {
-      x.slot = item - whole;
-      x.sliced = x.slot / slices;
-      tile = whole + x.sliced;
-    }
+    x.slice = 0;
+    x.slot = item;
+    x.sliced = tile;
     while (tile >= first_tile[group + 1]) ++group;
     const uint32_t r0 = start[group], r = start[group + 1] - r0;
     const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
@@ -181,10 +172,11 @@ template <int KIND, bool WGRAD> struct Items {
     x.rows = r;
     x.k0 = 0;
     x.blocks = WGRAD ? (r + 63u) / 64u : (group < p.groups ? p.col_dim : 0u);
-    if (item >= whole) {
+    if (slices > 1) {
       const uint32_t all = x.blocks;
-      x.slices = max(1u, min(slices, all / MIN_SLICE));
-      x.slice = x.slot - x.sliced * slices;
+      if (all >= MIN_SLICED)
+        x.slices = max(1u, min(min(slices, all / MIN_SLICE), static_cast<uint32_t>(sqrtf(50.f * all / x.cols))));
+      x.slice = item - tile * slices;
       if (x.slice >= x.slices) return false;
       x.k0 = all * x.slice / x.slices;
       x.blocks = all * (x.slice + 1) / x.slices - x.k0;
@@ -387,14 +379,22 @@ __device__ __forceinline__ bool join_slices(const GroupedParams &p, const Tile &
   for (uint32_t c = 0; c < cols; c += 16) {
     uint32_t v[16];
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) v[j] = __ldcg(first + (c + j) * BM_CTA);
-    for (uint32_t s = 1; s < x.slices; ++s) {
-      const uint32_t *part = first + static_cast<uint64_t>(s) * 2 * PART;
+    for (uint32_t j = 0; j < 16; ++j) v[j] = 0;
+    // several slices' values are on their way at once: one slice after the other took 2.8 us each for
+    // 256 columns
+#pragma unroll 1
+    for (uint32_t s = 0; s < x.slices; s += JOIN_AHEAD) {
+      uint32_t y[JOIN_AHEAD][16];
 #pragma unroll
-      for (uint32_t j = 0; j < 16; ++j) {
-        const uint32_t y = __ldcg(part + (c + j) * BM_CTA);
-        v[j] = KIND == kI8 ? v[j] + y : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(y));
-      }
+      for (uint32_t i = 0; i < JOIN_AHEAD; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j)
+          y[i][j] = s + i < x.slices ? __ldcg(first + static_cast<uint64_t>(s + i) * 2 * PART + (c + j) * BM_CTA) : 0u;
+#pragma unroll
+      for (uint32_t i = 0; i < JOIN_AHEAD; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j)
+          v[j] = KIND == kI8 ? v[j] + y[i][j] : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(y[i][j]));
     }
     ptx::tmem_st_32x32b_x16(taddr + c, v);
   }
@@ -1038,7 +1038,7 @@ std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
   // tiles there are at least: the groups of a product may leave some unfilled
   const uint64_t least = lane_tiles * (a.wgrad ? a.groups * static_cast<uint64_t>((a.col_dim + COLS - 1) / COLS)
                                                : (a.rows + COLS - 1) / COLS);
-  return least < SLICED_WAVES * pairs ? pairs * 2 * PART * sizeof(float) : 0;
+  return least <= pairs / 2 ? pairs * 2 * PART * sizeof(float) : 0;
 }
 
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream) {

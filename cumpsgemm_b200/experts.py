@@ -83,8 +83,8 @@ def _check(device: int, others, group_ends, groups: int) -> None:
         raise ValueError("group_ends must be a contiguous int32 vector")
     if group_ends.get_device() != device:
         raise ValueError("group_ends is on another device")
-    if len(group_ends) != groups:
-        raise ValueError(f"{len(group_ends)} group_ends for {groups} experts")
+    if group_ends.shape[0] != groups:
+        raise ValueError(f"{group_ends.shape[0]} group_ends for {groups} experts")
 
 
 def _output(out, beta, shape, dtype, like):
@@ -119,7 +119,8 @@ def grouped_matmul(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
         _, _, ldy = _rows_of(out, "out")
     out = _output(out, beta, (rows, n), dtype, x)
     handle.grouped_gemm(api.CUBLAS_OP_T if transpose_w else api.CUBLAS_OP_N, rows, n, k, groups,
-                        group_ends, alpha, x, ldx, w, ldw, stridew, beta, out, ldy, data_type, mode)
+                        None if group_ends is None else group_ends.data_ptr(), alpha, x.data_ptr(), ldx,
+                        w.data_ptr(), ldw, stridew, beta, out.data_ptr(), ldy, data_type, mode)
     return out
 
 
@@ -132,7 +133,7 @@ def grouped_matmul_wgrad(handle: api.Handle, x, dy, group_ends=None, transpose_w
     dy_rows, n, lddy = _rows_of(dy, "dy")
     if dy_rows != rows:
         raise ValueError(f"x has {rows} rows, dy {dy_rows}")
-    groups = 1 if group_ends is None else len(group_ends)
+    groups = 1 if group_ends is None else group_ends.numel()
     _check(x.get_device(), (dy,), group_ends, groups)
     dtype = x.dtype
     if dtype is not dy.dtype:
@@ -144,8 +145,9 @@ def grouped_matmul_wgrad(handle: api.Handle, x, dy, group_ends=None, transpose_w
         _, _, _, lddw, stridedw = _matrices_of(out, "out")
     out = _output(out, beta, shape, dtype, x)
     handle.grouped_gemm_wgrad(api.CUBLAS_OP_T if transpose_w else api.CUBLAS_OP_N, rows, n, k, groups,
-                              group_ends, alpha, x, ldx, dy, lddy, beta, out, lddw, stridedw,
-                              data_type, mode)
+                              None if group_ends is None else group_ends.data_ptr(), alpha, x.data_ptr(),
+                              ldx, dy.data_ptr(), lddy, beta, out.data_ptr(), lddw, stridedw, data_type,
+                              mode)
     return out
 
 
@@ -166,11 +168,13 @@ def quantize_rows(handle: api.Handle, x, row_index=None) -> Tuple[torch.Tensor, 
             raise ValueError("row_index must be a contiguous int32 vector")
         if row_index.get_device() != device:
             raise ValueError("row_index is on another device")
-        rows = len(row_index)
+        rows = row_index.shape[0]
     ldq = (k + 15) // 16 * 16
     q = x.new_empty((rows, ldq), dtype=torch.int8)
     scale = x.new_empty(rows, dtype=torch.float32)
-    handle.quantize_rows_i8(rows, k, x, ldx, data_type, row_index, src_rows, q, ldq, scale)
+    handle.quantize_rows_i8(rows, k, x.data_ptr(), ldx, data_type,
+                            None if row_index is None else row_index.data_ptr(), src_rows, q.data_ptr(),
+                            ldq, scale.data_ptr())
     return (q if ldq == k else q[:, :k]), scale
 
 
@@ -198,8 +202,10 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
         _, _, ldy = _rows_of(out, "out")
     data_type = _data_type(out_dtype)
     out = _output(out, 0.0, (rows, n), out_dtype, xq)
-    handle.i8_grouped_gemm(rows, n, k, groups, group_ends, xq, ldx, x_scale, wq, ldw, stridew, w_scale,
-                           bias, out, ldy, data_type)
+    handle.i8_grouped_gemm(rows, n, k, groups, None if group_ends is None else group_ends.data_ptr(),
+                           xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, stridew,
+                           w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                           ldy, data_type)
     return out
 
 

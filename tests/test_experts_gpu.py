@@ -497,3 +497,43 @@ def test_refusals(handle):
     handle.set_workspace_limit(0)
     # and the handle goes on working
     assert handle.grouped_gemm(**good) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", [[1], [20, 0, 300], [256]])
+def test_few_tiles_with_a_long_sum(handle, dtype, counts):
+    """Tiles fewer than half the pairs of SMs are cut along K and their sums added in a fixed order: at
+    most 15 more FP32 additions, 4 * 2^-22 S.  Without memory for the sums they stay whole."""
+    torch, api, experts = _setup()
+    dt = getattr(torch, dtype)
+    n, k, rows = 200, 5000, sum(counts)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, k, generator=g, device="cuda").to(dt)
+    w = torch.randn(len(counts), n, k, generator=g, device="cuda").to(dt)
+    want, size, spread = _product(torch, x, w, counts, True)
+    tol = _tolerance(torch, dt, k, want, size, spread) + 2.0 ** -20 * size
+    y = experts.grouped_matmul(handle, x, w, _ends(torch, counts), True)
+    _close(y, want, tol)
+    for _ in range(3):
+        assert torch.equal(y, experts.grouped_matmul(handle, x, w, _ends(torch, counts), True))
+    if dt != torch.float32:
+        handle.set_workspace_limit(1 << 10)
+        _close(experts.grouped_matmul(handle, x, w, _ends(torch, counts), True), want, tol)
+        handle.set_workspace_limit(0)
+    # the gradient of the weights, over rows that end inside a block
+    x = torch.randn(5000 + rows, 90, generator=g, device="cuda").to(dt)
+    dy = torch.randn(5000 + rows, n, generator=g, device="cuda").to(dt)
+    counts = [rows, 5000]
+    dw = experts.grouped_matmul_wgrad(handle, x, dy, _ends(torch, counts))
+    want, size, spread = _wgrad(torch, x, dy, counts, False)
+    _close(dw, want, _tolerance(torch, dt, 5000, want, size, spread) + 2.0 ** -20 * size)
+
+
+def test_few_tiles_with_a_long_integer_sum(handle):
+    torch, api, experts = _setup()
+    rows, n, k = 70, 130, 20000
+    xq = torch.randint(-128, 128, (rows, k), device="cuda", dtype=torch.int32).to(torch.int8)
+    wq = torch.randint(-128, 128, (n, k), device="cuda", dtype=torch.int32).to(torch.int8)
+    one = torch.ones(n, device="cuda")
+    y = experts.i8_matmul(handle, xq, one[:rows], wq, one, out_dtype=torch.float32)
+    assert torch.equal(y.double(), (xq.double() @ wq.double().t()).float().double())
