@@ -129,6 +129,14 @@ class Handle:
         if st != CUBLAS_STATUS_SUCCESS:
             raise CuMpSGEMMError(st, "cuMpSGEMM_create")
         self._h = h
+        self.stream = 0     # the raw stream that calls run on
+        self.device = None  # the number of its device, where torch is there to tell
+        try:
+            import torch
+
+            self.device = torch.cuda.current_device()
+        except ImportError:
+            pass
 
     # ------------------------------------------------------------------ life cycle
     def destroy(self) -> None:
@@ -158,6 +166,7 @@ class Handle:
         st = self._lib.cuMpSGEMM_set_stream(self._h, C.c_void_p(int(s)))
         if st != CUBLAS_STATUS_SUCCESS:
             raise CuMpSGEMMError(st, "cuMpSGEMM_set_stream")
+        self.stream = int(s)
 
     def use_current_torch_stream(self) -> None:
         import torch

@@ -11,7 +11,9 @@ the last total belong to no expert; their results are zero.
     y = i8_matmul(handle, q, s, wq, w_scale, ends)
 
 Everything goes through the C ABI (``cuMpSGEMM_grouped_gemm`` and its neighbours in
-``cumpsgemm_ext.h``) on the handle's stream; there is no other implementation behind it.
+``cumpsgemm_ext.h``); there is no other implementation behind it.  Results are allocated on the current
+stream and written on the handle's, so the two have to be one: ``handle.use_current_torch_stream()``
+wherever the current stream changes, or the call is refused.
 """
 from __future__ import annotations
 
@@ -69,9 +71,20 @@ def _matrices_of(t, what: str):
     return e, rows, n, ld, stride
 
 
-def _check(device: int, others, group_ends, groups: int) -> None:
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _check_place(handle, device: int) -> None:
     if device < 0:
         raise ValueError("operands must live in device memory")
+    if device != handle.device:
+        raise ValueError(f"operands are on device {device}, the handle is on {handle.device}")
+    if _current_stream(device) != handle.stream:
+        raise ValueError("the handle's stream is not the current one; call handle.use_current_torch_stream()")
+
+
+def _check(handle, device: int, others, group_ends, groups: int) -> None:
+    _check_place(handle, device)
     for t in others:
         if t.get_device() != device:
             raise ValueError("operands are on different devices")
@@ -109,7 +122,7 @@ def grouped_matmul(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
     groups, w_rows, w_cols, ldw, stridew = _matrices_of(w, "w")
     k, n = (w_cols, w_rows) if transpose_w else (w_rows, w_cols)
     rows, _, ldx = _rows_of(x, "x", k)
-    _check(x.get_device(), (w,), group_ends, groups)
+    _check(handle, x.get_device(), (w,), group_ends, groups)
     dtype = x.dtype
     if dtype is not w.dtype:
         raise ValueError(f"x is {dtype}, w is {w.dtype}")
@@ -134,7 +147,7 @@ def grouped_matmul_wgrad(handle: api.Handle, x, dy, group_ends=None, transpose_w
     if dy_rows != rows:
         raise ValueError(f"x has {rows} rows, dy {dy_rows}")
     groups = 1 if group_ends is None else group_ends.numel()
-    _check(x.get_device(), (dy,), group_ends, groups)
+    _check(handle, x.get_device(), (dy,), group_ends, groups)
     dtype = x.dtype
     if dtype is not dy.dtype:
         raise ValueError(f"x is {dtype}, dy is {dy.dtype}")
@@ -159,8 +172,7 @@ def quantize_rows(handle: api.Handle, x, row_index=None) -> Tuple[torch.Tensor, 
     (experts, n, k) is quantised as (experts * n, k) rows."""
     src_rows, k, ldx = _rows_of(x, "x")
     device = x.get_device()
-    if device < 0:
-        raise ValueError("operands must live in device memory")
+    _check_place(handle, device)
     data_type = _data_type(x.dtype)
     rows = src_rows
     if row_index is not None:
@@ -188,8 +200,8 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
         wq = wq.unsqueeze(0)
     groups, n, k, ldw, stridew = _matrices_of(wq, "wq")
     rows, _, ldx = _rows_of(xq, "xq", k)
-    _check(xq.get_device(), (x_scale, wq, w_scale) if bias is None else (x_scale, wq, w_scale, bias),
-           group_ends, groups)
+    _check(handle, xq.get_device(),
+           (x_scale, wq, w_scale) if bias is None else (x_scale, wq, w_scale, bias), group_ends, groups)
     if xq.dtype is not torch.int8 or wq.dtype is not torch.int8:
         raise ValueError(f"xq is {xq.dtype}, wq is {wq.dtype}: both must be int8")
     for t, what, count in ((x_scale, "x_scale", rows), (w_scale, "w_scale", groups * n),
@@ -209,6 +221,10 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
     return out
 
 
+def _dense_rows(t):
+    return t if t.stride(-1) == 1 and t.stride(-2) >= t.shape[-1] else t.contiguous()
+
+
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, group_ends, handle, transpose_w, mode):
@@ -220,8 +236,7 @@ class _GroupedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, group_ends = ctx.saved_tensors
         handle, transpose_w, mode = ctx.how
-        if dy.stride(-1) != 1 or dy.stride(0) < dy.shape[1]:  # e.g. of a sum: one value for all rows
-            dy = dy.contiguous()
+        dy = _dense_rows(dy)  # the gradient of a sum, say, is one value for all of them
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = grouped_matmul(handle, dy, w, group_ends, not transpose_w, mode=mode)
@@ -232,6 +247,6 @@ class _GroupedLinear(torch.autograd.Function):
 
 def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool = False, *,
                    mode: int = api.ComputeMode.FP16TCEC):
-    """``grouped_matmul`` with a backward pass: gradients of x and w.  Forward and backward run on the
-    handle's stream, which has to be the one that autograd runs on."""
-    return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode)
+    """``grouped_matmul`` with a backward pass: gradients of x and w.  Autograd runs the backward pass on the
+    stream of the forward pass."""
+    return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode)

@@ -417,7 +417,6 @@ def test_runs_repeat_bit_for_bit_on_another_stream_and_in_a_graph(handle):
     side.synchronize()
     assert torch.equal(first, again)
     y, y32, xf, wf = torch.empty_like(first), torch.empty_like(first32), x.float(), w.float()
-    q, s = experts.quantize_rows(handle, x)
     graph = torch.cuda.CUDAGraph()
     side.synchronize()
     with torch.cuda.graph(graph, stream=side):
@@ -495,6 +494,9 @@ def test_refusals(handle):
         experts.grouped_matmul(handle, *f, ends)
     assert e.value.status == api.CUBLAS_STATUS_ALLOC_FAILED
     handle.set_workspace_limit(0)
+    # results are allocated on the current stream and written on the handle's
+    with torch.cuda.stream(torch.cuda.Stream()), pytest.raises(ValueError, match="stream"):
+        experts.grouped_matmul(handle, x, w, ends)
     # and the handle goes on working
     assert handle.grouped_gemm(**good) == 0
 
