@@ -56,6 +56,7 @@ namespace {
 constexpr int BM_CTA = 128;            // lanes per CTA
 constexpr uint32_t LANES = 2 * BM_CTA; // per pair
 constexpr uint32_t COLS = 256;         // most columns of a tile
+constexpr uint32_t WIDTHS = 3;         // that a launch chooses from: 256, 128, 64
 constexpr uint32_t ROW_BYTES = kGemmRowBytes;
 constexpr uint32_t TILE_BYTES = 128 * ROW_BYTES; // an operand's part of a stage in one CTA
 constexpr uint32_t ATOM_BYTES = 64 * ROW_BYTES;  // lanes (columns) contiguous: 64 of them by 64 of K
@@ -84,15 +85,22 @@ template <int KIND> struct Cfg {
   static constexpr uint32_t STAGE_BYTES = 2 * PLANES * TILE_BYTES;
   static constexpr uint32_t STAGES = KIND == kTcec ? 3 : 6;
   static constexpr uint32_t K_ELEMS = KIND == kI8 ? 128 : 64; // of K in a stage
+  // What a step of K takes, in columns of products, and what a tile takes besides (about 3 us): a step is
+  // as long as its products or its loads, 128 lanes and half the columns in each CTA.
+  static __device__ __forceinline__ float step_cost(uint32_t cols) {
+    return fmaxf(static_cast<float>(cols), LOADS * static_cast<float>(256u + cols));
+  }
+  static constexpr float LOADS = KIND == kTcec ? 0.4f : KIND == kF16 ? 0.5f : 0.8f;
+  static constexpr float TILE_COST = KIND == kTcec ? 700.f : KIND == kF16 ? 2500.f : 5000.f;
   static constexpr uint32_t BARS = STAGES * STAGE_BYTES;      // offsets in shared memory
   static constexpr uint32_t FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
                             ACC_EMPTY = ACC_FULL + 16, TAIL = ACC_EMPTY + 16, NEXT_FULL = TAIL + 8 * STAGES,
                             NEXT_EMPTY = NEXT_FULL + 8 * AHEAD, WANT = NEXT_EMPTY + 8 * AHEAD, TMEM_PTR = WANT + 8,
-                            ABORT = TMEM_PTR + 4, NEXT = BARS + 256, START = NEXT + AHEAD * TILE_WORDS * 4,
+                            ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4, NEXT = BARS + 256, START = NEXT + AHEAD * TILE_WORDS * 4,
                             FIRST_TILE = START + 4 * (kMaxGroups + 2),
                             OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
                             BYTES = OUT + (KIND == kTcec ? 0 : NUM_EPI_WARPS * OUT_BYTES);
-  static_assert(ABORT + 4 <= NEXT && STAGES <= 32, "barriers and flags; phases are bits");
+  static_assert(WIDTH + 4 <= NEXT && STAGES <= 32, "barriers and flags; phases are bits");
   static constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 };
 
@@ -139,10 +147,12 @@ static_assert(sizeof(Tile) == TILE_WORDS * 4, "three times 16 bytes");
 template <int KIND, bool WGRAD> struct Items {
   const uint32_t *start, *first_tile;
   uint32_t group, total, slices; // slices: item numbers of a tile
+  uint32_t cols;                 // of a tile that is not a group's last
   __device__ __forceinline__ Items(const uint8_t *smem, const GroupedParams &p, uint32_t clusters) {
     start = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::START);
     first_tile = reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
     group = 0;
+    cols = *reinterpret_cast<const uint32_t *>(smem + Cfg<KIND>::WIDTH);
     const uint32_t tiles = first_tile[p.groups + 1];
     slices = p.parts != nullptr && tiles > 0 && tiles <= clusters / 2 ? min(clusters / tiles, MAX_SLICES) : 1u;
     total = tiles * slices;
@@ -159,15 +169,15 @@ template <int KIND, bool WGRAD> struct Items {
     const uint32_t r0 = start[group], r = start[group + 1] - r0;
     const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
     const uint32_t col_dim = WGRAD ? p.col_dim : r;
-    const uint32_t col_tiles = (col_dim + COLS - 1) / COLS;
+    const uint32_t col_tiles = (col_dim + cols - 1) / cols;
     const uint32_t local = tile - first_tile[group];
     const uint32_t band = local / (BAND * lane_tiles), in_band = local - band * BAND * lane_tiles;
     const uint32_t width = min(BAND, col_tiles - band * BAND);
     const uint32_t lt = in_band / width, ct = band * BAND + (in_band - lt * width);
     x.group = group;
     x.lane0 = lt * LANES;
-    x.cols = min(COLS, col_dim - ct * COLS);
-    x.col0 = ct * COLS + (WGRAD ? 0u : r0);
+    x.cols = min(cols, col_dim - ct * cols);
+    x.col0 = ct * cols + (WGRAD ? 0u : r0);
     x.row0 = r0;
     x.rows = r;
     x.k0 = 0;
@@ -230,17 +240,17 @@ template <int KIND, bool WARP> struct Tiles { // taken by a warp, or by one thre
   }
 };
 
-// First row and first tile of each group, by one warp.  What `ends` holds is never trusted: a total
-// that falls back or passes the number of rows is taken as the one in front of it, or as that number.
-// The rows behind the last group are a group of their own (product: its tiles have no blocks; wgrad:
-// it has no tiles).
+// First row and first tile of each group, and the width of the tiles, by one warp.  What `ends` holds is
+// never trusted: a total that falls back or passes the number of rows is taken as the one in front of it,
+// or as that number.  The rows behind the last group are a group of their own (product: its tiles have no
+// blocks; wgrad: it has no tiles).
 template <int KIND, bool WGRAD>
-__device__ __forceinline__ void find_groups(uint8_t *smem, const GroupedParams &p) {
+__device__ __forceinline__ void find_groups(uint8_t *smem, const GroupedParams &p, uint32_t clusters) {
   uint32_t *start = reinterpret_cast<uint32_t *>(smem + Cfg<KIND>::START);
   uint32_t *first_tile = reinterpret_cast<uint32_t *>(smem + Cfg<KIND>::FIRST_TILE);
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t lane_tiles = (p.lane_dim + LANES - 1) / LANES;
-  uint32_t end_before = 0, tiles_before = 0;
+  uint32_t end_before = 0, most = 0; // most rows of a group, of this lane's
   for (uint32_t g0 = 0; g0 < p.groups + 1; g0 += 32) {
     const uint32_t g = g0 + lane;
     uint32_t end = 0;
@@ -257,29 +267,74 @@ __device__ __forceinline__ void find_groups(uint8_t *smem, const GroupedParams &
     end = max(end, end_before);
     uint32_t begin = __shfl_up_sync(0xffffffffu, end, 1);
     if (lane == 0) begin = end_before;
-    uint32_t tiles = 0;
-    if constexpr (WGRAD) {
-      if (g < p.groups) tiles = lane_tiles * ((p.col_dim + COLS - 1) / COLS);
-    } else {
-      if (g <= p.groups) tiles = lane_tiles * ((end - begin + COLS - 1) / COLS);
+    if (g <= p.groups) start[g] = begin;
+    if (g == p.groups) start[g + 1] = end;
+    most = max(most, end - begin);
+    end_before = __shfl_sync(0xffffffffu, end, 31);
+  }
+  __syncwarp();
+  // tiles of group g (for g == groups, the rows behind the last) that are `cols` wide
+  auto tiles_of = [&](uint32_t g, uint32_t cols) {
+    if (WGRAD) return g < p.groups ? lane_tiles * ((p.col_dim + cols - 1) / cols) : 0u;
+    return lane_tiles * ((start[g + 1] - start[g] + cols - 1) / cols);
+  };
+  // The width.  With many tiles, the widest.  Else the one with the earliest end by this estimate: the
+  // work shared by all pairs and half a tile, or the longest tile where there are no more tiles than
+  // pairs.  (us with tiles of 256 / so: bfloat16 256 x 4096 x 1024 21.6 / 13.9, 1024^3 11.3 / 9.6, 1024 rows
+  // over 4 experts of 2048 x 2048 23.4 / 15.9, over 4 of 1024 x 1024 in FP32 34.6 / 23.4; 16 rows over 8
+  // experts, where there is nothing to choose, 8.6 / 8.8.)
+  uint32_t cols = COLS;
+  if (__any_sync(0xffffffffu, WGRAD ? p.col_dim > COLS >> (WIDTHS - 1) : most > COLS >> (WIDTHS - 1))) {
+    uint32_t tiles[WIDTHS];
+    float work[WIDTHS], longest[WIDTHS];
+#pragma unroll
+    for (uint32_t i = 0; i < WIDTHS; ++i) tiles[i] = 0, work[i] = longest[i] = 0.f;
+    for (uint32_t g = lane; g <= p.groups; g += 32) {
+      const uint32_t rows = start[g + 1] - start[g], col_dim = WGRAD ? p.col_dim : rows;
+      if (col_dim == 0 || (WGRAD && g == p.groups)) continue;
+      const float steps = static_cast<float>(WGRAD ? (rows + 63u) / 64u : g < p.groups ? p.col_dim : 0u);
+#pragma unroll
+      for (uint32_t i = 0; i < WIDTHS; ++i) {
+        const uint32_t w = COLS >> i, whole = col_dim / w, rest = (col_dim - whole * w + 31u) & ~31u;
+        const float wide = steps * Cfg<KIND>::step_cost(w) + Cfg<KIND>::TILE_COST,
+                    narrow = steps * Cfg<KIND>::step_cost(rest) + Cfg<KIND>::TILE_COST;
+        tiles[i] += lane_tiles * (whole + (rest > 0));
+        work[i] += lane_tiles * (whole * wide + (rest > 0 ? narrow : 0.f));
+        longest[i] = fmaxf(longest[i], whole > 0 ? wide : narrow);
+      }
     }
+    float best = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < WIDTHS; ++i) {
+      const uint32_t n = __reduce_add_sync(0xffffffffu, tiles[i]);
+      if (i == 0 && n >= 4 * clusters) break;
+      float sum = work[i];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      // (non-negative floats are ordered as their bits)
+      const float most_of_one = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(longest[i])));
+      const float ends_at = n <= clusters ? most_of_one : fmaxf(most_of_one, sum / clusters + 0.5f * most_of_one);
+      if (i == 0 || ends_at < 0.95f * best) {
+        best = ends_at;
+        cols = COLS >> i;
+      }
+    }
+  }
+  uint32_t tiles_before = 0;
+  for (uint32_t g0 = 0; g0 < p.groups + 1; g0 += 32) {
+    const uint32_t g = g0 + lane;
+    const uint32_t tiles = g <= p.groups ? tiles_of(g, cols) : 0u;
     uint32_t upto = tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
       if (static_cast<int>(lane) >= d) upto += o;
     }
-    if (g <= p.groups) {
-      start[g] = begin;
-      first_tile[g] = tiles_before + upto - tiles;
-      if (g == p.groups) {
-        start[g + 1] = end;
-        first_tile[g + 1] = tiles_before + upto;
-      }
-    }
-    end_before = __shfl_sync(0xffffffffu, end, 31);
+    if (g <= p.groups) first_tile[g] = tiles_before + upto - tiles;
+    if (g == p.groups) first_tile[g + 1] = tiles_before + upto;
     tiles_before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  if (lane == 0) *reinterpret_cast<uint32_t *>(smem + Cfg<KIND>::WIDTH) = cols;
 }
 
 template <int KIND>
@@ -576,7 +631,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   // not let in early: pairs end one by one, and the blocks of a pass over rows would crowd on the SMs that
   // are free first (FP32, 192 rows over 7 experts of 6469 x 2804, calls back to back: 513 us instead of 407).
   ptx::griddep_wait();
-  if (warp == 2) find_groups<KIND, WGRAD>(smem, p);
+  if (warp == 2) find_groups<KIND, WGRAD>(smem, p, clusters);
   ptx::tc_fence_before();
   __syncthreads();
   // both CTAs' barriers must exist before any remote arrive / remote TMA completion
