@@ -61,6 +61,9 @@ struct StageOperand {
   uint32_t batch;           // 1: outer runs over rows, of which those behind the last group are left out;
                             // a batch of weights leaves out the groups without rows
   bool rows_are_grouped;    // the first case
+  // How the rows are dealt (launch_stage sets it): 2^lanes_log2 lanes take a segment of a row at a time,
+  // of which there are `segments`, in so many steps.
+  uint32_t lanes_log2, segments, steps;
 };
 struct StageArgs {
   StageOperand op[2];

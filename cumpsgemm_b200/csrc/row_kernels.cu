@@ -40,24 +40,26 @@ __device__ __forceinline__ uint32_t last_end(const StageArgs &a) {
   return most;
 }
 
-// The rows of all operands, one after the other, dealt to the warps of the grid.
-struct RowCursor {
-  uint64_t first[3]; // first row number of each operand, and their end
-  uint32_t used_rows;
-  __device__ __forceinline__ RowCursor(const StageArgs &a) {
-    used_rows = last_end(a);
-    first[0] = 0;
-    for (int i = 0; i < 2; ++i)
-      first[i + 1] = first[i] + (i >= a.count ? 0
-                                 : a.op[i].rows_are_grouped
-                                     ? static_cast<uint64_t>(used_rows)
-                                     : static_cast<uint64_t>(a.op[i].batch) * a.op[i].outer);
-  }
-};
-
 // A row of `bytes` bytes at any address, read 16 bytes at a time.  Where the address is no multiple of
 // 16, two aligned accesses inside the row are shifted together (the second is the next lane's first,
-// and comes from L1): element by element, 55 million FP32 values in odd rows took 95 us to split.
+// and comes from L1): element by element, 55 million FP32 values in odd rows took 95 us to split, and
+// take 84 (5.3 TB/s).
+// bytes shift .. shift + 15 of the 32 in x and y; ES divides shift
+template <int ES>
+__device__ __forceinline__ uint4 shifted(const uint4 &x, const uint4 &y, uint32_t shift) {
+  uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = shift & 8u ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = shift & 4u ? w[i + 1] : w[i];
+  if constexpr (ES < 4) {
+    const uint32_t bits = (shift & 3u) * 8u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct RowReader {
   const uint8_t *p;
   uint64_t bytes;
@@ -85,21 +87,8 @@ struct RowReader {
       }
     }
     if (WHOLE || shift == 0) return;
-    const uint32_t bits = (shift & 3u) * 8u;
 #pragma unroll
-    for (uint32_t first = 0; first < 4; ++first)
-      if (shift >> 2 == first) { // the same for the whole row
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const uint32_t w[8] = {o[j].x,    o[j].y,    o[j].z,    o[j].w,
-                                 next[j].x, next[j].y, next[j].z, next[j].w};
-          uint32_t v[4];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            v[i] = ES == 4 ? w[first + i] : __funnelshift_r(w[first + i], w[first + i + 1], bits);
-          o[j] = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
+    for (int j = 0; j < N; ++j) o[j] = shifted<ES>(o[j], next[j], shift);
   }
   // the rest of such 16 bytes: at the ends of the row, element by element
   template <int ES> __device__ __forceinline__ uint4 load_end(uint64_t at) const {
@@ -136,39 +125,119 @@ struct RowReader {
 };
 constexpr uint32_t kBatch = 4; // 16-byte loads that a lane has on its way at once
 
+// The segments of all operands' rows, one after the other, dealt to the warps of the grid.  2^lanes_log2
+// lanes take one, so a warp takes several short rows together; a row is one segment, unless there are
+// too few of them to occupy all warps.  (With a row to a warp 110,000 rows of 183 bytes took 49 us, and
+// take 14, and 480 of 29 KB took 17 and take 8.)
+struct Segments {
+  uint32_t units[2];  // segments of each operand
+  uint64_t first[3];  // turns of a warp: first of each operand, and their end
+  __device__ __forceinline__ Segments(const StageArgs &a) {
+    const uint32_t used_rows = last_end(a);
+    first[0] = 0;
+    for (int i = 0; i < 2; ++i) {
+      const StageOperand &op = a.op[i];
+      units[i] = i >= a.count ? 0u
+                              : (op.rows_are_grouped ? used_rows : static_cast<uint32_t>(op.batch * op.outer)) *
+                                    op.segments;
+      first[i + 1] = first[i] + ((units[i] + (32u >> op.lanes_log2) - 1u) >> (5u - op.lanes_log2));
+    }
+  }
+};
+// One lane's part of a turn.
+struct Segment {
+  int o; // operand
+  uint32_t row, lanes, lane, first, steps; // first: of its pieces of 16 bytes; the next are `lanes` further on
+  bool ends;                               // the row's ends are this segment's too
+  uint64_t src_at;                         // of the row's first element
+  // false: there is none, or of weights that no row uses
+  __device__ __forceinline__ bool get(const StageArgs &a, const Segments &s, uint64_t turn) {
+    o = turn >= s.first[1];
+    const StageOperand &op = o ? a.op[1] : a.op[0];
+    const uint32_t all = threadIdx.x & 31u, log2 = op.lanes_log2, segments = op.segments;
+    lanes = 1u << log2;
+    lane = all & (lanes - 1u);
+    const uint32_t unit = (static_cast<uint32_t>(turn - s.first[o]) << (5u - log2)) + (all >> log2);
+    if (unit >= s.units[o]) return false;
+    row = unit / segments;
+    const uint32_t segment = unit - row * segments, outer = static_cast<uint32_t>(op.outer);
+    const uint32_t b = row / outer;
+    steps = op.steps;
+    first = segment * steps * kBatch * lanes + lane;
+    ends = segment == 0;
+    src_at = b * op.stride + (row - b * outer) * op.ld;
+    return op.rows_are_grouped || op.batch == 1 || group_is_used(a, b);
+  }
+};
+// The pieces of a row that aligned accesses inside it give: [from, to) in units of 16 bytes (RowReader::inside).
+struct Inside {
+  const uint4 *aligned; // the row's first byte and what lies in front of it in its 16 bytes
+  uint32_t shift, from, to;
+  __device__ __forceinline__ explicit Inside(const RowReader &row)
+      : aligned(reinterpret_cast<const uint4 *>(row.p - row.shift)), shift(row.shift), from(row.shift != 0) {
+    const uint64_t need = shift == 0 ? 16 : 32;
+    to = row.bytes + shift < need ? 0u : static_cast<uint32_t>((row.bytes + shift - need) / 16 + 1);
+  }
+  __device__ __forceinline__ bool has(uint32_t piece) const { return piece >= from && piece < to; }
+  template <int ES> // pieces at, at + lanes, ...; all loads are on their way before the first is looked at
+  __device__ __forceinline__ void load(uint32_t at, uint32_t lanes, uint4 (&x)[kBatch]) const {
+    uint4 next[kBatch];
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const uint32_t piece = at + j * lanes;
+      x[j] = next[j] = make_uint4(0, 0, 0, 0);
+      if (has(piece)) {
+        x[j] = __ldg(aligned + piece);
+        if (shift != 0) next[j] = __ldg(aligned + piece + 1);
+      }
+    }
+    if (shift == 0) return;
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) x[j] = shifted<ES>(x[j], next[j], shift);
+  }
+};
+
 // ---------------------------------------------------------------- scales of FP32 operands
 // records[op * kScaleRecords + block] = largest finite magnitude that block met.  Infinities and NaN
 // say nothing of the range of the others, and rows of no group may hold anything.
-__global__ void __launch_bounds__(kThreads) largest_magnitude_kernel(const StageArgs a) {
+// (Without the bound on blocks ptxas takes 32 registers and has a lane's loads wait for one another: 71 us
+// for 55 million values instead of 45.)
+__global__ void __launch_bounds__(kThreads, 4) largest_magnitude_kernel(const StageArgs a) {
   CUMPSGEMM_CHAINED_KERNEL_ENTRY();
-  const RowCursor rows(a);
+  const Segments all(a);
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWarps;
   float most[2] = {0.f, 0.f};
-  for (uint64_t r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows.first[2]; r += step) {
-    const int o = r >= rows.first[1];
-    const StageOperand &op = a.op[o];
-    const uint64_t at = r - rows.first[o];
-    const uint32_t b = static_cast<uint32_t>(at / op.outer);
-    if (!op.rows_are_grouped && op.batch > 1 && !group_is_used(a, b)) continue;
-    const float *src = static_cast<const float *>(op.src) + b * op.stride + (at - b * op.outer) * op.ld;
+  for (uint64_t turn = blockIdx.x * kWarps + (threadIdx.x >> 5); turn < all.first[2]; turn += step) {
+    Segment seg;
+    if (!seg.get(a, all, turn)) continue;
+    const StageOperand &op = seg.o ? a.op[1] : a.op[0];
+    const float *src = static_cast<const float *>(op.src) + seg.src_at;
     // in front of the first 16-byte boundary and behind the last one by one, 16 bytes at a time between
-    const uint64_t head = min(op.inner, static_cast<uint64_t>((0u - (reinterpret_cast<uintptr_t>(src) >> 2)) & 3u));
-    const uint64_t vectors = (op.inner - head) / 4, rest = head + 4 * vectors;
+    const uint32_t inner = static_cast<uint32_t>(op.inner);
+    const uint32_t head = min(inner, static_cast<uint32_t>(0u - (reinterpret_cast<uintptr_t>(src) >> 2)) & 3u);
+    const uint32_t vectors = (inner - head) / 4, rest = head + 4 * vectors;
+    const float4 *body = reinterpret_cast<const float4 *>(src + head);
+    float4 ends = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (seg.ends) { // (at least four lanes, and at most three values at either end)
+      if (seg.lane < head) ends.x = src[seg.lane];
+      if (rest + seg.lane < inner) ends.y = src[rest + seg.lane];
+    }
     float m = 0.f;
     auto take = [&](float v) { m = fmaxf(m, finite(v) ? fabsf(v) : 0.f); };
-    if (lane < head) take(src[lane]);
-    if (rest + lane < op.inner) take(src[rest + lane]);
-    const float4 *body = reinterpret_cast<const float4 *>(src + head);
-    for (uint64_t i = lane; i < vectors; i += kBatch * 32) {
+    uint32_t at = seg.first;
+    for (uint32_t t = 0; t < seg.steps; ++t, at += kBatch * seg.lanes) {
       float4 x[kBatch];
 #pragma unroll
-      for (uint32_t j = 0; j < kBatch; ++j)
-        x[j] = i + j * 32 < vectors ? __ldg(body + i + j * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t j = 0; j < kBatch; ++j) {
+        const uint32_t i = at + j * seg.lanes;
+        x[j] = i < vectors ? __ldg(body + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
       for (uint32_t j = 0; j < kBatch; ++j) take(x[j].x), take(x[j].y), take(x[j].z), take(x[j].w);
     }
-    most[o] = fmaxf(most[o], m);
+    take(ends.x), take(ends.y);
+    most[seg.o] = fmaxf(most[seg.o], m);
   }
   __shared__ uint32_t found[2];
   if (threadIdx.x < 2) found[threadIdx.x] = 0;
@@ -198,7 +267,7 @@ __device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
 template <int BYTES>
 __global__ void __launch_bounds__(kThreads) stage_kernel(const StageArgs a) {
   CUMPSGEMM_CHAINED_KERNEL_ENTRY();
-  const RowCursor rows(a);
+  const Segments all(a);
   const uint32_t lane = threadIdx.x & 31u;
   float scale[2] = {1.f, 1.f};
   if (BYTES == 4 && a.scale) {
@@ -224,20 +293,35 @@ __global__ void __launch_bounds__(kThreads) stage_kernel(const StageArgs a) {
     }
   }
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWarps;
-  for (uint64_t r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows.first[2]; r += step) {
-    const int o = r >= rows.first[1];
-    const StageOperand &op = a.op[o];
-    const uint64_t at = r - rows.first[o];
-    const uint32_t b = static_cast<uint32_t>(at / op.outer);
-    if (!op.rows_are_grouped && op.batch > 1 && !group_is_used(a, b)) continue;
-    const uint64_t src_at = b * op.stride + (at - b * op.outer) * op.ld;
+  for (uint64_t turn = blockIdx.x * kWarps + (threadIdx.x >> 5); turn < all.first[2]; turn += step) {
+    Segment seg;
+    if (!seg.get(a, all, turn)) continue;
+    const StageOperand &op = seg.o ? a.op[1] : a.op[0];
+    const RowReader row(static_cast<const uint8_t *>(op.src) + seg.src_at * BYTES, op.inner * BYTES);
+    const Inside in(row);
+    const uint64_t dst_at = seg.row * op.ld_dst;
+    // what is not inside, at most four pieces of a row, by the first lanes of its first segment
+    const uint64_t end = seg.ends && seg.lane < 4 ? row.end_piece(seg.lane) : row.bytes;
+    const bool has_end = end < row.bytes;
+    uint4 end_x = make_uint4(0, 0, 0, 0);
+    if (has_end) end_x = row.load_end<BYTES>(end);
+    auto all_pieces = [&](auto &&put) {
+      uint32_t at = seg.first;
+      for (uint32_t t = 0; t < seg.steps; ++t, at += kBatch * seg.lanes) {
+        uint4 x[kBatch];
+        in.load<BYTES>(at, seg.lanes, x);
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j)
+          if (in.has(at + j * seg.lanes)) put(at + j * seg.lanes, x[j]);
+      }
+      if (has_end) put(static_cast<uint32_t>(end / 16), end_x);
+    };
     if constexpr (BYTES == 4) {
-      const RowReader row(static_cast<const float *>(op.src) + src_at, op.inner * 4);
-      const float s = o ? scale[1] : scale[0];
-      __half *hi = static_cast<__half *>(op.dst) + at * op.ld_dst;
-      __half *lo = hi + static_cast<uint64_t>(op.batch) * op.outer * op.ld_dst;
-      auto put = [&](uint64_t i, const uint4 &x) { // four values from byte i on
-        const uint32_t b[4] = {x.x, x.y, x.z, x.w};
+      const float s = seg.o ? scale[1] : scale[0];
+      uint2 *hi = reinterpret_cast<uint2 *>(static_cast<__half *>(op.dst) + dst_at);
+      uint2 *lo = hi + static_cast<uint64_t>(op.batch) * op.outer * op.ld_dst / 4;
+      all_pieces([&](uint32_t piece, const uint4 &v) { // of four values
+        const uint32_t b[4] = {v.x, v.y, v.z, v.w};
         uint32_t h[2], l[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -248,30 +332,12 @@ __global__ void __launch_bounds__(kThreads) stage_kernel(const StageArgs a) {
           h[t] = *reinterpret_cast<const uint32_t *>(&hh);
           l[t] = *reinterpret_cast<const uint32_t *>(&ll);
         }
-        *reinterpret_cast<uint2 *>(hi + i / 4) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2 *>(lo + i / 4) = make_uint2(l[0], l[1]);
-      };
-      for (uint64_t i = 16ull * lane; i < row.bytes; i += kBatch * 512) {
-        uint4 x[kBatch];
-        row.load_inside<4, false>(i, 512, x);
-#pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j)
-          if (row.inside(i + j * 512)) put(i + j * 512, x[j]);
-      }
-      const uint64_t end = lane < 4 ? row.end_piece(lane) : row.bytes;
-      if (end < row.bytes) put(end, row.load_end<4>(end));
+        hi[piece] = make_uint2(h[0], h[1]);
+        lo[piece] = make_uint2(l[0], l[1]);
+      });
     } else {
-      const RowReader row(static_cast<const uint8_t *>(op.src) + src_at * BYTES, op.inner * BYTES);
-      uint8_t *dst = static_cast<uint8_t *>(op.dst) + at * op.ld_dst * BYTES; // rows of whole 16 bytes
-      for (uint64_t i = 16ull * lane; i < row.bytes; i += kBatch * 512) {
-        uint4 x[kBatch];
-        row.load_inside<BYTES, false>(i, 512, x);
-#pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j)
-          if (row.inside(i + j * 512)) *reinterpret_cast<uint4 *>(dst + i + j * 512) = x[j];
-      }
-      const uint64_t end = lane < 4 ? row.end_piece(lane) : row.bytes;
-      if (end < row.bytes) *reinterpret_cast<uint4 *>(dst + end) = row.load_end<BYTES>(end);
+      uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(op.dst) + dst_at * BYTES);
+      all_pieces([&](uint32_t piece, const uint4 &v) { dst[piece] = v; });
     }
   }
 }
@@ -495,12 +561,29 @@ template <class T> cudaError_t quantize(const QuantizeArgs &a, unsigned num_sms,
 
 } // namespace
 
-cudaError_t launch_stage(const StageArgs &a, unsigned num_sms, cudaStream_t stream) {
-  if (a.count == 0) return cudaSuccess;
-  uint64_t rows = 0;
-  for (int i = 0; i < a.count; ++i) rows += static_cast<uint64_t>(a.op[i].batch) * a.op[i].outer;
-  const uint64_t want = (rows + kWarps - 1) / kWarps, resident = static_cast<uint64_t>(num_sms) * 8;
-  const unsigned grid = static_cast<unsigned>(want < 1 ? 1 : want < resident ? want : resident);
+cudaError_t launch_stage(const StageArgs &args, unsigned num_sms, cudaStream_t stream) {
+  if (args.count == 0) return cudaSuccess;
+  StageArgs a = args;
+  uint64_t turns = 0;
+  for (int i = 0; i < 2; ++i) {
+    StageOperand &op = a.op[i];
+    const uint64_t pieces = (op.inner * static_cast<uint64_t>(a.elem_bytes) + 15) / 16;
+    op.lanes_log2 = 2;
+    while (op.lanes_log2 < 5 && (static_cast<uint64_t>(kBatch) << op.lanes_log2) < pieces) ++op.lanes_log2;
+    const uint64_t at_once = static_cast<uint64_t>(kBatch) << op.lanes_log2, steps = (pieces + at_once - 1) / at_once;
+    // two turns for each of 32 warps an SM, if the rows go so far
+    const uint64_t rows = op.outer * op.batch, wanted = (static_cast<uint64_t>(num_sms) * 64) << (5 - op.lanes_log2);
+    uint64_t segments = rows >= wanted || rows == 0 ? 1 : (wanted + rows - 1) / rows;
+    if (segments > steps) segments = steps;
+    op.steps = static_cast<uint32_t>(segments > 0 ? (steps + segments - 1) / segments : 1);
+    op.segments = static_cast<uint32_t>((steps + op.steps - 1) / op.steps);
+    if (i >= a.count) continue;
+    // (numbers of segments are 32-bit)
+    if (op.segments * op.outer >= (1ull << 32) / op.batch) return cudaErrorInvalidValue;
+    turns += ((op.segments * rows) >> (5 - op.lanes_log2)) + 1;
+  }
+  const uint64_t want = (turns + kWarps - 1) / kWarps, resident = static_cast<uint64_t>(num_sms) * 8;
+  const unsigned grid = static_cast<unsigned>(want < resident ? want : resident);
   if (a.elem_bytes == 4 && a.scale) {
     const cudaError_t e = launch_chained(largest_magnitude_kernel, kScaleRecords, kThreads, 0, stream, a);
     if (e != cudaSuccess) return e;
