@@ -129,14 +129,8 @@ class Handle:
         if st != CUBLAS_STATUS_SUCCESS:
             raise CuMpSGEMMError(st, "cuMpSGEMM_create")
         self._h = h
-        self.stream = 0     # the raw stream that calls run on
-        self.device = None  # the number of its device, where torch is there to tell
-        try:
-            import torch
-
-            self.device = torch.cuda.current_device()
-        except ImportError:
-            pass
+        self.stream = 0  # the raw stream that calls run on
+        self.device = self._lib.cuMpSGEMM_get_device(h)
 
     # ------------------------------------------------------------------ life cycle
     def destroy(self) -> None:

@@ -42,6 +42,7 @@ CUDA_SOURCES = [
     "static_scratch_gemm.cu",
     "tiny_gemm.cu",
     "grouped_gemm.cu",
+    "grouped_few_rows.cu",
     "row_kernels.cu",
     "grouped_api.cu",
 ]

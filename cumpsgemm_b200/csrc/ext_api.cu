@@ -220,6 +220,8 @@ int cuMpSGEMM_selftest_bounded_wait(cuMpSGEMM_handle_t h, unsigned limit_ms,
   return status;
 }
 
+int cuMpSGEMM_get_device(cuMpSGEMM_handle_t h) { return h == nullptr ? -1 : h->device; }
+
 void cuMpSGEMM_set_workspace_limit(cuMpSGEMM_handle_t h, size_t bytes) {
   h->workspace_limit_bytes = bytes;
 }

@@ -78,6 +78,18 @@ struct StageArgs {
 constexpr uint32_t kScaleRecords = 592;
 cudaError_t launch_stage(const StageArgs &a, unsigned num_sms, cudaStream_t stream);
 
+// The product of FP32 operands in FP32 arithmetic, for groups of few rows (grouped_few_rows.cu).
+struct FewRowsArgs {
+  bool op_n; // w is stored k by n, else n by k
+  const int32_t *ends;
+  const float *x, *w;
+  float *y;
+  uint64_t ldx, ldw, stridew, ldy;
+  uint32_t rows, groups, n, k;
+  float alpha, beta;
+};
+cudaError_t launch_few_rows(const FewRowsArgs &a, unsigned num_sms, cudaStream_t stream);
+
 struct QuantizeArgs {
   const void *x;
   int type; // GroupedOut

@@ -116,6 +116,11 @@ const char *check_sizes(uint64_t rows, uint64_t n, uint64_t k, uint32_t groups, 
   return nullptr;
 }
 
+// Whether an FP32 product goes to the kernel for few rows, which passes over a group's weights once for
+// every 8 of its rows: up to 6 for each group on average it is the shorter way (grouped_few_rows.cu has the
+// times), even if some groups have several times as many.
+bool takes_few_rows(uint64_t rows, uint32_t groups) { return rows <= 6ull * groups; }
+
 bool fp32_mode_ok(cuMpSGEMM_compute_mode_t mode) {
   return mode == CUMPSGEMM_FP16TCEC || mode == CUMPSGEMM_FP16TCEC_SCALING;
 }
@@ -151,6 +156,14 @@ extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm(
   if (rows == 0) return CUBLAS_STATUS_SUCCESS;
 
   DeviceGuard guard(h->device);
+  if (type == CUDA_R_32F && takes_few_rows(rows, num_groups)) {
+    const FewRowsArgs f = {w_n_contig, group_ends, static_cast<const float *>(x), static_cast<const float *>(w),
+                           static_cast<float *>(y), ldx, ldw, stridew, ldy, static_cast<uint32_t>(rows),
+                           num_groups, static_cast<uint32_t>(n), static_cast<uint32_t>(k), *alpha, *beta};
+    const cudaError_t e = launch_few_rows(f, h->num_sms, h->cuda_stream);
+    mark_stream_work(h);
+    return e == cudaSuccess ? CUBLAS_STATUS_SUCCESS : CUBLAS_STATUS_EXECUTION_FAILED;
+  }
   GroupedArgs g = {};
   g.kind = type == CUDA_R_32F ? GroupedKind::tcec : GroupedKind::f16;
   g.out_type = out_type(type);

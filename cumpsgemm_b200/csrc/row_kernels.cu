@@ -203,7 +203,8 @@ struct Inside {
 // (Without the bound on blocks ptxas takes 32 registers and has a lane's loads wait for one another: 71 us
 // for 55 million values instead of 45.)
 __global__ void __launch_bounds__(kThreads, 4) largest_magnitude_kernel(const StageArgs a) {
-  CUMPSGEMM_CHAINED_KERNEL_ENTRY();
+  // (the pass behind comes when this one is through: see grouped_few_rows.cu)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const Segments all(a);
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWarps;

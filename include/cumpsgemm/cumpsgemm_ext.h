@@ -150,6 +150,8 @@ int cuMpSGEMM_get_last_tile(cuMpSGEMM_handle_t handle, int *rows, int *cols);
  * the time the wait took.  The context stays usable; nothing faults. */
 int cuMpSGEMM_selftest_bounded_wait(cuMpSGEMM_handle_t handle, unsigned limit_ms,
                                     double *waited_ms);
+/* The device the handle was created on; -1 without a handle. */
+int cuMpSGEMM_get_device(cuMpSGEMM_handle_t handle);
 /* Cap (bytes) for the workspace a call may use at once: the panels of a strided batch beyond it are
  * (with the sums of K slices, where the pre-split route cuts K) are processed in chunks of at least
  * one matrix, and sums of K pieces that would take a call beyond a limit it otherwise keeps are left
@@ -359,7 +361,8 @@ cublasStatus_t cuMpSGEMM_sgemm_static_scratch(
  *     multiplies with error correction as the other calls do: CUMPSGEMM_FP16TCEC, or
  *     CUMPSGEMM_FP16TCEC_SCALING, which first brings the largest finite magnitude of each operand (of its
  *     rows in groups) to 2^14.  Other modes return CUBLAS_STATUS_NOT_SUPPORTED; 16-bit types do not look
- *     at it.
+ *     at it.  cuMpSGEMM_grouped_gemm multiplies FP32 operands with at most 6 rows for each group on average
+ *     in plain FP32 arithmetic, which reads the weights once.
  *   Any leading dimension, stride and alignment.  FP32 operands, and 8- and 16-bit ones whose address,
  *     leading dimension or stride is not a multiple of 16 bytes, go through the handle's workspace
  *     (CUBLAS_STATUS_ALLOC_FAILED where it cannot hold them).

@@ -4,6 +4,7 @@ import pytest
 
 def test_null_handle_is_refused(clib):
     one = 1
+    assert clib.cuMpSGEMM_get_device(None) == -1
     assert clib.cuMpSGEMM_grouped_gemm(None, 0, 1, 1, 1, one, None, None, None, 1, None, 1, 0, None, None, 1,
                                        0, 1) == 1
     assert clib.cuMpSGEMM_grouped_gemm_wgrad(None, 0, 1, 1, 1, one, None, None, None, 1, None, 1, None, None,

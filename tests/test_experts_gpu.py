@@ -7,6 +7,8 @@ Tolerances, element by element, with S = sum |x| |w| over the terms of that elem
 * FP32: an operand is hi + lo / 2^11 to 2^-22 of itself (2^-36 where lo is subnormal), lo * lo is left
   out: 3 * 2^-22 S.  Eight additions of the tensor core between drains, 9 * 2^-22 S; FP32 additions of the
   drained sums and the corrections, (k / 512 + 1) * 2^-22 S.
+  (Few rows are multiplied in FP32 arithmetic, k roundings of at most 2^-24 S, which with the random signs
+  here come to their square root: they are held to the same bound.)
 * 8 bits: the sums are exact; three FP32 roundings for conversion and scales, one for the bias, one
   for the result.
 """
@@ -200,8 +202,10 @@ def test_totals_are_not_trusted(handle):
     assert torch.equal(experts.grouped_matmul_wgrad(handle, x, dy, bad),
                        experts.grouped_matmul_wgrad(handle, x, dy, good))
     f = lambda t: t.float()  # noqa: E731
-    assert torch.equal(experts.grouped_matmul(handle, f(x), f(w), bad),
-                       experts.grouped_matmul(handle, f(x), f(w), good))
+    for xf in (f(x), f(x)[:30]):  # on the tensor core, and in FP32 arithmetic
+        good30 = good.clamp(max=xf.shape[0])
+        assert torch.equal(experts.grouped_matmul(handle, xf, f(w), bad),
+                           experts.grouped_matmul(handle, xf, f(w), good30))
 
 
 def test_no_rows_at_all(handle):
@@ -490,8 +494,8 @@ def test_refusals(handle):
     assert handle.quantize_rows_i8(8, 16, x, 16, api.CUDA_R_16BF, None, 7, y, 16, y,
                                    check=False) == api.CUBLAS_STATUS_INVALID_VALUE
     handle.set_workspace_limit(1 << 10)
-    with pytest.raises(api.CuMpSGEMMError) as e:
-        experts.grouped_matmul(handle, *f, ends)
+    with pytest.raises(api.CuMpSGEMMError) as e:  # (few rows need none)
+        experts.grouped_matmul(handle, torch.zeros(80, 16, device="cuda"), f[1], ends)
     assert e.value.status == api.CUBLAS_STATUS_ALLOC_FAILED
     handle.set_workspace_limit(0)
     # results are allocated on the current stream and written on the handle's
@@ -539,3 +543,33 @@ def test_few_tiles_with_a_long_integer_sum(handle):
     one = torch.ones(n, device="cuda")
     y = experts.i8_matmul(handle, xq, one[:rows], wq, one, out_dtype=torch.float32)
     assert torch.equal(y.double(), (xq.double() @ wq.double().t()).float().double())
+
+
+@pytest.mark.parametrize("transpose_w", [False, True])
+@pytest.mark.parametrize("counts", [[1], [6], [2, 0, 3, 1], [0] * 20 + [60, 1, 0, 9, 8, 7, 17], [1] * 40])
+@pytest.mark.parametrize("n,k,pad,offset", [(1, 1, 0, 0), (130, 4100, 0, 0), (300, 70, 3, 1), (1024, 2048, 0, 0)])
+def test_fp32_with_few_rows(handle, transpose_w, counts, n, k, pad, offset):
+    """At most six rows for each group on average: FP32 arithmetic, k + 16 roundings of at most 2^-24 S."""
+    torch, api, experts = _setup()
+    rows, e = sum(counts) + (1 if len(counts) > 3 else 0), len(counts)
+    assert rows <= 6 * e
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    x0 = torch.randn(rows, k, generator=g, device="cuda") * 1e-6
+    w0 = torch.randn(e, *((n, k) if transpose_w else (k, n)), generator=g, device="cuda") * 1e6
+    y0 = torch.randn(rows, n, generator=g, device="cuda")
+    for i, c in enumerate(counts):  # weights of experts without rows never count
+        if c == 0:
+            w0[i] = float("nan")
+    x0[sum(counts):] = float("nan")  # nor do rows of no expert
+    x, w = _matrix(torch, x0, k + pad, offset), _matrix(torch, w0, w0.shape[2] + pad, offset)
+    y = _matrix(torch, y0, n + pad, offset)
+    ends = _ends(torch, counts)
+    want, size, _ = _product(torch, x0, w0, counts, transpose_w)
+    for mode in (api.ComputeMode.FP16TCEC, api.ComputeMode.FP16TCEC_SCALING):
+        got = experts.grouped_matmul(handle, x, w, ends, transpose_w, mode=mode)
+        _close(got, want, (k + 16) * 2.0 ** -24 * size)
+        assert (got[sum(counts):] == 0).all()
+        assert torch.equal(got, experts.grouped_matmul(handle, x, w, ends, transpose_w, mode=mode))
+    experts.grouped_matmul(handle, x, w, ends, transpose_w, alpha=-2.0, beta=0.5, out=y)
+    want = -2.0 * want + 0.5 * y0.double()
+    _close(y, want, (k + 18) * 2.0 ** -24 * (2.0 * size + 0.5 * y0.double().abs()))
