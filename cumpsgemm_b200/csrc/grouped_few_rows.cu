@@ -5,9 +5,11 @@
 // do.  The tensor-core kernel (grouped_gemm.cu) wants them split first: read, written and read again, and
 // with FP16TCEC_SCALING read once more.  Here each is read once, at any address, and multiplied with up to 8
 // rows; more rows of a group pass over its weights again.  Weights of 16 experts, 2048 x 4096, which
-// memory delivers in 82 us: 1 / 4 / 8 rows for each take 104 / 115 / 145 us stored k by n and 115 / 142 / 192
-// stored n by k, and the tensor-core kernel 265, with scaling 350; 8 experts of 512 x 512, 4 rows each, 5.2
-// and 8.7 us against 14 and 21.  (16 rows at a time spilled: 273 and 589 us.)
+// memory delivers in 82 us: 1 / 4 / 6 rows for each take 119 / 146 / 183 us stored k by n and 115 / 142 / 179
+// stored n by k, and the tensor-core kernel 265, with scaling 350; one row, 4096 x 4096, 14 and 11 us against
+// 44 and 60; 8 experts of 512 x 512, 4 rows each, 5.3 against 14 and 21.  What bounds it: with one row
+// memory, with more the loads of x from shared memory, one for every four weights and row.  (16 rows at
+// a time spilled: 273 and 589 us.)
 //
 // op N (weights stored k by n): lanes side by side along n, the warps of a block share k and add their sums
 // in shared memory, in the order of the warps.  op T (n by k): lanes side by side along k, a warp has
