@@ -1053,8 +1053,12 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   // (any address does for an operand without rows; this one is 16-byte aligned)
   const void *fallback = a.dev_status;
   if (!operand_map(&map_a, a.a, ES, fallback, Cfg<KIND>::K_ELEMS, A_LANES ? 64 : BM_CTA) ||
-      !operand_map(&map_b, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, WGRAD ? 64 : BM_CTA) ||
       !operand_map(&map_b_few, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, WGRAD ? 64 : FEW_ROWS))
+    return cudaErrorInvalidValue;
+  // boxes of 128 rows are for tiles of more than 192
+  map_b = map_b_few;
+  if (!WGRAD && a.rows > 2 * (128 - FEW_ROWS) &&
+      !operand_map(&map_b, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, BM_CTA))
     return cudaErrorInvalidValue;
   GroupedParams p = {};
   p.ends = a.ends;

@@ -104,6 +104,11 @@ def _check(handle, device: int, others, group_ends, groups: int) -> None:
         raise ValueError(f"{group_ends.shape[0]} group_ends for {groups} experts")
 
 
+def _check_scales(t, what: str, count: int) -> None:
+    if t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous():
+        raise ValueError(f"{what} must be {count} contiguous float32 values")
+
+
 def _output(out, beta, shape, dtype, like):
     if out is None:
         if beta != 0.0:
@@ -204,14 +209,14 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
         wq = wq.unsqueeze(0)
     groups, n, k, ldw, stridew = _matrices_of(wq, "wq")
     rows, _, ldx = _rows_of(xq, "xq", k)
-    _check(handle, xq.get_device(),
-           (x_scale, wq, w_scale) if bias is None else (x_scale, wq, w_scale, bias), group_ends, groups)
+    others = (x_scale, wq, w_scale) if bias is None else (x_scale, wq, w_scale, bias)
+    _check(handle, xq.get_device(), others, group_ends, groups)
     if xq.dtype is not torch.int8 or wq.dtype is not torch.int8:
         raise ValueError(f"xq is {xq.dtype}, wq is {wq.dtype}: both must be int8")
-    for t, what, count in ((x_scale, "x_scale", rows), (w_scale, "w_scale", groups * n),
-                           (bias, "bias", groups * n)):
-        if t is not None and (t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous()):
-            raise ValueError(f"{what} must be {count} contiguous float32 values")
+    _check_scales(x_scale, "x_scale", rows)
+    _check_scales(w_scale, "w_scale", groups * n)
+    if bias is not None:
+        _check_scales(bias, "bias", groups * n)
     ldy = n
     if out is not None:
         out_dtype = out.dtype
