@@ -573,3 +573,17 @@ def test_fp32_with_few_rows(handle, transpose_w, counts, n, k, pad, offset):
     experts.grouped_matmul(handle, x, w, ends, transpose_w, alpha=-2.0, beta=0.5, out=y)
     want = -2.0 * want + 0.5 * y0.double()
     _close(y, want, (k + 18) * 2.0 ** -24 * (2.0 * size + 0.5 * y0.double().abs()))
+
+
+def test_a_wait_that_gave_up_leaves_the_handle_usable(handle):
+    """The status word raised (by the self-test's wait, which runs out): clearing it clears what the grouped
+    kernel counts with, and the next products are right."""
+    torch, api, experts = _setup()
+    x = torch.randn(90, 64, device="cuda").to(torch.bfloat16)
+    w = torch.randn(3, 64, 40, device="cuda").to(torch.bfloat16)
+    ends = _ends(torch, [30, 0, 60])
+    first = experts.grouped_matmul(handle, x, w, ends)
+    status, _ = handle.selftest_bounded_wait(50)
+    assert status != 0
+    assert torch.equal(first, experts.grouped_matmul(handle, x, w, ends))
+    assert handle.kernel_status() == 0
