@@ -231,9 +231,15 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
 
 
 def _dense_rows(t):
-    return t if t.stride(-1) == 1 and t.stride(-2) >= t.shape[-1] else t.contiguous()
+    """t, copied where its rows, or its matrices, do not lie one behind the other."""
+    rows, cols = t.shape[-2:]
+    dense = t.stride(-1) == 1 and t.stride(-2) >= cols and (
+        t.dim() < 3 or t.stride(-3) >= (rows - 1) * t.stride(-2) + cols)
+    return t if dense else t.contiguous()
 
 
+# The gradients of either product are products of the same two kinds, so each backward pass is made of these
+# functions again and can itself be differentiated, any number of times.
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, group_ends, handle, transpose_w, mode):
@@ -248,14 +254,49 @@ class _GroupedLinear(torch.autograd.Function):
         dy = _dense_rows(dy)  # the gradient of a sum, say, is one value for all of them
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = grouped_matmul(handle, dy, w, group_ends, not transpose_w, mode=mode)
+            dx = _linear(dy, w, group_ends, handle, not transpose_w, mode)
         if ctx.needs_input_grad[1]:
-            dw = grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode)
+            dw = _weight_gradient(x, dy, group_ends, handle, transpose_w, mode)
         return dx, dw, None, None, None, None
+
+
+class _WeightGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dy, group_ends, handle, transpose_w, mode):
+        ctx.save_for_backward(x, dy, group_ends)
+        ctx.how = (handle, transpose_w, mode)
+        return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode)
+
+    @staticmethod
+    def backward(ctx, v):
+        # dw_e = x_e^T dy_e: the gradient of x is dy v_e^T, that of dy is x v_e
+        x, dy, group_ends = ctx.saved_tensors
+        handle, transpose_w, mode = ctx.how
+        v = _dense_rows(v)
+        gx = gdy = None
+        if ctx.needs_input_grad[0]:
+            gx = _linear(dy, v, group_ends, handle, not transpose_w, mode)
+        if ctx.needs_input_grad[1]:
+            gdy = _linear(x, v, group_ends, handle, transpose_w, mode)
+        return gx, gdy, None, None, None, None
+
+
+# What backward passes are made of: without a graph to leave, which is the usual case, the products
+# themselves (10 us each shorter).
+def _linear(x, w, group_ends, handle, transpose_w, mode):
+    if torch.is_grad_enabled():
+        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode)
+    return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode)
+
+
+def _weight_gradient(x, dy, group_ends, handle, transpose_w, mode):
+    if torch.is_grad_enabled():
+        return _WeightGradient.apply(x, dy, group_ends, handle, transpose_w, mode)
+    return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode)
 
 
 def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool = False, *,
                    mode: int = api.ComputeMode.FP16TCEC):
-    """``grouped_matmul`` with a backward pass: gradients of x and w.  Autograd runs the backward pass on the
-    stream of the forward pass."""
+    """``grouped_matmul`` with a backward pass: gradients of x and w, which have gradients in turn
+    (``create_graph=True``).  Autograd runs the backward pass on the stream of the forward pass."""
     return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode)

@@ -1,0 +1,58 @@
+"""The grouped products under autograd, on the kernels: against the same expression in 64 bits."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+COUNTS = [30, 0, 77, 1]
+SPARE = 5  # rows of no expert
+
+
+def _case(dtype, transpose_w, n=64, k=96):
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from cumpsgemm_b200 import experts
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(sum(COUNTS) + SPARE, k, generator=g, device="cuda").to(dtype).requires_grad_()
+    shape = (n, k) if transpose_w else (k, n)
+    w = torch.randn(len(COUNTS), *shape, generator=g, device="cuda").to(dtype).requires_grad_()
+    return torch, experts, x, w, torch.tensor(COUNTS).cumsum(0).to(torch.int32).cuda()
+
+
+def _in_64_bits(torch, x, w, transpose_w):
+    """(x, w, y): copies in 64 bits and the product of them as autograd knows it."""
+    x, w = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    parts, at = [], 0
+    for e, c in enumerate(COUNTS):
+        parts.append(x[at:at + c] @ (w[e].t() if transpose_w else w[e]))
+        at += c
+    parts.append(x.new_zeros(x.shape[0] - at, parts[0].shape[1]))
+    return x, w, torch.cat(parts)
+
+
+def _near(got, want, limit):
+    off = (got.double() - want).norm() / want.norm()
+    assert off <= limit, float(off)
+
+
+@pytest.mark.parametrize("dtype,limit", [("float32", 2.0 ** -12), ("bfloat16", 0.1)])
+@pytest.mark.parametrize("transpose_w", [False, True])
+def test_a_penalty_on_the_gradients(handle, dtype, limit, transpose_w):
+    """Three products in a row.  FP32: 14 * 2^-22 of the sum of magnitudes for each, which in norm is at most 16
+    times the sum here.  bfloat16: six roundings of 2^-9, terms cancelling by no more than a factor of 8."""
+    import torch
+
+    _, experts, x, w, ends = _case(getattr(torch, dtype), transpose_w)
+    y = experts.grouped_linear(handle, x, w, ends, transpose_w)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w), create_graph=True)
+    # (the sum over the experts sends each of them one and the same matrix)
+    loss = dx.float().square().sum() + dw.float().square().sum() + dw.float().sum(0).square().sum()
+    got = torch.autograd.grad(loss, (x, w))
+    xd, wd, yd = _in_64_bits(torch, x, w, transpose_w)
+    dx, dw = torch.autograd.grad(yd.sum(), (xd, wd), create_graph=True)
+    want = torch.autograd.grad(dx.square().sum() + dw.square().sum() + dw.sum(0).square().sum(), (xd, wd))
+    _near(got[0], want[0], limit)
+    _near(got[1], want[1], limit)
+    assert (got[0][sum(COUNTS):] == 0).all() and (got[1][1] == 0).all()
