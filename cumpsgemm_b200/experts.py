@@ -242,9 +242,9 @@ def _dense_rows(t):
 # functions again and can itself be differentiated, any number of times.
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, group_ends, handle, transpose_w, mode):
+    def forward(ctx, x, w, group_ends, handle, transpose_w, mode, backward_mode):
         ctx.save_for_backward(x, w, group_ends)
-        ctx.how = (handle, transpose_w, mode)
+        ctx.how = (handle, transpose_w, backward_mode)
         return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode)
 
     @staticmethod
@@ -257,7 +257,7 @@ class _GroupedLinear(torch.autograd.Function):
             dx = _linear(dy, w, group_ends, handle, not transpose_w, mode)
         if ctx.needs_input_grad[1]:
             dw = _weight_gradient(x, dy, group_ends, handle, transpose_w, mode)
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 class _WeightGradient(torch.autograd.Function):
@@ -285,7 +285,7 @@ class _WeightGradient(torch.autograd.Function):
 # themselves (10 us each shorter).
 def _linear(x, w, group_ends, handle, transpose_w, mode):
     if torch.is_grad_enabled():
-        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode)
+        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode, mode)
     return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode)
 
 
@@ -296,7 +296,13 @@ def _weight_gradient(x, dy, group_ends, handle, transpose_w, mode):
 
 
 def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool = False, *,
-                   mode: int = api.ComputeMode.FP16TCEC):
+                   mode: int = api.ComputeMode.FP16TCEC,
+                   backward_mode: int = api.ComputeMode.FP16TCEC_SCALING):
     """``grouped_matmul`` with a backward pass: gradients of x and w, which have gradients in turn
-    (``create_graph=True``).  Autograd runs the backward pass on the stream of the forward pass."""
-    return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode)
+    (``create_graph=True``).  Autograd runs the backward pass on the stream of the forward pass.
+
+    ``mode`` multiplies FP32 operands of the forward pass, ``backward_mode`` those of the backward pass.
+    FP16TCEC knows an element to 2^-36 and none above 65504: enough for activations and weights of order one,
+    not for gradients, which FP16TCEC_SCALING takes at any magnitude.  16-bit operands look at neither."""
+    return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode,
+                                backward_mode)

@@ -85,3 +85,20 @@ def test_a_gradient_that_is_one_value_for_several_experts(experts):
     want = torch.autograd.grad((dw.sum(0) ** 2).sum(), (xd, wd))
     for g, e in zip(got, want):
         assert torch.allclose(g, e, rtol=1e-10, atol=1e-10)
+
+
+def test_gradients_are_multiplied_at_any_magnitude(experts):
+    """Each product of a backward pass, of a second one too, has its operands scaled; the forward pass does not."""
+    from cumpsgemm_b200.api import ComputeMode
+
+    module, calls = experts
+    x, w, ends = _operands(False)
+    y = module.grouped_linear(None, x, w, ends)
+    assert calls == [("matmul", ComputeMode.FP16TCEC)]
+    dx, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    dx.square().sum().backward()
+    assert len(calls) > 4 and all(mode == ComputeMode.FP16TCEC_SCALING for _, mode in calls[1:])
+    del calls[:]
+    module.grouped_linear(None, x, w, ends, mode=ComputeMode.FP16TCEC_SCALING,
+                          backward_mode=ComputeMode.FP16TCEC).sum().backward()
+    assert [mode for _, mode in calls] == [ComputeMode.FP16TCEC_SCALING] + 2 * [ComputeMode.FP16TCEC]

@@ -56,3 +56,35 @@ def test_a_penalty_on_the_gradients(handle, dtype, limit, transpose_w):
     _near(got[0], want[0], limit)
     _near(got[1], want[1], limit)
     assert (got[0][sum(COUNTS):] == 0).all() and (got[1][1] == 0).all()
+
+
+@pytest.mark.parametrize("magnitude", [1.0, 1e-6, 1e-9, 1e-20, 1e8])
+@pytest.mark.parametrize("counts", [COUNTS, [300, 0, 5, 40]])
+@pytest.mark.parametrize("transpose_w", [False, True])
+def test_fp32_gradients_of_any_magnitude(handle, magnitude, counts, transpose_w):
+    """Operands scaled by their largest element: each is hi + lo to 2^-22 of itself or 2^-50 of the largest.
+    Sums as in test_experts_gpu.py, (12 + terms / 512 + 1) * 2^-22 of the sum of magnitudes."""
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from cumpsgemm_b200 import experts
+
+    n, k, rows = 64, 96, sum(counts) + SPARE
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(rows, k, generator=g, device="cuda").requires_grad_()
+    w = torch.randn(len(counts), *((n, k) if transpose_w else (k, n)), generator=g, device="cuda").requires_grad_()
+    dy = torch.randn(rows, n, generator=g, device="cuda") * magnitude
+    ends = torch.tensor(counts).cumsum(0).to(torch.int32).cuda()
+    experts.grouped_linear(handle, x, w, ends, transpose_w).backward(dy)
+    xd, wd, dyd = x.detach().double(), w.detach().double(), dy.double()
+    at = 0
+    for e, c in enumerate(counts):
+        r, we = slice(at, at + c), wd[e] if transpose_w else wd[e].t()  # n x k
+        at += c
+        for got, a, b in ((x.grad[r], dyd[r], we),
+                          (w.grad[e] if transpose_w else w.grad[e].t(), dyd[r].t(), xd[r])):
+            terms = a.shape[1]
+            tol = (12 + terms / 512 + 1) * 2.0 ** -22 * (a.abs() @ b.abs())
+            tol = tol + 2.0 ** -50 * terms * float(dyd.abs().max()) * float(max(xd.abs().max(), wd.abs().max()))
+            assert ((got.double() - a @ b).abs() <= tol).all()
