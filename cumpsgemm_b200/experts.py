@@ -119,6 +119,16 @@ def _output(out, beta, shape, dtype, like):
     return out
 
 
+_BACKWARD_MODE = api.ComputeMode.FP16TCEC_SCALING  # FP32 gradients may have any magnitude
+
+
+def _no_graph_through(out, beta) -> None:
+    if out is not None:
+        raise ValueError("an operand requires a gradient, and what is written to out has none: use torch.no_grad()")
+    if beta != 0.0:
+        raise ValueError("beta needs an out to read")
+
+
 def grouped_matmul(handle: api.Handle, x, w, group_ends=None, transpose_w: bool = False, *,
                    mode: int = api.ComputeMode.FP16TCEC, alpha: float = 1.0, beta: float = 0.0,
                    out=None):
@@ -126,8 +136,12 @@ def grouped_matmul(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
 
     x is (rows, k), w (experts, k, n), or (experts, n, k) with ``transpose_w``; all of float16, bfloat16
     or float32, which ``mode`` multiplies (FP16TCEC or FP16TCEC_SCALING).  The gradient of x is
-    ``grouped_matmul(handle, dy, w, group_ends, not transpose_w)``.
+    ``grouped_matmul(handle, dy, w, group_ends, not transpose_w)``; autograd's where x or w requires one,
+    as with ``grouped_linear`` (without ``out``).
     """
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        _no_graph_through(out, beta)
+        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode, _BACKWARD_MODE, alpha)
     groups, w_rows, w_cols, ldw, stridew = _matrices_of(w, "w")
     k, n = (w_cols, w_rows) if transpose_w else (w_rows, w_cols)
     rows, _, ldx = _rows_of(x, "x", k)
@@ -150,7 +164,11 @@ def grouped_matmul_wgrad(handle: api.Handle, x, dy, group_ends=None, transpose_w
                          mode: int = api.ComputeMode.FP16TCEC, alpha: float = 1.0, beta: float = 0.0,
                          out=None):
     """``out[e] = alpha * x_e^T @ dy_e + beta * out[e]`` over the rows of each expert e, (experts, k, n);
-    its transpose, (experts, n, k), with ``transpose_w``.  Experts without rows: ``beta * out[e]``."""
+    its transpose, (experts, n, k), with ``transpose_w``.  Experts without rows: ``beta * out[e]``.  Has
+    gradients as ``grouped_matmul`` does."""
+    if torch.is_grad_enabled() and (x.requires_grad or dy.requires_grad):
+        _no_graph_through(out, beta)
+        return _WeightGradient.apply(x, dy, group_ends, handle, transpose_w, mode, _BACKWARD_MODE, alpha)
     rows, k, ldx = _rows_of(x, "x")
     dy_rows, n, lddy = _rows_of(dy, "dy")
     if dy_rows != rows:
@@ -242,62 +260,62 @@ def _dense_rows(t):
 # functions again and can itself be differentiated, any number of times.
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, group_ends, handle, transpose_w, mode, backward_mode):
+    def forward(ctx, x, w, group_ends, handle, transpose_w, mode, backward_mode, alpha):
         ctx.save_for_backward(x, w, group_ends)
-        ctx.how = (handle, transpose_w, backward_mode)
-        return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode)
+        ctx.how = (handle, transpose_w, backward_mode, alpha)
+        return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode, alpha=alpha)
 
     @staticmethod
     def backward(ctx, dy):
         x, w, group_ends = ctx.saved_tensors
-        handle, transpose_w, mode = ctx.how
+        handle, transpose_w, mode, alpha = ctx.how
         dy = _dense_rows(dy)  # the gradient of a sum, say, is one value for all of them
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = _linear(dy, w, group_ends, handle, not transpose_w, mode)
+            dx = _linear(dy, w, group_ends, handle, not transpose_w, mode, alpha)
         if ctx.needs_input_grad[1]:
-            dw = _weight_gradient(x, dy, group_ends, handle, transpose_w, mode)
-        return dx, dw, None, None, None, None, None
+            dw = _weight_gradient(x, dy, group_ends, handle, transpose_w, mode, alpha)
+        return dx, dw, None, None, None, None, None, None
 
 
 class _WeightGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dy, group_ends, handle, transpose_w, mode):
+    def forward(ctx, x, dy, group_ends, handle, transpose_w, mode, backward_mode, alpha):
         ctx.save_for_backward(x, dy, group_ends)
-        ctx.how = (handle, transpose_w, mode)
-        return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode)
+        ctx.how = (handle, transpose_w, backward_mode, alpha)
+        return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode, alpha=alpha)
 
     @staticmethod
     def backward(ctx, v):
         # dw_e = x_e^T dy_e: the gradient of x is dy v_e^T, that of dy is x v_e
         x, dy, group_ends = ctx.saved_tensors
-        handle, transpose_w, mode = ctx.how
+        handle, transpose_w, mode, alpha = ctx.how
         v = _dense_rows(v)
         gx = gdy = None
         if ctx.needs_input_grad[0]:
-            gx = _linear(dy, v, group_ends, handle, not transpose_w, mode)
+            gx = _linear(dy, v, group_ends, handle, not transpose_w, mode, alpha)
         if ctx.needs_input_grad[1]:
-            gdy = _linear(x, v, group_ends, handle, transpose_w, mode)
-        return gx, gdy, None, None, None, None
+            gdy = _linear(x, v, group_ends, handle, transpose_w, mode, alpha)
+        return gx, gdy, None, None, None, None, None, None
 
 
 # What backward passes are made of: without a graph to leave, which is the usual case, the products
 # themselves (10 us each shorter).
-def _linear(x, w, group_ends, handle, transpose_w, mode):
+def _linear(x, w, group_ends, handle, transpose_w, mode, alpha):
     if torch.is_grad_enabled():
-        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode, mode)
-    return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode)
+        return _GroupedLinear.apply(x, w, group_ends, handle, transpose_w, mode, mode, alpha)
+    return grouped_matmul(handle, x, w, group_ends, transpose_w, mode=mode, alpha=alpha)
 
 
-def _weight_gradient(x, dy, group_ends, handle, transpose_w, mode):
+def _weight_gradient(x, dy, group_ends, handle, transpose_w, mode, alpha):
     if torch.is_grad_enabled():
-        return _WeightGradient.apply(x, dy, group_ends, handle, transpose_w, mode)
-    return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode)
+        return _WeightGradient.apply(x, dy, group_ends, handle, transpose_w, mode, mode, alpha)
+    return grouped_matmul_wgrad(handle, x, dy, group_ends, transpose_w, mode=mode, alpha=alpha)
 
 
 def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool = False, *,
                    mode: int = api.ComputeMode.FP16TCEC,
-                   backward_mode: int = api.ComputeMode.FP16TCEC_SCALING):
+                   backward_mode: int = _BACKWARD_MODE):
     """``grouped_matmul`` with a backward pass: gradients of x and w, which have gradients in turn
     (``create_graph=True``).  Autograd runs the backward pass on the stream of the forward pass.
 
@@ -305,4 +323,4 @@ def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
     FP16TCEC knows an element to 2^-36 and none above 65504: enough for activations and weights of order one,
     not for gradients, which FP16TCEC_SCALING takes at any magnitude.  16-bit operands look at neither."""
     return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode,
-                                backward_mode)
+                                backward_mode, 1.0)

@@ -88,3 +88,29 @@ def test_fp32_gradients_of_any_magnitude(handle, magnitude, counts, transpose_w)
             tol = (12 + terms / 512 + 1) * 2.0 ** -22 * (a.abs() @ b.abs())
             tol = tol + 2.0 ** -50 * terms * float(dyd.abs().max()) * float(max(xd.abs().max(), wd.abs().max()))
             assert ((got.double() - a @ b).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("transpose_w", [False, True])
+def test_the_products_themselves_have_gradients(handle, transpose_w):
+    """grouped_matmul and grouped_matmul_wgrad of tensors that require gradients, alpha included; a result in
+    `out` has none to give and is refused.  Bounds as in the first test."""
+    import torch
+
+    _, experts, x, w, ends = _case(torch.float32, transpose_w)
+    y = experts.grouped_matmul(handle, x, w, ends, transpose_w, alpha=-0.5)
+    dw = experts.grouped_matmul_wgrad(handle, x, y, ends, transpose_w, alpha=3.0)  # x_e^T y_e
+    got = torch.autograd.grad(dw.sum() + y.square().sum(), (x, w))
+    xd, wd, yd = _in_64_bits(torch, x, w, transpose_w)
+    yd, at, total = -0.5 * yd, 0, 0.0
+    for c in COUNTS:
+        total = total + 3.0 * (xd[at:at + c].t() @ yd[at:at + c]).sum()
+        at += c
+    want = torch.autograd.grad(total + yd.square().sum(), (xd, wd))
+    _near(got[0], want[0], 2.0 ** -12)
+    _near(got[1], want[1], 2.0 ** -12)
+    with pytest.raises(ValueError, match="no_grad"):
+        experts.grouped_matmul(handle, x, w, ends, transpose_w, out=y.detach())
+    with pytest.raises(ValueError, match="no_grad"):
+        experts.grouped_matmul_wgrad(handle, x, y, ends, transpose_w, out=dw.detach())
+    with torch.no_grad():
+        assert not experts.grouped_matmul(handle, x, w, ends, transpose_w, out=y.detach()).requires_grad
