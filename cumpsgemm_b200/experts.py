@@ -116,6 +116,9 @@ def _output(out, beta, shape, dtype, like):
         return like.new_empty(shape, dtype=dtype)
     if tuple(out.shape) != shape or out.dtype is not dtype or out.get_device() != like.get_device():
         raise ValueError(f"out must be {dtype} of shape {shape} on {like.device}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out requires a gradient, which what is written to it has not: use torch.no_grad()")
+    torch.autograd.graph.increment_version(out)  # a backward pass that needs what stood there says so
     return out
 
 

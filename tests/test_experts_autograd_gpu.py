@@ -114,3 +114,27 @@ def test_the_products_themselves_have_gradients(handle, transpose_w):
         experts.grouped_matmul_wgrad(handle, x, y, ends, transpose_w, out=dw.detach())
     with torch.no_grad():
         assert not experts.grouped_matmul(handle, x, w, ends, transpose_w, out=y.detach()).requires_grad
+
+
+def test_a_result_in_out_is_seen_by_autograd(handle):
+    """What a graph has kept and a product overwrites is refused by the backward pass, not used."""
+    import torch
+
+    _, experts, x, w, ends = _case(torch.bfloat16, False)
+    x, w = x.detach(), w.detach()
+    xq, sx = experts.quantize_rows(handle, x)
+    wq, sw = experts.quantize_rows(handle, w.transpose(1, 2).reshape(-1, w.shape[1]))
+    wq = wq.unflatten(0, (len(COUNTS), w.shape[2]))
+    y, dw = x.new_zeros(x.shape[0], w.shape[2]), torch.zeros_like(w)
+    for out, call in ((y, lambda out: experts.grouped_matmul(handle, x, w, ends, out=out)),
+                      (dw, lambda out: experts.grouped_matmul_wgrad(handle, x, y, ends, out=out)),
+                      (y, lambda out: experts.i8_matmul(handle, xq, sx, wq, sw, ends, out=out))):
+        factor = torch.ones_like(out, requires_grad=True)
+        loss = (factor * out).sum()
+        call(out)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        with pytest.raises(ValueError, match="no_grad"):
+            call(factor)
+        with torch.no_grad():
+            call(factor)
