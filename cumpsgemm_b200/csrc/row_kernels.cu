@@ -344,11 +344,14 @@ __global__ void __launch_bounds__(kThreads) stage_kernel(const StageArgs a) {
 }
 
 // ---------------------------------------------------------------- rows to 8 bits
-// top = max_i |x_i|, scale = top / 127, q_i = rint(x_i * (127 / top)), the product not rounded in between:
-// |x_i| / top <= 1, so q_i stays within +-127, and an element is off by at most half a step of
-// top / 127.  A row of zeros has scale 0.  A row with an infinity or NaN has no scale: its scale is NaN,
-// its q_i are 0, and so every product with it is NaN.  Rows too small for 127 / top (below 2^-100) are
-// multiplied by 2^100 first.  A row whose index lies outside x reads as zeros.
+// top = max_i |x_i|, scale = top / 127, q_i = rint(x_i * (127 / top)), where 127 / top and the product are
+// rounded to FP32 first: |x_i| / top <= 1, so q_i stays within +-127, and an element is off by at most
+// half a step of top / 127 (and 2^-16 of one, by those roundings).  The product is not fused with the
+// addition that rounds it to an integer: halves are common (x_i = top / 2 in 16 bits), and unrounded such a
+// product goes the way of the error of 127 / top instead of to the even neighbour.  A row of zeros has scale
+// 0.  A row with an infinity or NaN has no scale: its scale is NaN, its q_i are 0, and so every product with
+// it is NaN.  Rows too small for 127 / top (below 2^-100) are multiplied by 2^100 first.  A row whose index
+// lies outside x reads as zeros.
 struct RowScale {
   float up, inverse, scale;
   bool none; // no scale
@@ -369,8 +372,8 @@ struct RowScale {
   __device__ __forceinline__ uint32_t four(float x, float y, float z, float w) const {
     if (up != 1.f) x *= up, y *= up, z *= up, w *= up;
     const float m = 12582912.f;
-    const uint32_t a = __float_as_uint(fmaf(x, inverse, m)), b = __float_as_uint(fmaf(y, inverse, m)),
-                   c = __float_as_uint(fmaf(z, inverse, m)), d = __float_as_uint(fmaf(w, inverse, m));
+    auto rounded = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inverse), m)); };
+    const uint32_t a = rounded(x), b = rounded(y), c = rounded(z), d = rounded(w);
     const uint32_t q = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     return none ? 0u : q;
   }
