@@ -350,8 +350,9 @@ __global__ void __launch_bounds__(kThreads) stage_kernel(const StageArgs a) {
 // addition that rounds it to an integer: halves are common (x_i = top / 2 in 16 bits), and unrounded such a
 // product goes the way of the error of 127 / top instead of to the even neighbour.  A row of zeros has scale
 // 0.  A row with an infinity or NaN has no scale: its scale is NaN, its q_i are 0, and so every product with
-// it is NaN.  Rows too small for 127 / top (below 2^-100) are multiplied by 2^100 first.  A row whose index
-// lies outside x reads as zeros.
+// it is NaN.  Rows too small for 127 / top (below 2^-100) are multiplied by 2^100 first.  Below 127 * 2^-126
+// the scale is subnormal, a multiple of 2^-149, and an element is off by up to another 127 * 2^-150; a row
+// whose scale comes to 0 so is one of zeros.  A row whose index lies outside x reads as zeros.
 struct RowScale {
   float up, inverse, scale;
   bool none; // no scale
@@ -365,7 +366,7 @@ struct RowScale {
     } else if (top > 0.f) {
       scale = __fdiv_rn(top, 127.f);
       if (top < 0x1p-100f) up = 0x1p100f;
-      inverse = __fdiv_rn(127.f, top * up);
+      if (scale > 0.f) inverse = __fdiv_rn(127.f, top * up);
     }
   }
   // Added to 1.5 * 2^23 the product is rounded to an integer, ties to even, whose low byte is the sum's.

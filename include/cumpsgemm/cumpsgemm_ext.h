@@ -399,10 +399,10 @@ cublasStatus_t cuMpSGEMM_i8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t row
                                          const float *w_scale, const float *bias, void *y, uint64_t ldy,
                                          cudaDataType_t y_type);
 /* Rows to 8 bits: with top the largest magnitude of a row, scale = top / 127 and
- * q[i] = rint(x[i] * (127 / top)), each step rounded to FP32, ties to even; a row of zeros has scale 0, a
- * row with an infinity or NaN has scale NaN and q = 0 (its products are NaN).  Row r is taken from row
- * row_index[r] of x (NULL: r); an index outside [0, src_rows) gives a row of zeros.  type: that of x, any of
- * the three. */
+ * q[i] = rint(x[i] * (127 / top)), each step rounded to FP32, ties to even; a row of zeros, or
+ * so small that its scale is 0 in FP32, has scale 0 and q = 0, a row with an infinity or NaN scale NaN and
+ * q = 0 (its products are NaN).  Row r is taken from row row_index[r] of x (NULL: r); an index outside
+ * [0, src_rows) gives a row of zeros.  type: that of x, any of the three. */
 cublasStatus_t cuMpSGEMM_quantize_rows_i8(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t k,
                                           const void *x, uint64_t ldx, cudaDataType_t type,
                                           const int32_t *row_index, uint64_t src_rows, int8_t *q,

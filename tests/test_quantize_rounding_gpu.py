@@ -42,3 +42,24 @@ def test_halves_go_to_the_even_neighbour(handle, dtype):
     x = torch.cat([3 * j + 1.5, torch.tensor([381.0], device="cuda")])[None].to(getattr(torch, dtype))
     q, _ = experts.quantize_rows(handle, x)
     assert torch.equal(q[0, :-1].float(), torch.round(j + 0.5)) and q[0, -1] == 127
+
+
+def test_rows_at_the_bottom_of_the_range(handle):
+    """scale * q is the row to half a step, and where the scale is subnormal to 127 / 2 of its smallest unit
+    more.  A row whose scale rounds to zero has zeros."""
+    import torch
+
+    from cumpsgemm_b200 import experts
+
+    tops = [2.0 ** e * f for e in range(-149, -110) for f in (1.0, 1.5)]
+    g = torch.Generator(device="cuda").manual_seed(9)
+    part = torch.rand(len(tops), 300, generator=g, device="cuda") * 2 - 1
+    part[:, 11] = 1
+    x = (part.double() * torch.tensor(tops, dtype=torch.float64, device="cuda")[:, None]).float()
+    q, scale = experts.quantize_rows(handle, x)
+    back = scale.double()[:, None] * q.double()
+    step = x.double().abs().amax(1, keepdim=True) / 127
+    tol = step * (0.5 + 2.0 ** -16) + torch.where(step < 2.0 ** -126, 127 * 2.0 ** -150, 127 * 2.0 ** -24 * step)
+    # (without a scale all that is left is the row itself, of at most 63 * 2^-149)
+    assert ((back - x.double()).abs() <= torch.where(scale[:, None] == 0, x.double().abs(), tol)).all()
+    assert (q[scale == 0] == 0).all() and (scale == 0).any() and (q[scale > 0][:, 11] == 127).all()
