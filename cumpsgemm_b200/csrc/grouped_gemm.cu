@@ -229,10 +229,11 @@ template <int KIND, bool WARP> struct Tiles { // taken by a warp, or by one thre
   }
   __device__ __forceinline__ void take(const Tile &x) {
     using C = Cfg<KIND>;
-    if (WARP) __syncwarp();
-    // the tile has been read when a word of it is compared (no group is ~0)
-    if (x.group != ~0u && (!WARP || (threadIdx.x & 31) == 0))
-      ptx::mbar_arrive_cluster_relaxed(ptx::map_to_cta(sbase + C::NEXT_EMPTY + 8 * turn, 0));
+    // The slot is given back relaxed, so its three reads have to have come in: a word of each is compared (none
+    // of these is ever ~0), by every lane that read.
+    bool has_come = max(max(x.group, x.k0), x.slices) != ~0u;
+    if (WARP) has_come = __all_sync(0xffffffffu, has_come) != 0 && (threadIdx.x & 31) == 0;
+    if (has_come) ptx::mbar_arrive_cluster_relaxed(ptx::map_to_cta(sbase + C::NEXT_EMPTY + 8 * turn, 0));
     if (++turn == AHEAD) {
       turn = 0;
       phase ^= 1u;
@@ -836,7 +837,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       while (more) {
         while (item < items.total && !items.get(p, item, x)) item = clusters + atomicAdd(p.counters, 1u);
         more = item < items.total;
-        if (!more) x.group = x.cols = 0;
+        if (!more) x = Tile{};
         if (!ptx::mbar_wait(sbase + C::NEXT_EMPTY + 8 * turn, ph, abort_flag, p.status, ptx::kErrWaitTile))
           break;
 #pragma unroll
