@@ -87,6 +87,7 @@ PROTOTYPES = {
     "cuMpSGEMM_sgemm_module": (i32, _GEMM_ARGS + [C.POINTER(u32)]),
     "cuMpSGEMM_get_kernel_status": (i32, [vp]),
     "cuMpSGEMM_selftest_bounded_wait": (i32, [vp, u32, C.POINTER(C.c_double)]),
+    "cuMpSGEMM_selftest_grouped_counters": (i32, [vp, C.c_ubyte]),
     "cuMpSGEMM_get_device": (i32, [vp]),
     "cuMpSGEMM_set_workspace_limit": (None, [vp, C.c_size_t]),
     "cuMpSGEMM_set_count_tail_padding": (None, [vp, i32]),

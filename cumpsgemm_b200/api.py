@@ -297,6 +297,11 @@ class Handle:
         st = self._lib.cuMpSGEMM_selftest_bounded_wait(self._h, limit_ms, C.byref(t))
         return st, t.value
 
+    def selftest_grouped_counters(self, byte: int = 0) -> int:
+        """How many of the words that grouped products count with are not zero; then, unless byte is 0, they are
+        filled with it and the status word is raised, as by a kernel that gave up."""
+        return self._lib.cuMpSGEMM_selftest_grouped_counters(self._h, byte)
+
     def set_workspace_limit(self, nbytes: int) -> None:
         self._lib.cuMpSGEMM_set_workspace_limit(self._h, nbytes)
 

@@ -1,5 +1,6 @@
 // extern "C" forwarding layer declared in include/cumpsgemm/cumpsgemm_ext.h.
 #include "internal.hpp"
+#include "ptx.cuh"
 
 #include <cstring>
 #include <cumpsgemm/cumpsgemm_ext.h>
@@ -218,6 +219,33 @@ int cuMpSGEMM_selftest_bounded_wait(cuMpSGEMM_handle_t h, unsigned limit_ms,
   const int status = cuMpSGEMM_get_kernel_status(h); // synchronises and clears
   if (waited_ms) *waited_ms = static_cast<double>(ns) * 1e-6;
   return status;
+}
+
+int cuMpSGEMM_selftest_grouped_counters(cuMpSGEMM_handle_t h, unsigned char byte) {
+  if (h == nullptr) return -1;
+  DeviceGuard guard(h->device);
+  const std::size_t words = grouped_counters(h->num_sms);
+  int raised = 0;
+  for (std::size_t at = 0; at < words;) {
+    unsigned some[256];
+    const std::size_t n = words - at < 256 ? words - at : 256;
+    if (cudaMemcpyAsync(some, h->dev_grouped_counters + at, n * sizeof(unsigned), cudaMemcpyDeviceToHost,
+                        h->cuda_stream) != cudaSuccess ||
+        cudaStreamSynchronize(h->cuda_stream) != cudaSuccess)
+      return -2;
+    for (std::size_t i = 0; i < n; ++i) raised += some[i] != 0;
+    at += n;
+  }
+  if (byte != 0) {
+    const int status = ptx::kErrWaitTile;
+    if (cudaMemsetAsync(h->dev_grouped_counters, byte, words * sizeof(unsigned), h->cuda_stream) !=
+            cudaSuccess ||
+        cudaMemcpyAsync(h->dev_status, &status, sizeof(status), cudaMemcpyHostToDevice, h->cuda_stream) !=
+            cudaSuccess ||
+        cudaStreamSynchronize(h->cuda_stream) != cudaSuccess)
+      return -3;
+  }
+  return raised;
 }
 
 int cuMpSGEMM_get_device(cuMpSGEMM_handle_t h) { return h == nullptr ? -1 : h->device; }

@@ -125,7 +125,10 @@ cublasStatus_t cuMpSGEMM_sgemm_module(
  * code in a device word.  This call synchronises the handle's stream, returns the word and
  * clears it.  0 = no error; 1 = a producer / converter waited for a free stage, 2 = the MMA
  * issuer for operands, 3 / 7 = the MMA issuer for the drain of an accumulator, 4 / 5 = the
- * epilogue for an accumulator, 6 = bad launch, 8 = a role of the grouped products for its next tile. */
+ * epilogue for an accumulator, 6 = bad launch, 8 = a role of the grouped products for its next tile.
+ * The results of a call in which a wait gave up are not valid, nor are those of products of rows grouped by
+ * expert that follow it on the handle before this call has cleared the word (they count with words that such
+ * a kernel leaves behind, and that are set right here). */
 int cuMpSGEMM_get_kernel_status(cuMpSGEMM_handle_t handle);
 /* Which kernels the handle's last GEMM call launched, and in *cut_along_k (nullable) whether any of
  * its tiles was cut along K; host state only, nothing is synchronised.  CUMPSGEMM_ROUTE_NONE: no call
@@ -150,6 +153,12 @@ int cuMpSGEMM_get_last_tile(cuMpSGEMM_handle_t handle, int *rows, int *cols);
  * the time the wait took.  The context stays usable; nothing faults. */
 int cuMpSGEMM_selftest_bounded_wait(cuMpSGEMM_handle_t handle, unsigned limit_ms,
                                     double *waited_ms);
+/* Self-test of what follows a wait that gave up: the words that the products of rows grouped by expert
+ * count tiles and slices with are zero between calls, and a kernel that gave up may leave them otherwise.
+ * Returns how many of them are not zero; then, unless byte is 0, sets every byte of them to it and the
+ * status word to 8, as such a kernel would.  No kernel runs; synchronises the handle's stream.
+ * cuMpSGEMM_get_kernel_status has to bring them back to zero.  Negative: a CUDA error. */
+int cuMpSGEMM_selftest_grouped_counters(cuMpSGEMM_handle_t handle, unsigned char byte);
 /* The device the handle was created on; -1 without a handle. */
 int cuMpSGEMM_get_device(cuMpSGEMM_handle_t handle);
 /* Cap (bytes) for the workspace a call may use at once: the panels of a strided batch beyond it are
