@@ -4,12 +4,15 @@
 // A step of decoding sends a handful of rows to each expert, and reading the weights is all there is to
 // do.  The tensor-core kernel (grouped_gemm.cu) wants them split first: read, written and read again, and
 // with FP16TCEC_SCALING read once more.  Here each is read once, at any address, and multiplied with up to 8
-// rows; more rows of a group pass over its weights again.  Weights of 16 experts, 2048 x 4096, which
-// memory delivers in 82 us: 1 / 4 / 6 rows for each take 119 / 146 / 183 us stored k by n and 115 / 142 / 179
-// stored n by k, and the tensor-core kernel 265, with scaling 350; one row, 4096 x 4096, 14 and 11 us against
-// 44 and 60; 8 experts of 512 x 512, 4 rows each, 5.3 against 14 and 21.  What bounds it: with one row
-// memory, with more the loads of x from shared memory, one for every four weights and row.  (16 rows at
-// a time spilled: 273 and 589 us.)
+// rows, a chunk of a group; other chunks of it pass over its weights again, in blocks of their own at the
+// same time, so that most of them come from L2.  Weights of 16 experts, 2048 x 4096, which memory delivers
+// in 82 us: 1 / 4 / 6 rows for each take 121 / 149 / 185 us stored k by n and 116 / 144 / 184 stored n by k, and
+// the tensor-core kernel 265, with scaling 350; one row, 4096 x 4096, 14 and 11 us against 44 and 60; 8 experts
+// of 512 x 512, 4 rows each, 5.3 against 14 and 21.  What bounds it: with one row memory, with more the
+// loads of x from shared memory, one for every four weights and row.  (16 rows at a time spilled: 273 and
+// 589 us.)  With all rows in one group: 384 of 64 groups of 2048 x 2048 take 143 and 190 us (evenly 285 and 340),
+// 1536 of 256 of 512 x 1024 76 and 111 (122 and 150); where the chunks of a group ran one after another in
+// its own blocks those took 1570 and 600, 3165 and 1290.
 //
 // op N (weights stored k by n): lanes side by side along n, the warps of a block share k and add their sums
 // in shared memory, in the order of the warps.  op T (n by k): lanes side by side along k, a warp has
@@ -47,24 +50,69 @@ struct FewRowsParams {
   float alpha, beta;
 };
 
-// First row of group blockIdx.y and how many it has, by all threads; totals are taken as find_groups does
-// (grouped_gemm.cu).  Group `groups` are the rows behind the last.
-__device__ __forceinline__ void group_rows(const FewRowsParams &p, uint32_t &begin, uint32_t &count) {
-  __shared__ uint32_t most;
-  const uint32_t g = blockIdx.y;
-  auto end_of = [&](uint32_t i) {
-    return p.ends == nullptr ? p.rows
-                             : static_cast<uint32_t>(min(max(__ldg(p.ends + i), 0), static_cast<int32_t>(p.rows)));
+// The rows of one group, at most kMostRows of them, that a block multiplies.
+struct Chunk {
+  uint32_t group, row0, rows; // rows == 0: there is none
+};
+// Chunk `number` (all threads give the same), and how many there are, by all threads, each of which has some
+// neighbouring groups; totals are taken as find_groups does (grouped_gemm.cu).  Group `groups` are the rows
+// behind the last.
+__device__ __forceinline__ Chunk find_chunk(const FewRowsParams &p, uint32_t number, uint32_t &all) {
+  constexpr uint32_t MOST = (kMaxGroups + kThreads) / kThreads;
+  __shared__ uint32_t chunks[kWarps];
+  __shared__ Chunk found;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t each = p.groups / kThreads + 1, first = threadIdx.x * each;
+  auto total = [&](uint32_t g) { // of rows up to the end of group g, as it stands there
+    return g >= p.groups || p.ends == nullptr
+               ? p.rows
+               : static_cast<uint32_t>(min(max(__ldg(p.ends + g), 0), static_cast<int32_t>(p.rows)));
   };
-  if (threadIdx.x == 0) most = 0;
+  uint32_t begin = first == 0 ? 0u : total(first - 1), end[MOST], last = begin;
+  bool falls = false;
+#pragma unroll
+  for (uint32_t i = 0; i < MOST; ++i) {
+    end[i] = i < each ? total(first + i) : last;
+    falls |= end[i] < last;
+    last = end[i];
+  }
+  if (__syncthreads_or(falls)) // a total that falls back is taken as the one in front of it
+    for (uint32_t g = 0; g < first && g < p.groups; ++g) begin = max(begin, total(g));
+  uint32_t mine = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < MOST; ++i) {
+    end[i] = max(end[i], i == 0 ? begin : end[i - 1]);
+    mine += (end[i] - (i == 0 ? begin : end[i - 1]) + kMostRows - 1) / kMostRows;
+  }
+  uint32_t at = mine; // chunks in front of the thread's
+#pragma unroll
+  for (uint32_t d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, at, d);
+    if (lane >= d) at += o;
+  }
+  if (lane == 31) chunks[warp] = at;
+  if (threadIdx.x == 0) found.rows = 0;
+  at -= mine;
   __syncthreads();
-  uint32_t m = 0;
-  for (uint32_t i = threadIdx.x; i < g; i += kThreads) m = max(m, end_of(i));
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m != 0) atomicMax(&most, m);
+  all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kWarps; ++w) {
+    if (w == warp) at += all;
+    all += chunks[w];
+  }
+  if (number >= at && number < at + mine) {
+#pragma unroll
+    for (uint32_t i = 0; i < MOST; ++i) {
+      const uint32_t from = i == 0 ? begin : end[i - 1], n = (end[i] - from + kMostRows - 1) / kMostRows;
+      if (number >= at && number < at + n) {
+        const uint32_t row0 = from + (number - at) * kMostRows;
+        found = {first + i, row0, min(end[i] - row0, kMostRows)};
+      }
+      at += n;
+    }
+  }
   __syncthreads();
-  begin = most;
-  count = max(begin, g < p.groups ? end_of(g) : p.rows) - begin;
+  return found;
 }
 
 // rows [row0, row0 + R) of x, those behind `have` as 0, values k0 .. k0 + kHeld / R - 1, as far as k goes
@@ -82,13 +130,13 @@ __device__ __forceinline__ void fetch_x(const FewRowsParams &p, float *xs, uint3
 
 // op N.  COL_LANES lanes along n, four columns each, 32 / COL_LANES along k; a block has 4 * COL_LANES columns.
 template <int R, int COL_LANES, bool VEC>
-__device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint32_t row0, uint32_t have) {
+__device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0, uint32_t have) {
   constexpr uint32_t STRETCH = kHeld / R, K_LANES = 32 / COL_LANES, COLS = 4 * COL_LANES, AT_ONCE = kWarps * K_LANES;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t cl = lane % COL_LANES, kl = lane / COL_LANES;
   const uint32_t col0 = blockIdx.x * COLS, col = col0 + 4 * cl;
   const uint32_t cols = col < p.n ? min(p.n - col, 4u) : 0u;
-  const float *w = p.w + blockIdx.y * p.stridew + col;
+  const float *w = p.w + group * p.stridew + col;
   float acc[R][4];
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0.f;
@@ -135,11 +183,11 @@ __device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint
 
 // op T.  A warp has NB rows of w.
 template <int R, int NB, bool VEC>
-__device__ __forceinline__ void rows_t(const FewRowsParams &p, float *smem, uint32_t row0, uint32_t have) {
+__device__ __forceinline__ void rows_t(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0, uint32_t have) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t n0 = (blockIdx.x * kWarps + warp) * NB;
   constexpr uint32_t STRETCH = kHeld / R;
-  const float *w = p.w + blockIdx.y * p.stridew + n0 * p.ldw;
+  const float *w = p.w + group * p.stridew + n0 * p.ldw;
   float acc[NB][R];
 #pragma unroll
   for (int j = 0; j < NB; ++j)
@@ -187,27 +235,29 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const FewRowsPara
   asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ float4 smem4[];
   float *smem = reinterpret_cast<float *>(smem4);
-  uint32_t begin, count;
-  group_rows(p, begin, count);
-  if (blockIdx.y == p.groups) { // rows of no group
-    constexpr uint32_t COLS = OP_N ? 4 * SHAPE : kWarps * SHAPE;
-    for (uint64_t i = threadIdx.x; i < static_cast<uint64_t>(count) * COLS; i += kThreads) {
-      const uint32_t c = blockIdx.x * COLS + static_cast<uint32_t>(i % COLS);
-      if (c >= p.n) continue;
-      float *at = p.y + (begin + i / COLS) * p.ldy + c;
-      *at = p.beta != 0.f ? p.beta * *at : 0.f;
+  // Chunks are dealt to the blocks of a column in turn: as many as groups are one each, unless some groups have
+  // more rows than a chunk and others have rows too.
+  uint32_t all = ~0u;
+  for (uint32_t number = blockIdx.y; number < all; number += gridDim.y) {
+    const Chunk c = find_chunk(p, number, all);
+    if (c.rows == 0) return;
+    if (c.group == p.groups) { // rows of no group
+      constexpr uint32_t COLS = OP_N ? 4 * SHAPE : kWarps * SHAPE;
+      for (uint32_t i = threadIdx.x; i < c.rows * COLS; i += kThreads) {
+        const uint32_t col = blockIdx.x * COLS + i % COLS;
+        if (col >= p.n) continue;
+        float *at = p.y + (c.row0 + i / COLS) * p.ldy + col;
+        *at = p.beta != 0.f ? p.beta * *at : 0.f;
+      }
+      continue;
     }
-    return;
-  }
-  for (uint32_t r = 0; r < count; r += kMostRows) {
-    const uint32_t have = min(count - r, kMostRows);
     auto go = [&](auto most) {
       constexpr int R = decltype(most)::value;
-      if constexpr (OP_N) rows_n<R, SHAPE, VEC>(p, smem, begin + r, have);
-      else rows_t<R, SHAPE, VEC>(p, smem, begin + r, have);
+      if constexpr (OP_N) rows_n<R, SHAPE, VEC>(p, smem, c.group, c.row0, c.rows);
+      else rows_t<R, SHAPE, VEC>(p, smem, c.group, c.row0, c.rows);
     };
-    if (have <= 2) go(std::integral_constant<int, 2>{});
-    else if (have <= 4) go(std::integral_constant<int, 4>{});
+    if (c.rows <= 2) go(std::integral_constant<int, 2>{});
+    else if (c.rows <= 4) go(std::integral_constant<int, 4>{});
     else go(std::integral_constant<int, 8>{});
   }
 }
@@ -221,7 +271,7 @@ cudaError_t launch(const FewRowsParams &p, cudaStream_t stream) {
   const auto kernel = few_rows_kernel<OP_N, SHAPE, VEC>;
   static_assert(smem <= 48 * 1024, "needs no attribute");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.n + COLS - 1) / COLS, p.groups + 1);
+  cfg.gridDim = dim3((p.n + COLS - 1) / COLS, p.groups + 1 < p.rows ? p.groups + 1 : p.rows);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -241,7 +291,7 @@ cudaError_t launch_few_rows(const FewRowsArgs &a, unsigned num_sms, cudaStream_t
   const bool vec = reinterpret_cast<uintptr_t>(a.w) % 16 == 0 && a.ldw % 4 == 0 &&
                    (a.groups == 1 || a.stridew % 4 == 0);
   // Blocks are narrower where there are few: how many of the groups have rows is known on the device only, and
-  // a narrow block of op N takes 5 to 25 % longer for the same weights, while 10 of 54 experts of 480 columns
+  // a narrow block of op N takes 5 to 28 % longer for the same weights, while 10 of 54 experts of 480 columns
   // made 40 wide blocks, which took 94 us and not 25.  (op T with one row of w for a warp was slower than with
   // two everywhere.)
   const uint64_t used = a.groups < a.rows ? a.groups : a.rows;

@@ -371,7 +371,7 @@ cublasStatus_t cuMpSGEMM_sgemm_static_scratch(
  *     CUMPSGEMM_FP16TCEC_SCALING, which first brings the largest finite magnitude of each operand (of its
  *     rows in groups) to 2^14.  Other modes return CUBLAS_STATUS_NOT_SUPPORTED; 16-bit types do not look
  *     at it.  cuMpSGEMM_grouped_gemm multiplies FP32 operands with at most 6 rows for each group on average
- *     in plain FP32 arithmetic, which reads the weights once.
+ *     in plain FP32 arithmetic, which passes over a group's weights once for every 8 of its rows.
  *   Any leading dimension, stride and alignment.  FP32 operands, and 8- and 16-bit ones whose address,
  *     leading dimension or stride is not a multiple of 16 bytes, go through the handle's workspace
  *     (CUBLAS_STATUS_ALLOC_FAILED where it cannot hold them).
