@@ -18,14 +18,14 @@
 // in shared memory, in the order of the warps.  op T (n by k): lanes side by side along k, a warp has
 // some rows of w to itself and adds its lanes by shuffles.  The rows of x are in shared memory as FP32, a
 // stretch of k at a time.  Nothing is atomic: results are the same from run to run.
-#include "grouped.hpp"
+#include "grouped_totals.cuh"
 
 #include <type_traits>
 
 namespace cumpsgemm_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kTotalsThreads;
 constexpr int kWarps = kThreads / 32;
 constexpr uint32_t kMostRows = 8;  // of a group at a time
 constexpr uint32_t kHeld = 8192;   // values of x in shared memory at a time
@@ -54,36 +54,16 @@ struct FewRowsParams {
 struct Chunk {
   uint32_t group, row0, rows; // rows == 0: there is none
 };
-// Chunk `number` (all threads give the same), and how many there are, by all threads, each of which has some
-// neighbouring groups; totals are taken as find_groups does (grouped_gemm.cu).  Group `groups` are the rows
-// behind the last.
+// Chunk `number` (all threads give the same), and how many there are, by all threads.
 __device__ __forceinline__ Chunk find_chunk(const FewRowsParams &p, uint32_t number, uint32_t &all) {
-  constexpr uint32_t MOST = (kMaxGroups + kThreads) / kThreads;
   __shared__ uint32_t chunks[kWarps];
   __shared__ Chunk found;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t each = p.groups / kThreads + 1, first = threadIdx.x * each;
-  auto total = [&](uint32_t g) { // of rows up to the end of group g, as it stands there
-    return g >= p.groups || p.ends == nullptr
-               ? p.rows
-               : static_cast<uint32_t>(min(max(__ldg(p.ends + g), 0), static_cast<int32_t>(p.rows)));
-  };
-  uint32_t begin = first == 0 ? 0u : total(first - 1), end[MOST], last = begin;
-  bool falls = false;
-#pragma unroll
-  for (uint32_t i = 0; i < MOST; ++i) {
-    end[i] = i < each ? total(first + i) : last;
-    falls |= end[i] < last;
-    last = end[i];
-  }
-  if (__syncthreads_or(falls)) // a total that falls back is taken as the one in front of it
-    for (uint32_t g = 0; g < first && g < p.groups; ++g) begin = max(begin, total(g));
+  const GroupTotals t(p.ends, p.groups, p.rows);
+  auto chunks_of = [&](uint32_t i) { return (t.end[i] - t.begin_of(i) + kMostRows - 1) / kMostRows; };
   uint32_t mine = 0;
 #pragma unroll
-  for (uint32_t i = 0; i < MOST; ++i) {
-    end[i] = max(end[i], i == 0 ? begin : end[i - 1]);
-    mine += (end[i] - (i == 0 ? begin : end[i - 1]) + kMostRows - 1) / kMostRows;
-  }
+  for (uint32_t i = 0; i < GroupTotals::MOST; ++i) mine += chunks_of(i);
   uint32_t at = mine; // chunks in front of the thread's
 #pragma unroll
   for (uint32_t d = 1; d < 32; d <<= 1) {
@@ -102,11 +82,11 @@ __device__ __forceinline__ Chunk find_chunk(const FewRowsParams &p, uint32_t num
   }
   if (number >= at && number < at + mine) {
 #pragma unroll
-    for (uint32_t i = 0; i < MOST; ++i) {
-      const uint32_t from = i == 0 ? begin : end[i - 1], n = (end[i] - from + kMostRows - 1) / kMostRows;
+    for (uint32_t i = 0; i < GroupTotals::MOST; ++i) {
+      const uint32_t n = chunks_of(i);
       if (number >= at && number < at + n) {
-        const uint32_t row0 = from + (number - at) * kMostRows;
-        found = {first + i, row0, min(end[i] - row0, kMostRows)};
+        const uint32_t row0 = t.begin_of(i) + (number - at) * kMostRows;
+        found = {t.first + i, row0, min(t.end[i] - row0, kMostRows)};
       }
       at += n;
     }

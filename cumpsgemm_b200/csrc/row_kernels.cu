@@ -1,7 +1,7 @@
 // Passes over rows in front of the grouped products (grouped_gemm.cu): operands brought into a form
 // that TMA and the tensor core read, and rows quantised to 8 bits.  All of them move bytes and
 // little else; a warp takes a row at a time, in 16-byte accesses where the row's address allows.
-#include "grouped.hpp"
+#include "grouped_totals.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -10,7 +10,7 @@
 namespace cumpsgemm_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kTotalsThreads;
 constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ bool finite(float v) {
@@ -18,27 +18,37 @@ __device__ __forceinline__ bool finite(float v) {
 }
 
 // Which rows of an operand are of use: rows in front of the last group's end; weights of groups with
-// rows.  (A running total that falls back ends an empty group here as it does for the product.)
-__device__ __forceinline__ uint32_t clamped_end(const int32_t *ends, uint32_t g, uint32_t rows) {
-  return static_cast<uint32_t>(min(max(__ldg(ends + g), 0), static_cast<int32_t>(rows)));
-}
-__device__ __forceinline__ bool group_is_used(const StageArgs &a, uint32_t g) {
-  if (a.ends == nullptr) return a.rows > 0;
-  return clamped_end(a.ends, g, a.rows) > (g > 0 ? clamped_end(a.ends, g - 1, a.rows) : 0u);
-}
-// by all threads of the block
-__device__ __forceinline__ uint32_t last_end(const StageArgs &a) {
-  if (a.ends == nullptr) return a.rows;
-  __shared__ uint32_t most;
-  if (threadIdx.x == 0) most = 0;
-  __syncthreads();
-  uint32_t e = 0;
-  for (uint32_t g = threadIdx.x; g < a.groups; g += kThreads) e = max(e, clamped_end(a.ends, g, a.rows));
-  e = __reduce_max_sync(0xffffffffu, e);
-  if ((threadIdx.x & 31) == 0) atomicMax(&most, e);
-  __syncthreads();
-  return most;
-}
+// rows.  By all threads of the block.
+struct Used {
+  uint32_t rows;
+  const uint32_t *groups; // a bit for each, in shared memory
+  __device__ __forceinline__ explicit Used(const StageArgs &a) {
+    __shared__ uint32_t most, bits[kMaxGroups / 32];
+    if (threadIdx.x < kMaxGroups / 32) bits[threadIdx.x] = 0;
+    if (threadIdx.x == 0) most = 0;
+    const GroupTotals t(a.ends, a.groups, a.rows); // (passes a barrier)
+    uint32_t upto = 0;
+    auto take = [&](uint32_t i) { // whether group i of the thread's is used
+      const bool some = i < t.each && t.first + i < a.groups && t.end[i] > t.begin_of(i);
+      if (some) upto = t.end[i];
+      return some;
+    };
+    if (t.each == 1) { // a warp has 32 groups side by side
+      const uint32_t word = __ballot_sync(0xffffffffu, take(0));
+      if ((threadIdx.x & 31) == 0) bits[threadIdx.x >> 5] = word;
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < GroupTotals::MOST; ++i)
+        if (take(i)) atomicOr(&bits[(t.first + i) / 32], 1u << ((t.first + i) % 32));
+    }
+    upto = __reduce_max_sync(0xffffffffu, upto);
+    if ((threadIdx.x & 31) == 0 && upto != 0) atomicMax(&most, upto);
+    __syncthreads();
+    rows = most;
+    groups = bits;
+  }
+  __device__ __forceinline__ bool has(uint32_t group) const { return (groups[group / 32] >> (group % 32)) & 1u; }
+};
 
 // A row of `bytes` bytes at any address, read 16 bytes at a time.  Where the address is no multiple of
 // 16, two aligned accesses inside the row are shifted together (the second is the next lane's first,
@@ -130,15 +140,15 @@ constexpr uint32_t kBatch = 4; // 16-byte loads that a lane has on its way at on
 // too few of them to occupy all warps.  (With a row to a warp 110,000 rows of 183 bytes took 49 us, and
 // take 14, and 480 of 29 KB took 17 and take 8.)
 struct Segments {
+  Used used;
   uint32_t units[2];  // segments of each operand
   uint64_t first[3];  // turns of a warp: first of each operand, and their end
-  __device__ __forceinline__ Segments(const StageArgs &a) {
-    const uint32_t used_rows = last_end(a);
+  __device__ __forceinline__ explicit Segments(const StageArgs &a) : used(a) {
     first[0] = 0;
     for (int i = 0; i < 2; ++i) {
       const StageOperand &op = a.op[i];
       units[i] = i >= a.count ? 0u
-                              : (op.rows_are_grouped ? used_rows : static_cast<uint32_t>(op.batch * op.outer)) *
+                              : (op.rows_are_grouped ? used.rows : static_cast<uint32_t>(op.batch * op.outer)) *
                                     op.segments;
       first[i + 1] = first[i] + ((units[i] + (32u >> op.lanes_log2) - 1u) >> (5u - op.lanes_log2));
     }
@@ -166,7 +176,7 @@ struct Segment {
     first = segment * steps * kBatch * lanes + lane;
     ends = segment == 0;
     src_at = b * op.stride + (row - b * outer) * op.ld;
-    return op.rows_are_grouped || op.batch == 1 || group_is_used(a, b);
+    return op.rows_are_grouped || op.batch == 1 || s.used.has(b);
   }
 };
 // The pieces of a row that aligned accesses inside it give: [from, to) in units of 16 bytes (RowReader::inside).
