@@ -7,7 +7,7 @@
 // rows, a chunk of a group; other chunks of it pass over its weights again, in blocks of their own at the
 // same time, so that most of them come from L2.  Weights of 16 experts, 2048 x 4096, which memory delivers
 // in 82 us: 1 / 4 / 6 rows for each take 121 / 149 / 185 us stored k by n and 116 / 144 / 184 stored n by k, and
-// the tensor-core kernel 265, with scaling 350; one row, 4096 x 4096, 14 and 11 us against 44 and 60; 8 experts
+// the tensor-core kernel 265, with scaling 350; one row, 4096 x 4096, 14 and 12 us against 44 and 60; 8 experts
 // of 512 x 512, 4 rows each, 5.3 against 14 and 21.  What bounds it: with one row memory, with more the
 // loads of x from shared memory, one for every four weights and row.  (16 rows at a time spilled: 273 and
 // 589 us.)  With all rows in one group: 384 of 64 groups of 2048 x 2048 take 143 and 190 us (evenly 285 and 340),
@@ -110,7 +110,8 @@ __device__ __forceinline__ void fetch_x(const FewRowsParams &p, float *xs, uint3
 
 // op N.  COL_LANES lanes along n, four columns each, 32 / COL_LANES along k; a block has 4 * COL_LANES columns.
 template <int R, int COL_LANES, bool VEC>
-__device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0, uint32_t have) {
+__device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0,
+                                       uint32_t have) {
   constexpr uint32_t STRETCH = kHeld / R, K_LANES = 32 / COL_LANES, COLS = 4 * COL_LANES, AT_ONCE = kWarps * K_LANES;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t cl = lane % COL_LANES, kl = lane / COL_LANES;
@@ -163,7 +164,8 @@ __device__ __forceinline__ void rows_n(const FewRowsParams &p, float *smem, uint
 
 // op T.  A warp has NB rows of w.
 template <int R, int NB, bool VEC>
-__device__ __forceinline__ void rows_t(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0, uint32_t have) {
+__device__ __forceinline__ void rows_t(const FewRowsParams &p, float *smem, uint64_t group, uint32_t row0,
+                                       uint32_t have) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t n0 = (blockIdx.x * kWarps + warp) * NB;
   constexpr uint32_t STRETCH = kHeld / R;

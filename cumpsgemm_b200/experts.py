@@ -6,14 +6,14 @@ same device, holds the running total of rows after each expert, so expert e has 
 the last total belong to no expert; their results are zero.
 
     ends = torch.bincount(expert_of_row, minlength=E).cumsum(0).to(torch.int32)
-    y = grouped_linear(handle, x, w, ends)              # training: has a backward pass
+    y = grouped_linear(handle, x, w, ends)              # training: gradients of x and w
     q, s = quantize_rows(handle, x, row_index=tokens)   # serving: gather and quantise in one pass
     y = i8_matmul(handle, q, s, wq, w_scale, ends)
 
 Everything goes through the C ABI (``cuMpSGEMM_grouped_gemm`` and its neighbours in
 ``cumpsgemm_ext.h``); there is no other implementation behind it.  Results are allocated on the current
 stream and written on the handle's, so the two have to be one: ``handle.use_current_torch_stream()``
-wherever the current stream changes, or the call is refused.
+wherever the current stream changes, or the call is refused.  The 8-bit calls have no gradients.
 """
 from __future__ import annotations
 

@@ -375,7 +375,10 @@ cublasStatus_t cuMpSGEMM_sgemm_static_scratch(
  *   Any leading dimension, stride and alignment.  FP32 operands, and 8- and 16-bit ones whose address,
  *     leading dimension or stride is not a multiple of 16 bytes, go through the handle's workspace
  *     (CUBLAS_STATUS_ALLOC_FAILED where it cannot hold them).
- *   Results are the same from run to run.  Outputs must not overlap inputs. */
+ *   Results are the same from run to run while the same calls have the same workspace: a call of few
+ *     tiles adds up in slices of K where it can have memory for their sums, which is another order of FP32
+ *     additions than without (under a workspace limit, or first made while the stream is being captured).
+ *   Outputs must not overlap inputs. */
 
 /* y[r, :] = alpha * x[r, :] op(w_e) + beta * y[r, :] for the rows r of each group e; rows of no group:
  * beta * y.  x is rows x k, y rows x n; w_e is stored k x n (op_W = CUBLAS_OP_N) or n x k (CUBLAS_OP_T).
