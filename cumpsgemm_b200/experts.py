@@ -44,7 +44,7 @@ def _rows_of(t, what: str, cols: Optional[int] = None):
     ld, step = t.stride()
     if cols is not None and n != cols:
         raise ValueError(f"{what} has {n} columns where {cols} are needed")
-    if step != 1 and n > 1:
+    if step != 1 and n > 1 and rows > 0:
         raise ValueError(f"the rows of {what} must be contiguous")
     if rows <= 1:
         return rows, n, n

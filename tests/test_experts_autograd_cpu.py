@@ -102,3 +102,19 @@ def test_gradients_are_multiplied_at_any_magnitude(experts):
     module.grouped_linear(None, x, w, ends, mode=ComputeMode.FP16TCEC_SCALING,
                           backward_mode=ComputeMode.FP16TCEC).sum().backward()
     assert [mode for _, mode in calls] == [ComputeMode.FP16TCEC_SCALING] + 2 * [ComputeMode.FP16TCEC]
+
+
+@pytest.mark.parametrize("transpose_w", [False, True])
+def test_no_rows_at_all(experts, transpose_w):
+    """The gradient of a sum over no rows: an empty tensor whose strides, 0 and 0, say nothing."""
+    module, _ = experts
+    _, w, _ = _operands(transpose_w)
+    x = torch.zeros(0, K, dtype=torch.float64, requires_grad=True)
+    ends = torch.zeros(len(COUNTS), dtype=torch.int32)
+    for create_graph in (False, True):
+        y = module.grouped_linear(None, x, w, ends, transpose_w)
+        dx, dw = torch.autograd.grad(y.sum(), (x, w), create_graph=create_graph)
+        assert dx.shape == (0, K) and dw.shape == w.shape and not dw.any()
+    assert module._rows_of(torch.zeros(()).expand(0, 5), "x", 5) == (0, 5, 5)
+    with pytest.raises(ValueError, match="columns"):
+        module._rows_of(torch.zeros(0, 4), "x", 5)
