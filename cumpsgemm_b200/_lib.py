@@ -139,6 +139,17 @@ PROTOTYPES = {
     "cuMpSGEMM_i8_grouped_gemm": (i32, [vp, u64, u64, u64, u32, vp, vp, u64, vp, vp, u64, u64, vp, vp, vp,
                                         u64, i32]),
     "cuMpSGEMM_quantize_rows_i8": (i32, [vp, u64, u64, vp, u64, i32, vp, u64, vp, u64, vp]),
+    "cuMpSGEMM_grouped_gemm_gated": (i32, [vp, u64, u64, u64, u32, vp, vp, u64, vp, u64, u64, i32, vp, u64, vp,
+                                           u64, i32, i32]),
+    "cuMpSGEMM_grouped_gemm_gated_grad": (i32, [vp, i32, u64, u64, u64, u32, vp, vp, u64, vp, u64, u64, i32, vp,
+                                                u64, vp, u64, i32, i32]),
+    "cuMpSGEMM_gated_rows": (i32, [vp, u64, u64, vp, u64, vp, u64, i32, vp, u64, i32]),
+    "cuMpSGEMM_quantize_rows_f8": (i32, [vp, u64, u64, vp, u64, i32, vp, u64, i32, vp, u64, i32, vp, u64, u64]),
+    "cuMpSGEMM_quantize_blocks_f8": (i32, [vp, u32, u64, u64, vp, u64, u64, i32, vp, u64, u64, i32, vp]),
+    "cuMpSGEMM_f8_grouped_gemm": (i32, [vp, u64, u64, u64, u32, vp, vp, u64, i32, vp, u64, u64, vp, u64, u64,
+                                        i32, vp, vp, vp, u64, i32]),
+    "cuMpSGEMM_f8_grouped_gemm_gated": (i32, [vp, u64, u64, u64, u32, vp, vp, u64, i32, vp, u64, u64, vp, u64,
+                                              u64, i32, vp, i32, vp, u64, i32, vp, u64, u64]),
     # intercepted cuBLAS symbols (prototypes of cublas_api.h)
     "cublasSgemm_v2": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, vp, i32]),
     "cublasCgemm_v2": (i32, [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i32, vp, vp, i32]),

@@ -24,6 +24,8 @@ CUBLAS_OP_C = 2
 CUDA_R_32F = 0
 CUDA_R_16F = 2
 CUDA_R_16BF = 14
+CUDA_R_8F_E4M3 = 28
+CUDA_R_8F_E5M2 = 29
 
 CUBLAS_STATUS_SUCCESS = 0
 CUBLAS_STATUS_NOT_INITIALIZED = 1
@@ -50,6 +52,16 @@ class ComputeMode(enum.IntEnum):
     UNDEFINED = 10
     FP16TCEC_SCALING = 11
     FP32_SIMT = 12
+
+
+class Activation(enum.IntEnum):
+    """cuMpSGEMM_activation_t."""
+
+    NONE = -1
+    SILU = 0
+    GELU = 1
+    GELU_TANH = 2
+    RELU = 3
 
 
 class CuMpSGEMMError(RuntimeError):
@@ -285,6 +297,86 @@ class Handle:
                                                   _ptr(scale))
         if check and st != CUBLAS_STATUS_SUCCESS:
             raise CuMpSGEMMError(st, "cuMpSGEMM_quantize_rows_i8")
+        return st
+
+    def grouped_gemm_gated(self, rows: int, hidden: int, k: int, num_groups: int, group_ends, X: DevPtr, ldx: int,
+                           W: DevPtr, ldw: int, stridew: int, activation: int, Y: DevPtr, ldy: int, pre,
+                           ldpre: int, data_type: int, mode: int = ComputeMode.FP16TCEC, check: bool = True) -> int:
+        """cuMpSGEMM_grouped_gemm_gated."""
+        st = self._lib.cuMpSGEMM_grouped_gemm_gated(
+            self._h, rows, hidden, k, num_groups, _ptr_or_null(group_ends), _ptr(X), ldx, _ptr(W), ldw, stridew,
+            int(activation), _ptr(Y), ldy, _ptr_or_null(pre), ldpre, data_type, int(mode))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_grouped_gemm_gated")
+        return st
+
+    def grouped_gemm_gated_grad(self, op_W: int, rows: int, hidden: int, k: int, num_groups: int, group_ends,
+                                dY: DevPtr, lddy: int, W: DevPtr, ldw: int, stridew: int, activation: int,
+                                pre: DevPtr, ldpre: int, dpre: DevPtr, lddpre: int, data_type: int,
+                                mode: int = ComputeMode.FP16TCEC, check: bool = True) -> int:
+        """cuMpSGEMM_grouped_gemm_gated_grad."""
+        st = self._lib.cuMpSGEMM_grouped_gemm_gated_grad(
+            self._h, op_W, rows, hidden, k, num_groups, _ptr_or_null(group_ends), _ptr(dY), lddy, _ptr(W), ldw,
+            stridew, int(activation), _ptr(pre), ldpre, _ptr(dpre), lddpre, data_type, int(mode))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_grouped_gemm_gated_grad")
+        return st
+
+    def gated_rows(self, rows: int, hidden: int, pre: DevPtr, ldpre: int, dh, lddh: int, activation: int,
+                   out: DevPtr, ldo: int, data_type: int, check: bool = True) -> int:
+        """cuMpSGEMM_gated_rows."""
+        st = self._lib.cuMpSGEMM_gated_rows(self._h, rows, hidden, _ptr(pre), ldpre, _ptr_or_null(dh), lddh,
+                                            int(activation), _ptr(out), ldo, data_type)
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_gated_rows")
+        return st
+
+    def quantize_rows_f8(self, rows: int, k: int, X: DevPtr, ldx: int, data_type: int, row_index, src_rows: int,
+                         activation: int, Q: DevPtr, ldq: int, q_type: int, scale: DevPtr, scale_row: int,
+                         scale_block: int, check: bool = True) -> int:
+        """cuMpSGEMM_quantize_rows_f8."""
+        st = self._lib.cuMpSGEMM_quantize_rows_f8(
+            self._h, rows, k, _ptr(X), ldx, data_type, _ptr_or_null(row_index), src_rows, int(activation), _ptr(Q),
+            ldq, q_type, _ptr(scale), scale_row, scale_block)
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_quantize_rows_f8")
+        return st
+
+    def quantize_blocks_f8(self, matrices: int, n: int, k: int, W: DevPtr, ldw: int, stridew: int, data_type: int,
+                           Q: DevPtr, ldq: int, strideq: int, q_type: int, scale: DevPtr,
+                           check: bool = True) -> int:
+        """cuMpSGEMM_quantize_blocks_f8."""
+        st = self._lib.cuMpSGEMM_quantize_blocks_f8(self._h, matrices, n, k, _ptr(W), ldw, stridew, data_type,
+                                                    _ptr(Q), ldq, strideq, q_type, _ptr(scale))
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_quantize_blocks_f8")
+        return st
+
+    def f8_grouped_gemm(self, rows: int, n: int, k: int, num_groups: int, group_ends, Xq: DevPtr, ldx: int,
+                        x_type: int, x_scale: DevPtr, x_scale_row: int, x_scale_block: int, Wq: DevPtr, ldw: int,
+                        stridew: int, w_type: int, w_scale: DevPtr, bias, Y: DevPtr, ldy: int, y_type: int,
+                        check: bool = True) -> int:
+        """cuMpSGEMM_f8_grouped_gemm."""
+        st = self._lib.cuMpSGEMM_f8_grouped_gemm(
+            self._h, rows, n, k, num_groups, _ptr_or_null(group_ends), _ptr(Xq), ldx, x_type, _ptr(x_scale),
+            x_scale_row, x_scale_block, _ptr(Wq), ldw, stridew, w_type, _ptr(w_scale), _ptr_or_null(bias), _ptr(Y),
+            ldy, y_type)
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_f8_grouped_gemm")
+        return st
+
+    def f8_grouped_gemm_gated(self, rows: int, hidden: int, k: int, num_groups: int, group_ends, Xq: DevPtr,
+                              ldx: int, x_type: int, x_scale: DevPtr, x_scale_row: int, x_scale_block: int,
+                              Wq: DevPtr, ldw: int, stridew: int, w_type: int, w_scale: DevPtr, activation: int,
+                              Q: DevPtr, ldq: int, q_type: int, scale: DevPtr, scale_row: int, scale_block: int,
+                              check: bool = True) -> int:
+        """cuMpSGEMM_f8_grouped_gemm_gated."""
+        st = self._lib.cuMpSGEMM_f8_grouped_gemm_gated(
+            self._h, rows, hidden, k, num_groups, _ptr_or_null(group_ends), _ptr(Xq), ldx, x_type, _ptr(x_scale),
+            x_scale_row, x_scale_block, _ptr(Wq), ldw, stridew, w_type, _ptr(w_scale), int(activation), _ptr(Q),
+            ldq, q_type, _ptr(scale), scale_row, scale_block)
+        if check and st != CUBLAS_STATUS_SUCCESS:
+            raise CuMpSGEMMError(st, "cuMpSGEMM_f8_grouped_gemm_gated")
         return st
 
     def kernel_status(self) -> int:

@@ -44,6 +44,8 @@ CUDA_SOURCES = [
     "grouped_gemm.cu",
     "grouped_few_rows.cu",
     "row_kernels.cu",
+    "f8_gemm.cu",
+    "block_rows.cu",
     "grouped_api.cu",
 ]
 CPP_SOURCES = ["cublas_shim.cpp", "default_rule.cpp"]

@@ -1,0 +1,56 @@
+// The activations of a gated feed-forward block, h = act(gate) * up, and their derivatives, in FP32.
+//
+//   silu       g p,  p = 1 / (1 + exp(-g))                    slope p + g p (1 - p)
+//   gelu       g P,  P = erfc(-g / sqrt 2) / 2                slope P + g exp(-g^2 / 2) / sqrt(2 pi)
+//   gelu_tanh  g (1 + tanh z) / 2 = g p,  p = 1 / (1 + exp(-2 z)),  z = sqrt(2 / pi) (g + 0.044715 g^3)
+//                                                             slope p + 2 g p (1 - p) z'
+//   relu       max(g, 0)                                      slope 1 above 0, else 0
+//
+// The forms with p and erfc lose nothing to cancellation where g is far below 0.  Where the second term of a
+// slope has come to 0 it is left out, so that an infinite g (times 0) does not make it NaN.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace cumpsgemm_b200 {
+
+enum class Activation : int { silu = 0, gelu = 1, gelu_tanh = 2, relu = 3 };
+
+struct ActResult {
+  float value, slope;
+};
+
+__device__ __forceinline__ float logistic(float v) { return 1.f / (1.f + expf(-v)); }
+
+// The slope costs nothing where it is not used.
+__device__ __forceinline__ ActResult activate(Activation a, float g) {
+  constexpr float kRootHalf = 0.707106781186547524f, kRootTwoOverPi = 0.797884560802865356f,
+                  kOverRootTwoPi = 0.398942280401432678f, kCubic = 0.044715f;
+  ActResult r;
+  switch (a) {
+  case Activation::silu: {
+    const float p = logistic(g), q = p * (1.f - p);
+    r.value = g * p;
+    r.slope = q != 0.f ? fmaf(g, q, p) : p;
+    break;
+  }
+  case Activation::gelu: {
+    const float p = 0.5f * erfcf(-g * kRootHalf), q = kOverRootTwoPi * expf(-0.5f * g * g);
+    r.value = g * p;
+    r.slope = q != 0.f ? fmaf(g, q, p) : p;
+    break;
+  }
+  case Activation::gelu_tanh: {
+    const float gg = g * g;
+    const float p = logistic(2.f * kRootTwoOverPi * g * fmaf(kCubic, gg, 1.f)), q = p * (1.f - p);
+    r.value = g * p;
+    r.slope = q != 0.f ? fmaf(2.f * g * q, kRootTwoOverPi * fmaf(3.f * kCubic, gg, 1.f), p) : p;
+    break;
+  }
+  default:
+    r.value = g < 0.f ? 0.f : g; // (NaN stays NaN)
+    r.slope = g > 0.f ? 1.f : 0.f;
+  }
+  return r;
+}
+
+} // namespace cumpsgemm_b200

@@ -1,0 +1,769 @@
+// Products of rows grouped by expert in 8-bit floating point, with a scale for each 128 values of a row and
+// each 128 x 128 of the weights, on CTA pairs (tcgen05 cta_group::2, kind::f8f6f4).
+//
+//   product  y[r, c] = sum over blocks b of 128 k's of  sx[r, b] sw_e[c / 128, b] sum_{k in b} xq[r, k] wq_e[c, k]
+//            (+ bias[e, c])                                            for the rows r of group e
+//   gated    h[r, f] = act(y[r, f]) y[r, hidden + f], which leaves as 8-bit values with scales of their own
+//
+// A block of K is a stage: its products go to a fresh accumulator, and the epilogue adds that, times its scale, to
+// sums in registers while the tensor core fills the other accumulator.  This is what bounds a long product: 128
+// x 256 multiply-adds of the epilogue for each stage of an SM, which the tensor core multiplies in 256 cycles.
+//
+// Which side is which.  Rows of x are the lanes of tensor memory and output features its columns, the other way
+// round than in grouped_gemm.cu.  So a thread has a row, and a stage has one scale for it, its own times the one of
+// the 128 features that its warp holds: a register, where scales that differ from column to column would have
+// to come from shared memory, whose port the operands need.  What it costs: a group's last 256 lanes are not all
+// rows.  Where groups have few rows the weights' way from memory is the longer one anyway (a stage of 256 features
+// is 32 KB, which memory gives a pair in 700 cycles).  Warps without rows read nothing, nor are rows loaded that
+// no lane needs.
+//
+// Gated: a CTA loads rows of the gate and the same ones of the projection it gates, so that the columns of an
+// epilogue warp are half the one and half the other, and a thread has both for its features; two warps
+// share the largest magnitude of 128 features.
+//
+// Tiles take equal time, so they are dealt to the pairs in turn.  A launch with few tiles cuts them into slices of
+// K, whose sums are parked and added in order by the warp that is the last to come.
+//
+// Barriers ("leader" = cluster rank 0):
+//   full[s]       leader's only: 2 arrivals, one from each CTA's producer, and the bytes of both CTAs' loads
+//   empty[s]      in both CTAs: commit multicast from the leader
+//   acc_full[b]   in both CTAs: commit multicast
+//   acc_empty[b]  leader's only: 16 arrivals, one from each epilogue warp of both CTAs
+//   pair[q]       own, gated: 2 arrivals, one from each epilogue warp that has quarter q of the lanes
+// Every wait is bounded; no TMA multicast is used.
+#include "activation.cuh"
+#include "block_scale.cuh"
+#include "gemm_common.cuh"
+#include "grouped.hpp"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <mutex>
+#include <type_traits>
+
+namespace cumpsgemm_b200 {
+namespace {
+
+constexpr uint32_t ROWS_CTA = 128, ROWS = 2 * ROWS_CTA; // lanes of a CTA and of a pair
+constexpr uint32_t COLS = 256;                          // most columns of a tile
+constexpr uint32_t WIDTHS = 3;                          // that a launch chooses from: 256, 128, 64
+constexpr uint32_t HALF = COLS / 2;                     // most columns of a warp
+constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
+constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
+constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
+constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 6;
+constexpr int NUM_THREADS = 384;
+constexpr int NUM_EPI_WARPS = 8;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t BAND = 8;        // row tiles that are walked together
+constexpr uint32_t MAX_SLICES = 16;
+constexpr uint32_t MIN_SLICE = 4;   // least blocks of K in a slice
+constexpr uint32_t PART = COLS * ROWS_CTA; // elements of a parked sum of one CTA
+constexpr uint32_t JOIN_AHEAD = 4;
+constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
+// Registers: 384 threads are launched with 168 each; the four warps that issue give back what the eight that
+// hold 128 sums each take.
+constexpr int REGS_REST = 64, REGS_EPI = 216;
+static_assert(128 * REGS_REST + 256 * REGS_EPI <= 384 * 168, "setmaxnreg draws on the launch's registers");
+
+constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
+                   ACC_EMPTY = ACC_FULL + 16, TMEM_PTR = ACC_EMPTY + 16, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 8,
+                   PAIR = WIDTH + 4, LAST = PAIR + 8 * 4, // gated, for each quarter of the lanes
+                   TOPS = BARS + 256,                     // gated: largest magnitudes, [tile's parity][half][lane]
+                   START = TOPS + 4 * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
+                   OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
+                   BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
+static_assert(PAIR % 8 == 0 && LAST + 4 * 4 <= TOPS, "barriers and flags");
+constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
+static_assert(SMEM <= 232448, "shared memory of a CTA");
+
+struct F8Params {
+  const int32_t *ends;
+  void *out; // gated: the 8-bit values
+  uint64_t ldo;
+  const float *x_scale;
+  uint64_t x_scale_row, x_scale_block;
+  const float *w_scale; // [groups][blocks of w's rows][blocks of K]
+  const float *bias;    // nullable; gated: none
+  float *out_scale;     // gated
+  uint64_t out_scale_row, out_scale_block;
+  float *parts; // nullable: sums of slices, [slot][CTA rank][COLS][ROWS_CTA]
+  unsigned *counters;
+  int *status;
+  uint32_t rows, groups, n, blocks; // n: features of the result
+  uint32_t idesc;
+  uint16_t out_type; // gated: F8Type
+  uint8_t activation;
+  uint8_t vector_out; // rows of the result allow 16-byte accesses
+};
+
+// A tile, or a slice of one: `rows` rows from row0 on, features from col0 on, blocks [k0, k0 + blocks) of K.
+struct Tile {
+  uint32_t group, row0, rows, col0, k0, blocks, slices, slice, slot, number;
+};
+
+// The items of a launch, which are tiles or slices of tiles, by their numbers: groups in turn; within one, bands
+// of row tiles that all column tiles pass over, so that what runs at the same time shares operands in L2.
+template <bool GATED> struct Items {
+  const uint32_t *start, *first_tile;
+  uint32_t group, total, slices, cols, features; // features: of the result, in a tile
+  __device__ __forceinline__ Items(const uint8_t *smem, const F8Params &p, uint32_t clusters) {
+    start = reinterpret_cast<const uint32_t *>(smem + START);
+    first_tile = reinterpret_cast<const uint32_t *>(smem + FIRST_TILE);
+    cols = *reinterpret_cast<const uint32_t *>(smem + WIDTH);
+    features = GATED ? cols / 2 : cols;
+    group = 0;
+    const uint32_t tiles = first_tile[p.groups + 1];
+    slices = p.parts != nullptr && tiles > 0 && tiles <= clusters / 2
+                 ? max(1u, min(min(clusters / tiles, p.blocks / MIN_SLICE), MAX_SLICES))
+                 : 1u;
+    total = tiles * slices;
+  }
+  // item < total, and not below that of an earlier call; false: it is none (a tile of zeros has one slice)
+  __device__ __forceinline__ bool get(const F8Params &p, uint32_t item, Tile &x) {
+    x.number = slices > 1 ? item / slices : item;
+    x.slot = item;
+    while (x.number >= first_tile[group + 1]) ++group;
+    const uint32_t r0 = start[group], r = start[group + 1] - r0;
+    const uint32_t row_tiles = (r + ROWS - 1) / ROWS, col_tiles = (p.n + features - 1) / features;
+    const uint32_t local = x.number - first_tile[group];
+    const uint32_t band = local / (BAND * col_tiles), in_band = local - band * BAND * col_tiles;
+    const uint32_t height = min(BAND, row_tiles - band * BAND);
+    const uint32_t ct = in_band / height, rt = band * BAND + (in_band - ct * height);
+    x.group = group;
+    x.row0 = r0 + rt * ROWS;
+    x.rows = min(ROWS, r - rt * ROWS);
+    x.col0 = ct * features;
+    x.slices = group < p.groups ? slices : 1u;
+    x.slice = slices > 1 ? item - x.number * slices : 0u;
+    if (x.slice >= x.slices) return false;
+    const uint32_t all = group < p.groups ? p.blocks : 0u;
+    x.k0 = all * x.slice / x.slices;
+    x.blocks = all * (x.slice + 1) / x.slices - x.k0;
+    return true;
+  }
+};
+
+// First row and first tile of each group, and the width of the tiles, by one warp.  What `ends` holds is never
+// trusted: a total that falls back or passes the number of rows is taken as the one in front of it, or as
+// that number.  The rows behind the last group are a group of their own, whose tiles have no blocks.
+template <bool GATED>
+__device__ __forceinline__ void find_groups(uint8_t *smem, const F8Params &p, uint32_t clusters) {
+  uint32_t *start = reinterpret_cast<uint32_t *>(smem + START);
+  uint32_t *first_tile = reinterpret_cast<uint32_t *>(smem + FIRST_TILE);
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t end_before = 0, row_tiles = 0; // row tiles in front
+  for (uint32_t g0 = 0; g0 < p.groups + 1; g0 += 32) {
+    const uint32_t g = g0 + lane;
+    uint32_t end = 0;
+    if (g < p.groups)
+      end = p.ends == nullptr ? p.rows
+                              : static_cast<uint32_t>(min(max(__ldg(p.ends + g), 0), static_cast<int32_t>(p.rows)));
+    else if (g == p.groups) end = p.rows;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, end, d);
+      if (static_cast<int>(lane) >= d) end = max(end, o);
+    }
+    end = max(end, end_before);
+    uint32_t begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = end_before;
+    uint32_t upto = g <= p.groups ? (end - begin + ROWS - 1) / ROWS : 0u;
+    const uint32_t mine = upto;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (static_cast<int>(lane) >= d) upto += o;
+    }
+    if (g <= p.groups) {
+      start[g] = begin;
+      first_tile[g] = row_tiles + upto - mine;
+    }
+    if (g == p.groups) start[g + 1] = end;
+    end_before = __shfl_sync(0xffffffffu, end, 31);
+    row_tiles += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  // The width.  With many tiles, the widest.  Else the one with the earliest end: waves of tiles, each as long as
+  // its steps (a narrow one's are bound by the loads of its rows) and what a tile takes besides.
+  uint32_t cols = COLS;
+  if constexpr (!GATED) { // (a gated tile has a whole block of 128 features)
+    if (row_tiles * ((p.n + COLS - 1) / COLS) < 4 * clusters) {
+      float best = 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < WIDTHS; ++i) {
+        const uint32_t w = COLS >> i, tiles = row_tiles * ((p.n + w - 1) / w), waves = (tiles + clusters - 1) / clusters;
+        const float ends_at = waves * (p.blocks * fmaxf(w, 0.6f * (COLS + w)) + 2500.f);
+        if (i == 0 || ends_at < 0.95f * best) {
+          best = ends_at;
+          cols = w;
+        }
+      }
+    }
+  }
+  const uint32_t features = GATED ? cols / 2 : cols, col_tiles = (p.n + features - 1) / features;
+  for (uint32_t g = lane; g <= p.groups; g += 32) first_tile[g] *= col_tiles;
+  if (lane == 0) {
+    first_tile[p.groups + 1] = row_tiles * col_tiles;
+    *reinterpret_cast<uint32_t *>(smem + WIDTH) = cols;
+  }
+}
+
+__device__ __forceinline__ unsigned long long both(float x) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(x));
+  return v;
+}
+__device__ __forceinline__ float low(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+
+// sums += scale * the first `cols` columns from taddr on (a multiple of 16), two columns to an instruction.  The
+// next 16 are on their way while these are added.  Gated: the second half of the columns has a scale of its own.
+template <bool GATED>
+__device__ __forceinline__ void drain(uint32_t taddr, unsigned long long (&sums)[HALF / 2], uint32_t cols,
+                                      unsigned long long s0, unsigned long long s1) {
+  uint32_t v[2][16];
+  ptx::tmem_ld_32x32b_x16(taddr, v[0]);
+#pragma unroll
+  for (uint32_t c = 0; c < HALF; c += 16) {
+    if (!GATED && c >= cols) break;
+    ptx::tmem_ld_wait();
+    if (c + 16 < HALF && (GATED || c + 16 < cols)) ptx::tmem_ld_32x32b_x16(taddr + c + 16, v[(c / 16 + 1) & 1]);
+    const uint32_t(&x)[16] = v[(c / 16) & 1];
+    const unsigned long long s = GATED && c >= HALF / 2 ? s1 : s0;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i += 2) {
+      unsigned long long y;
+      asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(x[i]), "r"(x[i + 1]));
+      asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[(c + i) / 2]) : "l"(y), "l"(s));
+    }
+  }
+}
+
+// A slice's sums are parked, column c of the warp at c * ROWS_CTA, for whoever is the last of the tile's slices
+// to do so and counts up to their number.  Nothing waits.
+__device__ __forceinline__ float *part_of(const F8Params &p, uint32_t slot, uint32_t rank, uint32_t quarter, uint32_t col) {
+  return p.parts + (static_cast<uint64_t>(slot) * 2 + rank) * PART + static_cast<uint64_t>(col) * ROWS_CTA +
+         quarter * 32u + (threadIdx.x & 31u);
+}
+__device__ __forceinline__ void park(float *mine, uint32_t cols, const unsigned long long (&sums)[HALF / 2]) {
+#pragma unroll
+  for (uint32_t c = 0; c < HALF; c += 2) {
+    if (c >= cols) break;
+    __stcg(mine + c * ROWS_CTA, low(sums[c / 2]));
+    __stcg(mine + (c + 1) * ROWS_CTA, high(sums[c / 2]));
+  }
+  __threadfence();
+  __syncwarp();
+}
+// by one lane: whether all other slices' sums of these lanes (and columns) have been parked
+__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) {
+  return atomicInc(p.counters + 2 + (x.number * 2 + rank) * NUM_EPI_WARPS + which, x.slices - 1) == x.slices - 1;
+}
+// the sums of all slices, the first of which is at `first`, added in their order
+__device__ __forceinline__ void join(const float *first, uint32_t slices, uint32_t cols,
+                                     unsigned long long (&sums)[HALF / 2]) {
+  __threadfence();
+#pragma unroll
+  for (uint32_t c = 0; c < HALF; c += 16) {
+    if (c >= cols) break;
+    float v[16];
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) v[j] = 0.f;
+#pragma unroll 1
+    for (uint32_t s = 0; s < slices; s += JOIN_AHEAD) {
+      float y[JOIN_AHEAD][16]; // several slices' values are on their way at once
+#pragma unroll
+      for (uint32_t i = 0; i < JOIN_AHEAD; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j)
+          y[i][j] = s + i < slices ? __ldcg(first + static_cast<uint64_t>(s + i) * 2 * PART + (c + j) * ROWS_CTA) : 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < JOIN_AHEAD; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) v[j] += y[i][j];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j += 2) sums[(c + j) / 2] = pair_of(v[j], v[j + 1]);
+  }
+}
+
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <class T> __device__ __forceinline__ T ld_shared_one(uint32_t addr) {
+  if constexpr (sizeof(T) == 1) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return static_cast<T>(v);
+  } else if constexpr (sizeof(T) == 2) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
+  } else {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+  }
+}
+
+// 64 bytes of each of a warp's rows, which its lanes have in w, to memory by way of the warp's buffer: a lane
+// stores its own as 16-byte chunks (those of two rows side by side XORed, so that neither side meets a bank twice)
+// and four lanes then write a row's together.  E: an element; `elems` of them in the row, `rows` rows.
+template <class E>
+__device__ __forceinline__ void store_64_bytes(uint32_t buf, const uint32_t (&w)[16], E *out, uint64_t ldo, uint32_t rows,
+                                               uint32_t elems, bool vector) {
+  constexpr uint32_t PER = 16 / sizeof(E), ALL = 4 * PER;
+  const uint32_t lane = threadIdx.x & 31u;
+  __syncwarp(); // the buffer has been read
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i)
+    st_shared(buf + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+  if (vector && elems >= ALL) {
+    const uint32_t chunk = lane & 3u;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t row = 8 * i + (lane >> 2);
+      const uint4 v = ld_shared(buf + row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4));
+      if (row < rows) *reinterpret_cast<uint4 *>(out + row * ldo + chunk * PER) = v;
+    }
+  } else { // element by element, neighbours by neighbouring lanes
+#pragma unroll 1
+    for (uint32_t i = lane; i < rows * ALL; i += 32) {
+      const uint32_t row = i / ALL, e = i - row * ALL;
+      if (e < elems)
+        out[row * ldo + e] = ld_shared_one<E>(buf + row * 64u + (((e / PER) ^ ((row >> 1) & 3u)) << 4) + (e % PER) * sizeof(E));
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+  uint32_t w;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  return w;
+}
+__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
+  uint32_t w;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  return w;
+}
+
+// A thread's sums, `cols` columns of its row, to the result: the one rounding.
+__device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, const unsigned long long (&sums)[HALF / 2],
+                                           uint64_t at, uint32_t rows, uint32_t cols) {
+  const auto type = static_cast<GroupedOut>(p.out_type);
+  if (type == GroupedOut::f32) {
+    uint32_t *out = static_cast<uint32_t *>(p.out) + at;
+#pragma unroll
+    for (uint32_t c = 0; c < HALF; c += 16) {
+      if (c >= cols) break;
+      uint32_t w[16];
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 2) {
+        w[i] = static_cast<uint32_t>(sums[(c + i) / 2]);
+        w[i + 1] = static_cast<uint32_t>(sums[(c + i) / 2] >> 32);
+      }
+      store_64_bytes(buf, w, out + c, p.ldo, rows, cols - c, p.vector_out != 0);
+    }
+  } else {
+    uint16_t *out = static_cast<uint16_t *>(p.out) + at;
+    const bool bf16 = type == GroupedOut::bf16;
+#pragma unroll
+    for (uint32_t c = 0; c < HALF; c += 32) {
+      if (c >= cols) break;
+      uint32_t w[16];
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const float x = low(sums[c / 2 + i]), y = high(sums[c / 2 + i]);
+        w[i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
+      }
+      store_64_bytes(buf, w, out + c, p.ldo, rows, cols - c, p.vector_out != 0);
+    }
+  }
+}
+
+template <F8Type TYPE>
+__device__ __forceinline__ void quantise_64(const BlockScale &s, const float (&h)[HALF / 2], uint32_t (&w)[16]) {
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+}
+
+template <bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+    f8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
+                   const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_few,
+                   const __grid_constant__ F8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *const smem =
+      reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t sbase = ptx::smem_u32(smem);
+  volatile int *const abort_flag = reinterpret_cast<volatile int *>(smem + ABORT);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+  const uint32_t cluster_id = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(sbase + FULL + 8 * s, 2);
+      ptx::mbar_init(sbase + EMPTY + 8 * s, 1);
+    }
+    for (uint32_t b = 0; b < 2; ++b) {
+      ptx::mbar_init(sbase + ACC_FULL + 8 * b, 1);
+      ptx::mbar_init(sbase + ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
+    }
+    for (uint32_t q = 0; q < 4; ++q) ptx::mbar_init(sbase + PAIR + 8 * q, 2);
+    *abort_flag = 0;
+    ptx::mbar_init_fence();
+    ptx::prefetch_tensormap(&map_x);
+    ptx::prefetch_tensormap(&map_x_few);
+    ptx::prefetch_tensormap(&map_w);
+    ptx::prefetch_tensormap(&map_w_few);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(sbase + TMEM_PTR, TMEM_COLS);
+    ptx::tmem_relinquish_pair();
+  }
+  // Everything above needs nothing of the kernel in front, everything below may.
+  ptx::griddep_wait();
+  if (warp == 2) find_groups<GATED>(smem, p, clusters);
+  ptx::tc_fence_before();
+  __syncthreads();
+  // both CTAs' barriers must exist before any remote arrive / remote TMA completion
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<const uint32_t *>(smem + TMEM_PTR);
+
+  if (warp < 4) {
+    ptx::setmaxnreg_dec<REGS_REST>();
+    Items<GATED> items(smem, p, clusters);
+    Tile x;
+    if (warp == 0) {
+      // ============================================================== TMA producer (both CTAs)
+      if (ptx::elect_one()) {
+        uint32_t s = 0, ph = 1;
+        bool ok = true;
+        const uint32_t half = items.cols / 2; // columns that this CTA loads
+        for (uint32_t item = cluster_id; ok && item < items.total; item += clusters) {
+          if (!items.get(p, item, x)) continue;
+          // boxes of rows: one of 128, or as many of 32 as it takes; none where this CTA has no rows
+          const uint32_t rows = x.rows > rank * ROWS_CTA ? min(x.rows - rank * ROWS_CTA, ROWS_CTA) : 0u;
+          const uint32_t x_boxes = (rows + BOX_ROWS - 1) / BOX_ROWS;
+          const bool x_whole = x_boxes == ROWS_CTA / BOX_ROWS;
+          const uint32_t bytes = (x_boxes * BOX_ROWS + half) * BLOCK;
+          const int row = static_cast<int>(x.row0 + rank * ROWS_CTA);
+          const int e = static_cast<int>(x.group);
+          for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+            ok = ptx::mbar_wait(sbase + EMPTY + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitEmpty);
+            if (!ok) break;
+            const uint32_t x_dst = sbase + s * STAGE_BYTES, w_dst = x_dst + TILE_BYTES;
+            const uint32_t full = ptx::map_to_cta(sbase + FULL + 8 * s, 0); // the leader's barrier
+            if (leader) ptx::mbar_arrive_expect_tx(sbase + FULL + 8 * s, bytes);
+            else ptx::mbar_arrive_expect_tx_cluster(full, bytes);
+            const int k = static_cast<int>((x.k0 + kb) * BLOCK);
+            if (x_whole) {
+              ptx::tma_load_3d_pair(x_dst, &map_x, full, k, row, 0);
+            } else {
+              for (uint32_t b = 0; b < x_boxes; ++b)
+                ptx::tma_load_3d_pair(x_dst + b * BOX_ROWS * BLOCK, &map_x_few, full, k,
+                                      row + static_cast<int>(b * BOX_ROWS), 0);
+            }
+            if constexpr (GATED) { // 64 rows of the gate, then the same of the projection
+              const int f = static_cast<int>(x.col0 + rank * (half / 2));
+              ptx::tma_load_3d_pair(w_dst, &map_w, full, k, f, e);
+              ptx::tma_load_3d_pair(w_dst + half / 2 * BLOCK, &map_w, full, k, static_cast<int>(p.n) + f, e);
+            } else {
+              const int c = static_cast<int>(x.col0 + rank * half);
+              if (half == HALF) {
+                ptx::tma_load_3d_pair(w_dst, &map_w, full, k, c, e);
+              } else {
+                for (uint32_t b = 0; b < half / BOX_ROWS; ++b)
+                  ptx::tma_load_3d_pair(w_dst + b * BOX_ROWS * BLOCK, &map_w_few, full, k,
+                                        c + static_cast<int>(b * BOX_ROWS), e);
+              }
+            }
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ============================================================== MMA issuer (leader only)
+      if (leader && ptx::elect_one()) {
+        constexpr uint16_t BOTH = 0x3;
+        constexpr uint64_t kStage = STAGE_BYTES >> 4;
+        const uint64_t a0 = ptx::make_kmajor_desc<BLOCK>(sbase), b0 = ptx::make_kmajor_desc<BLOCK>(sbase + TILE_BYTES);
+        const uint32_t idesc = p.idesc | ((items.cols >> 3) << 17);
+        uint32_t s = 0, ph = 0, acc = 0, e_ph = 1;
+        bool ok = true;
+        for (uint32_t item = cluster_id; ok && item < items.total; item += clusters) {
+          if (!items.get(p, item, x)) continue;
+          for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+            ok = ptx::mbar_wait(sbase + ACC_EMPTY + 8 * acc, e_ph, abort_flag, p.status, ptx::kErrWaitD0Empty) &&
+                 ptx::mbar_wait(sbase + FULL + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitFull);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t d = tmem_base + acc * COLS;
+#pragma unroll
+            for (uint32_t ks = 0; ks < 4; ++ks)
+              ptx::mma_f8_ss_pair(d, a0 + s * kStage + 2 * ks, b0 + s * kStage + 2 * ks, idesc, ks != 0);
+            ptx::tc_commit_pair(sbase + EMPTY + 8 * s, BOTH);
+            ptx::tc_commit_pair(sbase + ACC_FULL + 8 * acc, BOTH);
+            acc ^= 1u;
+            if (acc == 0) e_ph ^= 1u;
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ================================================================ epilogue (both CTAs)
+    ptx::setmaxnreg_inc<REGS_EPI>();
+    Items<GATED> items(smem, p, clusters);
+    Tile x;
+    const uint32_t epi = warp - 4, quarter = warp & 3u, second = epi >> 2;
+    const uint32_t half = items.cols / 2;
+    const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + second * half;
+    const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
+    const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
+    const uint32_t w_blocks = ((GATED ? 2 * p.n : p.n) + BLOCK - 1) / BLOCK;
+    uint32_t acc = 0, f_ph = 0, pair_ph = 0, parity = 0;
+    bool ok = true;
+    for (uint32_t item = cluster_id; item < items.total; item += clusters) {
+      if (!items.get(p, item, x)) continue;
+      const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in the tile
+      const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
+      const bool real = lane < rows;
+      unsigned long long sums[HALF / 2];
+#pragma unroll
+      for (uint32_t i = 0; i < HALF / 2; ++i) sums[i] = 0;
+      if (x.blocks > 0) {
+        // scales: of the next two blocks on their way
+        const float *xs = p.x_scale + (x.row0 + lane0 + (real ? lane : 0u)) * p.x_scale_row + x.k0 * p.x_scale_block;
+        const uint32_t wb = (x.col0 + (GATED ? 0u : second * half)) / BLOCK;
+        const float *ws = p.w_scale + (static_cast<uint64_t>(x.group) * w_blocks + min(wb, w_blocks - 1)) * p.blocks + x.k0;
+        const float *us = GATED ? ws + static_cast<uint64_t>(p.n / BLOCK) * p.blocks : nullptr;
+        auto scale_of = [&](uint32_t kb) { return real && kb < x.blocks ? __ldg(xs + kb * p.x_scale_block) : 0.f; };
+        auto weight_of = [&](const float *w, uint32_t kb) { return kb < x.blocks ? __ldg(w + kb) : 0.f; };
+        float sx = 0.f, sx1 = 0.f, sw = 0.f, sw1 = 0.f, su = 0.f, su1 = 0.f;
+        if (rows > 0) {
+          sx = scale_of(0), sx1 = scale_of(1);
+          sw = weight_of(ws, 0), sw1 = weight_of(ws, 1);
+          if constexpr (GATED) su = weight_of(us, 0), su1 = weight_of(us, 1);
+        }
+#pragma unroll 1
+        for (uint32_t kb = 0; kb < x.blocks; ++kb) {
+          float sx2 = 0.f, sw2 = 0.f, su2 = 0.f;
+          if (rows > 0) {
+            sx2 = scale_of(kb + 2);
+            sw2 = weight_of(ws, kb + 2);
+            if constexpr (GATED) su2 = weight_of(us, kb + 2);
+          }
+          ok = ptx::warp_agrees(ptx::mbar_wait(sbase + ACC_FULL + 8 * acc, f_ph, abort_flag, p.status, ptx::kErrWaitD0Full));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          if (rows > 0) drain<GATED>(t_lanes + acc * COLS, sums, half, both(sx * sw), GATED ? both(sx * su) : 0ull);
+          // The reads of tensor memory are complete (wait::ld): that is all there is to order.
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster_relaxed(acc_empty + 8 * acc);
+          acc ^= 1u;
+          if (acc == 0) f_ph ^= 1u;
+          sx = sx1, sx1 = sx2, sw = sw1, sw1 = sw2;
+          if constexpr (GATED) su = su1, su1 = su2;
+        }
+        if (!ok) break;
+      }
+      if constexpr (GATED) {
+        // (both warps that have these lanes have rows, or neither)
+        if (rows == 0) continue;
+        auto meet = [&]() { // the other warp; false: the wait gave up
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(sbase + PAIR + 8 * quarter);
+          const bool met = ptx::warp_agrees(
+              ptx::mbar_wait(sbase + PAIR + 8 * quarter, pair_ph, abort_flag, p.status, ptx::kErrWaitD1Full));
+          pair_ph ^= 1u;
+          return met;
+        };
+        if (x.slices > 1) { // both are last, or neither
+          park(part_of(p, x.slot, rank, quarter, second * half), half, sums);
+          ok = meet();
+          if (!ok) break;
+          volatile uint32_t *last = reinterpret_cast<volatile uint32_t *>(smem + LAST) + quarter;
+          if (second == 0 && lane == 0) *last = is_last(p, x, rank, quarter);
+          ok = meet();
+          if (!ok) break;
+          if (*last == 0) continue;
+          join(part_of(p, x.slot - x.slice, rank, quarter, second * half), x.slices, half, sums);
+        }
+        float h[HALF / 2];
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < HALF / 4; ++i) {
+          h[2 * i] = activate(static_cast<Activation>(p.activation), low(sums[i])).value * low(sums[HALF / 4 + i]);
+          h[2 * i + 1] = activate(static_cast<Activation>(p.activation), high(sums[i])).value * high(sums[HALF / 4 + i]);
+          top = max(top, max(__float_as_uint(h[2 * i]) & 0x7fffffffu, __float_as_uint(h[2 * i + 1]) & 0x7fffffffu));
+        }
+        // (written again two tiles on, when the other warp has long read them: it has been met since)
+        uint32_t *tops = reinterpret_cast<uint32_t *>(smem + TOPS) + parity * 2 * ROWS_CTA + quarter * 32u + lane;
+        parity ^= 1u;
+        tops[second * ROWS_CTA] = top;
+        ok = meet();
+        if (!ok) break;
+        top = max(top, tops[(second ^ 1u) * ROWS_CTA]);
+        const auto type = static_cast<F8Type>(p.out_type);
+        const BlockScale s(__uint_as_float(top), type);
+        uint32_t w[16];
+        if (type == F8Type::e4m3) quantise_64<F8Type::e4m3>(s, h, w);
+        else quantise_64<F8Type::e5m2>(s, h, w);
+        const uint64_t row = x.row0 + lane0;
+        store_64_bytes(buf, w, static_cast<uint8_t *>(p.out) + row * p.ldo + x.col0 + second * (HALF / 2), p.ldo, rows,
+                       HALF / 2, p.vector_out != 0);
+        if (second == 0 && real) p.out_scale[(row + lane) * p.out_scale_row + x.col0 / BLOCK * p.out_scale_block] = s.scale;
+      } else {
+        const uint32_t col = x.col0 + second * half;
+        const uint32_t cols = p.n > col ? min(half, p.n - col) : 0u;
+        if (rows == 0 || cols == 0) continue;
+        if (x.slices > 1) {
+          park(part_of(p, x.slot, rank, quarter, second * half), half, sums);
+          const bool last = lane == 0 && is_last(p, x, rank, epi);
+          if (!__any_sync(0xffffffffu, last)) continue;
+          join(part_of(p, x.slot - x.slice, rank, quarter, second * half), x.slices, half, sums);
+        }
+        if (p.bias != nullptr && x.group < p.groups) {
+          const float *bias = p.bias + static_cast<uint64_t>(x.group) * p.n + col;
+#pragma unroll
+          for (uint32_t c = 0; c < HALF; c += 2)
+            sums[c / 2] = pair_of(low(sums[c / 2]) + (c < cols ? __ldg(bias + c) : 0.f),
+                                  high(sums[c / 2]) + (c + 1 < cols ? __ldg(bias + c + 1) : 0.f));
+        }
+        store_sums(p, buf, sums, (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col, rows, cols);
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  // The peer's shared memory and TMEM are in use by the leader's MMAs until the last accumulator has
+  // been announced in both CTAs; neither CTA leaves before the other has finished its epilogue.
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (*abort_flag) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// Per device and kernel, once (any thread): shared-memory attribute and the pairs the device keeps resident.
+template <bool GATED> cudaError_t set_up(int *clusters_out) {
+  static std::once_flag once[64];
+  static cudaError_t setup_error[64];
+  static int max_clusters[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::call_once(once[dev], [&]() {
+    const auto kernel = f8_gemm_kernel<GATED>;
+    setup_error[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    int sms = 0;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int clusters = sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    int active = 0;
+    if (setup_error[dev] == cudaSuccess && cudaOccupancyMaxActiveClusters(&active, kernel, &cfg) == cudaSuccess) {
+      if (active > 0 && active < clusters) clusters = active;
+    } else {
+      cudaGetLastError();
+    }
+    max_clusters[dev] = clusters > 0 ? clusters : 1;
+  });
+  *clusters_out = max_clusters[dev];
+  return setup_error[dev];
+}
+
+bool operand_map(CUtensorMap *map, const GroupedOperand &o, uint32_t box_rows) {
+  return make_byte_map(map, 1, o.ptr, {o.inner, o.outer, o.batch}, {o.ld, o.batch > 1 ? o.stride : o.ld},
+                       {BLOCK, box_rows, 1}, true);
+}
+
+template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, cudaStream_t stream) {
+  int clusters = 1;
+  const cudaError_t se = set_up<GATED>(&clusters);
+  if (se != cudaSuccess) return se;
+  CUtensorMap map_x, map_x_few, map_w, map_w_few;
+  if (!operand_map(&map_x_few, a.b, BOX_ROWS) || !operand_map(&map_w, a.a, GATED ? HALF / 2 : HALF))
+    return cudaErrorInvalidValue;
+  // boxes of 128 rows are for tiles that have as many; narrow tiles are not gated
+  map_x = map_x_few;
+  map_w_few = map_w;
+  if (a.rows > ROWS_CTA - BOX_ROWS && !operand_map(&map_x, a.b, ROWS_CTA)) return cudaErrorInvalidValue;
+  if (!GATED && !operand_map(&map_w_few, a.a, BOX_ROWS)) return cudaErrorInvalidValue;
+  F8Params p = {};
+  p.ends = a.ends;
+  p.out = a.out;
+  p.ldo = a.ldo;
+  p.x_scale = a.col_scale;
+  p.x_scale_row = f.x_scale_row;
+  p.x_scale_block = f.x_scale_block;
+  p.w_scale = a.lane_scale;
+  p.bias = a.bias;
+  p.out_scale = f.out_scale;
+  p.out_scale_row = f.out_scale_row;
+  p.out_scale_block = f.out_scale_block;
+  p.parts = a.parts;
+  p.counters = a.counters;
+  p.status = a.dev_status;
+  p.rows = a.rows;
+  p.groups = a.groups;
+  p.n = a.lane_dim;
+  p.blocks = (a.k + BLOCK - 1) / BLOCK;
+  // FP32 sums; the formats of A (x) and B (w), e4m3 (0) or e5m2 (1)
+  p.idesc = (1u << 4) | (static_cast<uint32_t>(f.x_type) << 7) | (static_cast<uint32_t>(f.w_type) << 10) | ((ROWS >> 4) << 24);
+  p.out_type = static_cast<uint16_t>(GATED ? f.out_type : static_cast<int>(a.out_type));
+  p.activation = static_cast<uint8_t>(f.activation);
+  const uint64_t out_bytes = GATED ? 1 : a.out_type == GroupedOut::f32 ? 4 : 2;
+  p.vector_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo * out_bytes % 16 == 0;
+  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), NUM_THREADS, SMEM, stream, map_x,
+                        map_x_few, map_w, map_w_few, p);
+}
+
+} // namespace
+
+std::size_t f8_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
+  const uint64_t pairs = num_sms / 2, features = a.f8->gated ? COLS / 2 : COLS;
+  // tiles there are at least: groups may leave some unfilled
+  const uint64_t least = ((a.rows + ROWS - 1) / ROWS) * ((a.lane_dim + features - 1) / features);
+  return least <= pairs / 2 ? pairs * 2 * PART * sizeof(float) : 0;
+}
+
+cudaError_t launch_f8_gemm(const GroupedArgs &a, cudaStream_t stream) {
+  return a.f8->gated ? launch<true>(a, *a.f8, stream) : launch<false>(a, *a.f8, stream);
+}
+
+} // namespace cumpsgemm_b200

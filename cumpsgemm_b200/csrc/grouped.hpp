@@ -8,7 +8,7 @@ namespace cumpsgemm_b200 {
 constexpr uint32_t kMaxGroups = 1024;
 constexpr uint32_t kMaxK8 = 131071; // 2^14 * k has to stay below 2^31
 
-enum class GroupedKind : int { f16 = 0, tcec = 1, i8 = 2 };
+enum class GroupedKind : int { f16 = 0, tcec = 1, i8 = 2, f8 = 3 };
 enum class GroupedOut : int { f16 = 0, bf16 = 1, f32 = 2 };
 
 // One operand as the tensor core reads it: `planes` x `batch` matrices of `outer` rows of `inner`
@@ -24,6 +24,7 @@ struct GroupedOperand {
 // result is contiguous in memory.
 //   product  lanes = n, columns = rows of a group, reduction = k; A = w, B = x
 //   wgrad    lanes and columns = n and k, or k and n; reduction = rows of a group
+struct F8Args; // of kind f8 (f8_gemm.cu)
 struct GroupedArgs {
   GroupedKind kind;
   GroupedOut out_type;
@@ -39,9 +40,10 @@ struct GroupedArgs {
   uint64_t ldo, stride_o; // elements; stride_o: wgrad only
   float alpha, beta;
   const float *unscale;    // tcec, nullable: two factors that take the scales of the operands off
-  const float *lane_scale; // i8: [groups][lane_dim]
-  const float *col_scale;  // i8: [rows]
-  const float *bias;       // i8, nullable: [groups][lane_dim]
+  const float *lane_scale; // i8: [groups][lane_dim]; f8: [groups][blocks of w's rows][blocks of k]
+  const float *col_scale;  // i8: [rows]; f8: of each row and block of k, steps in F8Args
+  const float *bias;       // i8, f8, nullable: [groups][lane_dim]
+  const F8Args *f8;
   float *parts; // nullable: grouped_parts_bytes() of workspace for the sums of slices
   unsigned *counters; // grouped_counters() words, zero between calls
   int *dev_status;
@@ -49,6 +51,19 @@ struct GroupedArgs {
 // Memory with which a call may cut tiles into slices of K; 0 where it will not.
 std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms);
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream);
+
+// What the product of 8-bit floating-point operands has besides: a is w, b is x; lane_dim the features of the
+// result (gated: w has twice as many rows).
+struct F8Args {
+  int x_type, w_type; // F8Type
+  uint64_t x_scale_row, x_scale_block;
+  bool gated; // then the result is of 8 bits (out_type: F8Type), with a scale for each row and block of 128
+  int activation, out_type;
+  float *out_scale;
+  uint64_t out_scale_row, out_scale_block;
+};
+std::size_t f8_parts_bytes(const GroupedArgs &a, unsigned num_sms);
+cudaError_t launch_f8_gemm(const GroupedArgs &a, cudaStream_t stream);
 
 // An operand brought into the form above: 8- or 16-bit elements copied to rows that TMA can address,
 // or FP32 elements split into hi and lo FP16 planes, after a multiplication by a power of two.
@@ -101,5 +116,43 @@ struct QuantizeArgs {
   float *scale;
 };
 cudaError_t launch_quantize_rows(const QuantizeArgs &a, unsigned num_sms, cudaStream_t stream);
+
+// Rows to 8-bit floating point with a scale for each block of 128 columns (block_rows.cu).
+struct BlockRowsArgs {
+  const void *x;
+  int type;       // GroupedOut
+  int q_type;     // F8Type
+  int activation; // Activation: act(gate) * up of rows of 2 * k is quantised; -1: the rows themselves
+  uint64_t ldx;
+  const int32_t *row_index; // nullable
+  uint32_t src_rows, rows, k;
+  uint8_t *q;
+  uint64_t ldq;
+  float *scale;
+  uint64_t scale_row, scale_block; // steps
+};
+cudaError_t launch_block_rows(const BlockRowsArgs &a, unsigned num_sms, cudaStream_t stream);
+// Matrices, with a scale for each 128 x 128: scale[matrix][block of n][block of k].
+struct WeightBlocksArgs {
+  const void *w;
+  int type, q_type;
+  uint64_t ldw, stridew;
+  uint32_t matrices, n, k;
+  uint8_t *q;
+  uint64_t ldq, strideq;
+  float *scale;
+};
+cudaError_t launch_weight_blocks(const WeightBlocksArgs &a, unsigned num_sms, cudaStream_t stream);
+
+// The elementwise passes of a gated block: pre is rows x 2 * hidden, the gate in front.
+struct GatedRowsArgs {
+  const void *pre;
+  const void *dh; // null: out = act(gate) * up (rows x hidden); else out = the gradient of pre
+  int type, activation;
+  uint64_t ldpre, lddh, ldo;
+  uint32_t rows, hidden;
+  void *out;
+};
+cudaError_t launch_gated_rows(const GatedRowsArgs &a, unsigned num_sms, cudaStream_t stream);
 
 } // namespace cumpsgemm_b200

@@ -1,5 +1,7 @@
 // C ABI of the products of rows grouped by expert (include/cumpsgemm/cumpsgemm_ext.h): checks of the
 // arguments, workspace, and what has to be done to the operands in front of the kernel.
+#include "activation.cuh"
+#include "block_scale.cuh"
 #include "grouped.hpp"
 
 #include <cumpsgemm/cumpsgemm_ext.h>
@@ -122,6 +124,14 @@ const char *check_sizes(uint64_t rows, uint64_t n, uint64_t k, uint32_t groups, 
 // 2048 x 2048 285 against 508.  With all of those rows in one group there is less to read for both: 97 against
 // 41 and 143 (stored n by k 190) against 52, so the most it costs is less than what it saves.
 bool takes_few_rows(uint64_t rows, uint32_t groups) { return rows <= 6ull * groups; }
+
+bool known_activation(int a) { return a >= 0 && a <= static_cast<int>(Activation::relu); }
+bool known_f8(cudaDataType_t t) { return t == CUDA_R_8F_E4M3 || t == CUDA_R_8F_E5M2; }
+int f8_type(cudaDataType_t t) { return static_cast<int>(t == CUDA_R_8F_E4M3 ? F8Type::e4m3 : F8Type::e5m2); }
+cublasStatus_t done(cuMpSGEMM_handle *h, cudaError_t e) {
+  mark_stream_work(h);
+  return e == cudaSuccess ? CUBLAS_STATUS_SUCCESS : CUBLAS_STATUS_EXECUTION_FAILED;
+}
 
 bool fp32_mode_ok(cuMpSGEMM_compute_mode_t mode) {
   return mode == CUMPSGEMM_FP16TCEC || mode == CUMPSGEMM_FP16TCEC_SCALING;
@@ -309,4 +319,254 @@ extern "C" cublasStatus_t cuMpSGEMM_quantize_rows_i8(cuMpSGEMM_handle_t h, uint6
   const cudaError_t e = launch_quantize_rows(a, h->num_sms, h->cuda_stream);
   mark_stream_work(h);
   return e == cudaSuccess ? CUBLAS_STATUS_SUCCESS : CUBLAS_STATUS_EXECUTION_FAILED;
+}
+
+static cublasStatus_t gated_rows(cuMpSGEMM_handle_t h, uint64_t rows, uint64_t hidden, const void *pre, uint64_t ldpre,
+                                 const void *dh, uint64_t lddh, int activation, void *out, uint64_t ldo,
+                                 cudaDataType_t type) {
+  GatedRowsArgs a = {};
+  a.pre = pre;
+  a.dh = dh;
+  a.type = static_cast<int>(out_type(type));
+  a.activation = activation;
+  a.ldpre = ldpre;
+  a.lddh = lddh;
+  a.ldo = ldo;
+  a.rows = static_cast<uint32_t>(rows);
+  a.hidden = static_cast<uint32_t>(hidden);
+  a.out = out;
+  return done(h, launch_gated_rows(a, h->num_sms, h->cuda_stream));
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_gated_rows(cuMpSGEMM_handle_t h, uint64_t rows, uint64_t hidden, const void *pre,
+                                               uint64_t ldpre, const void *dh, uint64_t lddh,
+                                               cuMpSGEMM_activation_t activation, void *out, uint64_t ldo,
+                                               cudaDataType_t type) {
+  static const char where[] = "cuMpSGEMM_gated_rows";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (hidden == 0) return refuse(where, "hidden must not be 0");
+  if (rows > kMaxDim || hidden > kMaxDim / 2) return refuse(where, "a size does not fit 31 bits");
+  if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (!known_activation(activation)) return refuse(where, "unknown activation");
+  if (ldpre < 2 * hidden || (dh != nullptr && lddh < hidden) || ldo < (dh != nullptr ? 2 * hidden : hidden))
+    return refuse(where, "a leading dimension is too small");
+  if (rows > 0 && (pre == nullptr || out == nullptr)) return refuse(where, "null pointer");
+  if (rows == 0) return CUBLAS_STATUS_SUCCESS;
+  DeviceGuard guard(h->device);
+  return gated_rows(h, rows, hidden, pre, ldpre, dh, lddh, activation, out, ldo, type);
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm_gated(
+    cuMpSGEMM_handle_t h, uint64_t rows, uint64_t hidden, uint64_t k, uint32_t num_groups, const int32_t *group_ends,
+    const void *x, uint64_t ldx, const void *w, uint64_t ldw, uint64_t stridew, cuMpSGEMM_activation_t activation,
+    void *y, uint64_t ldy, void *pre, uint64_t ldpre, cudaDataType_t type, cuMpSGEMM_compute_mode_t mode) {
+  static const char where[] = "cuMpSGEMM_grouped_gemm_gated";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (hidden > kMaxDim / 2) return refuse(where, "a size does not fit 31 bits");
+  if (const char *why = check_sizes(rows, 2 * hidden, k, num_groups, group_ends)) return refuse(where, why);
+  if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (!known_activation(activation)) return refuse(where, "unknown activation");
+  if (w == nullptr || (rows > 0 && (x == nullptr || y == nullptr || pre == nullptr))) return refuse(where, "null pointer");
+  if (ldx < k || ldy < hidden || ldw < k || (num_groups > 1 && stridew < (2 * hidden - 1) * ldw + k) ||
+      (pre != nullptr && ldpre < 2 * hidden))
+    return refuse(where, "a leading dimension or the stride of w is too small");
+  if (type == CUDA_R_32F && !fp32_mode_ok(mode)) {
+    log_error(std::string(where) + ": FP32 operands take FP16TCEC or FP16TCEC_SCALING");
+    return CUBLAS_STATUS_NOT_SUPPORTED;
+  }
+  if (rows == 0) return CUBLAS_STATUS_SUCCESS;
+
+  const float one = 1.f, zero = 0.f;
+  const cublasStatus_t st = cuMpSGEMM_grouped_gemm(h, CUBLAS_OP_T, rows, 2 * hidden, k, num_groups, group_ends, &one, x, ldx,
+                                                   w, ldw, stridew, &zero, pre, ldpre, type, mode);
+  if (st != CUBLAS_STATUS_SUCCESS) return st;
+  DeviceGuard guard(h->device);
+  return gated_rows(h, rows, hidden, pre, ldpre, nullptr, 0, activation, y, ldy, type);
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm_gated_grad(
+    cuMpSGEMM_handle_t h, cublasOperation_t op_W, uint64_t rows, uint64_t hidden, uint64_t k, uint32_t num_groups,
+    const int32_t *group_ends, const void *dy, uint64_t lddy, const void *w, uint64_t ldw, uint64_t stridew,
+    cuMpSGEMM_activation_t activation, const void *pre, uint64_t ldpre, void *dpre, uint64_t lddpre,
+    cudaDataType_t type, cuMpSGEMM_compute_mode_t mode) {
+  static const char where[] = "cuMpSGEMM_grouped_gemm_gated_grad";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (hidden > kMaxDim / 2) return refuse(where, "a size does not fit 31 bits");
+  if (const char *why = check_sizes(rows, hidden, k, num_groups, group_ends)) return refuse(where, why);
+  if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (!known_activation(activation)) return refuse(where, "unknown activation");
+  if (op_W != CUBLAS_OP_N && op_W != CUBLAS_OP_T && op_W != CUBLAS_OP_C) return refuse(where, "unknown op_W");
+  if (w == nullptr || (rows > 0 && (dy == nullptr || pre == nullptr || dpre == nullptr))) return refuse(where, "null pointer");
+  const bool w_n_contig = op_W == CUBLAS_OP_N;
+  const uint64_t w_inner = w_n_contig ? hidden : k, w_outer = w_n_contig ? k : hidden;
+  if (lddy < k || ldpre < 2 * hidden || lddpre < 2 * hidden || ldw < w_inner ||
+      (num_groups > 1 && stridew < (w_outer - 1) * ldw + w_inner))
+    return refuse(where, "a leading dimension or the stride of w is too small");
+  if (type == CUDA_R_32F && !fp32_mode_ok(mode)) {
+    log_error(std::string(where) + ": FP32 operands take FP16TCEC or FP16TCEC_SCALING");
+    return CUBLAS_STATUS_NOT_SUPPORTED;
+  }
+  if (rows == 0) return CUBLAS_STATUS_SUCCESS;
+
+  // dh goes to the first half of dpre, and the elementwise pass takes it from there
+  const float one = 1.f, zero = 0.f;
+  const cublasStatus_t st = cuMpSGEMM_grouped_gemm(h, op_W, rows, hidden, k, num_groups, group_ends, &one, dy, lddy, w, ldw,
+                                                   stridew, &zero, dpre, lddpre, type, mode);
+  if (st != CUBLAS_STATUS_SUCCESS) return st;
+  DeviceGuard guard(h->device);
+  return gated_rows(h, rows, hidden, pre, ldpre, dpre, lddpre, activation, dpre, lddpre, type);
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_quantize_rows_f8(cuMpSGEMM_handle_t h, uint64_t rows, uint64_t k, const void *x,
+                                                     uint64_t ldx, cudaDataType_t type, const int32_t *row_index,
+                                                     uint64_t src_rows, int activation, void *q, uint64_t ldq,
+                                                     cudaDataType_t q_type, float *scale, uint64_t scale_row,
+                                                     uint64_t scale_block) {
+  static const char where[] = "cuMpSGEMM_quantize_rows_f8";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (k == 0) return refuse(where, "k must not be 0");
+  if (rows > kMaxDim || k > kMaxDim / 2 || src_rows > kMaxDim) return refuse(where, "a size does not fit 31 bits");
+  if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (!known_f8(q_type)) return refuse(where, "q_type is not CUDA_R_8F_E4M3 or CUDA_R_8F_E5M2");
+  if (activation != CUMPSGEMM_ACTIVATION_NONE && !known_activation(activation)) return refuse(where, "unknown activation");
+  if (ldx < (activation == CUMPSGEMM_ACTIVATION_NONE ? k : 2 * k) || ldq < k)
+    return refuse(where, "a leading dimension is too small");
+  if (rows > 0 && (q == nullptr || scale == nullptr || (src_rows > 0 && x == nullptr))) return refuse(where, "null pointer");
+  if (row_index == nullptr && src_rows < rows) return refuse(where, "fewer rows in x than asked for, and no row_index");
+  if (rows == 0) return CUBLAS_STATUS_SUCCESS;
+
+  DeviceGuard guard(h->device);
+  BlockRowsArgs a = {};
+  a.x = x;
+  a.type = static_cast<int>(out_type(type));
+  a.q_type = f8_type(q_type);
+  a.activation = activation;
+  a.ldx = ldx;
+  a.row_index = row_index;
+  a.src_rows = static_cast<uint32_t>(src_rows);
+  a.rows = static_cast<uint32_t>(rows);
+  a.k = static_cast<uint32_t>(k);
+  a.q = static_cast<uint8_t *>(q);
+  a.ldq = ldq;
+  a.scale = scale;
+  a.scale_row = scale_row;
+  a.scale_block = scale_block;
+  return done(h, launch_block_rows(a, h->num_sms, h->cuda_stream));
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_quantize_blocks_f8(cuMpSGEMM_handle_t h, uint32_t matrices, uint64_t n, uint64_t k,
+                                                       const void *w, uint64_t ldw, uint64_t stridew, cudaDataType_t type,
+                                                       void *q, uint64_t ldq, uint64_t strideq, cudaDataType_t q_type,
+                                                       float *scale) {
+  static const char where[] = "cuMpSGEMM_quantize_blocks_f8";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (n == 0 || k == 0) return refuse(where, "n and k must not be 0");
+  if (n > kMaxDim || k > kMaxDim) return refuse(where, "a size does not fit 31 bits");
+  if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (!known_f8(q_type)) return refuse(where, "q_type is not CUDA_R_8F_E4M3 or CUDA_R_8F_E5M2");
+  if (ldw < k || ldq < k || (matrices > 1 && (stridew < (n - 1) * ldw + k || strideq < (n - 1) * ldq + k)))
+    return refuse(where, "a leading dimension or stride is too small");
+  if (matrices > 0 && (w == nullptr || q == nullptr || scale == nullptr)) return refuse(where, "null pointer");
+  if (matrices == 0) return CUBLAS_STATUS_SUCCESS;
+
+  DeviceGuard guard(h->device);
+  WeightBlocksArgs a = {};
+  a.w = w;
+  a.type = static_cast<int>(out_type(type));
+  a.q_type = f8_type(q_type);
+  a.ldw = ldw;
+  a.stridew = stridew;
+  a.matrices = matrices;
+  a.n = static_cast<uint32_t>(n);
+  a.k = static_cast<uint32_t>(k);
+  a.q = static_cast<uint8_t *>(q);
+  a.ldq = ldq;
+  a.strideq = strideq;
+  a.scale = scale;
+  return done(h, launch_weight_blocks(a, h->num_sms, h->cuda_stream));
+}
+
+// What both products of 8-bit floating-point operands check and set; n: rows of w.
+static cublasStatus_t f8_product(cuMpSGEMM_handle_t h, const char *where, uint64_t rows, uint64_t n, uint64_t k,
+                                 uint32_t num_groups, const int32_t *group_ends, const void *xq, uint64_t ldx,
+                                 cudaDataType_t x_type, const float *x_scale, const void *wq, uint64_t ldw, uint64_t stridew,
+                                 cudaDataType_t w_type, const float *w_scale, GroupedArgs &g, F8Args &f) {
+  if (const char *why = check_sizes(rows, n, k, num_groups, group_ends)) return refuse(where, why);
+  if (!known_f8(x_type) || !known_f8(w_type))
+    return refuse(where, "x_type or w_type is not CUDA_R_8F_E4M3 or CUDA_R_8F_E5M2");
+  if (wq == nullptr || w_scale == nullptr || (rows > 0 && (xq == nullptr || x_scale == nullptr || g.out == nullptr)))
+    return refuse(where, "null pointer");
+  if (ldx < k || ldw < k || (num_groups > 1 && stridew < (n - 1) * ldw + k))
+    return refuse(where, "a leading dimension or the stride of wq is too small");
+  if (rows == 0) return CUBLAS_STATUS_SUCCESS;
+
+  DeviceGuard guard(h->device);
+  g.kind = GroupedKind::f8;
+  g.a = {wq, k, n, ldw, stridew, 0, num_groups, 1};
+  g.b = {xq, k, rows, ldx, 0, 0, 1, 1};
+  g.ends = group_ends;
+  g.rows = static_cast<uint32_t>(rows);
+  g.groups = num_groups;
+  g.k = static_cast<uint32_t>(k);
+  g.lane_scale = w_scale;
+  g.col_scale = x_scale;
+  g.dev_status = h->dev_status;
+  g.f8 = &f;
+  f.x_type = f8_type(x_type);
+  f.w_type = f8_type(w_type);
+  const cublasStatus_t st = stage(h, where, g, 1, true, false);
+  return st == CUBLAS_STATUS_SUCCESS ? finish(h, g) : st;
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_f8_grouped_gemm(
+    cuMpSGEMM_handle_t h, uint64_t rows, uint64_t n, uint64_t k, uint32_t num_groups, const int32_t *group_ends,
+    const void *xq, uint64_t ldx, cudaDataType_t x_type, const float *x_scale, uint64_t x_scale_row, uint64_t x_scale_block,
+    const void *wq, uint64_t ldw, uint64_t stridew, cudaDataType_t w_type, const float *w_scale, const float *bias, void *y,
+    uint64_t ldy, cudaDataType_t y_type) {
+  static const char where[] = "cuMpSGEMM_f8_grouped_gemm";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (!known_type(y_type)) return refuse(where, "y_type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
+  if (ldy < n) return refuse(where, "the leading dimension of y is too small");
+  GroupedArgs g = {};
+  F8Args f = {};
+  g.out_type = out_type(y_type);
+  g.lane_dim = static_cast<uint32_t>(n);
+  g.out = y;
+  g.ldo = ldy;
+  g.bias = bias;
+  f.x_scale_row = x_scale_row;
+  f.x_scale_block = x_scale_block;
+  return f8_product(h, where, rows, n, k, num_groups, group_ends, xq, ldx, x_type, x_scale, wq, ldw, stridew, w_type, w_scale,
+                    g, f);
+}
+
+extern "C" cublasStatus_t cuMpSGEMM_f8_grouped_gemm_gated(
+    cuMpSGEMM_handle_t h, uint64_t rows, uint64_t hidden, uint64_t k, uint32_t num_groups, const int32_t *group_ends,
+    const void *xq, uint64_t ldx, cudaDataType_t x_type, const float *x_scale, uint64_t x_scale_row, uint64_t x_scale_block,
+    const void *wq, uint64_t ldw, uint64_t stridew, cudaDataType_t w_type, const float *w_scale,
+    cuMpSGEMM_activation_t activation, void *q, uint64_t ldq, cudaDataType_t q_type, float *scale, uint64_t scale_row,
+    uint64_t scale_block) {
+  static const char where[] = "cuMpSGEMM_f8_grouped_gemm_gated";
+  if (h == nullptr) return CUBLAS_STATUS_NOT_INITIALIZED;
+  if (hidden == 0 || hidden % 128 != 0) return refuse(where, "hidden is not a multiple of 128");
+  if (hidden > kMaxDim / 2) return refuse(where, "a size does not fit 31 bits");
+  if (!known_activation(activation)) return refuse(where, "unknown activation");
+  if (!known_f8(q_type)) return refuse(where, "q_type is not CUDA_R_8F_E4M3 or CUDA_R_8F_E5M2");
+  if (ldq < hidden) return refuse(where, "the leading dimension of q is too small");
+  if (rows > 0 && scale == nullptr) return refuse(where, "null pointer");
+  GroupedArgs g = {};
+  F8Args f = {};
+  g.lane_dim = static_cast<uint32_t>(hidden);
+  g.out = q;
+  g.ldo = ldq;
+  f.x_scale_row = x_scale_row;
+  f.x_scale_block = x_scale_block;
+  f.gated = true;
+  f.activation = activation;
+  f.out_type = f8_type(q_type);
+  f.out_scale = scale;
+  f.out_scale_row = scale_row;
+  f.out_scale_block = scale_block;
+  return f8_product(h, where, rows, 2 * hidden, k, num_groups, group_ends, xq, ldx, x_type, x_scale, wq, ldw, stridew, w_type,
+                    w_scale, g, f);
 }

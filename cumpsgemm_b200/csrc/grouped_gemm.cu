@@ -1094,6 +1094,7 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
 } // namespace
 
 std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
+  if (a.kind == GroupedKind::f8) return f8_parts_bytes(a, num_sms);
   const uint64_t pairs = num_sms / 2, lane_tiles = (a.lane_dim + LANES - 1) / LANES;
   // tiles there are at least: the groups of a product may leave some unfilled
   const uint64_t least = lane_tiles * (a.wgrad ? a.groups * static_cast<uint64_t>((a.col_dim + COLS - 1) / COLS)
@@ -1102,6 +1103,7 @@ std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
 }
 
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream) {
+  if (a.kind == GroupedKind::f8) return launch_f8_gemm(a, stream);
   if (a.kind == GroupedKind::i8) {
     if (a.wgrad || a.a_lane_contig) return cudaErrorInvalidValue;
     return launch<kI8, false, false>(a, stream);

@@ -7,8 +7,11 @@ the last total belong to no expert; their results are zero.
 
     ends = torch.bincount(expert_of_row, minlength=E).cumsum(0).to(torch.int32)
     y = grouped_linear(handle, x, w, ends)              # training: gradients of x and w
+    y = gated_feed_forward(handle, x, gate_up, down, ends)  # a gated block: gradients of all three
     q, s = quantize_rows(handle, x, row_index=tokens)   # serving: gather and quantise in one pass
     y = i8_matmul(handle, q, s, wq, w_scale, ends)
+    q, s = quantize_blocks(handle, x, row_index=tokens)  # the same in 8-bit floating point
+    y = f8_matmul(handle, q, s, wq, w_scale, ends)
 
 Everything goes through the C ABI (``cuMpSGEMM_grouped_gemm`` and its neighbours in
 ``cumpsgemm_ext.h``); there is no other implementation behind it.  Results are allocated on the current
@@ -23,6 +26,11 @@ import torch
 
 from . import api
 
+_F8_TYPES = {torch.float8_e4m3fn: api.CUDA_R_8F_E4M3, torch.float8_e5m2: api.CUDA_R_8F_E5M2}
+_ACTIVATIONS = {"silu": api.Activation.SILU, "gelu": api.Activation.GELU, "gelu_tanh": api.Activation.GELU_TANH,
+                "relu": api.Activation.RELU}
+_BLOCK = 128  # columns, or rows and columns, that share a scale in 8-bit floating point
+
 _DATA_TYPES = {torch.float16: api.CUDA_R_16F, torch.bfloat16: api.CUDA_R_16BF,
                torch.float32: api.CUDA_R_32F}
 
@@ -32,6 +40,20 @@ def _data_type(dtype) -> int:
         return _DATA_TYPES[dtype]
     except KeyError:
         raise ValueError(f"expected float16, bfloat16 or float32, got {dtype}") from None
+
+
+def _f8_type(dtype, what: str) -> int:
+    try:
+        return _F8_TYPES[dtype]
+    except KeyError:
+        raise ValueError(f"{what} must be float8_e4m3fn or float8_e5m2, got {dtype}") from None
+
+
+def _activation(name) -> int:
+    try:
+        return _ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {name!r}") from None
 
 
 # A call with few rows takes as long as its checks: they ask a tensor for each thing once.
@@ -327,3 +349,285 @@ def grouped_linear(handle: api.Handle, x, w, group_ends=None, transpose_w: bool 
     not for gradients, which FP16TCEC_SCALING takes at any magnitude.  16-bit operands look at neither."""
     return _GroupedLinear.apply(_dense_rows(x), _dense_rows(w), group_ends, handle, transpose_w, mode,
                                 backward_mode, 1.0)
+
+
+# ---------------------------------------------------------------- gated feed-forward blocks
+def _gated_shapes(handle, x, gate_up, group_ends):
+    """What a gated product checks; (rows, hidden, width, groups, leading dimensions ..., data type)."""
+    groups, both, width, ldw, stridew = _matrices_of(gate_up, "gate_up")
+    if both % 2:
+        raise ValueError(f"gate_up has {both} rows: as many of the gate as of what it gates are needed")
+    rows, _, ldx = _rows_of(x, "x", width)
+    _check(handle, x.get_device(), (gate_up,), group_ends, groups)
+    if x.dtype is not gate_up.dtype:
+        raise ValueError(f"x is {x.dtype}, gate_up is {gate_up.dtype}")
+    return rows, both // 2, width, groups, ldx, ldw, stridew, _data_type(x.dtype)
+
+
+def _gated(handle, x, gate_up, group_ends, act, mode, out=None):
+    """(act(gate) * up, both in front of that)."""
+    rows, hidden, width, groups, ldx, ldw, stridew, data_type = _gated_shapes(handle, x, gate_up, group_ends)
+    ldy = hidden
+    if out is not None:
+        _, _, ldy = _rows_of(out, "out")
+    out = _output(out, 0.0, (rows, hidden), x.dtype, x)
+    pre = x.new_empty((rows, 2 * hidden))
+    handle.grouped_gemm_gated(rows, hidden, width, groups, None if group_ends is None else group_ends.data_ptr(),
+                              x.data_ptr(), ldx, gate_up.data_ptr(), ldw, stridew, act, out.data_ptr(), ldy,
+                              pre.data_ptr(), 2 * hidden, data_type, mode)
+    return out, pre
+
+
+def _gated_rows_grad(handle, pre, dh, act):
+    rows, both = pre.shape
+    _, _, lddh = _rows_of(dh, "the gradient", both // 2)
+    _check_place(handle, dh.get_device())
+    if dh.dtype is not pre.dtype:
+        raise ValueError(f"the gradient is {dh.dtype}, the operands are {pre.dtype}")
+    dpre = torch.empty_like(pre)
+    handle.gated_rows(rows, both // 2, pre.data_ptr(), both, dh.data_ptr(), lddh, act, dpre.data_ptr(), both,
+                      _data_type(pre.dtype))
+    return dpre
+
+
+def _gated_grad(handle, dy, down, group_ends, pre, act, mode):
+    """The gradient of pre from that of the block's result."""
+    groups, width, hidden, ldw, stridew = _matrices_of(down, "down")
+    rows, _, lddy = _rows_of(dy, "the gradient", width)
+    _check(handle, dy.get_device(), (down,), group_ends, groups)
+    if dy.dtype is not pre.dtype:
+        raise ValueError(f"the gradient is {dy.dtype}, the operands are {pre.dtype}")
+    dpre = torch.empty_like(pre)
+    handle.grouped_gemm_gated_grad(api.CUBLAS_OP_N, rows, hidden, width, groups,
+                                   None if group_ends is None else group_ends.data_ptr(), dy.data_ptr(), lddy,
+                                   down.data_ptr(), ldw, stridew, act, pre.data_ptr(), 2 * hidden,
+                                   dpre.data_ptr(), 2 * hidden, _data_type(pre.dtype), mode)
+    return dpre
+
+
+def _composed(handle, x, gate_up, down, group_ends, act, mode):
+    """The same made of products that have gradients of any order, for those of gradients."""
+    f = torch.nn.functional
+    gate, up = _linear(x, gate_up, group_ends, handle, True, mode, 1.0).float().chunk(2, -1)
+    gate = {api.Activation.SILU: f.silu, api.Activation.GELU: f.gelu, api.Activation.RELU: f.relu,
+            api.Activation.GELU_TANH: lambda v: f.gelu(v, approximate="tanh")}[act](gate)
+    h = (gate * up).to(x.dtype)
+    return h if down is None else _linear(h, down, group_ends, handle, True, mode, 1.0)
+
+
+def _composed_gradients(ctx, dy, operands, handle, group_ends, act, mode):
+    wanted = [t for t, need in zip(operands, ctx.needs_input_grad) if need]
+    x, gate_up, down = operands if len(operands) == 3 else (*operands, None)
+    grads = iter(torch.autograd.grad(_composed(handle, x, gate_up, down, group_ends, act, mode), wanted, dy,
+                                     create_graph=True))
+    return [next(grads) if need else None for _, need in zip(operands, ctx.needs_input_grad)]
+
+
+class _GatedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_up, group_ends, handle, act, mode, backward_mode):
+        h, pre = _gated(handle, x, gate_up, group_ends, act, mode)
+        ctx.save_for_backward(x, gate_up, group_ends, pre)
+        ctx.how = (handle, act, backward_mode)
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        x, gate_up, group_ends, pre = ctx.saved_tensors
+        handle, act, mode = ctx.how
+        if torch.is_grad_enabled():
+            return (*_composed_gradients(ctx, dh, (x, gate_up), handle, group_ends, act, mode), *(None,) * 5)
+        dpre = _gated_rows_grad(handle, pre, _dense_rows(dh), act)
+        dx = dgate_up = None
+        if ctx.needs_input_grad[0]:
+            dx = grouped_matmul(handle, dpre, gate_up, group_ends, mode=mode)
+        if ctx.needs_input_grad[1]:
+            dgate_up = grouped_matmul_wgrad(handle, x, dpre, group_ends, True, mode=mode)
+        return dx, dgate_up, None, None, None, None, None
+
+
+class _GatedFeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_up, down, group_ends, handle, act, mode, backward_mode):
+        h, pre = _gated(handle, x, gate_up, group_ends, act, mode)
+        ctx.save_for_backward(x, gate_up, down, group_ends, pre, h)
+        ctx.how = (handle, act, backward_mode)
+        return grouped_matmul(handle, h, down, group_ends, True, mode=mode)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, gate_up, down, group_ends, pre, h = ctx.saved_tensors
+        handle, act, mode = ctx.how
+        if torch.is_grad_enabled():
+            return (*_composed_gradients(ctx, dy, (x, gate_up, down), handle, group_ends, act, mode), *(None,) * 5)
+        dy = _dense_rows(dy)
+        dx = dgate_up = ddown = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            dpre = _gated_grad(handle, dy, down, group_ends, pre, act, mode)
+        if ctx.needs_input_grad[0]:
+            dx = grouped_matmul(handle, dpre, gate_up, group_ends, mode=mode)
+        if ctx.needs_input_grad[1]:
+            dgate_up = grouped_matmul_wgrad(handle, x, dpre, group_ends, True, mode=mode)
+        if ctx.needs_input_grad[2]:
+            ddown = grouped_matmul_wgrad(handle, h, dy, group_ends, True, mode=mode)
+        return dx, dgate_up, ddown, None, None, None, None, None
+
+
+def gated_matmul(handle: api.Handle, x, gate_up, group_ends=None, *, activation: str = "silu",
+                 mode: int = api.ComputeMode.FP16TCEC, backward_mode: int = _BACKWARD_MODE, out=None):
+    """``out[r] = act(x[r] @ gate_e^T) * (x[r] @ up_e^T)`` for the rows r of each expert e; rows of none: 0.
+
+    x is (rows, width), gate_up (experts, 2 * hidden, width) with the rows of the gate first; all of float16,
+    bfloat16 or float32 (``mode``).  activation: "silu", "gelu" (by the error function), "gelu_tanh" or
+    "relu".  Products, activation and their product are FP32, rounded once.  Differentiable in x and
+    gate_up (without ``out``), any number of times; ``backward_mode`` as in ``grouped_linear``."""
+    act = _activation(activation)
+    x, gate_up = _dense_rows(x), _dense_rows(gate_up)
+    if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad):
+        _no_graph_through(out, 0.0)
+        return _GatedMatmul.apply(x, gate_up, group_ends, handle, act, mode, backward_mode)
+    return _gated(handle, x, gate_up, group_ends, act, mode, out)[0]
+
+
+def gated_feed_forward(handle: api.Handle, x, gate_up, down, group_ends=None, *, activation: str = "silu",
+                       mode: int = api.ComputeMode.FP16TCEC, backward_mode: int = _BACKWARD_MODE):
+    """``gated_matmul(handle, x, gate_up, ...) @ down_e^T`` for the rows of each expert e: a gated feed-forward
+    block, or one for each expert.  down is (experts, width, hidden).
+
+    Differentiable in x, gate_up and down, any number of times.  The block in between is rounded to the
+    operands' type, as is the gradient in front of the activation.  One expert without ``group_ends`` is a
+    dense block."""
+    act = _activation(activation)
+    x, gate_up, down = _dense_rows(x), _dense_rows(gate_up), _dense_rows(down)
+    if down.dim() != 3 or gate_up.dim() != 3 or down.shape[2] * 2 != gate_up.shape[1] or down.shape[0] != gate_up.shape[0]:
+        raise ValueError(f"down {tuple(down.shape)} does not fit gate_up {tuple(gate_up.shape)}")
+    if down.dtype is not x.dtype:
+        raise ValueError(f"x is {x.dtype}, down is {down.dtype}")
+    if down.get_device() != x.get_device():
+        raise ValueError("operands are on different devices")
+    if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad):
+        return _GatedFeedForward.apply(x, gate_up, down, group_ends, handle, act, mode, backward_mode)
+    return grouped_matmul(handle, _gated(handle, x, gate_up, group_ends, act, mode)[0], down, group_ends, True, mode=mode)
+
+
+# ---------------------------------------------------------------- 8-bit floating point
+def _blocks(n: int) -> int:
+    return (n + _BLOCK - 1) // _BLOCK
+
+
+def _f8_rows(like, rows: int, k: int, dtype):
+    """Room for such rows, which start at multiples of 16 bytes, and for their scales, rows side by side."""
+    ldq = (k + 15) // 16 * 16
+    q = like.new_empty((rows, ldq), dtype=dtype)
+    scale = like.new_empty((_blocks(k), rows), dtype=torch.float32)
+    return (q if ldq == k else q[:, :k]), ldq, scale.t()
+
+
+def quantize_blocks(handle: api.Handle, x, row_index=None, *, activation: Optional[str] = None,
+                    dtype=torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale): 8-bit floating-point rows with a float32 scale for each 128 columns, (rows, ceil(k / 128)):
+    ``scale[r, j // 128] * q[r, j]`` stands for ``x[r, j]``, or with ``row_index`` (int32) for
+    ``x[row_index[r], j]``; an index outside x gives a row of zeros.  dtype: float8_e4m3fn or float8_e5m2.
+
+    With an activation, x is (rows, 2 * k), and ``act(gate) * up`` of its halves is what is quantised.
+    q's rows start at multiples of 16 bytes, and a block's scales of all rows lie side by side, which is
+    what ``f8_matmul`` reads fastest.  No gradients."""
+    act = api.Activation.NONE if activation is None else _activation(activation)
+    src_rows, k, ldx = _rows_of(x, "x")
+    if activation is not None:
+        if k % 2:
+            raise ValueError(f"x has {k} columns: as many of the gate as of what it gates are needed")
+        k //= 2
+    device = x.get_device()
+    _check_place(handle, device)
+    data_type, q_type = _data_type(x.dtype), _f8_type(dtype, "dtype")
+    rows = src_rows
+    if row_index is not None:
+        if row_index.dtype is not torch.int32 or row_index.dim() != 1 or not row_index.is_contiguous():
+            raise ValueError("row_index must be a contiguous int32 vector")
+        if row_index.get_device() != device:
+            raise ValueError("row_index is on another device")
+        rows = row_index.shape[0]
+    q, ldq, scale = _f8_rows(x, rows, k, dtype)
+    handle.quantize_rows_f8(rows, k, x.data_ptr(), ldx, data_type,
+                            None if row_index is None else row_index.data_ptr(), src_rows, act, q.data_ptr(), ldq,
+                            q_type, scale.data_ptr(), 1, rows)
+    return q, scale
+
+
+def quantize_weight_blocks(handle: api.Handle, w, *, dtype=torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of weights (experts, n, k) or (n, k), with a float32 scale for each 128 x 128 of a matrix:
+    (experts, ceil(n / 128), ceil(k / 128)), or without the first.  No gradients."""
+    stack = w if w.dim() == 3 else w.unsqueeze(0)
+    matrices, n, k, ldw, stridew = _matrices_of(stack, "w")
+    _check_place(handle, w.get_device())
+    ldq = (k + 15) // 16 * 16
+    q = w.new_empty((matrices, n, ldq), dtype=dtype)
+    scale = w.new_empty((matrices, _blocks(n), _blocks(k)), dtype=torch.float32)
+    handle.quantize_blocks_f8(matrices, n, k, stack.data_ptr(), ldw, stridew, _data_type(w.dtype), q.data_ptr(), ldq,
+                              n * ldq, _f8_type(dtype, "dtype"), scale.data_ptr())
+    q = q if ldq == k else q[..., :k]
+    return (q, scale) if w.dim() == 3 else (q[0], scale[0])
+
+
+def _f8_operands(handle, xq, x_scale, wq, w_scale, group_ends, others=()):
+    """What both products check: (rows, n, k, groups, ldx, ldw, stridew, types, steps of x_scale)."""
+    groups, n, k, ldw, stridew = _matrices_of(wq, "wq")
+    rows, _, ldx = _rows_of(xq, "xq", k)
+    _check(handle, xq.get_device(), (x_scale, wq, w_scale, *others), group_ends, groups)
+    x_type, w_type = _f8_type(xq.dtype, "xq"), _f8_type(wq.dtype, "wq")
+    if x_scale.dtype is not torch.float32 or tuple(x_scale.shape) != (rows, _blocks(k)):
+        raise ValueError(f"x_scale must be float32 of shape {(rows, _blocks(k))}")
+    _check_scales(w_scale, "w_scale", groups * _blocks(n) * _blocks(k))
+    return rows, n, k, groups, ldx, ldw, stridew, x_type, w_type, x_scale.stride()
+
+
+def f8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, bias=None, out=None,
+              out_dtype=torch.bfloat16):
+    """``out[r] = x[r] @ w_e^T + bias[e]`` for the rows r of each expert e, x and w being what 8-bit values and
+    scales stand for; rows of none: 0.
+
+    xq is (rows, k) and wq (experts, n, k), each of float8_e4m3fn or float8_e5m2; x_scale (rows, ceil(k / 128)),
+    w_scale (experts, ceil(n / 128), ceil(k / 128)) and bias (experts, n), float32.  A (n, k) wq with
+    its scales is one expert of all rows: a plain linear layer.  No gradients."""
+    if wq.dim() == 2:
+        wq = wq.unsqueeze(0)
+    rows, n, k, groups, ldx, ldw, stridew, x_type, w_type, steps = _f8_operands(
+        handle, xq, x_scale, wq, w_scale, group_ends, () if bias is None else (bias,))
+    if bias is not None:
+        _check_scales(bias, "bias", groups * n)
+    ldy = n
+    if out is not None:
+        out_dtype = out.dtype
+        _, _, ldy = _rows_of(out, "out")
+    data_type = _data_type(out_dtype)
+    out = _output(out, 0.0, (rows, n), out_dtype, xq)
+    handle.f8_grouped_gemm(rows, n, k, groups, None if group_ends is None else group_ends.data_ptr(), xq.data_ptr(),
+                           ldx, x_type, x_scale.data_ptr(), steps[0], steps[1], wq.data_ptr(), ldw, stridew, w_type,
+                           w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), ldy,
+                           data_type)
+    return out
+
+
+def f8_gated_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, activation: str = "silu",
+                    dtype=torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of ``act(x[r] @ gate_e^T) * (x[r] @ up_e^T)`` as ``quantize_blocks`` gives them, for ``f8_matmul``
+    with the weights behind: operands as there, wq being (experts, 2 * hidden, k) with the rows of the gate
+    first.  Products, activation and their product are FP32.  Where hidden is a multiple of 128 nothing else
+    reaches memory; other sizes take a product to FP32 and a pass over it.  No gradients."""
+    act = _activation(activation)
+    if wq.dim() == 2:
+        wq = wq.unsqueeze(0)
+    if wq.dim() == 3 and wq.shape[1] % 2:
+        raise ValueError(f"wq has {wq.shape[1]} rows: as many of the gate as of what it gates are needed")
+    if wq.dim() != 3 or (wq.shape[1] // 2) % _BLOCK:
+        pre = f8_matmul(handle, xq, x_scale, wq, w_scale, group_ends, out_dtype=torch.float32)
+        return quantize_blocks(handle, pre, activation=activation, dtype=dtype)
+    rows, n, k, groups, ldx, ldw, stridew, x_type, w_type, steps = _f8_operands(handle, xq, x_scale, wq, w_scale, group_ends)
+    q_type = _f8_type(dtype, "dtype")
+    q, ldq, scale = _f8_rows(xq, rows, n // 2, dtype)
+    handle.f8_grouped_gemm_gated(rows, n // 2, k, groups, None if group_ends is None else group_ends.data_ptr(),
+                                 xq.data_ptr(), ldx, x_type, x_scale.data_ptr(), steps[0], steps[1], wq.data_ptr(), ldw,
+                                 stridew, w_type, w_scale.data_ptr(), act, q.data_ptr(), ldq, q_type, scale.data_ptr(),
+                                 1, rows)
+    return q, scale

@@ -420,6 +420,81 @@ cublasStatus_t cuMpSGEMM_quantize_rows_i8(cuMpSGEMM_handle_t handle, uint64_t ro
                                           const int32_t *row_index, uint64_t src_rows, int8_t *q,
                                           uint64_t ldq, float *scale);
 
+/* Gated feed-forward blocks: h = act(gate) * up, where gate and up are the halves of pre = x w^T; w_e is stored
+ * 2 hidden x k, the rows of the gate first.  Sums, the activation and its derivative are FP32, and each result is
+ * rounded once.  gelu is x (1 + erf(x / sqrt 2)) / 2, gelu_tanh its usual approximation by tanh. */
+typedef enum {
+  CUMPSGEMM_ACTIVATION_NONE = -1,
+  CUMPSGEMM_ACTIVATION_SILU = 0,
+  CUMPSGEMM_ACTIVATION_GELU = 1,
+  CUMPSGEMM_ACTIVATION_GELU_TANH = 2,
+  CUMPSGEMM_ACTIVATION_RELU = 3
+} cuMpSGEMM_activation_t;
+/* y[r, :] = act(x[r] gate_e^T) * (x[r] up_e^T) for the rows r of each group e; rows of no group: 0.  x is rows x k,
+ * y rows x hidden; pre (rows x 2 hidden) receives the rounded products, which the backward pass needs. */
+cublasStatus_t cuMpSGEMM_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
+                                            uint64_t k, uint32_t num_groups, const int32_t *group_ends,
+                                            const void *x, uint64_t ldx, const void *w, uint64_t ldw,
+                                            uint64_t stridew, cuMpSGEMM_activation_t activation, void *y,
+                                            uint64_t ldy, void *pre, uint64_t ldpre, cudaDataType_t type,
+                                            cuMpSGEMM_compute_mode_t mode);
+/* Backwards through the product behind it as well: with dh = dy op(w_e) (dy rows x k, w_e stored k x hidden,
+ * CUBLAS_OP_N, or hidden x k, CUBLAS_OP_T), dpre = [dh * up * act'(gate), dh * act(gate)].  pre: as the call above
+ * left it.  Rows of no group: 0. */
+cublasStatus_t cuMpSGEMM_grouped_gemm_gated_grad(cuMpSGEMM_handle_t handle, cublasOperation_t op_W,
+                                                 uint64_t rows, uint64_t hidden, uint64_t k,
+                                                 uint32_t num_groups, const int32_t *group_ends,
+                                                 const void *dy, uint64_t lddy, const void *w, uint64_t ldw,
+                                                 uint64_t stridew, cuMpSGEMM_activation_t activation,
+                                                 const void *pre, uint64_t ldpre, void *dpre, uint64_t lddpre,
+                                                 cudaDataType_t type, cuMpSGEMM_compute_mode_t mode);
+/* The elementwise passes by themselves: out = act(gate) * up (rows x hidden), or where dh (rows x hidden) is not
+ * NULL, out = dpre (rows x 2 hidden) as above. */
+cublasStatus_t cuMpSGEMM_gated_rows(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
+                                    const void *pre, uint64_t ldpre, const void *dh, uint64_t lddh,
+                                    cuMpSGEMM_activation_t activation, void *out, uint64_t ldo,
+                                    cudaDataType_t type);
+
+/* 8-bit floating point (CUDA_R_8F_E4M3, CUDA_R_8F_E5M2) with a scale for each block of 128 columns of a row, or of
+ * 128 x 128 of a matrix; the last blocks may be smaller.  With top the largest magnitude in a block and M the type's
+ * largest value (448, 57344), scale = top / M and q[i] is the value nearest to x[i] M / top (product and quotient
+ * rounded to FP32).  A block of zeros, or so small that its scale is 0 in FP32, has scale 0 and q = 0, one with an
+ * infinity or NaN scale NaN and q = 0 (its products are NaN).
+ *   Scales of rows lie at scale[row * scale_row + block * scale_block], those of weights one behind the other:
+ *   [matrix][block of n][block of k]. */
+/* Row r is taken from row row_index[r] of x (NULL: r); an index outside [0, src_rows) gives a row of zeros.  With an
+ * activation, x has rows of 2 k, and act(gate) * up of their halves, in FP32, is what is brought to 8 bits. */
+cublasStatus_t cuMpSGEMM_quantize_rows_f8(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t k, const void *x,
+                                          uint64_t ldx, cudaDataType_t type, const int32_t *row_index,
+                                          uint64_t src_rows, int activation, void *q, uint64_t ldq,
+                                          cudaDataType_t q_type, float *scale, uint64_t scale_row,
+                                          uint64_t scale_block);
+cublasStatus_t cuMpSGEMM_quantize_blocks_f8(cuMpSGEMM_handle_t handle, uint32_t matrices, uint64_t n, uint64_t k,
+                                            const void *w, uint64_t ldw, uint64_t stridew, cudaDataType_t type,
+                                            void *q, uint64_t ldq, uint64_t strideq, cudaDataType_t q_type,
+                                            float *scale);
+/* y[r, c] = sum over blocks b of k of x_scale[r, b] w_scale[e, c / 128, b] sum_{i in b} xq[r, i] wq_e[c, i]
+ * (+ bias[e * n + c]) for the rows r of each group e; rows of no group: 0.  wq_e is stored n x k.  The products of a
+ * block are added in FP32 by the tensor core, the blocks in FP32, and the result is rounded once to y_type. */
+cublasStatus_t cuMpSGEMM_f8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t n, uint64_t k,
+                                         uint32_t num_groups, const int32_t *group_ends, const void *xq,
+                                         uint64_t ldx, cudaDataType_t x_type, const float *x_scale,
+                                         uint64_t x_scale_row, uint64_t x_scale_block, const void *wq,
+                                         uint64_t ldw, uint64_t stridew, cudaDataType_t w_type,
+                                         const float *w_scale, const float *bias, void *y, uint64_t ldy,
+                                         cudaDataType_t y_type);
+/* The gated product with such operands, act(x gate_e^T) * (x up_e^T) of unrounded FP32 products, brought to 8 bits
+ * again: q (rows x hidden) and its scales.  wq_e is stored 2 hidden x k; hidden is a multiple of 128. */
+cublasStatus_t cuMpSGEMM_f8_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
+                                               uint64_t k, uint32_t num_groups, const int32_t *group_ends,
+                                               const void *xq, uint64_t ldx, cudaDataType_t x_type,
+                                               const float *x_scale, uint64_t x_scale_row,
+                                               uint64_t x_scale_block, const void *wq, uint64_t ldw,
+                                               uint64_t stridew, cudaDataType_t w_type, const float *w_scale,
+                                               cuMpSGEMM_activation_t activation, void *q, uint64_t ldq,
+                                               cudaDataType_t q_type, float *scale, uint64_t scale_row,
+                                               uint64_t scale_block);
+
 #ifdef __cplusplus
 }
 #endif
