@@ -19,29 +19,35 @@ struct ActResult {
   float value, slope;
 };
 
-__device__ __forceinline__ float logistic(float v) { return 1.f / (1.f + expf(-v)); }
+// FAST: for results of 16 or 8 bits.  exp by the approximation of 2^x, whose relative error is 2^-22 + |v| 2^-23, and
+// the quotient to 2 units in the last place; both are far inside the rounding that follows.  Where exp(-v) passes
+// 2^126 the quotient is 0 for what is at most 2^-126.
+template <bool FAST> __device__ __forceinline__ float logistic(float v) {
+  if constexpr (FAST) return __fdividef(1.f, 1.f + __expf(-v));
+  else return 1.f / (1.f + expf(-v));
+}
 
 // The slope costs nothing where it is not used.
-__device__ __forceinline__ ActResult activate(Activation a, float g) {
+template <bool FAST = false> __device__ __forceinline__ ActResult activate(Activation a, float g) {
   constexpr float kRootHalf = 0.707106781186547524f, kRootTwoOverPi = 0.797884560802865356f,
                   kOverRootTwoPi = 0.398942280401432678f, kCubic = 0.044715f;
   ActResult r;
   switch (a) {
   case Activation::silu: {
-    const float p = logistic(g), q = p * (1.f - p);
+    const float p = logistic<FAST>(g), q = p * (1.f - p);
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(g, q, p) : p;
     break;
   }
   case Activation::gelu: {
-    const float p = 0.5f * erfcf(-g * kRootHalf), q = kOverRootTwoPi * expf(-0.5f * g * g);
+    const float p = 0.5f * erfcf(-g * kRootHalf), e = -0.5f * g * g, q = kOverRootTwoPi * (FAST ? __expf(e) : expf(e));
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(g, q, p) : p;
     break;
   }
   case Activation::gelu_tanh: {
     const float gg = g * g;
-    const float p = logistic(2.f * kRootTwoOverPi * g * fmaf(kCubic, gg, 1.f)), q = p * (1.f - p);
+    const float p = logistic<FAST>(2.f * kRootTwoOverPi * g * fmaf(kCubic, gg, 1.f)), q = p * (1.f - p);
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(2.f * g * q, kRootTwoOverPi * fmaf(3.f * kCubic, gg, 1.f), p) : p;
     break;

@@ -18,7 +18,7 @@
 // no lane needs.
 //
 // Gated: a CTA loads rows of the gate and the same ones of the projection it gates, so that the columns of an
-// epilogue warp are half the one and half the other, and a thread has both for its features; two warps
+// epilogue warp are half the one and half the other, and a thread has both for its features; four warps
 // share the largest magnitude of 128 features.
 //
 // Tiles take equal time, so they are dealt to the pairs in turn.  A launch with few tiles cuts them into slices of
@@ -28,11 +28,14 @@
 //   full[s]       leader's only: 2 arrivals, one from each CTA's producer, and the bytes of both CTAs' loads
 //   empty[s]      in both CTAs: commit multicast from the leader
 //   acc_full[b]   in both CTAs: commit multicast
-//   acc_empty[b]  leader's only: 16 arrivals, one from each epilogue warp of both CTAs
-//   pair[q]       own, gated: 2 arrivals, one from each epilogue warp that has quarter q of the lanes
+//   acc_empty[b]  leader's only: 32 arrivals, one from each epilogue warp of both CTAs
+//   tile_full[i]  own: 1 arrival, from the warp that works out the tiles
+//   tile_empty[i] own: 1 arrival from each role that took the tile
+//   pair[q]       own, gated: 4 arrivals, one from each epilogue warp that has quarter q of the lanes
 // Every wait is bounded; no TMA multicast is used.
 #include "activation.cuh"
 #include "block_scale.cuh"
+#include "epilogue.cuh"
 #include "gemm_common.cuh"
 #include "grouped.hpp"
 #include "ptx.cuh"
@@ -48,33 +51,40 @@ namespace {
 constexpr uint32_t ROWS_CTA = 128, ROWS = 2 * ROWS_CTA; // lanes of a CTA and of a pair
 constexpr uint32_t COLS = 256;                          // most columns of a tile
 constexpr uint32_t WIDTHS = 3;                          // that a launch chooses from: 256, 128, 64
-constexpr uint32_t HALF = COLS / 2;                     // most columns of a warp
+constexpr uint32_t PARTS = 4;                           // epilogue warps that share the columns of 32 lanes
+constexpr uint32_t MOST = COLS / PARTS;                 // most columns of a warp
 constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
 constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
 constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
-constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 6;
-constexpr int NUM_THREADS = 384;
-constexpr int NUM_EPI_WARPS = 8;
+constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 5;
+constexpr int NUM_EPI_WARPS = 4 * PARTS;
+constexpr int NUM_THREADS = 128 + 32 * NUM_EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t BAND = 8;        // row tiles that are walked together
 constexpr uint32_t MAX_SLICES = 16;
 constexpr uint32_t MIN_SLICE = 4;   // least blocks of K in a slice
 constexpr uint32_t PART = COLS * ROWS_CTA; // elements of a parked sum of one CTA
 constexpr uint32_t JOIN_AHEAD = 4;
+constexpr uint32_t RING = 4;        // blocks of K whose scales a warp has in shared memory or on their way
+constexpr uint32_t SCALE_BYTES = RING * (32 + 2) * 4; // of a warp: each lane's own, then those of the weights
+constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
 constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
-// Registers: 384 threads are launched with 168 each; the four warps that issue give back what the eight that
-// hold 128 sums each take.
-constexpr int REGS_REST = 64, REGS_EPI = 216;
-static_assert(128 * REGS_REST + 256 * REGS_EPI <= 384 * 168, "setmaxnreg draws on the launch's registers");
+// Registers: 640 threads are launched with 96 each; the four warps that issue give back what the sixteen that
+// hold 64 sums a thread take.
+constexpr int REGS_LAUNCH = PARTS == 4 ? 96 : 168, REGS_REST = 64, REGS_EPI = PARTS == 4 ? 104 : 216;
+static_assert(128 * REGS_REST + 32 * NUM_EPI_WARPS * REGS_EPI <= NUM_THREADS * REGS_LAUNCH,
+              "setmaxnreg draws on the launch's registers");
 
 constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
-                   ACC_EMPTY = ACC_FULL + 16, TMEM_PTR = ACC_EMPTY + 16, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 8,
-                   PAIR = WIDTH + 4, LAST = PAIR + 8 * 4, // gated, for each quarter of the lanes
-                   TOPS = BARS + 256,                     // gated: largest magnitudes, [tile's parity][half][lane]
-                   START = TOPS + 4 * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
-                   OUT = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                   BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
-static_assert(PAIR % 8 == 0 && LAST + 4 * 4 <= TOPS, "barriers and flags");
+                   ACC_EMPTY = ACC_FULL + 16, TILE_FULL = ACC_EMPTY + 16, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
+                   PAIR = TILE_EMPTY + 8 * AHEAD, // gated, for each quarter of the lanes
+                   LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
+                   TILE = BARS + 320,                // the tiles of the roles
+                   TOPS = TILE + AHEAD * 48,         // gated: largest magnitudes, [tile's parity][part][lane]
+                   START = TOPS + 2 * PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
+                   SCALE = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
+                   OUT = SCALE + NUM_EPI_WARPS * SCALE_BYTES, BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
+static_assert(PAIR % 8 == 0 && WIDTH + 4 <= TILE && TILE % 16 == 0 && OUT % 16 == 0, "barriers and flags");
 constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 static_assert(SMEM <= 232448, "shared memory of a CTA");
 
@@ -99,35 +109,60 @@ struct F8Params {
 };
 
 // A tile, or a slice of one: `rows` rows from row0 on, features from col0 on, blocks [k0, k0 + blocks) of K.
-struct Tile {
-  uint32_t group, row0, rows, col0, k0, blocks, slices, slice, slot, number;
+struct alignas(16) Tile {
+  uint32_t group, row0, rows, col0; // rows == 0: there are no more tiles
+  uint32_t k0, blocks, slices, slice;
+  uint32_t slot, number, pad0, pad1;
 };
+static_assert(sizeof(Tile) == 48, "three times 16 bytes");
+
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+template <class T> __device__ __forceinline__ T ld_shared_one(uint32_t addr) {
+  if constexpr (sizeof(T) == 1) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return static_cast<T>(v);
+  } else if constexpr (sizeof(T) == 2) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return v;
+  } else {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+  }
+}
 
 // The items of a launch, which are tiles or slices of tiles, by their numbers: groups in turn; within one, bands
 // of row tiles that all column tiles pass over, so that what runs at the same time shares operands in L2.
 template <bool GATED> struct Items {
-  const uint32_t *start, *first_tile;
-  uint32_t group, total, slices, cols, features; // features: of the result, in a tile
-  __device__ __forceinline__ Items(const uint8_t *smem, const F8Params &p, uint32_t clusters) {
-    start = reinterpret_cast<const uint32_t *>(smem + START);
-    first_tile = reinterpret_cast<const uint32_t *>(smem + FIRST_TILE);
-    cols = *reinterpret_cast<const uint32_t *>(smem + WIDTH);
-    features = GATED ? cols / 2 : cols;
-    group = 0;
-    const uint32_t tiles = first_tile[p.groups + 1];
+  uint32_t sbase, group, total, slices, cols;
+  __device__ __forceinline__ Items(uint32_t sbase_, const F8Params &p, uint32_t clusters) : sbase(sbase_), group(0) {
+    cols = ld_shared_one<uint32_t>(sbase + WIDTH);
+    const uint32_t tiles = first_tile(p.groups + 1);
     slices = p.parts != nullptr && tiles > 0 && tiles <= clusters / 2
                  ? max(1u, min(min(clusters / tiles, p.blocks / MIN_SLICE), MAX_SLICES))
                  : 1u;
     total = tiles * slices;
   }
+  __device__ __forceinline__ uint32_t start(uint32_t g) const { return ld_shared_one<uint32_t>(sbase + START + 4 * g); }
+  __device__ __forceinline__ uint32_t first_tile(uint32_t g) const { return ld_shared_one<uint32_t>(sbase + FIRST_TILE + 4 * g); }
   // item < total, and not below that of an earlier call; false: it is none (a tile of zeros has one slice)
   __device__ __forceinline__ bool get(const F8Params &p, uint32_t item, Tile &x) {
     x.number = slices > 1 ? item / slices : item;
     x.slot = item;
-    while (x.number >= first_tile[group + 1]) ++group;
-    const uint32_t r0 = start[group], r = start[group + 1] - r0;
+    while (x.number >= first_tile(group + 1)) ++group;
+    const uint32_t features = GATED ? cols / 2 : cols; // of the result, in a tile
+    const uint32_t r0 = start(group), r = start(group + 1) - r0;
     const uint32_t row_tiles = (r + ROWS - 1) / ROWS, col_tiles = (p.n + features - 1) / features;
-    const uint32_t local = x.number - first_tile[group];
+    const uint32_t local = x.number - first_tile(group);
     const uint32_t band = local / (BAND * col_tiles), in_band = local - band * BAND * col_tiles;
     const uint32_t height = min(BAND, row_tiles - band * BAND);
     const uint32_t ct = in_band / height, rt = band * BAND + (in_band - ct * height);
@@ -142,6 +177,45 @@ template <bool GATED> struct Items {
     x.k0 = all * x.slice / x.slices;
     x.blocks = all * (x.slice + 1) / x.slices - x.k0;
     return true;
+  }
+};
+
+// The tiles a role takes, as a warp of its CTA works them out: a handful of divisions, 500 cycles.
+template <bool WARP> struct Tiles { // taken by a warp, or by one thread
+  uint32_t sbase, turn, phase;
+  __device__ __forceinline__ explicit Tiles(uint32_t sbase_) : sbase(sbase_), turn(0), phase(0) {}
+  // the next tile is there; false: the wait gave up
+  __device__ __forceinline__ bool wait(int *status) const {
+    const bool ok = ptx::mbar_wait_s(sbase + TILE_FULL + 8 * turn, phase, sbase + ABORT, status, ptx::kErrWaitTile);
+    return WARP ? ptx::warp_agrees(ok) : ok;
+  }
+  __device__ __forceinline__ uint32_t advance() { // returns the turn it was
+    const uint32_t was = turn;
+    if (++turn == AHEAD) {
+      turn = 0;
+      phase ^= 1u;
+    }
+    return was;
+  }
+  __device__ __forceinline__ void read(uint32_t at, Tile &x) const {
+    const uint4 a = ld_shared(sbase + TILE + 48 * at), b = ld_shared(sbase + TILE + 48 * at + 16),
+                c = ld_shared(sbase + TILE + 48 * at + 32);
+    x.group = a.x, x.row0 = a.y, x.rows = a.z, x.col0 = a.w;
+    x.k0 = b.x, x.blocks = b.y, x.slices = b.z, x.slice = b.w;
+    x.slot = c.x, x.number = c.y;
+  }
+  // by all of the warp, or the thread, when what was read has come (its words have been used)
+  __device__ __forceinline__ void give_back(uint32_t at) const {
+    if (WARP) __syncwarp();
+    if (!WARP || (threadIdx.x & 31u) == 0) ptx::mbar_arrive(sbase + TILE_EMPTY + 8 * at);
+  }
+  // one thread: the next tile; false at the end, or where the wait gave up
+  __device__ __forceinline__ bool next(int *status, Tile &x) {
+    if (!wait(status)) return false;
+    const uint32_t at = advance();
+    read(at, x);
+    give_back(at); // (a release: the reads are in front of it)
+    return x.rows != 0;
   }
 };
 
@@ -209,54 +283,55 @@ __device__ __forceinline__ void find_groups(uint8_t *smem, const F8Params &p, ui
   }
 }
 
-__device__ __forceinline__ unsigned long long both(float x) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(x));
-  return v;
+__device__ __forceinline__ void copy_word(uint32_t to, const float *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ float low(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float high(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-  return v;
-}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// sums += scale * the first `cols` columns from taddr on (a multiple of 16), two columns to an instruction.  The
-// next 16 are on their way while these are added.  Gated: the second half of the columns has a scale of its own.
+// sums += scale * the first `cols` columns from taddr on (a multiple of 16).  Gated: the second half of the columns
+// has a scale of its own.  (Packed in pairs, fma.rn.f32x2, the additions took twice as long: 680 cycles a stage
+// against 366, 16 warps of 64 columns; the unit's rate is the same, and the pairs have to be moved together.)
 template <bool GATED>
-__device__ __forceinline__ void drain(uint32_t taddr, unsigned long long (&sums)[HALF / 2], uint32_t cols,
-                                      unsigned long long s0, unsigned long long s1) {
-  uint32_t v[2][16];
-  ptx::tmem_ld_32x32b_x16(taddr, v[0]);
+__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[MOST], uint32_t cols, float s0, float s1) {
 #pragma unroll
-  for (uint32_t c = 0; c < HALF; c += 16) {
+  for (uint32_t c = 0; c < MOST; c += 16) {
     if (!GATED && c >= cols) break;
+    uint32_t x[16];
+    ptx::tmem_ld_32x32b_x16(taddr + c, x);
     ptx::tmem_ld_wait();
-    if (c + 16 < HALF && (GATED || c + 16 < cols)) ptx::tmem_ld_32x32b_x16(taddr + c + 16, v[(c / 16 + 1) & 1]);
-    const uint32_t(&x)[16] = v[(c / 16) & 1];
-    const unsigned long long s = GATED && c >= HALF / 2 ? s1 : s0;
+    const float s = GATED && c >= MOST / 2 ? s1 : s0;
 #pragma unroll
-    for (uint32_t i = 0; i < 16; i += 2) {
-      unsigned long long y;
-      asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(x[i]), "r"(x[i + 1]));
-      asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sums[(c + i) / 2]) : "l"(y), "l"(s));
-    }
+    for (uint32_t i = 0; i < 16; ++i) sums[c + i] = fmaf(__uint_as_float(x[i]), s, sums[c + i]);
   }
 }
+// the way back
+__device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
+#pragma unroll
+  for (uint32_t c = 0; c < MOST; c += 16) {
+    if (c >= cols) break;
+    uint32_t v[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(sums[c + i]);
+    ptx::tmem_st_32x32b_x16(taddr + c, v);
+  }
+  ptx::tmem_st_wait();
+}
 
-// A slice's sums are parked, column c of the warp at c * ROWS_CTA, for whoever is the last of the tile's slices
-// to do so and counts up to their number.  Nothing waits.
+// `cols` columns of a slice's sums (a multiple of 16) are parked, column c of the warp at c * ROWS_CTA, for whoever
+// is the last of the tile's slices to do so and counts up to their number.  Nothing waits.
 __device__ __forceinline__ float *part_of(const F8Params &p, uint32_t slot, uint32_t rank, uint32_t quarter, uint32_t col) {
   return p.parts + (static_cast<uint64_t>(slot) * 2 + rank) * PART + static_cast<uint64_t>(col) * ROWS_CTA +
          quarter * 32u + (threadIdx.x & 31u);
 }
-__device__ __forceinline__ void park(float *mine, uint32_t cols, const unsigned long long (&sums)[HALF / 2]) {
+__device__ __forceinline__ void park(float *mine, uint32_t cols, uint32_t taddr) {
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += 16) {
+    uint32_t v[16];
+    ptx::tmem_ld_32x32b_x16(taddr + c, v);
+    ptx::tmem_ld_wait();
 #pragma unroll
-  for (uint32_t c = 0; c < HALF; c += 2) {
-    if (c >= cols) break;
-    __stcg(mine + c * ROWS_CTA, low(sums[c / 2]));
-    __stcg(mine + (c + 1) * ROWS_CTA, high(sums[c / 2]));
+    for (uint32_t j = 0; j < 16; ++j) __stcg(mine + (c + j) * ROWS_CTA, __uint_as_float(v[j]));
   }
   __threadfence();
   __syncwarp();
@@ -265,13 +340,11 @@ __device__ __forceinline__ void park(float *mine, uint32_t cols, const unsigned 
 __device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) {
   return atomicInc(p.counters + 2 + (x.number * 2 + rank) * NUM_EPI_WARPS + which, x.slices - 1) == x.slices - 1;
 }
-// the sums of all slices, the first of which is at `first`, added in their order
-__device__ __forceinline__ void join(const float *first, uint32_t slices, uint32_t cols,
-                                     unsigned long long (&sums)[HALF / 2]) {
+// the sums of all slices, the first of which is at `first`, added in their order, back to tensor memory
+__device__ __forceinline__ void join(const float *first, uint32_t slices, uint32_t cols, uint32_t taddr) {
   __threadfence();
-#pragma unroll
-  for (uint32_t c = 0; c < HALF; c += 16) {
-    if (c >= cols) break;
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += 16) {
     float v[16];
 #pragma unroll
     for (uint32_t j = 0; j < 16; ++j) v[j] = 0.f;
@@ -288,33 +361,12 @@ __device__ __forceinline__ void join(const float *first, uint32_t slices, uint32
 #pragma unroll
         for (uint32_t j = 0; j < 16; ++j) v[j] += y[i][j];
     }
+    uint32_t w[16];
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j += 2) sums[(c + j) / 2] = pair_of(v[j], v[j + 1]);
+    for (uint32_t j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j]);
+    ptx::tmem_st_32x32b_x16(taddr + c, w);
   }
-}
-
-__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-template <class T> __device__ __forceinline__ T ld_shared_one(uint32_t addr) {
-  if constexpr (sizeof(T) == 1) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return static_cast<T>(v);
-  } else if constexpr (sizeof(T) == 2) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return v;
-  } else {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-  }
+  ptx::tmem_st_wait();
 }
 
 // 64 bytes of each of a warp's rows, which its lanes have in w, to memory by way of the warp's buffer: a lane
@@ -330,13 +382,17 @@ __device__ __forceinline__ void store_64_bytes(uint32_t buf, const uint32_t (&w)
   for (uint32_t i = 0; i < 4; ++i)
     st_shared(buf + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   __syncwarp();
-  if (vector && elems >= ALL) {
-    const uint32_t chunk = lane & 3u;
+  if (vector) {
+    const uint32_t chunk = lane & 3u, n = elems > chunk * PER ? min(elems - chunk * PER, PER) : 0u;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       const uint32_t row = 8 * i + (lane >> 2);
       const uint4 v = ld_shared(buf + row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4));
-      if (row < rows) *reinterpret_cast<uint4 *>(out + row * ldo + chunk * PER) = v;
+      E *at = out + row * ldo + chunk * PER;
+      if (row < rows && n == PER) *reinterpret_cast<uint4 *>(at) = v;
+      else if (row < rows && n > 0) // the last features of a width that fills no 16 bytes
+        for (uint32_t e = 0; e < n; ++e)
+          at[e] = ld_shared_one<E>(buf + row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4) + e * sizeof(E));
     }
   } else { // element by element, neighbours by neighbouring lanes
 #pragma unroll 1
@@ -359,44 +415,58 @@ __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
   return w;
 }
 
-// A thread's sums, `cols` columns of its row, to the result: the one rounding.
-__device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, const unsigned long long (&sums)[HALF / 2],
-                                           uint64_t at, uint32_t rows, uint32_t cols) {
+// 16 columns of a warp's sums; where there are none (zero) the product is 0
+__device__ __forceinline__ void fetch(uint32_t taddr, bool zero, uint32_t (&v)[16]) {
+  if (zero) {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) v[j] = 0;
+  } else {
+    ptx::tmem_ld_32x32b_x16(taddr, v);
+    ptx::tmem_ld_wait();
+  }
+}
+
+// `cols` columns of a warp's sums to the result, from `at` on: the one rounding.
+__device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint32_t taddr, bool zero, uint64_t at,
+                                           uint32_t rows, uint32_t cols, const float *bias) {
   const auto type = static_cast<GroupedOut>(p.out_type);
+  auto sixteen = [&](uint32_t c, uint32_t (&v)[16]) {
+    fetch(taddr + c, zero, v);
+    if (bias != nullptr) {
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j)
+        v[j] = __float_as_uint(__uint_as_float(v[j]) + (c + j < cols ? __ldg(bias + c + j) : 0.f));
+    }
+  };
+  uint32_t v[16], w[16];
   if (type == GroupedOut::f32) {
-    uint32_t *out = static_cast<uint32_t *>(p.out) + at;
-#pragma unroll
-    for (uint32_t c = 0; c < HALF; c += 16) {
-      if (c >= cols) break;
-      uint32_t w[16];
-#pragma unroll
-      for (uint32_t i = 0; i < 16; i += 2) {
-        w[i] = static_cast<uint32_t>(sums[(c + i) / 2]);
-        w[i + 1] = static_cast<uint32_t>(sums[(c + i) / 2] >> 32);
-      }
-      store_64_bytes(buf, w, out + c, p.ldo, rows, cols - c, p.vector_out != 0);
+#pragma unroll 1
+    for (uint32_t c = 0; c < cols; c += 16) {
+      sixteen(c, v);
+      store_64_bytes(buf, v, static_cast<uint32_t *>(p.out) + at + c, p.ldo, rows, cols - c, p.vector_out != 0);
     }
   } else {
-    uint16_t *out = static_cast<uint16_t *>(p.out) + at;
     const bool bf16 = type == GroupedOut::bf16;
+#pragma unroll 1
+    for (uint32_t c = 0; c < cols; c += 32) {
 #pragma unroll
-    for (uint32_t c = 0; c < HALF; c += 32) {
-      if (c >= cols) break;
-      uint32_t w[16];
+      for (uint32_t h = 0; h < 2; ++h) { // (the second half of a narrow tile's columns is its neighbour's)
+        sixteen(c + 16 * h, v);
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        const float x = low(sums[c / 2 + i]), y = high(sums[c / 2 + i]);
-        w[i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
+        for (uint32_t i = 0; i < 8; ++i) {
+          const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+          w[8 * h + i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
+        }
       }
-      store_64_bytes(buf, w, out + c, p.ldo, rows, cols - c, p.vector_out != 0);
+      store_64_bytes(buf, w, static_cast<uint16_t *>(p.out) + at + c, p.ldo, rows, cols - c, p.vector_out != 0);
     }
   }
 }
 
 template <F8Type TYPE>
-__device__ __forceinline__ void quantise_64(const BlockScale &s, const float (&h)[HALF / 2], uint32_t (&w)[16]) {
+__device__ __forceinline__ void quantise(const BlockScale &s, const float (&h)[MOST / 2], uint32_t (&w)[16]) {
 #pragma unroll
-  for (uint32_t i = 0; i < 16; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  for (uint32_t i = 0; i < MOST / 8; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
 }
 
 template <bool GATED>
@@ -423,7 +493,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       ptx::mbar_init(sbase + ACC_FULL + 8 * b, 1);
       ptx::mbar_init(sbase + ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
     }
-    for (uint32_t q = 0; q < 4; ++q) ptx::mbar_init(sbase + PAIR + 8 * q, 2);
+    for (uint32_t q = 0; q < 4; ++q) ptx::mbar_init(sbase + PAIR + 8 * q, PARTS);
+    for (uint32_t i = 0; i < AHEAD; ++i) {
+      ptx::mbar_init(sbase + TILE_FULL + 8 * i, 1);
+      ptx::mbar_init(sbase + TILE_EMPTY + 8 * i, NUM_EPI_WARPS + (leader ? 2 : 1)); // and the producer, the issuer
+    }
     *abort_flag = 0;
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_x);
@@ -448,16 +522,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 
   if (warp < 4) {
     ptx::setmaxnreg_dec<REGS_REST>();
-    Items<GATED> items(smem, p, clusters);
+    const uint32_t width = ld_shared_one<uint32_t>(sbase + WIDTH);
     Tile x;
     if (warp == 0) {
       // ============================================================== TMA producer (both CTAs)
       if (ptx::elect_one()) {
         uint32_t s = 0, ph = 1;
         bool ok = true;
-        const uint32_t half = items.cols / 2; // columns that this CTA loads
-        for (uint32_t item = cluster_id; ok && item < items.total; item += clusters) {
-          if (!items.get(p, item, x)) continue;
+        const uint32_t half = width / 2; // columns that this CTA loads
+        Tiles<false> tiles(sbase);
+        while (ok && tiles.next(p.status, x)) {
           // boxes of rows: one of 128, or as many of 32 as it takes; none where this CTA has no rows
           const uint32_t rows = x.rows > rank * ROWS_CTA ? min(x.rows - rank * ROWS_CTA, ROWS_CTA) : 0u;
           const uint32_t x_boxes = (rows + BOX_ROWS - 1) / BOX_ROWS;
@@ -480,13 +554,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
                 ptx::tma_load_3d_pair(x_dst + b * BOX_ROWS * BLOCK, &map_x_few, full, k,
                                       row + static_cast<int>(b * BOX_ROWS), 0);
             }
-            if constexpr (GATED) { // 64 rows of the gate, then the same of the projection
-              const int f = static_cast<int>(x.col0 + rank * (half / 2));
-              ptx::tma_load_3d_pair(w_dst, &map_w, full, k, f, e);
-              ptx::tma_load_3d_pair(w_dst + half / 2 * BLOCK, &map_w, full, k, static_cast<int>(p.n) + f, e);
+            if constexpr (GATED) { // for each warp's columns rows of the gate, then the same of the projection
+#pragma unroll
+              for (uint32_t b = 0; b < COLS / 2 / BOX_ROWS; ++b) {
+                const uint32_t local = b * BOX_ROWS % MOST, f = x.col0 + (rank * (COLS / 2) + b * BOX_ROWS) / MOST * (MOST / 2);
+                ptx::tma_load_3d_pair(w_dst + b * BOX_ROWS * BLOCK, &map_w_few, full, k,
+                                      static_cast<int>(local < MOST / 2 ? f + local : p.n + f + local - MOST / 2), e);
+              }
             } else {
               const int c = static_cast<int>(x.col0 + rank * half);
-              if (half == HALF) {
+              if (half == COLS / 2) {
                 ptx::tma_load_3d_pair(w_dst, &map_w, full, k, c, e);
               } else {
                 for (uint32_t b = 0; b < half / BOX_ROWS; ++b)
@@ -507,11 +584,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         constexpr uint16_t BOTH = 0x3;
         constexpr uint64_t kStage = STAGE_BYTES >> 4;
         const uint64_t a0 = ptx::make_kmajor_desc<BLOCK>(sbase), b0 = ptx::make_kmajor_desc<BLOCK>(sbase + TILE_BYTES);
-        const uint32_t idesc = p.idesc | ((items.cols >> 3) << 17);
+        const uint32_t idesc = p.idesc | ((width >> 3) << 17);
         uint32_t s = 0, ph = 0, acc = 0, e_ph = 1;
         bool ok = true;
-        for (uint32_t item = cluster_id; ok && item < items.total; item += clusters) {
-          if (!items.get(p, item, x)) continue;
+        Tiles<false> tiles(sbase);
+        while (ok && tiles.next(p.status, x)) {
           for (uint32_t kb = 0; kb < x.blocks; ++kb) {
             ok = ptx::mbar_wait(sbase + ACC_EMPTY + 8 * acc, e_ph, abort_flag, p.status, ptx::kErrWaitD0Empty) &&
                  ptx::mbar_wait(sbase + FULL + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitFull);
@@ -521,8 +598,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
             for (uint32_t ks = 0; ks < 4; ++ks)
               ptx::mma_f8_ss_pair(d, a0 + s * kStage + 2 * ks, b0 + s * kStage + 2 * ks, idesc, ks != 0);
-            ptx::tc_commit_pair(sbase + EMPTY + 8 * s, BOTH);
             ptx::tc_commit_pair(sbase + ACC_FULL + 8 * acc, BOTH);
+            ptx::tc_commit_pair(sbase + EMPTY + 8 * s, BOTH);
             acc ^= 1u;
             if (acc == 0) e_ph ^= 1u;
             if (++s == STAGES) {
@@ -532,131 +609,201 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           }
         }
       }
+    } else if (warp == 2) {
+      // ============================================================== the next tiles (both CTAs, each its own)
+      if (ptx::elect_one()) {
+        Items<GATED> items(sbase, p, clusters);
+        uint32_t turn = 0, ph = 1;
+        for (uint32_t item = cluster_id;; item += clusters) {
+          const bool more = item < items.total;
+          if (more && !items.get(p, item, x)) continue;
+          if (!more) x = Tile{};
+          if (!ptx::mbar_wait_backoff(sbase + TILE_EMPTY + 8 * turn, ph, abort_flag, p.status, ptx::kErrWaitTile, 64)) break;
+          const uint32_t to = sbase + TILE + 48 * turn;
+          st_shared(to, x.group, x.row0, x.rows, x.col0);
+          st_shared(to + 16, x.k0, x.blocks, x.slices, x.slice);
+          st_shared(to + 32, x.slot, x.number, 0, 0);
+          ptx::mbar_arrive(sbase + TILE_FULL + 8 * turn);
+          if (!more) break;
+          if (++turn == AHEAD) {
+            turn = 0;
+            ph ^= 1u;
+          }
+        }
+      }
     }
   } else {
     // ================================================================ epilogue (both CTAs)
     ptx::setmaxnreg_inc<REGS_EPI>();
-    Items<GATED> items(smem, p, clusters);
     Tile x;
-    const uint32_t epi = warp - 4, quarter = warp & 3u, second = epi >> 2;
-    const uint32_t half = items.cols / 2;
-    const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + second * half;
+    const uint32_t epi = warp - 4, quarter = warp & 3u, part = epi >> 2;
+    const uint32_t mine = ld_shared_one<uint32_t>(sbase + WIDTH) / PARTS; // columns of the warp, from part * mine on
+    const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + part * mine;
     const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
-    const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
-    const uint32_t w_blocks = ((GATED ? 2 * p.n : p.n) + BLOCK - 1) / BLOCK;
+    const uint32_t buf = sbase + OUT + epi * OUT_BYTES, ring = sbase + SCALE + epi * SCALE_BYTES;
+    const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in a tile
     uint32_t acc = 0, f_ph = 0, pair_ph = 0, parity = 0;
     bool ok = true;
-    for (uint32_t item = cluster_id; item < items.total; item += clusters) {
-      if (!items.get(p, item, x)) continue;
-      const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in the tile
-      const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
-      const bool real = lane < rows;
-      unsigned long long sums[HALF / 2];
+    // The reads of tensor memory are complete (wait::ld): that is all there is to order.
+    auto give_back = [&]() {
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(acc_empty + 8 * acc);
+      acc ^= 1u;
+      if (acc == 0) f_ph ^= 1u;
+    };
+    // Scales: a lane copies the one of its row, lanes 0 and 1 those of the weights, RING - 1 blocks ahead, the first
+    // of a tile before the one in front of it is stored.  A register that waits for them, or a warp that passes
+    // them on by barriers, took 250 to 300 cycles of each stage.
+    const float *xs = nullptr, *ws = nullptr; // of the block to be fetched next
+    uint32_t left = 0, at = 0;                // blocks of the tile to be fetched; slot of the block in turn
+    auto fetch_scales = [&](uint32_t slot) {
+      if (left > 0) {
+        if (xs != nullptr) copy_word(ring + (slot % RING) * 128u + lane * 4u, xs);
+        if (ws != nullptr) copy_word(ring + RING * 128u + ((slot % RING) * 2u + lane) * 4u, ws);
+        --left;
+        if (xs != nullptr) xs += p.x_scale_block;
+        if (ws != nullptr) ++ws;
+      }
+      commit_copies();
+    };
+    auto first_scales = [&](const Tile &y) {
+      xs = ws = nullptr;
+      left = y.rows > lane0 ? y.blocks : 0u;
+      if (lane0 + lane < y.rows)
+        xs = p.x_scale + (static_cast<uint64_t>(y.row0) + lane0 + lane) * p.x_scale_row + y.k0 * p.x_scale_block;
+      if (lane < (GATED ? 2u : 1u)) {
+        const uint32_t w_blocks = ((GATED ? 2 * p.n : p.n) + BLOCK - 1) / BLOCK;
+        const uint32_t block = GATED ? (y.col0 + lane * p.n) / BLOCK : (y.col0 + part * mine) / BLOCK;
+        // (a warp whose columns are all behind the last one has any)
+        ws = p.w_scale + (static_cast<uint64_t>(y.group) * w_blocks + min(block, w_blocks - 1)) * p.blocks + y.k0;
+      }
 #pragma unroll
-      for (uint32_t i = 0; i < HALF / 2; ++i) sums[i] = 0;
-      if (x.blocks > 0) {
-        // scales: of the next two blocks on their way
-        const float *xs = p.x_scale + (x.row0 + lane0 + (real ? lane : 0u)) * p.x_scale_row + x.k0 * p.x_scale_block;
-        const uint32_t wb = (x.col0 + (GATED ? 0u : second * half)) / BLOCK;
-        const float *ws = p.w_scale + (static_cast<uint64_t>(x.group) * w_blocks + min(wb, w_blocks - 1)) * p.blocks + x.k0;
-        const float *us = GATED ? ws + static_cast<uint64_t>(p.n / BLOCK) * p.blocks : nullptr;
-        auto scale_of = [&](uint32_t kb) { return real && kb < x.blocks ? __ldg(xs + kb * p.x_scale_block) : 0.f; };
-        auto weight_of = [&](const float *w, uint32_t kb) { return kb < x.blocks ? __ldg(w + kb) : 0.f; };
-        float sx = 0.f, sx1 = 0.f, sw = 0.f, sw1 = 0.f, su = 0.f, su1 = 0.f;
-        if (rows > 0) {
-          sx = scale_of(0), sx1 = scale_of(1);
-          sw = weight_of(ws, 0), sw1 = weight_of(ws, 1);
-          if constexpr (GATED) su = weight_of(us, 0), su1 = weight_of(us, 1);
-        }
+      for (uint32_t i = 0; i + 1 < RING; ++i) fetch_scales(at + i);
+    };
+    Tiles<true> tiles(sbase);
+    ok = tiles.wait(p.status);
+    uint32_t slot = tiles.advance();
+    if (ok) {
+      tiles.read(slot, x);
+      if (x.rows > 0) first_scales(x);
+    }
+    while (ok && x.rows > 0) {
+      float sums[MOST];
+#pragma unroll
+      for (uint32_t i = 0; i < MOST; ++i) sums[i] = 0.f;
+      const bool zero = x.blocks == 0;
+      if (!zero) {
+        const bool some = x.rows > lane0;
+        const uint32_t blocks = x.blocks;
 #pragma unroll 1
-        for (uint32_t kb = 0; kb < x.blocks; ++kb) {
-          float sx2 = 0.f, sw2 = 0.f, su2 = 0.f;
-          if (rows > 0) {
-            sx2 = scale_of(kb + 2);
-            sw2 = weight_of(ws, kb + 2);
-            if constexpr (GATED) su2 = weight_of(us, kb + 2);
+        for (uint32_t kb = 0; kb < blocks; ++kb) {
+          float t0 = 0.f, t1 = 0.f;
+          if (some) {
+            wait_copies<RING - 2>();
+            __syncwarp();
+            const float own = __uint_as_float(ld_shared_one<uint32_t>(ring + (at % RING) * 128u + lane * 4u));
+            const uint32_t w = ring + RING * 128u + (at % RING) * 8u;
+            t0 = own * __uint_as_float(ld_shared_one<uint32_t>(w));
+            if constexpr (GATED) t1 = own * __uint_as_float(ld_shared_one<uint32_t>(w + 4));
+            fetch_scales(at + RING - 1); // (the slot that all lanes have read a block ago)
+            ++at;
           }
-          ok = ptx::warp_agrees(ptx::mbar_wait(sbase + ACC_FULL + 8 * acc, f_ph, abort_flag, p.status, ptx::kErrWaitD0Full));
+          ok = ptx::warp_agrees(ptx::mbar_wait_s(sbase + ACC_FULL + 8 * acc, f_ph, sbase + ABORT, p.status, ptx::kErrWaitD0Full));
           if (!ok) break;
           ptx::tc_fence_after();
-          if (rows > 0) drain<GATED>(t_lanes + acc * COLS, sums, half, both(sx * sw), GATED ? both(sx * su) : 0ull);
-          // The reads of tensor memory are complete (wait::ld): that is all there is to order.
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster_relaxed(acc_empty + 8 * acc);
-          acc ^= 1u;
-          if (acc == 0) f_ph ^= 1u;
-          sx = sx1, sx1 = sx2, sw = sw1, sw1 = sw2;
-          if constexpr (GATED) su = su1, su1 = su2;
+          if (some) drain<GATED>(t_lanes + acc * COLS, sums, mine, t0, t1);
+          if (kb + 1 < blocks) give_back();
         }
         if (!ok) break;
+        // The sums take the place of the last accumulator: what follows has few registers, and little code.
+        // (From registers it pushed sums to local memory, which came back from L2.)
+        if (some) put_back(t_lanes + acc * COLS, sums, mine);
       }
+      // The next tile's first scales, then this tile again: kept over the loop it took registers from the sums.
+      ok = tiles.wait(p.status);
+      if (!ok) break;
+      const uint32_t next_slot = tiles.advance();
+      tiles.read(next_slot, x);
+      if (x.rows > 0) first_scales(x);
+      tiles.read(slot, x);
+      const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
+      const bool real = lane < rows;
+      const uint32_t t_sums = t_lanes + acc * COLS;
+      bool done = rows == 0;
       if constexpr (GATED) {
-        // (both warps that have these lanes have rows, or neither)
-        if (rows == 0) continue;
-        auto meet = [&]() { // the other warp; false: the wait gave up
+        // (all warps that have these lanes have rows, or none)
+        auto meet = [&]() { // the other warps; false: the wait gave up
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(sbase + PAIR + 8 * quarter);
           const bool met = ptx::warp_agrees(
-              ptx::mbar_wait(sbase + PAIR + 8 * quarter, pair_ph, abort_flag, p.status, ptx::kErrWaitD1Full));
+              ptx::mbar_wait_s(sbase + PAIR + 8 * quarter, pair_ph, sbase + ABORT, p.status, ptx::kErrWaitD1Full));
           pair_ph ^= 1u;
           return met;
         };
-        if (x.slices > 1) { // both are last, or neither
-          park(part_of(p, x.slot, rank, quarter, second * half), half, sums);
+        if (!done && x.slices > 1) { // all are last, or none
+          park(part_of(p, x.slot, rank, quarter, part * mine), mine, t_sums);
           ok = meet();
           if (!ok) break;
           volatile uint32_t *last = reinterpret_cast<volatile uint32_t *>(smem + LAST) + quarter;
-          if (second == 0 && lane == 0) *last = is_last(p, x, rank, quarter);
+          if (part == 0 && lane == 0) *last = is_last(p, x, rank, quarter);
           ok = meet();
           if (!ok) break;
-          if (*last == 0) continue;
-          join(part_of(p, x.slot - x.slice, rank, quarter, second * half), x.slices, half, sums);
+          done = *last == 0;
+          if (!done) join(part_of(p, x.slot - x.slice, rank, quarter, part * mine), x.slices, mine, t_sums);
         }
-        float h[HALF / 2];
-        uint32_t top = 0;
+        if (!done) {
+          float h[MOST / 2];
+          uint32_t top = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < HALF / 4; ++i) {
-          h[2 * i] = activate(static_cast<Activation>(p.activation), low(sums[i])).value * low(sums[HALF / 4 + i]);
-          h[2 * i + 1] = activate(static_cast<Activation>(p.activation), high(sums[i])).value * high(sums[HALF / 4 + i]);
-          top = max(top, max(__float_as_uint(h[2 * i]) & 0x7fffffffu, __float_as_uint(h[2 * i + 1]) & 0x7fffffffu));
+          for (uint32_t c = 0; c < MOST / 2; c += 16) {
+            uint32_t gate[16], up[16];
+            fetch(t_sums + c, zero, gate);
+            fetch(t_sums + MOST / 2 + c, zero, up);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+              h[c + i] = activate<true>(static_cast<Activation>(p.activation), __uint_as_float(gate[i])).value * __uint_as_float(up[i]);
+              top = max(top, __float_as_uint(h[c + i]) & 0x7fffffffu);
+            }
+          }
+          // (written again two tiles on, when the other warps have long read them: they have been met since)
+          uint32_t *tops = reinterpret_cast<uint32_t *>(smem + TOPS) + parity * PARTS * ROWS_CTA + quarter * 32u + lane;
+          parity ^= 1u;
+          tops[part * ROWS_CTA] = top;
+          ok = meet();
+          if (!ok) break;
+#pragma unroll
+          for (uint32_t i = 0; i < PARTS; ++i) top = max(top, tops[i * ROWS_CTA]);
+          const auto type = static_cast<F8Type>(p.out_type);
+          const BlockScale s(__uint_as_float(top), type);
+          uint32_t w[16] = {};
+          if (type == F8Type::e4m3) quantise<F8Type::e4m3>(s, h, w);
+          else quantise<F8Type::e5m2>(s, h, w);
+          const uint64_t row = x.row0 + lane0;
+          store_64_bytes(buf, w, static_cast<uint8_t *>(p.out) + row * p.ldo + x.col0 + part * (MOST / 2), p.ldo, rows, MOST / 2,
+                         p.vector_out != 0);
+          if (part == 0 && real) p.out_scale[(row + lane) * p.out_scale_row + x.col0 / BLOCK * p.out_scale_block] = s.scale;
         }
-        // (written again two tiles on, when the other warp has long read them: it has been met since)
-        uint32_t *tops = reinterpret_cast<uint32_t *>(smem + TOPS) + parity * 2 * ROWS_CTA + quarter * 32u + lane;
-        parity ^= 1u;
-        tops[second * ROWS_CTA] = top;
-        ok = meet();
-        if (!ok) break;
-        top = max(top, tops[(second ^ 1u) * ROWS_CTA]);
-        const auto type = static_cast<F8Type>(p.out_type);
-        const BlockScale s(__uint_as_float(top), type);
-        uint32_t w[16];
-        if (type == F8Type::e4m3) quantise_64<F8Type::e4m3>(s, h, w);
-        else quantise_64<F8Type::e5m2>(s, h, w);
-        const uint64_t row = x.row0 + lane0;
-        store_64_bytes(buf, w, static_cast<uint8_t *>(p.out) + row * p.ldo + x.col0 + second * (HALF / 2), p.ldo, rows,
-                       HALF / 2, p.vector_out != 0);
-        if (second == 0 && real) p.out_scale[(row + lane) * p.out_scale_row + x.col0 / BLOCK * p.out_scale_block] = s.scale;
       } else {
-        const uint32_t col = x.col0 + second * half;
-        const uint32_t cols = p.n > col ? min(half, p.n - col) : 0u;
-        if (rows == 0 || cols == 0) continue;
-        if (x.slices > 1) {
-          park(part_of(p, x.slot, rank, quarter, second * half), half, sums);
+        const uint32_t col = x.col0 + part * mine;
+        const uint32_t cols = p.n > col ? min(mine, p.n - col) : 0u;
+        done |= cols == 0;
+        if (!done && x.slices > 1) {
+          park(part_of(p, x.slot, rank, quarter, part * mine), mine, t_sums);
           const bool last = lane == 0 && is_last(p, x, rank, epi);
-          if (!__any_sync(0xffffffffu, last)) continue;
-          join(part_of(p, x.slot - x.slice, rank, quarter, second * half), x.slices, half, sums);
+          done = !__any_sync(0xffffffffu, last);
+          if (!done) join(part_of(p, x.slot - x.slice, rank, quarter, part * mine), x.slices, mine, t_sums);
         }
-        if (p.bias != nullptr && x.group < p.groups) {
-          const float *bias = p.bias + static_cast<uint64_t>(x.group) * p.n + col;
-#pragma unroll
-          for (uint32_t c = 0; c < HALF; c += 2)
-            sums[c / 2] = pair_of(low(sums[c / 2]) + (c < cols ? __ldg(bias + c) : 0.f),
-                                  high(sums[c / 2]) + (c + 1 < cols ? __ldg(bias + c + 1) : 0.f));
-        }
-        store_sums(p, buf, sums, (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col, rows, cols);
+        if (!done)
+          store_sums(p, buf, t_sums, zero, (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col, rows, cols,
+                     p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr);
       }
+      if (!zero) give_back();
+      tiles.give_back(slot);
+      slot = next_slot;
+      tiles.read(slot, x);
     }
+    wait_copies<0>();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -717,13 +864,13 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
   const cudaError_t se = set_up<GATED>(&clusters);
   if (se != cudaSuccess) return se;
   CUtensorMap map_x, map_x_few, map_w, map_w_few;
-  if (!operand_map(&map_x_few, a.b, BOX_ROWS) || !operand_map(&map_w, a.a, GATED ? HALF / 2 : HALF))
+  if (!operand_map(&map_x_few, a.b, BOX_ROWS) || !operand_map(&map_w_few, a.a, BOX_ROWS))
     return cudaErrorInvalidValue;
-  // boxes of 128 rows are for tiles that have as many; narrow tiles are not gated
+  // boxes of 128 rows are for tiles that have as many, and not for gated ones' weights
   map_x = map_x_few;
-  map_w_few = map_w;
+  map_w = map_w_few;
   if (a.rows > ROWS_CTA - BOX_ROWS && !operand_map(&map_x, a.b, ROWS_CTA)) return cudaErrorInvalidValue;
-  if (!GATED && !operand_map(&map_w_few, a.a, BOX_ROWS)) return cudaErrorInvalidValue;
+  if (!GATED && !operand_map(&map_w, a.a, COLS / 2)) return cudaErrorInvalidValue;
   F8Params p = {};
   p.ends = a.ends;
   p.out = a.out;
