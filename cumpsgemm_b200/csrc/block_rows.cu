@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) quantize_block_rows_kernel(const Blo
         gate[j].values(v[j]);
         up[j].values(u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = activate(static_cast<Activation>(a.activation), v[j][i]).value * u[i];
+        for (int i = 0; i < 8; ++i) v[j][i] = activate<true>(static_cast<Activation>(a.activation), v[j][i]).value * u[i];
       }
     } else {
       Eight<T, WHOLE> x[kAtOnce];
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(const GatedRowsArg
       if constexpr (GRAD) dh[j].values(d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const ActResult act = activate(static_cast<Activation>(a.activation), g[i]);
+        const ActResult act = activate<sizeof(T) == 2>(static_cast<Activation>(a.activation), g[i]);
         if constexpr (GRAD) {
           g[i] = d[i] * u[i] * act.slope;
           u[i] = d[i] * act.value;

@@ -11,6 +11,8 @@ constexpr uint32_t kMaxK8 = 131071; // 2^14 * k has to stay below 2^31
 enum class GroupedKind : int { f16 = 0, tcec = 1, i8 = 2, f8 = 3 };
 enum class GroupedOut : int { f16 = 0, bf16 = 1, f32 = 2 };
 
+enum class GatedKind : int { none = 0, gated = 1, grad = 2 };
+
 // One operand as the tensor core reads it: `planes` x `batch` matrices of `outer` rows of `inner`
 // contiguous elements.  A plane is the operand itself, or (tcec) its hi and its lo half.
 struct GroupedOperand {
@@ -44,6 +46,13 @@ struct GroupedArgs {
   const float *col_scale;  // i8: [rows]; f8: of each row and block of k, steps in F8Args
   const float *bias;       // i8, f8, nullable: [groups][lane_dim]
   const F8Args *f8;
+  // f16: what follows a product.  gated: w has the rows of the gate and of what it gates (lane_dim: of both), out is
+  // act(gate) * up, and pre, if not null, receives both.  gated_grad: the product is the gradient of that, out
+  // receives the gradient of pre (lane_dim: of the product).
+  GatedKind gated;
+  int activation; // Activation
+  void *pre;
+  uint64_t ldpre;
   float *parts; // nullable: grouped_parts_bytes() of workspace for the sums of slices
   unsigned *counters; // grouped_counters() words, zero between calls
   int *dev_status;

@@ -366,7 +366,8 @@ extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm_gated(
   if (const char *why = check_sizes(rows, 2 * hidden, k, num_groups, group_ends)) return refuse(where, why);
   if (!known_type(type)) return refuse(where, "type is not CUDA_R_16F, CUDA_R_16BF or CUDA_R_32F");
   if (!known_activation(activation)) return refuse(where, "unknown activation");
-  if (w == nullptr || (rows > 0 && (x == nullptr || y == nullptr || pre == nullptr))) return refuse(where, "null pointer");
+  if (w == nullptr || (rows > 0 && (x == nullptr || y == nullptr || (pre == nullptr && type == CUDA_R_32F))))
+    return refuse(where, "null pointer");
   if (ldx < k || ldy < hidden || ldw < k || (num_groups > 1 && stridew < (2 * hidden - 1) * ldw + k) ||
       (pre != nullptr && ldpre < 2 * hidden))
     return refuse(where, "a leading dimension or the stride of w is too small");
@@ -376,6 +377,30 @@ extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm_gated(
   }
   if (rows == 0) return CUBLAS_STATUS_SUCCESS;
 
+  if (type != CUDA_R_32F) {
+    DeviceGuard guard(h->device);
+    GroupedArgs g = {};
+    g.kind = GroupedKind::f16;
+    g.out_type = out_type(type);
+    g.bf16 = type == CUDA_R_16BF;
+    g.a = {w, k, 2 * hidden, ldw, stridew, 0, num_groups, 1};
+    g.b = {x, k, rows, ldx, 0, 0, 1, 1};
+    g.ends = group_ends;
+    g.rows = static_cast<uint32_t>(rows);
+    g.groups = num_groups;
+    g.lane_dim = static_cast<uint32_t>(2 * hidden);
+    g.k = static_cast<uint32_t>(k);
+    g.out = y;
+    g.ldo = ldy;
+    g.alpha = 1.f;
+    g.dev_status = h->dev_status;
+    g.gated = GatedKind::gated;
+    g.activation = activation;
+    g.pre = pre;
+    g.ldpre = ldpre;
+    const cublasStatus_t st = stage(h, where, g, 2, true, false);
+    return st == CUBLAS_STATUS_SUCCESS ? finish(h, g) : st;
+  }
   const float one = 1.f, zero = 0.f;
   const cublasStatus_t st = cuMpSGEMM_grouped_gemm(h, CUBLAS_OP_T, rows, 2 * hidden, k, num_groups, group_ends, &one, x, ldx,
                                                    w, ldw, stridew, &zero, pre, ldpre, type, mode);
@@ -408,6 +433,31 @@ extern "C" cublasStatus_t cuMpSGEMM_grouped_gemm_gated_grad(
   }
   if (rows == 0) return CUBLAS_STATUS_SUCCESS;
 
+  if (type != CUDA_R_32F) {
+    DeviceGuard guard(h->device);
+    GroupedArgs g = {};
+    g.kind = GroupedKind::f16;
+    g.out_type = out_type(type);
+    g.bf16 = type == CUDA_R_16BF;
+    g.a_lane_contig = w_n_contig;
+    g.a = {w, w_inner, w_outer, ldw, stridew, 0, num_groups, 1};
+    g.b = {dy, k, rows, lddy, 0, 0, 1, 1};
+    g.ends = group_ends;
+    g.rows = static_cast<uint32_t>(rows);
+    g.groups = num_groups;
+    g.lane_dim = static_cast<uint32_t>(hidden);
+    g.k = static_cast<uint32_t>(k);
+    g.out = dpre;
+    g.ldo = lddpre;
+    g.alpha = 1.f;
+    g.dev_status = h->dev_status;
+    g.gated = GatedKind::grad;
+    g.activation = activation;
+    g.pre = const_cast<void *>(pre);
+    g.ldpre = ldpre;
+    const cublasStatus_t st = stage(h, where, g, 2, true, false);
+    return st == CUBLAS_STATUS_SUCCESS ? finish(h, g) : st;
+  }
   // dh goes to the first half of dpre, and the elementwise pass takes it from there
   const float one = 1.f, zero = 0.f;
   const cublasStatus_t st = cuMpSGEMM_grouped_gemm(h, op_W, rows, hidden, k, num_groups, group_ends, &one, dy, lddy, w, ldw,

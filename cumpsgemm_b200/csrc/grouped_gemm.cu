@@ -39,6 +39,7 @@
 //   next_empty[i] leader's only: one arrival from each role that took the tile
 //   want          leader's only: 1 arrival, from its producer towards the end of each tile
 // Every wait is bounded; no TMA multicast is used.
+#include "activation.cuh"
 #include "epilogue.cuh"
 #include "gemm_common.cuh"
 #include "grouped.hpp"
@@ -74,6 +75,7 @@ constexpr uint32_t MIN_SLICE = 8;
 constexpr uint32_t MAX_SLICES = 16;
 constexpr uint32_t JOIN_AHEAD = 4;   // slices whose sums are fetched together
 constexpr uint32_t PART = COLS * BM_CTA; // elements of a parked sum of one CTA
+constexpr uint32_t GATED_ROWS = 16;  // of the gate, and of what it gates, that lie side by side in the lanes
 constexpr uint32_t OUT_COLS = 32;    // columns that a warp stores at a time
 constexpr uint32_t OUT_BYTES = OUT_COLS * 32 * 2; // 32 lanes of 16-bit elements
 
@@ -117,8 +119,11 @@ struct GroupedParams {
   uint32_t col_dim; // wgrad; product: steps of K
   uint32_t idesc;
   float alpha, beta;
-  uint16_t out_type;
-  uint16_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0
+  uint8_t out_type;
+  uint8_t activation;
+  uint16_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0; bit 1: rows of pre do
+  void *pre;           // gated; nullable where it is written
+  uint64_t ldpre;
 };
 static_assert(sizeof(GroupedParams) <= 128, "read from the constant bank (gemm_common.cuh)");
 
@@ -581,7 +586,185 @@ __device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, T *out,
   }
 }
 
-template <int KIND, bool A_LANES, bool WGRAD>
+// ---- what follows a product of a gated block (16-bit types)
+constexpr int kPlain = static_cast<int>(GatedKind::none), kGated = static_cast<int>(GatedKind::gated),
+              kGatedGrad = static_cast<int>(GatedKind::grad);
+
+// 8 elements of a row, of which there are `elems`
+template <class T> __device__ __forceinline__ void store_piece(T *at, const uint4 &v, uint32_t elems, bool vector) {
+  if (vector && elems >= 8) {
+    *reinterpret_cast<uint4 *>(at) = v;
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+      if (i < elems) reinterpret_cast<uint16_t *>(at)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+template <class T> __device__ __forceinline__ uint4 load_piece(const T *at, uint32_t elems, bool vector) {
+  if (vector && elems >= 8) return __ldg(reinterpret_cast<const uint4 *>(at));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i)
+    if (i < elems) w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(at) + i)) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T> __device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t least(uint32_t all, uint32_t from, uint32_t most) { // of `all` from `from` on
+  return all > from ? min(all - from, most) : 0u;
+}
+
+// h = act(gate) * up.  A CTA's lanes are 16 rows of the gate and the same 16 of what it gates in turn (the loads put
+// them there), so of the two fragments that a warp reads of its 32 lanes the one is the gate and the other up, of the
+// same features and columns in the same registers: no exchange.  They are multiplied before they are rounded.
+// out, pre: at the warp's first feature and column; features: of the 16 that there are.
+template <class T>
+__device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, const GroupedParams &p, T *pre, uint32_t buf,
+                                            uint32_t cols, uint32_t features, uint32_t hidden) {
+  const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u;
+  const bool vector = (p.vector_out & 1u) != 0, vector_pre = (p.vector_out & 2u) != 0;
+  const auto act = static_cast<Activation>(p.activation);
+  // pre, as in store_by_rows
+  const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
+  const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
+  // h: 32 bytes for each column, the two 16-byte chunks of every other four columns exchanged
+  const uint32_t in_h = buf + (8u * (lane >> 4) + (lane & 7u)) * 32u + ((((lane >> 3) ^ (lane >> 2)) & 1u) << 4);
+  const uint32_t back_h = buf + (lane >> 1) * 32u + (((lane ^ (lane >> 3)) & 1u) << 4);
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += OUT_COLS) {
+    uint32_t lo[16], hi[16];
+    if (!zero) {
+      ptx::tmem_ld_16x256b_x4(taddr + c, lo);
+      ptx::tmem_ld_16x256b_x4(taddr + c + (16u << 16), hi);
+      ptx::tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) lo[i] = hi[i] = 0;
+    }
+    if (pre != nullptr) {
+      __syncwarp(); // the buffer has been read
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g) {
+        uint32_t w[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          w[i] = pack_results<T>(__uint_as_float(lo[4 * g + 2 * i]), __uint_as_float(lo[4 * g + 2 * i + 1]));
+          w[2 + i] = pack_results<T>(__uint_as_float(hi[4 * g + 2 * i]), __uint_as_float(hi[4 * g + 2 * i + 1]));
+        }
+        ptx::stmatrix_x4_trans(in + g * 512u, w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+      const uint32_t elems = least(features, 8 * (chunk & 1u), 8);
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g) {
+        uint4 v;
+        ld_shared_v4(back + g * 512u, v.x, v.y, v.z, v.w);
+        const uint32_t col = c + 8 * g + (lane >> 2);
+        if (col < cols)
+          store_piece(pre + col * p.ldpre + (chunk >> 1) * static_cast<uint64_t>(hidden) + 8 * (chunk & 1u), v, elems, vector_pre);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t g = 0; g < 4; g += 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) { // group g + i / 2, features 8 (i % 2) on
+        const uint32_t at = 4 * (g + i / 2) + 2 * (i & 1u);
+        w[i] = pack_results<T>(activate<true>(act, __uint_as_float(lo[at])).value * __uint_as_float(hi[at]),
+                               activate<true>(act, __uint_as_float(lo[at + 1])).value * __uint_as_float(hi[at + 1]));
+      }
+      ptx::stmatrix_x4_trans(in_h + g * 256u, w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    const uint32_t elems = least(features, 8 * (lane & 1u), 8);
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      uint4 v;
+      ld_shared_v4(back_h + j * 512u, v.x, v.y, v.z, v.w);
+      const uint32_t col = c + 16 * j + (lane >> 1);
+      if (col < cols) store_piece(out + col * p.ldo + 8 * (lane & 1u), v, elems, vector);
+    }
+  }
+}
+
+// The gradient of pre, dgate = dh up act'(gate) and dup = dh act(gate), dh being the product, which is not rounded: pre
+// comes the way the results leave, 16 bytes a lane, and through the warp's buffer to the fragments of the sums.
+// pre, out: at the warp's first feature and column; features: of the 32 that there are.
+template <class T>
+__device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *out, const GroupedParams &p, const T *pre,
+                                                 uint32_t buf, uint32_t cols, uint32_t features, uint32_t hidden) {
+  const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u;
+  const uint32_t elems = least(features, 8 * chunk, 8);
+  const bool vector = (p.vector_out & 1u) != 0, vector_pre = (p.vector_out & 2u) != 0;
+  const auto act = static_cast<Activation>(p.activation);
+  const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
+  const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += OUT_COLS) {
+    const uint32_t first = c + (lane >> 2);
+    uint32_t w[2][4][4]; // gate and up, then their gradients: of columns 8 g on, features 8 i on
+    if (!zero) {
+      uint4 v[2][4];
+      const T *from = pre + first * p.ldpre + 8 * chunk;
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+        for (uint32_t q = 0; q < 2; ++q)
+          v[q][g] = load_piece(from + 8 * g * p.ldpre + q * static_cast<uint64_t>(hidden), first + 8 * g < cols ? elems : 0u,
+                               vector_pre);
+      uint32_t lo[16], hi[16];
+      ptx::tmem_ld_16x256b_x4(taddr + c, lo);
+      ptx::tmem_ld_16x256b_x4(taddr + c + (16u << 16), hi);
+#pragma unroll
+      for (uint32_t q = 0; q < 2; ++q) {
+        __syncwarp(); // the buffer has been read
+#pragma unroll
+        for (uint32_t g = 0; g < 4; ++g) st_shared_v4(back + g * 512u, v[q][g].x, v[q][g].y, v[q][g].z, v[q][g].w);
+        __syncwarp();
+#pragma unroll
+        for (uint32_t g = 0; g < 4; ++g)
+          ptx::ldmatrix_x4_trans(in + g * 512u, w[q][g][0], w[q][g][1], w[q][g][2], w[q][g][3]);
+      }
+      ptx::tmem_ld_wait();
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const float x = __uint_as_float(i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4]),
+                      y = __uint_as_float(i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3]);
+          const float2 gate = unpack<T>(w[0][g][i]), up = unpack<T>(w[1][g][i]);
+          const ActResult a = activate<true>(act, gate.x), b = activate<true>(act, gate.y);
+          w[0][g][i] = pack_results<T>(x * up.x * a.slope, y * up.y * b.slope);
+          w[1][g][i] = pack_results<T>(x * a.value, y * b.value);
+        }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 32; ++i) w[i / 16][i / 4 % 4][i % 4] = 0;
+    }
+    T *to = out + first * p.ldo + 8 * chunk;
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q) {
+      __syncwarp();
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g)
+        ptx::stmatrix_x4_trans(in + g * 512u, w[q][g][0], w[q][g][1], w[q][g][2], w[q][g][3]);
+      __syncwarp();
+#pragma unroll
+      for (uint32_t g = 0; g < 4; ++g) {
+        uint4 v;
+        ld_shared_v4(back + g * 512u, v.x, v.y, v.z, v.w);
+        if (first + 8 * g < cols)
+          store_piece(to + 8 * g * p.ldo + q * static_cast<uint64_t>(hidden), v, elems, vector);
+      }
+    }
+  }
+}
+
+template <int KIND, bool A_LANES, bool WGRAD, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                         const __grid_constant__ CUtensorMap map_b,
@@ -679,7 +862,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           for (uint32_t pl = 0; pl < PLANES; ++pl) {
             const uint32_t a_dst = st + pl * TILE_BYTES, b_dst = st + (PLANES + pl) * TILE_BYTES;
             const int za = static_cast<int>(WGRAD ? pl : pl * p.groups + x.group);
-            if constexpr (A_LANES) {
+            if constexpr (EPI == kGated) { // 16 rows of the gate, the same of what it gates, and so on
+              const uint32_t f = (x.lane0 + rank * BM_CTA) / 2, hidden = p.lane_dim / 2;
+#pragma unroll
+              for (uint32_t b = 0; b < BM_CTA / GATED_ROWS; ++b)
+                load(a_dst + b * GATED_ROWS * ROW_BYTES, &map_a, red,
+                     static_cast<int>((b & 1u) * hidden + f + b / 2 * GATED_ROWS), za);
+            } else if constexpr (A_LANES) {
               load(a_dst, &map_a, a_lane, red, za);
               load(a_dst + ATOM_BYTES, &map_a, a_lane + 64, red, za);
             } else {
@@ -959,7 +1148,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         return f;
       };
       const auto type = static_cast<GroupedOut>(p.out_type);
-      if (KIND != kTcec && p.vector_out != 0) {
+      if constexpr (EPI != kPlain) {
+        const uint32_t hidden = EPI == kGated ? p.lane_dim / 2 : p.lane_dim;
+        const uint32_t f = EPI == kGated ? lane0 / 2 : lane0, features = least(hidden, f, EPI == kGated ? 16u : 32u);
+        const uint64_t row = x.col0 + col;
+        auto go = [&](auto *out) {
+          using T = std::remove_pointer_t<decltype(out)>;
+          T *pre = static_cast<T *>(p.pre);
+          if (pre != nullptr) pre += row * p.ldpre + f;
+          if constexpr (EPI == kGated) store_gated(t_sums, zero, out + row * p.ldo + f, p, pre, buf, cols, features, hidden);
+          else store_gated_grad(t_sums, zero, out + row * p.ldo + f, p, pre, buf, cols, features, hidden);
+        };
+        if (type == GroupedOut::bf16) go(static_cast<__nv_bfloat16 *>(p.out));
+        else go(static_cast<__half *>(p.out));
+      } else if (KIND != kTcec && p.vector_out != 0) {
         const uint32_t l = static_cast<uint32_t>(lane) >> 2;
         const Finish f[4] = {finish_of(l), finish_of(l + 8), finish_of(l + 16), finish_of(l + 24)};
         const uint32_t lanes = p.lane_dim > lane0 ? p.lane_dim - lane0 : 0u;
@@ -1002,7 +1204,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 
 // Per device and kernel, once (any thread): shared-memory attribute and the pairs the device keeps
 // resident.  (A kernel of each instance has a type of its own here: its statics are its own.)
-template <int KIND, bool A_LANES, bool WGRAD> cudaError_t set_up(int *clusters_out) {
+template <int KIND, bool A_LANES, bool WGRAD, int EPI> cudaError_t set_up(int *clusters_out) {
   static std::once_flag once[64];
   static cudaError_t setup_error[64];
   static int max_clusters[64];
@@ -1010,7 +1212,7 @@ template <int KIND, bool A_LANES, bool WGRAD> cudaError_t set_up(int *clusters_o
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() {
-    const auto kernel = grouped_gemm_kernel<KIND, A_LANES, WGRAD>;
+    const auto kernel = grouped_gemm_kernel<KIND, A_LANES, WGRAD, EPI>;
     setup_error[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             Cfg<KIND>::SMEM);
     int sms = 0;
@@ -1044,16 +1246,16 @@ bool operand_map(CUtensorMap *map, const GroupedOperand &o, int elem_bytes, cons
                        {inner_box, outer_box, 1}, true);
 }
 
-template <int KIND, bool A_LANES, bool WGRAD>
+template <int KIND, bool A_LANES, bool WGRAD, int EPI = kPlain>
 cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   int clusters = 1;
-  const cudaError_t se = set_up<KIND, A_LANES, WGRAD>(&clusters);
+  const cudaError_t se = set_up<KIND, A_LANES, WGRAD, EPI>(&clusters);
   if (se != cudaSuccess) return se;
   constexpr int ES = KIND == kI8 ? 1 : 2;
   CUtensorMap map_a, map_b, map_b_few;
   // (any address does for an operand without rows; this one is 16-byte aligned)
   const void *fallback = a.dev_status;
-  if (!operand_map(&map_a, a.a, ES, fallback, Cfg<KIND>::K_ELEMS, A_LANES ? 64 : BM_CTA) ||
+  if (!operand_map(&map_a, a.a, ES, fallback, Cfg<KIND>::K_ELEMS, EPI == kGated ? GATED_ROWS : A_LANES ? 64 : BM_CTA) ||
       !operand_map(&map_b_few, a.b, ES, fallback, Cfg<KIND>::K_ELEMS, WGRAD ? 64 : FEW_ROWS))
     return cudaErrorInvalidValue;
   // boxes of 128 rows are for tiles of more than 192
@@ -1083,11 +1285,19 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
             (WGRAD ? 1u << 16 : 0u) | ((LANES >> 4) << 24);
   p.alpha = a.alpha;
   p.beta = a.beta;
-  p.out_type = static_cast<uint16_t>(a.out_type);
+  p.out_type = static_cast<uint8_t>(a.out_type);
+  p.activation = static_cast<uint8_t>(a.activation);
+  p.pre = a.pre;
+  p.ldpre = a.ldpre;
   p.vector_out = a.out_type != GroupedOut::f32 && a.beta == 0.f &&
                  (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo % 8 == 0 &&
                  (!a.wgrad || a.groups == 1 || a.stride_o % 8 == 0);
-  return launch_chained(grouped_gemm_kernel<KIND, A_LANES, WGRAD>, static_cast<unsigned>(2 * clusters),
+  if constexpr (EPI != kPlain) { // pre, and the gradient of it, have their second half `hidden` elements on
+    const bool halves = (EPI == kGated ? a.lane_dim / 2 : a.lane_dim) % 8 == 0;
+    if (EPI == kGatedGrad && !halves) p.vector_out = 0;
+    if (halves && (reinterpret_cast<uintptr_t>(a.pre) & 15u) == 0 && a.ldpre % 8 == 0) p.vector_out |= 2;
+  }
+  return launch_chained(grouped_gemm_kernel<KIND, A_LANES, WGRAD, EPI>, static_cast<unsigned>(2 * clusters),
                         NUM_THREADS, Cfg<KIND>::SMEM, stream, map_a, map_b, map_b_few, p);
 }
 
@@ -1112,6 +1322,9 @@ cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream) {
     return a.wgrad            ? launch<kTcec, true, true>(a, stream)
            : a.a_lane_contig  ? launch<kTcec, true, false>(a, stream)
                               : launch<kTcec, false, false>(a, stream);
+  if (a.gated == GatedKind::gated) return launch<kF16, false, false, kGated>(a, stream);
+  if (a.gated == GatedKind::grad)
+    return a.a_lane_contig ? launch<kF16, true, false, kGatedGrad>(a, stream) : launch<kF16, false, false, kGatedGrad>(a, stream);
   return a.wgrad           ? launch<kF16, true, true>(a, stream)
          : a.a_lane_contig ? launch<kF16, true, false>(a, stream)
                            : launch<kF16, false, false>(a, stream);

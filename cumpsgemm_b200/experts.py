@@ -364,17 +364,17 @@ def _gated_shapes(handle, x, gate_up, group_ends):
     return rows, both // 2, width, groups, ldx, ldw, stridew, _data_type(x.dtype)
 
 
-def _gated(handle, x, gate_up, group_ends, act, mode, out=None):
-    """(act(gate) * up, both in front of that)."""
+def _gated(handle, x, gate_up, group_ends, act, mode, out=None, keep=False):
+    """(act(gate) * up, both in front of that if they are to be kept)."""
     rows, hidden, width, groups, ldx, ldw, stridew, data_type = _gated_shapes(handle, x, gate_up, group_ends)
     ldy = hidden
     if out is not None:
         _, _, ldy = _rows_of(out, "out")
     out = _output(out, 0.0, (rows, hidden), x.dtype, x)
-    pre = x.new_empty((rows, 2 * hidden))
+    pre = x.new_empty((rows, 2 * hidden)) if keep or data_type == api.CUDA_R_32F else None
     handle.grouped_gemm_gated(rows, hidden, width, groups, None if group_ends is None else group_ends.data_ptr(),
                               x.data_ptr(), ldx, gate_up.data_ptr(), ldw, stridew, act, out.data_ptr(), ldy,
-                              pre.data_ptr(), 2 * hidden, data_type, mode)
+                              None if pre is None else pre.data_ptr(), 2 * hidden, data_type, mode)
     return out, pre
 
 
@@ -426,7 +426,7 @@ def _composed_gradients(ctx, dy, operands, handle, group_ends, act, mode):
 class _GatedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, group_ends, handle, act, mode, backward_mode):
-        h, pre = _gated(handle, x, gate_up, group_ends, act, mode)
+        h, pre = _gated(handle, x, gate_up, group_ends, act, mode, keep=True)
         ctx.save_for_backward(x, gate_up, group_ends, pre)
         ctx.how = (handle, act, backward_mode)
         return h
@@ -449,7 +449,7 @@ class _GatedMatmul(torch.autograd.Function):
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, down, group_ends, handle, act, mode, backward_mode):
-        h, pre = _gated(handle, x, gate_up, group_ends, act, mode)
+        h, pre = _gated(handle, x, gate_up, group_ends, act, mode, keep=True)
         ctx.save_for_backward(x, gate_up, down, group_ends, pre, h)
         ctx.how = (handle, act, backward_mode)
         return grouped_matmul(handle, h, down, group_ends, True, mode=mode)

@@ -431,7 +431,8 @@ typedef enum {
   CUMPSGEMM_ACTIVATION_RELU = 3
 } cuMpSGEMM_activation_t;
 /* y[r, :] = act(x[r] gate_e^T) * (x[r] up_e^T) for the rows r of each group e; rows of no group: 0.  x is rows x k,
- * y rows x hidden; pre (rows x 2 hidden) receives the rounded products, which the backward pass needs. */
+ * y rows x hidden; pre (rows x 2 hidden), if not NULL, receives the rounded products, which the backward pass
+ * needs.  FP32 needs it in any case.  y comes of unrounded products. */
 cublasStatus_t cuMpSGEMM_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
                                             uint64_t k, uint32_t num_groups, const int32_t *group_ends,
                                             const void *x, uint64_t ldx, const void *w, uint64_t ldw,
