@@ -31,6 +31,8 @@
 //   acc_empty[b]  leader's only: 32 arrivals, one from each epilogue warp of both CTAs
 //   tile_full[i]  own: 1 arrival, from the warp that works out the tiles
 //   tile_empty[i] own: 1 arrival from each role that took the tile
+//   sc_full[b]    own: 32 arrivals, of the copies of each lane of the warp that fetches scales
+//   sc_empty[b]   own: 16 arrivals, one from each epilogue warp
 //   pair[q]       own, gated: 4 arrivals, one from each epilogue warp that has quarter q of the lanes
 // Every wait is bounded; no TMA multicast is used.
 #include "activation.cuh"
@@ -65,8 +67,8 @@ constexpr uint32_t MAX_SLICES = 16;
 constexpr uint32_t MIN_SLICE = 4;   // least blocks of K in a slice
 constexpr uint32_t PART = COLS * ROWS_CTA; // elements of a parked sum of one CTA
 constexpr uint32_t JOIN_AHEAD = 4;
-constexpr uint32_t RING = 4;        // blocks of K whose scales a warp has in shared memory or on their way
-constexpr uint32_t SCALE_BYTES = RING * (32 + 2) * 4; // of a warp: each lane's own, then those of the weights
+constexpr uint32_t AT_ONCE = 4;     // blocks of K whose scales are copied together, into two buffers in turn
+constexpr uint32_t SCALE_WORDS = ROWS_CTA + 4; // of a block: the rows', then two of the weights'
 constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
 constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
 // Registers: 640 threads are launched with 96 each; the four warps that issue give back what the sixteen that
@@ -77,13 +79,14 @@ static_assert(128 * REGS_REST + 32 * NUM_EPI_WARPS * REGS_EPI <= NUM_THREADS * R
 
 constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
                    ACC_EMPTY = ACC_FULL + 16, TILE_FULL = ACC_EMPTY + 16, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
-                   PAIR = TILE_EMPTY + 8 * AHEAD, // gated, for each quarter of the lanes
+                   SC_FULL = TILE_EMPTY + 8 * AHEAD, SC_EMPTY = SC_FULL + 16,
+                   PAIR = SC_EMPTY + 16, // gated, for each quarter of the lanes
                    LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
                    TILE = BARS + 320,                // the tiles of the roles
                    TOPS = TILE + AHEAD * 48,         // gated: largest magnitudes, [tile's parity][part][lane]
                    START = TOPS + 2 * PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
                    SCALE = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                   OUT = SCALE + NUM_EPI_WARPS * SCALE_BYTES, BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
+                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
 static_assert(PAIR % 8 == 0 && WIDTH + 4 <= TILE && TILE % 16 == 0 && OUT % 16 == 0, "barriers and flags");
 constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -286,8 +289,11 @@ __device__ __forceinline__ void find_groups(uint8_t *smem, const F8Params &p, ui
 __device__ __forceinline__ void copy_word(uint32_t to, const float *from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// an arrival of this thread, when what it has copied has come
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // sums += scale * the first `cols` columns from taddr on (a multiple of 16).  Gated: the second half of the columns
 // has a scale of its own.  (Packed in pairs, fma.rn.f32x2, the additions took twice as long: 680 cycles a stage
@@ -496,7 +502,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     for (uint32_t q = 0; q < 4; ++q) ptx::mbar_init(sbase + PAIR + 8 * q, PARTS);
     for (uint32_t i = 0; i < AHEAD; ++i) {
       ptx::mbar_init(sbase + TILE_FULL + 8 * i, 1);
-      ptx::mbar_init(sbase + TILE_EMPTY + 8 * i, NUM_EPI_WARPS + (leader ? 2 : 1)); // and the producer, the issuer
+      ptx::mbar_init(sbase + TILE_EMPTY + 8 * i, NUM_EPI_WARPS + (leader ? 3 : 2)); // and who loads, copies, issues
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      ptx::mbar_init(sbase + SC_FULL + 8 * i, 32);
+      ptx::mbar_init(sbase + SC_EMPTY + 8 * i, NUM_EPI_WARPS);
     }
     *abort_flag = 0;
     ptx::mbar_init_fence();
@@ -631,6 +641,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           }
         }
       }
+    } else {
+      // ============================================================== scales (both CTAs)
+      // Asynchronous copies that announce themselves: nothing waits for memory.  (An epilogue warp with loads of its own
+      // on their way waits for them at every read of tensor memory: its stages took 600 cycles instead of 370.)
+      const uint32_t w_blocks = ((GATED ? 2 * p.n : p.n) + BLOCK - 1) / BLOCK;
+      uint32_t b = 0, ph = 1;
+      bool ok = true;
+      Tiles<true> tiles(sbase);
+      while (ok) {
+        ok = tiles.wait(p.status);
+        if (!ok) break;
+        const uint32_t turn = tiles.advance();
+        tiles.read(turn, x);
+        tiles.give_back(turn);
+        if (x.rows == 0) break;
+        const uint32_t row0 = rank * ROWS_CTA, rows = x.rows > row0 ? min(x.rows - row0, ROWS_CTA) : 0u;
+        const float *xs = p.x_scale + (static_cast<uint64_t>(x.row0) + row0 + lane) * p.x_scale_row + x.k0 * p.x_scale_block;
+        const uint32_t block = GATED ? (x.col0 + lane * p.n) / BLOCK : x.col0 / BLOCK + lane;
+        // (columns behind the last block have any)
+        const float *ws = p.w_scale + (static_cast<uint64_t>(x.group) * w_blocks + min(block, w_blocks - 1)) * p.blocks + x.k0;
+        for (uint32_t kb = 0; kb < x.blocks; kb += AT_ONCE) {
+          ok = ptx::warp_agrees(ptx::mbar_wait_backoff(sbase + SC_EMPTY + 8 * b, ph, abort_flag, p.status, ptx::kErrWaitTile, 64));
+          if (!ok) break;
+          for (uint32_t i = 0; i < AT_ONCE && kb + i < x.blocks; ++i) {
+            const uint32_t to = sbase + SCALE + (b * AT_ONCE + i) * (SCALE_WORDS * 4) + lane * 4u;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+              if (lane + 32 * j < rows) copy_word(to + 128u * j, xs + 32 * j * p.x_scale_row);
+            if (lane < 2) copy_word(to + ROWS_CTA * 4, ws);
+            xs += p.x_scale_block;
+            ++ws;
+          }
+          copies_arrive(sbase + SC_FULL + 8 * b);
+          b ^= 1u;
+          if (b == 0) ph ^= 1u;
+        }
+      }
+      wait_copies();
     }
   } else {
     // ================================================================ epilogue (both CTAs)
@@ -640,9 +688,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     const uint32_t mine = ld_shared_one<uint32_t>(sbase + WIDTH) / PARTS; // columns of the warp, from part * mine on
     const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + part * mine;
     const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
-    const uint32_t buf = sbase + OUT + epi * OUT_BYTES, ring = sbase + SCALE + epi * SCALE_BYTES;
+    const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
     const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in a tile
-    uint32_t acc = 0, f_ph = 0, pair_ph = 0, parity = 0;
+    uint32_t acc = 0, f_ph = 0, sc = 0, sc_ph = 0, pair_ph = 0, parity = 0;
     bool ok = true;
     // The reads of tensor memory are complete (wait::ld): that is all there is to order.
     auto give_back = [&]() {
@@ -652,42 +700,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       acc ^= 1u;
       if (acc == 0) f_ph ^= 1u;
     };
-    // Scales: a lane copies the one of its row, lanes 0 and 1 those of the weights, RING - 1 blocks ahead, the first
-    // of a tile before the one in front of it is stored.  A register that waits for them, or a warp that passes
-    // them on by barriers, took 250 to 300 cycles of each stage.
-    const float *xs = nullptr, *ws = nullptr; // of the block to be fetched next
-    uint32_t left = 0, at = 0;                // blocks of the tile to be fetched; slot of the block in turn
-    auto fetch_scales = [&](uint32_t slot) {
-      if (left > 0) {
-        if (xs != nullptr) copy_word(ring + (slot % RING) * 128u + lane * 4u, xs);
-        if (ws != nullptr) copy_word(ring + RING * 128u + ((slot % RING) * 2u + lane) * 4u, ws);
-        --left;
-        if (xs != nullptr) xs += p.x_scale_block;
-        if (ws != nullptr) ++ws;
-      }
-      commit_copies();
-    };
-    auto first_scales = [&](const Tile &y) {
-      xs = ws = nullptr;
-      left = y.rows > lane0 ? y.blocks : 0u;
-      if (lane0 + lane < y.rows)
-        xs = p.x_scale + (static_cast<uint64_t>(y.row0) + lane0 + lane) * p.x_scale_row + y.k0 * p.x_scale_block;
-      if (lane < (GATED ? 2u : 1u)) {
-        const uint32_t w_blocks = ((GATED ? 2 * p.n : p.n) + BLOCK - 1) / BLOCK;
-        const uint32_t block = GATED ? (y.col0 + lane * p.n) / BLOCK : (y.col0 + part * mine) / BLOCK;
-        // (a warp whose columns are all behind the last one has any)
-        ws = p.w_scale + (static_cast<uint64_t>(y.group) * w_blocks + min(block, w_blocks - 1)) * p.blocks + y.k0;
-      }
-#pragma unroll
-      for (uint32_t i = 0; i + 1 < RING; ++i) fetch_scales(at + i);
-    };
     Tiles<true> tiles(sbase);
     ok = tiles.wait(p.status);
     uint32_t slot = tiles.advance();
-    if (ok) {
-      tiles.read(slot, x);
-      if (x.rows > 0) first_scales(x);
-    }
+    if (ok) tiles.read(slot, x);
     while (ok && x.rows > 0) {
       float sums[MOST];
 #pragma unroll
@@ -696,36 +712,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       if (!zero) {
         const bool some = x.rows > lane0;
         const uint32_t blocks = x.blocks;
+        const uint32_t scales = sbase + SCALE + (quarter * 32u + lane) * 4u;
+        const uint32_t weights = sbase + SCALE + (ROWS_CTA + (GATED ? 0u : part * mine / BLOCK)) * 4u;
 #pragma unroll 1
-        for (uint32_t kb = 0; kb < blocks; ++kb) {
-          float t0 = 0.f, t1 = 0.f;
-          if (some) {
-            wait_copies<RING - 2>();
-            __syncwarp();
-            const float own = __uint_as_float(ld_shared_one<uint32_t>(ring + (at % RING) * 128u + lane * 4u));
-            const uint32_t w = ring + RING * 128u + (at % RING) * 8u;
-            t0 = own * __uint_as_float(ld_shared_one<uint32_t>(w));
-            if constexpr (GATED) t1 = own * __uint_as_float(ld_shared_one<uint32_t>(w + 4));
-            fetch_scales(at + RING - 1); // (the slot that all lanes have read a block ago)
-            ++at;
+        for (uint32_t kb = 0, at = 0; kb < blocks; ++kb) {
+          if (at == 0) {
+            ok = ptx::warp_agrees(ptx::mbar_wait_s(sbase + SC_FULL + 8 * sc, sc_ph, sbase + ABORT, p.status, ptx::kErrWaitTile));
+            if (!ok) break;
           }
+          const uint32_t offset = (sc * AT_ONCE + at) * (SCALE_WORDS * 4);
+          const float own = __uint_as_float(ld_shared_one<uint32_t>(scales + offset));
+          const float t0 = own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset)),
+                      t1 = GATED ? own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset + 4)) : 0.f;
+          const bool last = ++at == AT_ONCE || kb + 1 == blocks; // of the scales that were copied together
           ok = ptx::warp_agrees(ptx::mbar_wait_s(sbase + ACC_FULL + 8 * acc, f_ph, sbase + ABORT, p.status, ptx::kErrWaitD0Full));
           if (!ok) break;
           ptx::tc_fence_after();
           if (some) drain<GATED>(t_lanes + acc * COLS, sums, mine, t0, t1);
           if (kb + 1 < blocks) give_back();
+          if (last) {
+            if (lane == 0) ptx::mbar_arrive_relaxed(sbase + SC_EMPTY + 8 * sc);
+            at = 0;
+            sc ^= 1u;
+            if (sc == 0) sc_ph ^= 1u;
+          }
         }
         if (!ok) break;
         // The sums take the place of the last accumulator: what follows has few registers, and little code.
         // (From registers it pushed sums to local memory, which came back from L2.)
         if (some) put_back(t_lanes + acc * COLS, sums, mine);
       }
-      // The next tile's first scales, then this tile again: kept over the loop it took registers from the sums.
-      ok = tiles.wait(p.status);
-      if (!ok) break;
-      const uint32_t next_slot = tiles.advance();
-      tiles.read(next_slot, x);
-      if (x.rows > 0) first_scales(x);
+      // The tile again: kept over the loop it took registers from the sums.
       tiles.read(slot, x);
       const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
       const bool real = lane < rows;
@@ -800,10 +817,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       }
       if (!zero) give_back();
       tiles.give_back(slot);
-      slot = next_slot;
+      ok = tiles.wait(p.status);
+      if (!ok) break;
+      slot = tiles.advance();
       tiles.read(slot, x);
     }
-    wait_copies<0>();
   }
 
   // ---------------------------------------------------------------- teardown
