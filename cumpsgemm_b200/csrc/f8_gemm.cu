@@ -28,11 +28,11 @@
 //   full[s]       leader's only: 2 arrivals, one from each CTA's producer, and the bytes of both CTAs' loads
 //   empty[s]      in both CTAs: commit multicast from the leader
 //   acc_full[b]   in both CTAs: commit multicast
-//   acc_empty[b]  leader's only: 32 arrivals, one from each epilogue warp of both CTAs
+//   acc_empty[b]  leader's only: one arrival from each epilogue warp of both CTAs
 //   tile_full[i]  own: 1 arrival, from the warp that works out the tiles
 //   tile_empty[i] own: 1 arrival from each role that took the tile
 //   sc_full[b]    own: 32 arrivals, of the copies of each lane of the warp that fetches scales
-//   sc_empty[b]   own: 16 arrivals, one from each epilogue warp
+//   sc_empty[b]   own: one arrival from each epilogue warp
 //   pair[q]       own, gated: 4 arrivals, one from each epilogue warp that has quarter q of the lanes
 // Every wait is bounded; no TMA multicast is used.
 #include "activation.cuh"
@@ -53,14 +53,10 @@ namespace {
 constexpr uint32_t ROWS_CTA = 128, ROWS = 2 * ROWS_CTA; // lanes of a CTA and of a pair
 constexpr uint32_t COLS = 256;                          // most columns of a tile
 constexpr uint32_t WIDTHS = 3;                          // that a launch chooses from: 256, 128, 64
-constexpr uint32_t PARTS = 4;                           // epilogue warps that share the columns of 32 lanes
-constexpr uint32_t MOST = COLS / PARTS;                 // most columns of a warp
 constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
 constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
 constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 5;
-constexpr int NUM_EPI_WARPS = 4 * PARTS;
-constexpr int NUM_THREADS = 128 + 32 * NUM_EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t BAND = 8;        // row tiles that are walked together
 constexpr uint32_t MAX_SLICES = 16;
@@ -71,11 +67,20 @@ constexpr uint32_t AT_ONCE = 4;     // blocks of K whose scales are copied toget
 constexpr uint32_t SCALE_WORDS = ROWS_CTA + 4; // of a block: the rows', then two of the weights'
 constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
 constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
-// Registers: 640 threads are launched with 96 each; the four warps that issue give back what the sixteen that
-// hold 64 sums a thread take.
-constexpr int REGS_LAUNCH = PARTS == 4 ? 96 : 168, REGS_REST = 64, REGS_EPI = PARTS == 4 ? 104 : 216;
-static_assert(128 * REGS_REST + 32 * NUM_EPI_WARPS * REGS_EPI <= NUM_THREADS * REGS_LAUNCH,
-              "setmaxnreg draws on the launch's registers");
+// Epilogue warps and registers.  8192 x 8192 x 8192 took 598 us with sixteen warps of 64 columns and 565 with eight of
+// 128, which leave room to read 32 columns ahead.  The gated product of 32764 rows x 2048 x 2 x 4096 took 1190 us with
+// eight and takes 850 with sixteen: its activations are as much work again, and latency.
+// The four warps that issue give back registers that the epilogue's take.
+template <bool GATED> struct Cfg {
+  static constexpr uint32_t PARTS = GATED ? 4 : 2;   // epilogue warps that share the columns of 32 lanes
+  static constexpr uint32_t MOST = COLS / PARTS;     // most columns of a warp
+  static constexpr uint32_t READ = GATED ? 16 : 32;  // columns that it reads at a time
+  static constexpr int EPI_WARPS = 4 * PARTS, THREADS = 128 + 32 * EPI_WARPS;
+  static constexpr int REGS_LAUNCH = GATED ? 96 : 168, REGS_REST = 64, REGS_EPI = GATED ? 104 : 216;
+  static_assert(128 * REGS_REST + 32 * EPI_WARPS * REGS_EPI <= THREADS * REGS_LAUNCH,
+                "setmaxnreg draws on the launch's registers");
+};
+constexpr uint32_t MOST_PARTS = 4;
 
 constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
                    ACC_EMPTY = ACC_FULL + 16, TILE_FULL = ACC_EMPTY + 16, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
@@ -84,9 +89,9 @@ constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * 
                    LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
                    TILE = BARS + 320,                // the tiles of the roles
                    TOPS = TILE + AHEAD * 48,         // gated: largest magnitudes, [tile's parity][part][lane]
-                   START = TOPS + 2 * PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
+                   START = TOPS + 2 * MOST_PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
                    SCALE = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + NUM_EPI_WARPS * OUT_BYTES;
+                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + 4 * MOST_PARTS * OUT_BYTES;
 static_assert(PAIR % 8 == 0 && WIDTH + 4 <= TILE && TILE % 16 == 0 && OUT % 16 == 0, "barriers and flags");
 constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -295,24 +300,30 @@ __device__ __forceinline__ void copies_arrive(uint32_t bar) {
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// sums += scale * the first `cols` columns from taddr on (a multiple of 16).  Gated: the second half of the columns
+__device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[16]) { ptx::tmem_ld_32x32b_x16(taddr, v); }
+__device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32b_x32(taddr, v); }
+
+// sums += scale * the first `cols` columns from taddr on (a multiple of 32).  Gated: the second half of the columns
 // has a scale of its own.  (Packed in pairs, fma.rn.f32x2, the additions took twice as long: 680 cycles a stage
 // against 366, 16 warps of 64 columns; the unit's rate is the same, and the pairs have to be moved together.)
 template <bool GATED>
-__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[MOST], uint32_t cols, float s0, float s1) {
+__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[Cfg<GATED>::MOST], uint32_t cols, float s0, float s1) {
+  constexpr uint32_t MOST = Cfg<GATED>::MOST, READ = Cfg<GATED>::READ;
+  uint32_t x[2][READ];
+  read_columns(taddr, x[0]);
 #pragma unroll
-  for (uint32_t c = 0; c < MOST; c += 16) {
+  for (uint32_t c = 0; c < MOST; c += READ) {
     if (!GATED && c >= cols) break;
-    uint32_t x[16];
-    ptx::tmem_ld_32x32b_x16(taddr + c, x);
     ptx::tmem_ld_wait();
+    // (the next are on their way while these are added; behind the last of a narrow tile's, its neighbour's)
+    if (c + READ < MOST) read_columns(taddr + c + READ, x[(c / READ + 1) & 1]);
     const float s = GATED && c >= MOST / 2 ? s1 : s0;
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) sums[c + i] = fmaf(__uint_as_float(x[i]), s, sums[c + i]);
+    for (uint32_t i = 0; i < READ; ++i) sums[c + i] = fmaf(__uint_as_float(x[(c / READ) & 1][i]), s, sums[c + i]);
   }
 }
 // the way back
-__device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
+template <uint32_t MOST> __device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
 #pragma unroll
   for (uint32_t c = 0; c < MOST; c += 16) {
     if (c >= cols) break;
@@ -343,8 +354,8 @@ __device__ __forceinline__ void park(float *mine, uint32_t cols, uint32_t taddr)
   __syncwarp();
 }
 // by one lane: whether all other slices' sums of these lanes (and columns) have been parked
-__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) {
-  return atomicInc(p.counters + 2 + (x.number * 2 + rank) * NUM_EPI_WARPS + which, x.slices - 1) == x.slices - 1;
+__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) { // (which < 16)
+  return atomicInc(p.counters + 2 + (x.number * 2 + rank) * 16 + which, x.slices - 1) == x.slices - 1;
 }
 // the sums of all slices, the first of which is at `first`, added in their order, back to tensor memory
 __device__ __forceinline__ void join(const float *first, uint32_t slices, uint32_t cols, uint32_t taddr) {
@@ -470,16 +481,17 @@ __device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint
 }
 
 template <F8Type TYPE>
-__device__ __forceinline__ void quantise(const BlockScale &s, const float (&h)[MOST / 2], uint32_t (&w)[16]) {
+__device__ __forceinline__ void quantise(const BlockScale &s, const float (&h)[Cfg<true>::MOST / 2], uint32_t (&w)[16]) {
 #pragma unroll
-  for (uint32_t i = 0; i < MOST / 8; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
 }
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS, 1)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_few,
                    const __grid_constant__ F8Params p) {
+  constexpr uint32_t PARTS = Cfg<GATED>::PARTS, MOST = Cfg<GATED>::MOST, NUM_EPI_WARPS = Cfg<GATED>::EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem =
       reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -531,7 +543,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   const uint32_t tmem_base = *reinterpret_cast<const uint32_t *>(smem + TMEM_PTR);
 
   if (warp < 4) {
-    ptx::setmaxnreg_dec<REGS_REST>();
+    ptx::setmaxnreg_dec<Cfg<GATED>::REGS_REST>();
     const uint32_t width = ld_shared_one<uint32_t>(sbase + WIDTH);
     Tile x;
     if (warp == 0) {
@@ -682,7 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     }
   } else {
     // ================================================================ epilogue (both CTAs)
-    ptx::setmaxnreg_inc<REGS_EPI>();
+    ptx::setmaxnreg_inc<Cfg<GATED>::REGS_EPI>();
     Tile x;
     const uint32_t epi = warp - 4, quarter = warp & 3u, part = epi >> 2;
     const uint32_t mine = ld_shared_one<uint32_t>(sbase + WIDTH) / PARTS; // columns of the warp, from part * mine on
@@ -858,7 +870,7 @@ template <bool GATED> cudaError_t set_up(int *clusters_out) {
     int clusters = sms / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
-    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.blockDim = dim3(Cfg<GATED>::THREADS);
     cfg.dynamicSmemBytes = SMEM;
     int active = 0;
     if (setup_error[dev] == cudaSuccess && cudaOccupancyMaxActiveClusters(&active, kernel, &cfg) == cudaSuccess) {
@@ -914,7 +926,7 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
   p.activation = static_cast<uint8_t>(f.activation);
   const uint64_t out_bytes = GATED ? 1 : a.out_type == GroupedOut::f32 ? 4 : 2;
   p.vector_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo * out_bytes % 16 == 0;
-  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), NUM_THREADS, SMEM, stream, map_x,
+  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), Cfg<GATED>::THREADS, SMEM, stream, map_x,
                         map_x_few, map_w, map_w_few, p);
 }
 
