@@ -28,35 +28,45 @@ template <bool FAST> __device__ __forceinline__ float logistic(float v) {
 }
 
 // The slope costs nothing where it is not used.
-template <bool FAST = false> __device__ __forceinline__ ActResult activate(Activation a, float g) {
+template <Activation ACT, bool FAST> __device__ __forceinline__ ActResult activate(float g) {
   constexpr float kRootHalf = 0.707106781186547524f, kRootTwoOverPi = 0.797884560802865356f,
                   kOverRootTwoPi = 0.398942280401432678f, kCubic = 0.044715f;
   ActResult r;
-  switch (a) {
-  case Activation::silu: {
+  if constexpr (ACT == Activation::silu) {
     const float p = logistic<FAST>(g), q = p * (1.f - p);
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(g, q, p) : p;
-    break;
-  }
-  case Activation::gelu: {
+  } else if constexpr (ACT == Activation::gelu) {
     const float p = 0.5f * erfcf(-g * kRootHalf), e = -0.5f * g * g, q = kOverRootTwoPi * (FAST ? __expf(e) : expf(e));
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(g, q, p) : p;
-    break;
-  }
-  case Activation::gelu_tanh: {
+  } else if constexpr (ACT == Activation::gelu_tanh) {
     const float gg = g * g;
     const float p = logistic<FAST>(2.f * kRootTwoOverPi * g * fmaf(kCubic, gg, 1.f)), q = p * (1.f - p);
     r.value = g * p;
     r.slope = q != 0.f ? fmaf(2.f * g * q, kRootTwoOverPi * fmaf(3.f * kCubic, gg, 1.f), p) : p;
-    break;
-  }
-  default:
+  } else {
     r.value = g < 0.f ? 0.f : g; // (NaN stays NaN)
     r.slope = g > 0.f ? 1.f : 0.f;
   }
   return r;
+}
+
+// f(ActivationIs<a>{}): a loop asks once, and not for each of its values.
+template <Activation A> struct ActivationIs {
+  static constexpr Activation value = A;
+};
+template <class F> __device__ __forceinline__ void with_activation(int a, F &&f) {
+  switch (static_cast<Activation>(a)) {
+  case Activation::silu:
+    return f(ActivationIs<Activation::silu>{});
+  case Activation::gelu:
+    return f(ActivationIs<Activation::gelu>{});
+  case Activation::gelu_tanh:
+    return f(ActivationIs<Activation::gelu_tanh>{});
+  default:
+    return f(ActivationIs<Activation::relu>{});
+  }
 }
 
 } // namespace cumpsgemm_b200

@@ -53,14 +53,16 @@ __global__ void __launch_bounds__(kThreads) quantize_block_rows_kernel(const Blo
       Eight<T, WHOLE> gate[kAtOnce], up[kAtOnce];
       Eight<T, WHOLE>::load(RowReader(row, bytes), first, 32, gate);
       Eight<T, WHOLE>::load(RowReader(row + a.k, bytes), first, 32, up);
+      with_activation(a.activation, [&](auto act) {
 #pragma unroll
-      for (uint32_t j = 0; j < kAtOnce; ++j) {
-        float u[8];
-        gate[j].values(v[j]);
-        up[j].values(u);
+        for (uint32_t j = 0; j < kAtOnce; ++j) {
+          float u[8];
+          gate[j].values(v[j]);
+          up[j].values(u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = activate<true>(static_cast<Activation>(a.activation), v[j][i]).value * u[i];
-      }
+          for (int i = 0; i < 8; ++i) v[j][i] = activate<act.value, true>(v[j][i]).value * u[i];
+        }
+      });
     } else {
       Eight<T, WHOLE> x[kAtOnce];
       Eight<T, WHOLE>::load(RowReader(row, bytes), first, 32, x);
@@ -178,28 +180,30 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(const GatedRowsArg
       // (dh may be the first half of out: a thread reads its values before it writes there)
       Eight<T, WHOLE>::template load<false>(RowReader(static_cast<const T *>(a.dh) + r * a.lddh, bytes), first, 32, dh);
     T *out = static_cast<T *>(a.out) + r * a.ldo;
+    with_activation(a.activation, [&](auto kind) {
 #pragma unroll
-    for (uint32_t j = 0; j < kGatedAtOnce; ++j) {
-      const uint32_t col = 8 * (first + 32 * j);
-      if (col >= a.hidden) continue;
-      const uint32_t n = min(8u, a.hidden - col);
-      float g[8], u[8], d[8];
-      gate[j].values(g);
-      up[j].values(u);
-      if constexpr (GRAD) dh[j].values(d);
+      for (uint32_t j = 0; j < kGatedAtOnce; ++j) {
+        const uint32_t col = 8 * (first + 32 * j);
+        if (col >= a.hidden) continue;
+        const uint32_t n = min(8u, a.hidden - col);
+        float g[8], u[8], d[8];
+        gate[j].values(g);
+        up[j].values(u);
+        if constexpr (GRAD) dh[j].values(d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const ActResult act = activate<sizeof(T) == 2>(static_cast<Activation>(a.activation), g[i]);
-        if constexpr (GRAD) {
-          g[i] = d[i] * u[i] * act.slope;
-          u[i] = d[i] * act.value;
-        } else {
-          g[i] = act.value * u[i];
+        for (int i = 0; i < 8; ++i) {
+          const ActResult act = activate<kind.value, sizeof(T) == 2>(g[i]);
+          if constexpr (GRAD) {
+            g[i] = d[i] * u[i] * act.slope;
+            u[i] = d[i] * act.value;
+          } else {
+            g[i] = act.value * u[i];
+          }
         }
+        store_values(out + col, n, g);
+        if constexpr (GRAD) store_values(out + a.hidden + col, n, u);
       }
-      store_values(out + col, n, g);
-      if constexpr (GRAD) store_values(out + a.hidden + col, n, u);
-    }
+    });
   }
 }
 

@@ -36,6 +36,19 @@ struct BlockScale {
     const float p = __fmul_rn(x * up, most), q = __fmul_rn(p, inverse);
     return __fmaf_rn(__fmaf_rn(-q, top, p), inverse, q);
   }
+  // The same, rounded three times: for values that are sums themselves, where no tie is meant.  Where the factor
+  // would over- or underflow, by quotient().
+  __device__ __forceinline__ bool plain(float &factor) const {
+    factor = __fmul_rn(up, __fmul_rn(most, inverse));
+    return factor > 0x1p-100f && factor < 0x1p100f;
+  }
+  template <F8Type TYPE> __device__ __forceinline__ uint32_t four_of_sums(float x, float y, float z, float w) const {
+    float f;
+    if (!plain(f) || zero) return four<TYPE>(x, y, z, w);
+    constexpr auto kind = TYPE == F8Type::e4m3 ? __NV_E4M3 : __NV_E5M2;
+    return __nv_cvt_float2_to_fp8x2(make_float2(x * f, y * f), __NV_SATFINITE, kind) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(z * f, w * f), __NV_SATFINITE, kind)) << 16;
+  }
   template <F8Type TYPE> __device__ __forceinline__ uint32_t pair(float x, float y) const {
     return __nv_cvt_float2_to_fp8x2(make_float2(quotient(x), quotient(y)), __NV_SATFINITE,
                                     TYPE == F8Type::e4m3 ? __NV_E4M3 : __NV_E5M2);

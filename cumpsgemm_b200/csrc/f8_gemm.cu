@@ -483,7 +483,7 @@ __device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint
 template <F8Type TYPE>
 __device__ __forceinline__ void quantise(const BlockScale &s, const float (&h)[Cfg<true>::MOST / 2], uint32_t (&w)[16]) {
 #pragma unroll
-  for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i) w[i] = s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i) w[i] = s.four_of_sums<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
 }
 
 template <bool GATED>
@@ -789,11 +789,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
             uint32_t gate[16], up[16];
             fetch(t_sums + c, zero, gate);
             fetch(t_sums + MOST / 2 + c, zero, up);
+            with_activation(p.activation, [&](auto act) {
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-              h[c + i] = activate<true>(static_cast<Activation>(p.activation), __uint_as_float(gate[i])).value * __uint_as_float(up[i]);
-              top = max(top, __float_as_uint(h[c + i]) & 0x7fffffffu);
-            }
+              for (uint32_t i = 0; i < 16; ++i)
+                h[c + i] = activate<act.value, true>(__uint_as_float(gate[i])).value * __uint_as_float(up[i]);
+            });
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) top = max(top, __float_as_uint(h[c + i]) & 0x7fffffffu);
           }
           // (written again two tiles on, when the other warps have long read them: they have been met since)
           uint32_t *tops = reinterpret_cast<uint32_t *>(smem + TOPS) + parity * PARTS * ROWS_CTA + quarter * 32u + lane;

@@ -626,7 +626,6 @@ __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, c
                                             uint32_t cols, uint32_t features, uint32_t hidden) {
   const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u;
   const bool vector = (p.vector_out & 1u) != 0, vector_pre = (p.vector_out & 2u) != 0;
-  const auto act = static_cast<Activation>(p.activation);
   // pre, as in store_by_rows
   const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
   const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
@@ -667,6 +666,11 @@ __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, c
           store_piece(pre + col * p.ldpre + (chunk >> 1) * static_cast<uint64_t>(hidden) + 8 * (chunk & 1u), v, elems, vector_pre);
       }
     }
+    with_activation(p.activation, [&](auto act) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        lo[i] = __float_as_uint(activate<act.value, true>(__uint_as_float(lo[i])).value * __uint_as_float(hi[i]));
+    });
     __syncwarp();
 #pragma unroll
     for (uint32_t g = 0; g < 4; g += 2) {
@@ -674,8 +678,7 @@ __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, c
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) { // group g + i / 2, features 8 (i % 2) on
         const uint32_t at = 4 * (g + i / 2) + 2 * (i & 1u);
-        w[i] = pack_results<T>(activate<true>(act, __uint_as_float(lo[at])).value * __uint_as_float(hi[at]),
-                               activate<true>(act, __uint_as_float(lo[at + 1])).value * __uint_as_float(hi[at + 1]));
+        w[i] = pack_results<T>(__uint_as_float(lo[at]), __uint_as_float(lo[at + 1]));
       }
       ptx::stmatrix_x4_trans(in_h + g * 256u, w[0], w[1], w[2], w[3]);
     }
@@ -700,7 +703,6 @@ __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *o
   const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u;
   const uint32_t elems = least(features, 8 * chunk, 8);
   const bool vector = (p.vector_out & 1u) != 0, vector_pre = (p.vector_out & 2u) != 0;
-  const auto act = static_cast<Activation>(p.activation);
   const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
   const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
 #pragma unroll 1
@@ -730,17 +732,19 @@ __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *o
           ptx::ldmatrix_x4_trans(in + g * 512u, w[q][g][0], w[q][g][1], w[q][g][2], w[q][g][3]);
       }
       ptx::tmem_ld_wait();
+      with_activation(p.activation, [&](auto act) {
 #pragma unroll
-      for (uint32_t g = 0; g < 4; ++g)
+        for (uint32_t g = 0; g < 4; ++g)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const float x = __uint_as_float(i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4]),
-                      y = __uint_as_float(i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3]);
-          const float2 gate = unpack<T>(w[0][g][i]), up = unpack<T>(w[1][g][i]);
-          const ActResult a = activate<true>(act, gate.x), b = activate<true>(act, gate.y);
-          w[0][g][i] = pack_results<T>(x * up.x * a.slope, y * up.y * b.slope);
-          w[1][g][i] = pack_results<T>(x * a.value, y * b.value);
-        }
+          for (uint32_t i = 0; i < 4; ++i) {
+            const float x = __uint_as_float(i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4]),
+                        y = __uint_as_float(i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3]);
+            const float2 gate = unpack<T>(w[0][g][i]), up = unpack<T>(w[1][g][i]);
+            const ActResult a = activate<act.value, true>(gate.x), b = activate<act.value, true>(gate.y);
+            w[0][g][i] = pack_results<T>(x * up.x * a.slope, y * up.y * b.slope);
+            w[1][g][i] = pack_results<T>(x * a.value, y * b.value);
+          }
+      });
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < 32; ++i) w[i / 16][i / 4 % 4][i % 4] = 0;
