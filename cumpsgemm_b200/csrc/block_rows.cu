@@ -18,10 +18,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr uint32_t kBlock = 128;
 
 // the largest magnitude of 16 neighbouring lanes' values
-__device__ __forceinline__ float half_warp_largest(uint32_t bits) {
+__device__ __forceinline__ uint32_t half_warp_largest(uint32_t bits) {
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-  return __uint_as_float(bits);
+  return bits;
 }
 __device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
   uint32_t top = 0; // (ordered as the magnitudes, NaN above all)
@@ -41,38 +41,63 @@ __global__ void __launch_bounds__(kThreads) quantize_block_rows_kernel(const Blo
   CUMPSGEMM_CHAINED_KERNEL_ENTRY();
   const uint32_t lane = threadIdx.x & 31u, segments = (a.k + kSegment - 1) / kSegment;
   const uint64_t tasks = static_cast<uint64_t>(a.rows) * segments, step = static_cast<uint64_t>(gridDim.x) * kWarps;
-  for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < tasks; t += step) {
-    const uint32_t r = static_cast<uint32_t>(t / segments), seg = static_cast<uint32_t>(t - static_cast<uint64_t>(r) * segments);
+  uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  Eight<T, WHOLE> x[kAtOnce], up[GATED ? kAtOnce : 1];
+  auto fetch = [&](uint64_t task) {
+    const uint32_t r = static_cast<uint32_t>(task / segments);
+    const uint32_t first = static_cast<uint32_t>(task - static_cast<uint64_t>(r) * segments) * (kSegment / 8) + lane;
     const int64_t from = a.row_index != nullptr ? __ldg(a.row_index + r) : static_cast<int64_t>(r);
     const bool real = from >= 0 && from < static_cast<int64_t>(a.src_rows);
     const T *row = static_cast<const T *>(a.x) + (real ? from : 0) * a.ldx;
     const uint64_t bytes = real ? a.k * static_cast<uint64_t>(sizeof(T)) : 0;
-    const uint32_t first = seg * (kSegment / 8) + lane;
+    Eight<T, WHOLE>::load(RowReader(row, bytes), first, 32, x);
+    if constexpr (GATED) Eight<T, WHOLE>::load(RowReader(row + a.k, bytes), first, 32, up);
+  };
+  if (t < tasks) fetch(t);
+  for (; t < tasks; t += step) {
+    const uint32_t r = static_cast<uint32_t>(t / segments);
+    const uint32_t first = static_cast<uint32_t>(t - static_cast<uint64_t>(r) * segments) * (kSegment / 8) + lane;
     float v[kAtOnce][8];
+    uint32_t top[kAtOnce]; // the bits of each lane's largest magnitude
     if constexpr (GATED) {
-      Eight<T, WHOLE> gate[kAtOnce], up[kAtOnce];
-      Eight<T, WHOLE>::load(RowReader(row, bytes), first, 32, gate);
-      Eight<T, WHOLE>::load(RowReader(row + a.k, bytes), first, 32, up);
       with_activation(a.activation, [&](auto act) {
 #pragma unroll
         for (uint32_t j = 0; j < kAtOnce; ++j) {
           float u[8];
-          gate[j].values(v[j]);
+          x[j].values(v[j]);
           up[j].values(u);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[j][i] = activate<act.value, true>(v[j][i]).value * u[i];
+          top[j] = largest_bits(v[j]);
         }
       });
     } else {
-      Eight<T, WHOLE> x[kAtOnce];
-      Eight<T, WHOLE>::load(RowReader(row, bytes), first, 32, x);
 #pragma unroll
       for (uint32_t j = 0; j < kAtOnce; ++j) x[j].values(v[j]);
+      if constexpr (sizeof(T) == 2) { // two values to an instruction, and two blocks
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; j += 2) {
+          const uint32_t a0 = x[j].largest(0), a1 = x[j + 1].largest(0);
+          uint32_t both = __vmaxu2(__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632));
+#pragma unroll
+          for (int d = 8; d > 0; d >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+          top[j] = __float_as_uint(value_of<T>(both & 0xffffu));
+          top[j + 1] = __float_as_uint(value_of<T>(both >> 16));
+        }
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j) top[j] = largest_bits(v[j]);
+      }
+    }
+    if (t + step < tasks) fetch(t + step); // on its way while this one's leaves
+    if constexpr (GATED || sizeof(T) == 4) {
+#pragma unroll
+      for (uint32_t j = 0; j < kAtOnce; ++j) top[j] = half_warp_largest(top[j]);
     }
     uint8_t *dst = a.q + r * a.ldq;
 #pragma unroll
     for (uint32_t j = 0; j < kAtOnce; ++j) {
-      const BlockScale s(half_warp_largest(largest_bits(v[j])), TYPE);
+      const BlockScale s(__uint_as_float(top[j]), TYPE);
       const uint32_t col = 8 * (first + 32 * j);
       if (col < a.k) {
         store_eight(reinterpret_cast<int8_t *>(dst), col, a.k, eight<TYPE>(s, v[j]));

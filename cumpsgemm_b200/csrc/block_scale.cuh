@@ -17,29 +17,38 @@ namespace cumpsgemm_b200 {
 enum class F8Type : int { e4m3 = 0, e5m2 = 1 };
 
 struct BlockScale {
-  float scale, up, top, inverse, most;
+  float scale, up, top, inverse; // up: a power of two that brings the largest near 1, times the type's largest value
   bool zero; // q is 0
   __device__ __forceinline__ BlockScale(float largest, F8Type type) {
-    most = type == F8Type::e4m3 ? 448.f : 57344.f;
+    const float most = type == F8Type::e4m3 ? 448.f : 57344.f;
     const uint32_t e = __float_as_uint(largest) >> 23; // (largest is not negative)
     const bool none = e == 255u;
-    scale = none ? __uint_as_float(0x7fffffffu) : __fdiv_rn(largest, most);
+    scale = none ? __uint_as_float(0x7fffffffu) : over(largest, most, type);
     zero = none || scale == 0.f;
-    // by a power of two that brings the largest near 1: nothing over- or underflows that counts
-    up = __uint_as_float(min(max(254u - min(e, 254u), 1u), 254u) << 23);
-    top = zero ? 1.f : largest * up;
-    inverse = __frcp_rn(top);
+    // (at most 2^108, so that nothing overflows; what underflows is 0 in 8 bits)
+    const float power = __uint_as_float(min(max(254u - min(e, 254u), 1u), 235u) << 23);
+    top = zero ? 1.f : largest * power;
+    const float about = __fdividef(1.f, top); // (one Newton step more; quotient() needs no more than that)
+    inverse = __fmaf_rn(__fmaf_rn(-top, about, 1.f), about, about);
+    up = power * most; // (exact)
   }
-  // x * most / top: a product with the reciprocal, whose error one more step takes off (Markstein's, with the
-  // remainder from a fused multiply-add)
+  // largest / most, rounded once.  The step that makes a product with the rounded reciprocal the rounded quotient
+  // (Markstein's, with the remainder from a fused multiply-add) holds where nothing comes near the subnormals.
+  static __device__ __forceinline__ float over(float largest, float most, F8Type type) {
+    if (largest < 0x1p-90f) return __fdiv_rn(largest, most);
+    const float r = type == F8Type::e4m3 ? 1.f / 448.f : 1.f / 57344.f, q = __fmul_rn(largest, r);
+    return __fmaf_rn(__fmaf_rn(-q, most, largest), r, q);
+  }
+  // x * most / top: the same step.  Where the quotient is a tie between two 8-bit values, the remainder is exact, its
+  // product with the reciprocal is off by 2^-22 of itself, and the sum is rounded to the tie.
   __device__ __forceinline__ float quotient(float x) const {
-    const float p = __fmul_rn(x * up, most), q = __fmul_rn(p, inverse);
+    const float p = __fmul_rn(x, up), q = __fmul_rn(p, inverse);
     return __fmaf_rn(__fmaf_rn(-q, top, p), inverse, q);
   }
-  // The same, rounded three times: for values that are sums themselves, where no tie is meant.  Where the factor
+  // The same with one factor, rounded twice: for values that are sums themselves, where no tie is meant.  Where it
   // would over- or underflow, by quotient().
   __device__ __forceinline__ bool plain(float &factor) const {
-    factor = __fmul_rn(up, __fmul_rn(most, inverse));
+    factor = __fmul_rn(up, inverse);
     return factor > 0x1p-100f && factor < 0x1p100f;
   }
   template <F8Type TYPE> __device__ __forceinline__ uint32_t four_of_sums(float x, float y, float z, float w) const {
