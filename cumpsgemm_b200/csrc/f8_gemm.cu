@@ -52,12 +52,14 @@ namespace {
 
 constexpr uint32_t ROWS_CTA = 128, ROWS = 2 * ROWS_CTA; // lanes of a CTA and of a pair
 constexpr uint32_t COLS = 256;                          // most columns of a tile
-constexpr uint32_t WIDTHS = 3;                          // that a launch chooses from: 256, 128, 64
+constexpr uint32_t WIDTHS = 2;                          // that a launch chooses from: 256, 128
 constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
 constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
 constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 5;
 constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t MOST_SLOTS = 4;      // accumulators, of TMEM_COLS / slots columns
+__device__ __forceinline__ uint32_t slots_of(uint32_t width) { return width > 128 ? 2u : MOST_SLOTS; }
 constexpr uint32_t BAND = 8;        // row tiles that are walked together
 constexpr uint32_t MAX_SLICES = 16;
 constexpr uint32_t MIN_SLICE = 4;   // least blocks of K in a slice
@@ -74,7 +76,7 @@ constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of
 template <bool GATED> struct Cfg {
   static constexpr uint32_t PARTS = GATED ? 4 : 2;   // epilogue warps that share the columns of 32 lanes
   static constexpr uint32_t MOST = COLS / PARTS;     // most columns of a warp
-  static constexpr uint32_t READ = GATED ? 16 : 32;  // columns that it reads at a time
+  static constexpr uint32_t READ = 16;               // columns that it reads at a time
   static constexpr int EPI_WARPS = 4 * PARTS, THREADS = 128 + 32 * EPI_WARPS;
   static constexpr int REGS_LAUNCH = GATED ? 96 : 168, REGS_REST = 64, REGS_EPI = GATED ? 104 : 216;
   static_assert(128 * REGS_REST + 32 * EPI_WARPS * REGS_EPI <= THREADS * REGS_LAUNCH,
@@ -83,7 +85,7 @@ template <bool GATED> struct Cfg {
 constexpr uint32_t MOST_PARTS = 4;
 
 constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
-                   ACC_EMPTY = ACC_FULL + 16, TILE_FULL = ACC_EMPTY + 16, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
+                   ACC_EMPTY = ACC_FULL + 8 * MOST_SLOTS, TILE_FULL = ACC_EMPTY + 8 * MOST_SLOTS, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
                    SC_FULL = TILE_EMPTY + 8 * AHEAD, SC_EMPTY = SC_FULL + 16,
                    PAIR = SC_EMPTY + 16, // gated, for each quarter of the lanes
                    LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
@@ -303,25 +305,53 @@ __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;
 __device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[16]) { ptx::tmem_ld_32x32b_x16(taddr, v); }
 __device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32b_x32(taddr, v); }
 
-// sums += scale * the first `cols` columns from taddr on (a multiple of 32).  Gated: the second half of the columns
-// has a scale of its own.  (Packed in pairs, fma.rn.f32x2, the additions took twice as long: 680 cycles a stage
-// against 366, 16 warps of 64 columns; the unit's rate is the same, and the pairs have to be moved together.)
-template <bool GATED>
-__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[Cfg<GATED>::MOST], uint32_t cols, float s0, float s1) {
-  constexpr uint32_t MOST = Cfg<GATED>::MOST, READ = Cfg<GATED>::READ;
+// sums += scale * COLUMNS columns from taddr on; the next are on their way while these are added.  Gated: the second
+// half of the columns has a scale of its own.
+template <bool GATED, uint32_t COLUMNS>
+__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[Cfg<GATED>::MOST], float s0, float s1) {
+  constexpr uint32_t READ = Cfg<GATED>::READ;
   uint32_t x[2][READ];
   read_columns(taddr, x[0]);
 #pragma unroll
-  for (uint32_t c = 0; c < MOST; c += READ) {
-    if (!GATED && c >= cols) break;
+  for (uint32_t c = 0; c < COLUMNS; c += READ) {
     ptx::tmem_ld_wait();
-    // (the next are on their way while these are added; behind the last of a narrow tile's, its neighbour's)
-    if (c + READ < MOST) read_columns(taddr + c + READ, x[(c / READ + 1) & 1]);
-    const float s = GATED && c >= MOST / 2 ? s1 : s0;
+    if (c + READ < COLUMNS) read_columns(taddr + c + READ, x[(c / READ + 1) & 1]);
+    const float s = GATED && c >= COLUMNS / 2 ? s1 : s0;
 #pragma unroll
     for (uint32_t i = 0; i < READ; ++i) sums[c + i] = fmaf(__uint_as_float(x[(c / READ) & 1][i]), s, sums[c + i]);
   }
 }
+
+// Whether both phases are over.  For the loops over stages, in which a branch costs a warp some 30 cycles: one
+// question, and arrivals that are not branched around.
+__device__ __forceinline__ bool both_over(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(done)
+      : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ void arrive_if(bool yes, uint32_t bar) { // own barrier; a release
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(bar),
+               "r"(static_cast<uint32_t>(yes))
+               : "memory");
+}
+__device__ __forceinline__ void arrive_cluster_relaxed_if(bool yes, uint32_t cluster_addr) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}\n" ::"r"(cluster_addr),
+      "r"(static_cast<uint32_t>(yes))
+      : "memory");
+}
+
 // the way back
 template <uint32_t MOST> __device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
 #pragma unroll
@@ -507,7 +537,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
       ptx::mbar_init(sbase + FULL + 8 * s, 2);
       ptx::mbar_init(sbase + EMPTY + 8 * s, 1);
     }
-    for (uint32_t b = 0; b < 2; ++b) {
+    for (uint32_t b = 0; b < MOST_SLOTS; ++b) {
       ptx::mbar_init(sbase + ACC_FULL + 8 * b, 1);
       ptx::mbar_init(sbase + ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
     }
@@ -607,23 +637,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
         constexpr uint64_t kStage = STAGE_BYTES >> 4;
         const uint64_t a0 = ptx::make_kmajor_desc<BLOCK>(sbase), b0 = ptx::make_kmajor_desc<BLOCK>(sbase + TILE_BYTES);
         const uint32_t idesc = p.idesc | ((width >> 3) << 17);
+        const uint32_t slots = slots_of(width), slot_cols = TMEM_COLS / slots;
         uint32_t s = 0, ph = 0, acc = 0, e_ph = 1;
         bool ok = true;
         Tiles<false> tiles(sbase);
         while (ok && tiles.next(p.status, x)) {
           for (uint32_t kb = 0; kb < x.blocks; ++kb) {
-            ok = ptx::mbar_wait(sbase + ACC_EMPTY + 8 * acc, e_ph, abort_flag, p.status, ptx::kErrWaitD0Empty) &&
-                 ptx::mbar_wait(sbase + FULL + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitFull);
+            // (the accumulator last: what follows its wait lengthens the way round)
+            ok = ptx::mbar_wait(sbase + FULL + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitFull) &&
+                 ptx::mbar_wait(sbase + ACC_EMPTY + 8 * acc, e_ph, abort_flag, p.status, ptx::kErrWaitD0Empty);
             if (!ok) break;
             ptx::tc_fence_after();
-            const uint32_t d = tmem_base + acc * COLS;
+            const uint32_t d = tmem_base + acc * slot_cols;
 #pragma unroll
             for (uint32_t ks = 0; ks < 4; ++ks)
               ptx::mma_f8_ss_pair(d, a0 + s * kStage + 2 * ks, b0 + s * kStage + 2 * ks, idesc, ks != 0);
             ptx::tc_commit_pair(sbase + ACC_FULL + 8 * acc, BOTH);
             ptx::tc_commit_pair(sbase + EMPTY + 8 * s, BOTH);
-            acc ^= 1u;
-            if (acc == 0) e_ph ^= 1u;
+            if (++acc == slots) {
+              acc = 0;
+              e_ph ^= 1u;
+            }
             if (++s == STAGES) {
               s = 0;
               ph ^= 1u;
@@ -697,20 +731,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
     ptx::setmaxnreg_inc<Cfg<GATED>::REGS_EPI>();
     Tile x;
     const uint32_t epi = warp - 4, quarter = warp & 3u, part = epi >> 2;
-    const uint32_t mine = ld_shared_one<uint32_t>(sbase + WIDTH) / PARTS; // columns of the warp, from part * mine on
+    const uint32_t width = ld_shared_one<uint32_t>(sbase + WIDTH), slots = slots_of(width), slot_cols = TMEM_COLS / slots;
+    const uint32_t mine = width / PARTS; // columns of the warp, from part * mine on
     const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + part * mine;
     const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
     const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
     const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in a tile
-    uint32_t acc = 0, f_ph = 0, sc = 0, sc_ph = 0, pair_ph = 0, parity = 0;
+    uint32_t turn = 0, group = 0, pair_ph = 0, parity = 0; // accumulators and groups of scales that are behind
     bool ok = true;
-    // The reads of tensor memory are complete (wait::ld): that is all there is to order.
-    auto give_back = [&]() {
+    const uint32_t slots_log2 = slots == 2 ? 1u : 2u;
+    auto slot_now = [&]() { return turn & (slots - 1u); };
+    // An accumulator is given back when its reads are complete (wait::ld): that is all there is to order.
+    auto give_back = [&](bool yes) {
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(acc_empty + 8 * acc);
-      acc ^= 1u;
-      if (acc == 0) f_ph ^= 1u;
+      arrive_cluster_relaxed_if(yes && lane == 0, acc_empty + 8 * slot_now());
+      turn += yes;
+    };
+    // The stages of a tile; the last accumulator is not given back.
+    auto all_stages = [&](uint32_t blocks, auto &&add) {
+      const uint32_t scales = sbase + SCALE + (quarter * 32u + lane) * 4u;
+      const uint32_t weights = sbase + SCALE + (ROWS_CTA + (GATED ? 0u : part * mine / BLOCK)) * 4u;
+#pragma unroll 1
+      for (uint32_t kb = 0; kb < blocks; ++kb) {
+        const uint32_t b = group & 1u, sc_full = sbase + SC_FULL + 8 * b, full = sbase + ACC_FULL + 8 * slot_now();
+        const uint32_t sc_ph = (group >> 1) & 1u, ph = (turn >> slots_log2) & 1u;
+        if (!ptx::warp_agrees(both_over(sc_full, sc_ph, full, ph))) {
+          ok = ptx::warp_agrees(ptx::mbar_wait_s(sc_full, sc_ph, sbase + ABORT, p.status, ptx::kErrWaitTile) &&
+                                ptx::mbar_wait_s(full, ph, sbase + ABORT, p.status, ptx::kErrWaitD0Full));
+          if (!ok) break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t offset = (b * AT_ONCE + kb % AT_ONCE) * (SCALE_WORDS * 4);
+        const float own = __uint_as_float(ld_shared_one<uint32_t>(scales + offset));
+        const float t0 = own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset)),
+                    t1 = GATED ? own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset + 4)) : 0.f;
+        add(t_lanes + slot_now() * slot_cols, t0, t1);
+        give_back(kb + 1 < blocks);
+        const bool last = kb % AT_ONCE == AT_ONCE - 1 || kb + 1 == blocks; // of the scales that were copied together
+        arrive_if(last && lane == 0, sbase + SC_EMPTY + 8 * b);
+        group += last;
+      }
     };
     Tiles<true> tiles(sbase);
     ok = tiles.wait(p.status);
@@ -722,43 +783,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
       for (uint32_t i = 0; i < MOST; ++i) sums[i] = 0.f;
       const bool zero = x.blocks == 0;
       if (!zero) {
-        const bool some = x.rows > lane0;
-        const uint32_t blocks = x.blocks;
-        const uint32_t scales = sbase + SCALE + (quarter * 32u + lane) * 4u;
-        const uint32_t weights = sbase + SCALE + (ROWS_CTA + (GATED ? 0u : part * mine / BLOCK)) * 4u;
-#pragma unroll 1
-        for (uint32_t kb = 0, at = 0; kb < blocks; ++kb) {
-          if (at == 0) {
-            ok = ptx::warp_agrees(ptx::mbar_wait_s(sbase + SC_FULL + 8 * sc, sc_ph, sbase + ABORT, p.status, ptx::kErrWaitTile));
-            if (!ok) break;
-          }
-          const uint32_t offset = (sc * AT_ONCE + at) * (SCALE_WORDS * 4);
-          const float own = __uint_as_float(ld_shared_one<uint32_t>(scales + offset));
-          const float t0 = own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset)),
-                      t1 = GATED ? own * __uint_as_float(ld_shared_one<uint32_t>(weights + offset + 4)) : 0.f;
-          const bool last = ++at == AT_ONCE || kb + 1 == blocks; // of the scales that were copied together
-          ok = ptx::warp_agrees(ptx::mbar_wait_s(sbase + ACC_FULL + 8 * acc, f_ph, sbase + ABORT, p.status, ptx::kErrWaitD0Full));
-          if (!ok) break;
-          ptx::tc_fence_after();
-          if (some) drain<GATED>(t_lanes + acc * COLS, sums, mine, t0, t1);
-          if (kb + 1 < blocks) give_back();
-          if (last) {
-            if (lane == 0) ptx::mbar_arrive_relaxed(sbase + SC_EMPTY + 8 * sc);
-            at = 0;
-            sc ^= 1u;
-            if (sc == 0) sc_ph ^= 1u;
-          }
+        if (x.rows <= lane0) {
+          all_stages(x.blocks, [](uint32_t, float, float) {});
+        } else if (GATED || mine == MOST) {
+          all_stages(x.blocks, [&](uint32_t from, float t0, float t1) { drain<GATED, MOST>(from, sums, t0, t1); });
+        } else {
+          all_stages(x.blocks, [&](uint32_t from, float t0, float t1) { drain<GATED, MOST / 2>(from, sums, t0, t1); });
         }
         if (!ok) break;
         // The sums take the place of the last accumulator: what follows has few registers, and little code.
         // (From registers it pushed sums to local memory, which came back from L2.)
-        if (some) put_back(t_lanes + acc * COLS, sums, mine);
+        if (x.rows > lane0) put_back(t_lanes + slot_now() * slot_cols, sums, mine);
       }
       // The tile again: kept over the loop it took registers from the sums.
       tiles.read(slot, x);
       const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
       const bool real = lane < rows;
-      const uint32_t t_sums = t_lanes + acc * COLS;
+      const uint32_t t_sums = t_lanes + slot_now() * slot_cols;
       bool done = rows == 0;
       if constexpr (GATED) {
         // (all warps that have these lanes have rows, or none)
@@ -829,7 +870,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
           store_sums(p, buf, t_sums, zero, (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col, rows, cols,
                      p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr);
       }
-      if (!zero) give_back();
+      if (!zero) give_back(true);
       tiles.give_back(slot);
       ok = tiles.wait(p.status);
       if (!ok) break;
