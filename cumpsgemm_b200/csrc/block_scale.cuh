@@ -51,9 +51,8 @@ struct BlockScale {
     factor = __fmul_rn(up, inverse);
     return factor > 0x1p-100f && factor < 0x1p100f;
   }
-  template <F8Type TYPE> __device__ __forceinline__ uint32_t four_of_sums(float x, float y, float z, float w) const {
-    float f;
-    if (!plain(f) || zero) return four<TYPE>(x, y, z, w);
+  template <F8Type TYPE>
+  static __device__ __forceinline__ uint32_t four_by(float f, float x, float y, float z, float w) {
     constexpr auto kind = TYPE == F8Type::e4m3 ? __NV_E4M3 : __NV_E5M2;
     return __nv_cvt_float2_to_fp8x2(make_float2(x * f, y * f), __NV_SATFINITE, kind) |
            static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(z * f, w * f), __NV_SATFINITE, kind)) << 16;

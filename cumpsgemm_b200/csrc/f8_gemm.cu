@@ -418,36 +418,45 @@ __device__ __forceinline__ void join(const float *first, uint32_t slices, uint32
 
 // 64 bytes of each of a warp's rows, which its lanes have in w, to memory by way of the warp's buffer: a lane
 // stores its own as 16-byte chunks (those of two rows side by side XORed, so that neither side meets a bank twice)
-// and four lanes then write a row's together.  E: an element; `elems` of them in the row, `rows` rows.
-template <class E>
-__device__ __forceinline__ void store_64_bytes(uint32_t buf, const uint32_t (&w)[16], E *out, uint64_t ldo, uint32_t rows,
-                                               uint32_t elems, bool vector) {
-  constexpr uint32_t PER = 16 / sizeof(E), ALL = 4 * PER;
+// and four lanes then write a row's together.
+__device__ __forceinline__ void to_buffer(uint32_t buf, const uint32_t (&w)[16]) {
   const uint32_t lane = threadIdx.x & 31u;
   __syncwarp(); // the buffer has been read
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i)
     st_shared(buf + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   __syncwarp();
-  if (vector) {
-    const uint32_t chunk = lane & 3u, n = elems > chunk * PER ? min(elems - chunk * PER, PER) : 0u;
+}
+// Whole 64 bytes of `rows` rows, at 16-byte aligned addresses; out: at the lane's chunk of row lane / 4, `step` bytes
+// from a row to the one 8 further on.  No branches: with one for each store a round took 1000 cycles.
+__device__ __forceinline__ void store_whole(uint32_t buf, const uint32_t (&w)[16], uint8_t *out, uint64_t step, uint32_t rows) {
+  to_buffer(buf, w);
+  const uint32_t lane = threadIdx.x & 31u, row = lane >> 2;
+  const uint32_t from = buf + row * 64u + (((lane & 3u) ^ ((row >> 1) & 3u)) << 4);
+  uint4 v[4];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      const uint32_t row = 8 * i + (lane >> 2);
-      const uint4 v = ld_shared(buf + row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4));
-      E *at = out + row * ldo + chunk * PER;
-      if (row < rows && n == PER) *reinterpret_cast<uint4 *>(at) = v;
-      else if (row < rows && n > 0) // the last features of a width that fills no 16 bytes
-        for (uint32_t e = 0; e < n; ++e)
-          at[e] = ld_shared_one<E>(buf + row * 64u + ((chunk ^ ((row >> 1) & 3u)) << 4) + e * sizeof(E));
-    }
-  } else { // element by element, neighbours by neighbouring lanes
-#pragma unroll 1
-    for (uint32_t i = lane; i < rows * ALL; i += 32) {
-      const uint32_t row = i / ALL, e = i - row * ALL;
-      if (e < elems)
-        out[row * ldo + e] = ld_shared_one<E>(buf + row * 64u + (((e / PER) ^ ((row >> 1) & 3u)) << 4) + (e % PER) * sizeof(E));
-    }
+  for (uint32_t i = 0; i < 4; ++i) v[i] = ld_shared(from + 512u * i);
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %5, %6;\n\t@p st.global.v4.u32 [%0], {%1, %2, %3, %4};\n\t}\n" ::"l"(
+                     out + i * step),
+                 "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w), "r"(row + 8 * i), "r"(rows)
+                 : "memory");
+}
+// `elems` elements of each of `rows` rows, at any address: element by element, neighbours by neighbouring lanes
+template <class E>
+__device__ __forceinline__ void store_elements(uint32_t buf, const uint32_t (&w)[16], E *out, uint64_t ldo, uint32_t rows,
+                                               uint32_t elems) {
+  constexpr uint32_t PER = 16 / sizeof(E), ALL = 4 * PER;
+  to_buffer(buf, w);
+  const uint32_t lane = threadIdx.x & 31u, e = lane % ALL, first = lane / ALL; // (its rows are a step of 32 / ALL apart)
+  out += first * ldo + e;
+#pragma unroll 8
+  for (uint32_t i = 0; i < ALL; ++i) {
+    const uint32_t row = first + i * (32 / ALL);
+    const E v = ld_shared_one<E>(buf + row * 64u + (((e / PER) ^ ((row >> 1) & 3u)) << 4) + (e % PER) * sizeof(E));
+    if (row < rows && e < elems) *out = v;
+    out += (32 / ALL) * ldo;
   }
 }
 
@@ -462,58 +471,66 @@ __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
   return w;
 }
 
-// 16 columns of a warp's sums; where there are none (zero) the product is 0
-__device__ __forceinline__ void fetch(uint32_t taddr, bool zero, uint32_t (&v)[16]) {
+// N columns of a warp's sums; where there are none (zero) the product is 0
+template <uint32_t N> __device__ __forceinline__ void fetch(uint32_t taddr, bool zero, uint32_t (&v)[N]) {
   if (zero) {
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) v[j] = 0;
+    for (uint32_t j = 0; j < N; ++j) v[j] = 0;
   } else {
-    ptx::tmem_ld_32x32b_x16(taddr, v);
+    read_columns(taddr, v);
     ptx::tmem_ld_wait();
   }
 }
 
-// `cols` columns of a warp's sums to the result, from `at` on: the one rounding.
+// `cols` columns of a warp's sums to the result, from `at` on: the one rounding.  full: they are as many as the warp
+// has, a multiple of PER.  E: an element of the result, PER of them 64 bytes.
+template <class E>
 __device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint32_t taddr, bool zero, uint64_t at,
-                                           uint32_t rows, uint32_t cols, const float *bias) {
-  const auto type = static_cast<GroupedOut>(p.out_type);
-  auto sixteen = [&](uint32_t c, uint32_t (&v)[16]) {
+                                           uint32_t rows, uint32_t cols, bool full, const float *bias) {
+  constexpr uint32_t PER = 64 / sizeof(E);
+  const uint32_t lane = threadIdx.x & 31u;
+  const bool bf16 = static_cast<GroupedOut>(p.out_type) == GroupedOut::bf16, whole = full && p.vector_out != 0;
+  E *out = static_cast<E *>(p.out) + at;
+  uint8_t *mine = reinterpret_cast<uint8_t *>(out + (lane >> 2) * p.ldo) + (lane & 3u) * 16u;
+#pragma unroll 1
+  for (uint32_t c = 0; c < cols; c += PER) {
+    uint32_t v[PER], w[16];
     fetch(taddr + c, zero, v);
     if (bias != nullptr) {
 #pragma unroll
-      for (uint32_t j = 0; j < 16; ++j)
+      for (uint32_t j = 0; j < PER; ++j)
         v[j] = __float_as_uint(__uint_as_float(v[j]) + (c + j < cols ? __ldg(bias + c + j) : 0.f));
     }
-  };
-  uint32_t v[16], w[16];
-  if (type == GroupedOut::f32) {
-#pragma unroll 1
-    for (uint32_t c = 0; c < cols; c += 16) {
-      sixteen(c, v);
-      store_64_bytes(buf, v, static_cast<uint32_t *>(p.out) + at + c, p.ldo, rows, cols - c, p.vector_out != 0);
-    }
-  } else {
-    const bool bf16 = type == GroupedOut::bf16;
-#pragma unroll 1
-    for (uint32_t c = 0; c < cols; c += 32) {
+    if constexpr (sizeof(E) == 4) {
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) { // (the second half of a narrow tile's columns is its neighbour's)
-        sixteen(c + 16 * h, v);
+      for (uint32_t i = 0; i < 16; ++i) w[i] = v[i];
+    } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
-          w[8 * h + i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
-        }
+      for (uint32_t i = 0; i < 16; ++i) {
+        const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+        w[i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
       }
-      store_64_bytes(buf, w, static_cast<uint16_t *>(p.out) + at + c, p.ldo, rows, cols - c, p.vector_out != 0);
     }
+    if (whole) store_whole(buf, w, mine + c * sizeof(E), 8 * p.ldo * sizeof(E), rows);
+    else store_elements(buf, w, out + c, p.ldo, rows, cols - c);
   }
 }
 
+// The warp asks once whether all of its rows can be brought to 8 bits by one factor.
 template <F8Type TYPE>
-__device__ __forceinline__ void quantise(const BlockScale &s, const float (&h)[Cfg<true>::MOST / 2], uint32_t (&w)[16]) {
+__device__ __forceinline__ void quantise(const BlockScale &s, bool real, const float (&h)[Cfg<true>::MOST / 2], uint32_t (&w)[8]) {
+  float f;
+  const bool one = s.plain(f) && !s.zero;
+  if (__all_sync(0xffffffffu, one || !real)) {
 #pragma unroll
-  for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i) w[i] = s.four_of_sums<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+    for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i)
+      w[i] = BlockScale::four_by<TYPE>(f, h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i)
+      w[i] = one ? BlockScale::four_by<TYPE>(f, h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3])
+                 : s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+  }
 }
 
 template <bool GATED>
@@ -735,7 +752,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
     const uint32_t mine = width / PARTS; // columns of the warp, from part * mine on
     const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + part * mine;
     const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
-    const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
+    [[maybe_unused]] const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
     const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in a tile
     uint32_t turn = 0, group = 0, pair_ph = 0, parity = 0; // accumulators and groups of scales that are behind
     bool ok = true;
@@ -848,12 +865,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
           for (uint32_t i = 0; i < PARTS; ++i) top = max(top, tops[i * ROWS_CTA]);
           const auto type = static_cast<F8Type>(p.out_type);
           const BlockScale s(__uint_as_float(top), type);
-          uint32_t w[16] = {};
-          if (type == F8Type::e4m3) quantise<F8Type::e4m3>(s, h, w);
-          else quantise<F8Type::e5m2>(s, h, w);
+          uint32_t w[8];
+          if (type == F8Type::e4m3) quantise<F8Type::e4m3>(s, real, h, w);
+          else quantise<F8Type::e5m2>(s, real, h, w);
           const uint64_t row = x.row0 + lane0;
-          store_64_bytes(buf, w, static_cast<uint8_t *>(p.out) + row * p.ldo + x.col0 + part * (MOST / 2), p.ldo, rows, MOST / 2,
-                         p.vector_out != 0);
+          // 32 bytes of a lane's own row
+          uint8_t *out = static_cast<uint8_t *>(p.out) + (row + lane) * p.ldo + x.col0 + part * (MOST / 2);
+          if (real && p.vector_out != 0) {
+            reinterpret_cast<uint4 *>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4 *>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else if (real) {
+#pragma unroll
+            for (uint32_t i = 0; i < MOST / 2; ++i) out[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3u)));
+          }
           if (part == 0 && real) p.out_scale[(row + lane) * p.out_scale_row + x.col0 / BLOCK * p.out_scale_block] = s.scale;
         }
       } else {
@@ -866,9 +890,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
           done = !__any_sync(0xffffffffu, last);
           if (!done) join(part_of(p, x.slot - x.slice, rank, quarter, part * mine), x.slices, mine, t_sums);
         }
-        if (!done)
-          store_sums(p, buf, t_sums, zero, (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col, rows, cols,
-                     p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr);
+        if (!done) {
+          const uint64_t at = (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col;
+          const float *bias = p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr;
+          if (static_cast<GroupedOut>(p.out_type) == GroupedOut::f32)
+            store_sums<uint32_t>(p, buf, t_sums, zero, at, rows, cols, cols == mine, bias);
+          else store_sums<uint16_t>(p, buf, t_sums, zero, at, rows, cols, cols == mine, bias);
+        }
       }
       if (!zero) give_back(true);
       tiles.give_back(slot);
