@@ -6,9 +6,12 @@
 //   gated    h[r, f] = act(y[r, f]) y[r, hidden + f], which leaves as 8-bit values with scales of their own
 //
 // A block of K is a stage: its products go to a fresh accumulator, and the epilogue adds that, times its scale, to
-// sums in registers while the tensor core fills the other accumulator.  This is what bounds a long product: 128
-// x 256 multiply-adds of the epilogue for each stage of an SM, which the tensor core multiplies in 256 cycles.
-//
+// sums in registers while the tensor core fills the other.  Tensor memory holds two accumulators of 256 columns.  What
+// bounds a long product is the way round: the products of a stage take 512 cycles, their end is known 180 cycles
+// later, an epilogue warp takes 400 to 500 to add 128 columns up (two warps share a scheduler, and 256 of them are
+// multiply-adds), and it is another 200 until the leader knows that both CTAs have, the one's word to the other going
+// through the cluster.  So with two accumulators a stage takes some 820 cycles, which at 8192^3 in a loop, where
+// the power cap leaves 1.55 GHz, is 486 us: 2.26 PFLOP/s.
 // Which side is which.  Rows of x are the lanes of tensor memory and output features its columns, the other way
 // round than in grouped_gemm.cu.  So a thread has a row, and a stage has one scale for it, its own times the one of
 // the 128 features that its warp holds: a register, where scales that differ from column to column would have
@@ -18,7 +21,7 @@
 // no lane needs.
 //
 // Gated: a CTA loads rows of the gate and the same ones of the projection it gates, so that the columns of an
-// epilogue warp are half the one and half the other, and a thread has both for its features; four warps
+// epilogue warp are half the one and half the other, and a thread has both for its features; two warps
 // share the largest magnitude of 128 features.
 //
 // Tiles take equal time, so they are dealt to the pairs in turn.  A launch with few tiles cuts them into slices of
@@ -33,7 +36,7 @@
 //   tile_empty[i] own: 1 arrival from each role that took the tile
 //   sc_full[b]    own: 32 arrivals, of the copies of each lane of the warp that fetches scales
 //   sc_empty[b]   own: one arrival from each epilogue warp
-//   pair[q]       own, gated: 4 arrivals, one from each epilogue warp that has quarter q of the lanes
+//   pair[q]       own, gated: 2 arrivals, one from each epilogue warp that has quarter q of the lanes
 // Every wait is bounded; no TMA multicast is used.
 #include "activation.cuh"
 #include "block_scale.cuh"
@@ -56,7 +59,7 @@ constexpr uint32_t WIDTHS = 2;                          // that a launch chooses
 constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
 constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
 constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
-constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 5;
+constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 6;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t MOST_SLOTS = 4;      // accumulators, of TMEM_COLS / slots columns
 __device__ __forceinline__ uint32_t slots_of(uint32_t width) { return width > 128 ? 2u : MOST_SLOTS; }
@@ -69,20 +72,15 @@ constexpr uint32_t AT_ONCE = 4;     // blocks of K whose scales are copied toget
 constexpr uint32_t SCALE_WORDS = ROWS_CTA + 4; // of a block: the rows', then two of the weights'
 constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
 constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
-// Epilogue warps and registers.  8192 x 8192 x 8192 took 598 us with sixteen warps of 64 columns and 565 with eight of
-// 128, which leave room to read 32 columns ahead.  The gated product of 32764 rows x 2048 x 2 x 4096 took 1190 us with
-// eight and takes 850 with sixteen: its activations are as much work again, and latency.
-// The four warps that issue give back registers that the epilogue's take.
-template <bool GATED> struct Cfg {
-  static constexpr uint32_t PARTS = GATED ? 4 : 2;   // epilogue warps that share the columns of 32 lanes
-  static constexpr uint32_t MOST = COLS / PARTS;     // most columns of a warp
-  static constexpr uint32_t READ = 16;               // columns that it reads at a time
-  static constexpr int EPI_WARPS = 4 * PARTS, THREADS = 128 + 32 * EPI_WARPS;
-  static constexpr int REGS_LAUNCH = GATED ? 96 : 168, REGS_REST = 64, REGS_EPI = GATED ? 104 : 216;
-  static_assert(128 * REGS_REST + 32 * EPI_WARPS * REGS_EPI <= THREADS * REGS_LAUNCH,
-                "setmaxnreg draws on the launch's registers");
-};
-constexpr uint32_t MOST_PARTS = 4;
+// Two epilogue warps share the 256 columns of 32 lanes.  (With four of 64 columns 8192 x 8192 x 8192 took 598 us where
+// these took 565, and the gated product of 32764 rows x 2048 x 2 x 4096 takes 726 where these take 643: a stage costs a
+// warp what it costs with half as many columns, and twice as many warps want to issue.)  The four warps that
+// issue give back registers that the epilogue's take.
+constexpr uint32_t PARTS = 2, MOST = COLS / PARTS; // most columns of a warp
+constexpr uint32_t READ = 16;                      // that it reads at a time
+constexpr int EPI_WARPS = 4 * PARTS, THREADS = 128 + 32 * EPI_WARPS;
+constexpr int REGS_LAUNCH = 168, REGS_REST = 64, REGS_EPI = 216;
+static_assert(128 * REGS_REST + 32 * EPI_WARPS * REGS_EPI <= THREADS * REGS_LAUNCH, "setmaxnreg draws on the launch's registers");
 
 constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
                    ACC_EMPTY = ACC_FULL + 8 * MOST_SLOTS, TILE_FULL = ACC_EMPTY + 8 * MOST_SLOTS, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
@@ -91,9 +89,9 @@ constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * 
                    LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
                    TILE = BARS + 320,                // the tiles of the roles
                    TOPS = TILE + AHEAD * 48,         // gated: largest magnitudes, [tile's parity][part][lane]
-                   START = TOPS + 2 * MOST_PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
+                   START = TOPS + 2 * PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
                    SCALE = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + 4 * MOST_PARTS * OUT_BYTES;
+                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + EPI_WARPS * OUT_BYTES;
 static_assert(PAIR % 8 == 0 && WIDTH + 4 <= TILE && TILE % 16 == 0 && OUT % 16 == 0, "barriers and flags");
 constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
 static_assert(SMEM <= 232448, "shared memory of a CTA");
@@ -308,8 +306,7 @@ __device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[32]) 
 // sums += scale * COLUMNS columns from taddr on; the next are on their way while these are added.  Gated: the second
 // half of the columns has a scale of its own.
 template <bool GATED, uint32_t COLUMNS>
-__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[Cfg<GATED>::MOST], float s0, float s1) {
-  constexpr uint32_t READ = Cfg<GATED>::READ;
+__device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[MOST], float s0, float s1) {
   uint32_t x[2][READ];
   read_columns(taddr, x[0]);
 #pragma unroll
@@ -353,7 +350,7 @@ __device__ __forceinline__ void arrive_cluster_relaxed_if(bool yes, uint32_t clu
 }
 
 // the way back
-template <uint32_t MOST> __device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
+__device__ __forceinline__ void put_back(uint32_t taddr, const float (&sums)[MOST], uint32_t cols) {
 #pragma unroll
   for (uint32_t c = 0; c < MOST; c += 16) {
     if (c >= cols) break;
@@ -384,7 +381,7 @@ __device__ __forceinline__ void park(float *mine, uint32_t cols, uint32_t taddr)
   __syncwarp();
 }
 // by one lane: whether all other slices' sums of these lanes (and columns) have been parked
-__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) { // (which < 16)
+__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) { // 
   return atomicInc(p.counters + 2 + (x.number * 2 + rank) * 16 + which, x.slices - 1) == x.slices - 1;
 }
 // the sums of all slices, the first of which is at `first`, added in their order, back to tensor memory
@@ -518,27 +515,26 @@ __device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint
 
 // The warp asks once whether all of its rows can be brought to 8 bits by one factor.
 template <F8Type TYPE>
-__device__ __forceinline__ void quantise(const BlockScale &s, bool real, const float (&h)[Cfg<true>::MOST / 2], uint32_t (&w)[8]) {
+__device__ __forceinline__ void quantise(const BlockScale &s, bool real, const float (&h)[MOST / 2], uint32_t (&w)[MOST / 8]) {
   float f;
   const bool one = s.plain(f) && !s.zero;
   if (__all_sync(0xffffffffu, one || !real)) {
 #pragma unroll
-    for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i)
+    for (uint32_t i = 0; i < MOST / 8; ++i)
       w[i] = BlockScale::four_by<TYPE>(f, h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < Cfg<true>::MOST / 8; ++i)
+    for (uint32_t i = 0; i < MOST / 8; ++i)
       w[i] = one ? BlockScale::four_by<TYPE>(f, h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3])
                  : s.four<TYPE>(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
   }
 }
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_few,
                    const __grid_constant__ F8Params p) {
-  constexpr uint32_t PARTS = Cfg<GATED>::PARTS, MOST = Cfg<GATED>::MOST, NUM_EPI_WARPS = Cfg<GATED>::EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem =
       reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -556,16 +552,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
     }
     for (uint32_t b = 0; b < MOST_SLOTS; ++b) {
       ptx::mbar_init(sbase + ACC_FULL + 8 * b, 1);
-      ptx::mbar_init(sbase + ACC_EMPTY + 8 * b, 2 * NUM_EPI_WARPS);
+      ptx::mbar_init(sbase + ACC_EMPTY + 8 * b, 2 * EPI_WARPS);
     }
     for (uint32_t q = 0; q < 4; ++q) ptx::mbar_init(sbase + PAIR + 8 * q, PARTS);
     for (uint32_t i = 0; i < AHEAD; ++i) {
       ptx::mbar_init(sbase + TILE_FULL + 8 * i, 1);
-      ptx::mbar_init(sbase + TILE_EMPTY + 8 * i, NUM_EPI_WARPS + (leader ? 3 : 2)); // and who loads, copies, issues
+      ptx::mbar_init(sbase + TILE_EMPTY + 8 * i, EPI_WARPS + (leader ? 3 : 2)); // and who loads, copies, issues
     }
     for (uint32_t i = 0; i < 2; ++i) {
       ptx::mbar_init(sbase + SC_FULL + 8 * i, 32);
-      ptx::mbar_init(sbase + SC_EMPTY + 8 * i, NUM_EPI_WARPS);
+      ptx::mbar_init(sbase + SC_EMPTY + 8 * i, EPI_WARPS);
     }
     *abort_flag = 0;
     ptx::mbar_init_fence();
@@ -590,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
   const uint32_t tmem_base = *reinterpret_cast<const uint32_t *>(smem + TMEM_PTR);
 
   if (warp < 4) {
-    ptx::setmaxnreg_dec<Cfg<GATED>::REGS_REST>();
+    ptx::setmaxnreg_dec<REGS_REST>();
     const uint32_t width = ld_shared_one<uint32_t>(sbase + WIDTH);
     Tile x;
     if (warp == 0) {
@@ -745,7 +741,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
     }
   } else {
     // ================================================================ epilogue (both CTAs)
-    ptx::setmaxnreg_inc<Cfg<GATED>::REGS_EPI>();
+    ptx::setmaxnreg_inc<REGS_EPI>();
     Tile x;
     const uint32_t epi = warp - 4, quarter = warp & 3u, part = epi >> 2;
     const uint32_t width = ld_shared_one<uint32_t>(sbase + WIDTH), slots = slots_of(width), slot_cols = TMEM_COLS / slots;
@@ -865,15 +861,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<GATED>::THREADS,
           for (uint32_t i = 0; i < PARTS; ++i) top = max(top, tops[i * ROWS_CTA]);
           const auto type = static_cast<F8Type>(p.out_type);
           const BlockScale s(__uint_as_float(top), type);
-          uint32_t w[8];
+          uint32_t w[MOST / 8];
           if (type == F8Type::e4m3) quantise<F8Type::e4m3>(s, real, h, w);
           else quantise<F8Type::e5m2>(s, real, h, w);
           const uint64_t row = x.row0 + lane0;
-          // 32 bytes of a lane's own row
+          // whole sectors of a lane's own row
           uint8_t *out = static_cast<uint8_t *>(p.out) + (row + lane) * p.ldo + x.col0 + part * (MOST / 2);
           if (real && p.vector_out != 0) {
-            reinterpret_cast<uint4 *>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            reinterpret_cast<uint4 *>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+            for (uint32_t i = 0; i < MOST / 32; ++i)
+              reinterpret_cast<uint4 *>(out)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           } else if (real) {
 #pragma unroll
             for (uint32_t i = 0; i < MOST / 2; ++i) out[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3u)));
@@ -941,7 +938,7 @@ template <bool GATED> cudaError_t set_up(int *clusters_out) {
     int clusters = sms / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
-    cfg.blockDim = dim3(Cfg<GATED>::THREADS);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM;
     int active = 0;
     if (setup_error[dev] == cudaSuccess && cudaOccupancyMaxActiveClusters(&active, kernel, &cfg) == cudaSuccess) {
@@ -997,7 +994,7 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
   p.activation = static_cast<uint8_t>(f.activation);
   const uint64_t out_bytes = GATED ? 1 : a.out_type == GroupedOut::f32 ? 4 : 2;
   p.vector_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo * out_bytes % 16 == 0;
-  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), Cfg<GATED>::THREADS, SMEM, stream, map_x,
+  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), THREADS, SMEM, stream, map_x,
                         map_x_few, map_w, map_w_few, p);
 }
 
