@@ -67,7 +67,7 @@ constexpr uint32_t BAND = 8;        // row tiles that are walked together
 constexpr uint32_t MAX_SLICES = 16;
 constexpr uint32_t MIN_SLICE = 4;   // least blocks of K in a slice
 constexpr uint32_t PART = COLS * ROWS_CTA; // elements of a parked sum of one CTA
-constexpr uint32_t JOIN_AHEAD = 4;
+constexpr uint32_t JOIN_AHEAD = 8;  // slices whose sums are fetched together
 constexpr uint32_t AT_ONCE = 4;     // blocks of K whose scales are copied together, into two buffers in turn
 constexpr uint32_t SCALE_WORDS = ROWS_CTA + 4; // of a block: the rows', then two of the weights'
 constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
@@ -148,6 +148,21 @@ template <class T> __device__ __forceinline__ T ld_shared_one(uint32_t addr) {
   }
 }
 
+// What a launch is expected to take, in cycles: a stage of a tile `width` columns wide (8192 x 8192 x 8192: 820 with 256,
+// 620 with 128), and the join of slices, which passes over the columns of a warp.
+__device__ __forceinline__ float stage_cycles(uint32_t width) { return 560.f + width; }
+__device__ __forceinline__ float join_cycles(uint32_t width, uint32_t slices) {
+  return slices > 1 ? 4000.f + width * (30.f + 4.f * slices) : 0.f;
+}
+// Slices of K that tiles are cut into, where there are at most half as many as pairs: as many as make the sum of both
+// least, if that is less than a whole tile.
+__device__ __forceinline__ uint32_t slices_of(const F8Params &p, uint32_t tiles, uint32_t clusters, uint32_t width) {
+  if (p.parts == nullptr || tiles == 0 || tiles > clusters / 2) return 1;
+  const uint32_t most = min(min(clusters / tiles, p.blocks / MIN_SLICE), MAX_SLICES);
+  const uint32_t cut = max(1u, min(most, static_cast<uint32_t>(sqrtf(p.blocks * stage_cycles(width) / (4.f * width)))));
+  return (p.blocks - (p.blocks + cut - 1) / cut) * stage_cycles(width) > join_cycles(width, cut) ? cut : 1u;
+}
+
 // The items of a launch, which are tiles or slices of tiles, by their numbers: groups in turn; within one, bands
 // of row tiles that all column tiles pass over, so that what runs at the same time shares operands in L2.
 template <bool GATED> struct Items {
@@ -155,9 +170,7 @@ template <bool GATED> struct Items {
   __device__ __forceinline__ Items(uint32_t sbase_, const F8Params &p, uint32_t clusters) : sbase(sbase_), group(0) {
     cols = ld_shared_one<uint32_t>(sbase + WIDTH);
     const uint32_t tiles = first_tile(p.groups + 1);
-    slices = p.parts != nullptr && tiles > 0 && tiles <= clusters / 2
-                 ? max(1u, min(min(clusters / tiles, p.blocks / MIN_SLICE), MAX_SLICES))
-                 : 1u;
+    slices = slices_of(p, tiles, clusters, cols);
     total = tiles * slices;
   }
   __device__ __forceinline__ uint32_t start(uint32_t g) const { return ld_shared_one<uint32_t>(sbase + START + 4 * g); }
@@ -266,16 +279,17 @@ __device__ __forceinline__ void find_groups(uint8_t *smem, const F8Params &p, ui
     end_before = __shfl_sync(0xffffffffu, end, 31);
     row_tiles += __shfl_sync(0xffffffffu, upto, 31);
   }
-  // The width.  With many tiles, the widest.  Else the one with the earliest end: waves of tiles, each as long as
-  // its steps (a narrow one's are bound by the loads of its rows) and what a tile takes besides.
+  // The width.  With many tiles, the widest.  Else the one with the earliest end: waves of tiles (or slices), with some
+  // 6000 cycles for what a tile takes besides its stages.
   uint32_t cols = COLS;
   if constexpr (!GATED) { // (a gated tile has a whole block of 128 features)
     if (row_tiles * ((p.n + COLS - 1) / COLS) < 4 * clusters) {
       float best = 0.f;
 #pragma unroll
       for (uint32_t i = 0; i < WIDTHS; ++i) {
-        const uint32_t w = COLS >> i, tiles = row_tiles * ((p.n + w - 1) / w), waves = (tiles + clusters - 1) / clusters;
-        const float ends_at = waves * (p.blocks * fmaxf(w, 0.6f * (COLS + w)) + 2500.f);
+        const uint32_t w = COLS >> i, tiles = row_tiles * ((p.n + w - 1) / w), cut = slices_of(p, tiles, clusters, w),
+                       waves = (tiles * cut + clusters - 1) / clusters, blocks = (p.blocks + cut - 1) / cut;
+        const float ends_at = waves * (blocks * stage_cycles(w) + 6000.f) + join_cycles(w, cut);
         if (i == 0 || ends_at < 0.95f * best) {
           best = ends_at;
           cols = w;
@@ -381,7 +395,7 @@ __device__ __forceinline__ void park(float *mine, uint32_t cols, uint32_t taddr)
   __syncwarp();
 }
 // by one lane: whether all other slices' sums of these lanes (and columns) have been parked
-__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) { // 
+__device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) {
   return atomicInc(p.counters + 2 + (x.number * 2 + rank) * 16 + which, x.slices - 1) == x.slices - 1;
 }
 // the sums of all slices, the first of which is at `first`, added in their order, back to tensor memory
