@@ -11,7 +11,9 @@
 // later, an epilogue warp takes 400 to 500 to add 128 columns up (two warps share a scheduler, and 256 of them are
 // multiply-adds), and it is another 200 until the leader knows that both CTAs have, the one's word to the other going
 // through the cluster.  So with two accumulators a stage takes some 820 cycles, which at 8192^3 in a loop, where
-// the power cap leaves 1.55 GHz, is 486 us: 2.26 PFLOP/s.
+// the power cap leaves 1.55 GHz, is 486 us: 2.26 PFLOP/s.  (As two accumulators of 128 columns each, with products and
+// barriers of their own, the same took 579: products of 128 columns are not twice as fast.)
+//
 // Which side is which.  Rows of x are the lanes of tensor memory and output features its columns, the other way
 // round than in grouped_gemm.cu.  So a thread has a row, and a stage has one scale for it, its own times the one of
 // the 128 features that its warp holds: a register, where scales that differ from column to column would have

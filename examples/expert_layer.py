@@ -1,4 +1,5 @@
-"""A mixture-of-experts layer on the grouped products: training steps, then the same weights in 8 bits.
+"""A mixture-of-experts layer on the grouped products: training steps, then the same weights in 8 bits, integer and
+floating point.
 
 Each token goes to ``topk`` of the experts; an expert is a gated feed-forward block,
 ``(silu(x gate^T) * (x up^T)) down^T``.  The tokens' rows are sorted by expert on the device, and nothing
@@ -39,15 +40,29 @@ class ExpertLayer(torch.nn.Module):
 
     def forward(self, x):
         tokens, weight, ends = route(x @ self.router.t(), self.topk)
-        h = experts.grouped_linear(self.handle, x[tokens], self.gate_up, ends, transpose_w=True)
-        gate, up = h.chunk(2, -1)
-        h = torch.nn.functional.silu(gate) * up
-        y = experts.grouped_linear(self.handle, h, self.down, ends, transpose_w=True)
+        y = experts.gated_feed_forward(self.handle, x[tokens], self.gate_up, self.down, ends)
         return torch.zeros_like(x).index_add_(0, tokens, y * weight[:, None].to(y.dtype))
 
     @torch.no_grad()
+    def quantised_f8(self):
+        """The layer's forward pass in 8-bit floating point: weights with a scale for each 128 x 128, activations with
+        one for each 128 columns of a row."""
+        gate_up, down = (experts.quantize_weight_blocks(self.handle, w) for w in (self.gate_up, self.down))
+        router, topk, handle = self.router.detach().clone(), self.topk, self.handle
+
+        @torch.no_grad()
+        def forward(x):
+            tokens, weight, ends = route(x @ router.t(), topk)
+            q, scale = experts.quantize_blocks(handle, x, row_index=tokens.to(torch.int32))
+            q, scale = experts.f8_gated_matmul(handle, q, scale, *gate_up, ends)
+            y = experts.f8_matmul(handle, q, scale, *down, ends, out_dtype=x.dtype)
+            return torch.zeros_like(x).index_add_(0, tokens, y * weight[:, None].to(y.dtype))
+
+        return forward
+
+    @torch.no_grad()
     def quantised(self):
-        """The layer's forward pass with 8-bit weights and activations."""
+        """The layer's forward pass with 8-bit integer weights and activations."""
         def channels(w):
             q, scale = experts.quantize_rows(self.handle, w.flatten(0, 1))
             return q.unflatten(0, w.shape[:2]), scale.view(w.shape[:2])
@@ -98,12 +113,12 @@ def main():
             optimiser.step()
             if step % 5 == 0 or step == a.steps - 1:
                 print(f"step {step:3d}  loss {loss.item():.5f}")
-        serve = layer.quantised()
         x = torch.randn(a.tokens, a.width, device="cuda", dtype=torch.bfloat16)
         with torch.no_grad():
             full = layer(x).float()
-        off = (serve(x).float() - full).norm() / full.norm()
-        print(f"8-bit layer against bfloat16: relative difference {off.item():.4f}")
+        for name, serve in (("integer", layer.quantised()), ("floating-point", layer.quantised_f8())):
+            off = (serve(x).float() - full).norm() / full.norm()
+            print(f"8-bit {name} layer against bfloat16: relative difference {off.item():.4f}")
         if handle.kernel_status() != 0:
             raise SystemExit("a kernel gave up waiting")
 
