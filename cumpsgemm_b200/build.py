@@ -45,6 +45,7 @@ CUDA_SOURCES = [
     "grouped_few_rows.cu",
     "row_kernels.cu",
     "f8_gemm.cu",
+    "f8_few_rows.cu",
     "block_rows.cu",
     "grouped_api.cu",
 ]

@@ -42,7 +42,7 @@
 // Every wait is bounded; no TMA multicast is used.
 #include "activation.cuh"
 #include "block_scale.cuh"
-#include "epilogue.cuh"
+#include "f8_common.cuh"
 #include "gemm_common.cuh"
 #include "grouped.hpp"
 #include "ptx.cuh"
@@ -125,30 +125,6 @@ struct alignas(16) Tile {
   uint32_t slot, number, pad0, pad1;
 };
 static_assert(sizeof(Tile) == 48, "three times 16 bytes");
-
-__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-template <class T> __device__ __forceinline__ T ld_shared_one(uint32_t addr) {
-  if constexpr (sizeof(T) == 1) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return static_cast<T>(v);
-  } else if constexpr (sizeof(T) == 2) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-    return v;
-  } else {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-  }
-}
 
 // What a launch is expected to take, in cycles: a stage of a tile `width` columns wide (8192 x 8192 x 8192: 820 with 256,
 // 620 with 128), and the join of slices, which passes over the columns of a warp.
@@ -307,15 +283,6 @@ __device__ __forceinline__ void find_groups(uint8_t *smem, const F8Params &p, ui
   }
 }
 
-__device__ __forceinline__ void copy_word(uint32_t to, const float *from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
-// an arrival of this thread, when what it has copied has come
-__device__ __forceinline__ void copies_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 __device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[16]) { ptx::tmem_ld_32x32b_x16(taddr, v); }
 __device__ __forceinline__ void read_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32b_x32(taddr, v); }
 
@@ -335,28 +302,6 @@ __device__ __forceinline__ void drain(uint32_t taddr, float (&sums)[MOST], float
   }
 }
 
-// Whether both phases are over.  For the loops over stages, in which a branch costs a warp some 30 cycles: one
-// question, and arrivals that are not branched around.
-__device__ __forceinline__ bool both_over(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p, q;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
-      "and.pred p, p, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(done)
-      : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
-      : "memory");
-  return done != 0;
-}
-__device__ __forceinline__ void arrive_if(bool yes, uint32_t bar) { // own barrier; a release
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(bar),
-               "r"(static_cast<uint32_t>(yes))
-               : "memory");
-}
 __device__ __forceinline__ void arrive_cluster_relaxed_if(bool yes, uint32_t cluster_addr) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t"
@@ -471,17 +416,6 @@ __device__ __forceinline__ void store_elements(uint32_t buf, const uint32_t (&w)
     if (row < rows && e < elems) *out = v;
     out += (32 / ALL) * ldo;
   }
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
-  uint32_t w;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
-  return w;
-}
-__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
-  uint32_t w;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
-  return w;
 }
 
 // N columns of a warp's sums; where there are none (zero) the product is 0
@@ -1017,6 +951,7 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
 } // namespace
 
 std::size_t f8_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
+  if (a.f8->few_rows) return f8_few_rows_parts_bytes(a, num_sms);
   const uint64_t pairs = num_sms / 2, features = a.f8->gated ? COLS / 2 : COLS;
   // tiles there are at least: groups may leave some unfilled
   const uint64_t least = ((a.rows + ROWS - 1) / ROWS) * ((a.lane_dim + features - 1) / features);
@@ -1024,6 +959,7 @@ std::size_t f8_parts_bytes(const GroupedArgs &a, unsigned num_sms) {
 }
 
 cudaError_t launch_f8_gemm(const GroupedArgs &a, cudaStream_t stream) {
+  if (a.f8->few_rows) return launch_f8_few_rows(a, stream);
   return a.f8->gated ? launch<true>(a, *a.f8, stream) : launch<false>(a, *a.f8, stream);
 }
 

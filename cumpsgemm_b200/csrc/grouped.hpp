@@ -55,6 +55,8 @@ struct GroupedArgs {
   uint64_t ldpre;
   float *parts; // nullable: grouped_parts_bytes() of workspace for the sums of slices
   unsigned *counters; // grouped_counters() words, zero between calls
+  uint64_t scratch_bytes; // of workspace, besides what the operands need
+  void *scratch;
   int *dev_status;
 };
 // Memory with which a call may cut tiles into slices of K; 0 where it will not.
@@ -66,6 +68,7 @@ cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream);
 struct F8Args {
   int x_type, w_type; // F8Type
   uint64_t x_scale_row, x_scale_block;
+  bool few_rows; // the kernel for groups of few rows (f8_few_rows.cu), which has no gated form
   bool gated; // then the result is of 8 bits (out_type: F8Type), with a scale for each row and block of 128
   int activation, out_type;
   float *out_scale;
@@ -73,6 +76,8 @@ struct F8Args {
 };
 std::size_t f8_parts_bytes(const GroupedArgs &a, unsigned num_sms);
 cudaError_t launch_f8_gemm(const GroupedArgs &a, cudaStream_t stream);
+std::size_t f8_few_rows_parts_bytes(const GroupedArgs &a, unsigned num_sms);
+cudaError_t launch_f8_few_rows(const GroupedArgs &a, cudaStream_t stream);
 
 // An operand brought into the form above: 8- or 16-bit elements copied to rows that TMA can address,
 // or FP32 elements split into hi and lo FP16 planes, after a multiplication by a power of two.

@@ -74,6 +74,8 @@ cublasStatus_t stage(cuMpSGEMM_handle *h, const char *where, GroupedArgs &g, int
   }
   const uint64_t records_at = bytes;
   if (scale && s.count > 0) bytes += round_up((2 * kScaleRecords + 2) * sizeof(float), 1024);
+  const uint64_t scratch_at = bytes;
+  bytes += round_up(g.scratch_bytes, 1024);
   // the sums of slices are a matter of speed: without room for them tiles stay whole
   const uint64_t parts_at = bytes, parts = grouped_parts_bytes(g, h->num_sms);
   const bool with_parts = parts > 0 && bytes + parts <= workspace_limit(h) && ensure_workspace(h, bytes + parts);
@@ -84,6 +86,7 @@ cublasStatus_t stage(cuMpSGEMM_handle *h, const char *where, GroupedArgs &g, int
   }
   char *ws = static_cast<char *>(h->workspace);
   if (with_parts) g.parts = reinterpret_cast<float *>(ws + parts_at);
+  if (g.scratch_bytes > 0) g.scratch = ws + scratch_at;
   g.counters = h->dev_grouped_counters;
   if (s.count == 0) return CUBLAS_STATUS_SUCCESS;
   for (int i = 0; i < s.count; ++i) {
@@ -131,6 +134,16 @@ int f8_type(cudaDataType_t t) { return static_cast<int>(t == CUDA_R_8F_E4M3 ? F8
 cublasStatus_t done(cuMpSGEMM_handle *h, cudaError_t e) {
   mark_stream_work(h);
   return e == cudaSuccess ? CUBLAS_STATUS_SUCCESS : CUBLAS_STATUS_EXECUTION_FAILED;
+}
+
+// Whether a product of 8-bit floating-point operands goes to the kernel for groups of few rows, which passes over a
+// group's weights once for every 64 of its rows, and whose tiles are half as high and half as wide.  Up to 32 rows for
+// each group on average, however they are spread: 32 groups of 4096 x 4096 with 32 rows each 85 us against 125; with all
+// of those rows in one group some 50 against 30.  One group with up to 64 rows, and any call whose tiles all have an SM of
+// their own: 256 rows of 4096 x 4096 15 against 21 (512, which are more tiles than that, 25 against 19).
+bool f8_takes_few_rows(uint64_t rows, uint64_t n, uint32_t groups, unsigned num_sms) {
+  const uint64_t most_tiles = (rows + 63ull * groups) / 64 * ((n + 127) / 128);
+  return rows <= (groups == 1 ? 64ull : 32ull * groups) || most_tiles <= num_sms;
 }
 
 bool fp32_mode_ok(cuMpSGEMM_compute_mode_t mode) {
@@ -551,6 +564,7 @@ static cublasStatus_t f8_product(cuMpSGEMM_handle_t h, const char *where, uint64
   if (rows == 0) return CUBLAS_STATUS_SUCCESS;
 
   DeviceGuard guard(h->device);
+  f.few_rows = !f.gated && f8_takes_few_rows(rows, n, num_groups, h->num_sms);
   g.kind = GroupedKind::f8;
   g.a = {wq, k, n, ldw, stridew, 0, num_groups, 1};
   g.b = {xq, k, rows, ldx, 0, 0, 1, 1};
@@ -565,7 +579,9 @@ static cublasStatus_t f8_product(cuMpSGEMM_handle_t h, const char *where, uint64
   f.x_type = f8_type(x_type);
   f.w_type = f8_type(w_type);
   const cublasStatus_t st = stage(h, where, g, 1, true, false);
-  return st == CUBLAS_STATUS_SUCCESS ? finish(h, g) : st;
+  if (st != CUBLAS_STATUS_SUCCESS) return st;
+  if (g.scratch_bytes > 0) g.out = g.scratch;
+  return finish(h, g);
 }
 
 extern "C" cublasStatus_t cuMpSGEMM_f8_grouped_gemm(
@@ -604,6 +620,40 @@ extern "C" cublasStatus_t cuMpSGEMM_f8_grouped_gemm_gated(
   if (!known_f8(q_type)) return refuse(where, "q_type is not CUDA_R_8F_E4M3 or CUDA_R_8F_E5M2");
   if (ldq < hidden) return refuse(where, "the leading dimension of q is too small");
   if (rows > 0 && scale == nullptr) return refuse(where, "null pointer");
+  // Few rows: the product in FP32 to the workspace, and a pass over it (256 rows over 32 groups, 4096 x 2 x 2048: 89 us
+  // against 142 of the one kernel, whose way round costs a stage of weights more than memory does).
+  if (rows > 0 && rows <= kMaxDim && num_groups > 0 && f8_takes_few_rows(rows, 2 * hidden, num_groups, h->num_sms) &&
+      rows * 2 * hidden * sizeof(float) <= workspace_limit(h)) {
+    GroupedArgs g = {};
+    F8Args f = {};
+    g.out_type = GroupedOut::f32;
+    g.lane_dim = static_cast<uint32_t>(2 * hidden);
+    g.out = q; // (checked; the workspace takes its place)
+    g.ldo = 2 * hidden;
+    g.scratch_bytes = rows * 2 * hidden * sizeof(float);
+    f.x_scale_row = x_scale_row;
+    f.x_scale_block = x_scale_block;
+    const cublasStatus_t st = f8_product(h, where, rows, 2 * hidden, k, num_groups, group_ends, xq, ldx, x_type, x_scale, wq, ldw,
+                                         stridew, w_type, w_scale, g, f);
+    if (st == CUBLAS_STATUS_SUCCESS) {
+      DeviceGuard guard(h->device);
+      BlockRowsArgs a = {};
+      a.x = g.scratch;
+      a.type = static_cast<int>(GroupedOut::f32);
+      a.q_type = f8_type(q_type);
+      a.activation = activation;
+      a.ldx = 2 * hidden;
+      a.src_rows = a.rows = static_cast<uint32_t>(rows);
+      a.k = static_cast<uint32_t>(hidden);
+      a.q = static_cast<uint8_t *>(q);
+      a.ldq = ldq;
+      a.scale = scale;
+      a.scale_row = scale_row;
+      a.scale_block = scale_block;
+      return done(h, launch_block_rows(a, h->num_sms, h->cuda_stream));
+    }
+    if (st != CUBLAS_STATUS_ALLOC_FAILED) return st; // (without room for that, the one kernel)
+  }
   GroupedArgs g = {};
   F8Args f = {};
   g.lane_dim = static_cast<uint32_t>(hidden);

@@ -475,8 +475,8 @@ cublasStatus_t cuMpSGEMM_quantize_blocks_f8(cuMpSGEMM_handle_t handle, uint32_t 
                                             void *q, uint64_t ldq, uint64_t strideq, cudaDataType_t q_type,
                                             float *scale);
 /* y[r, c] = sum over blocks b of k of x_scale[r, b] w_scale[e, c / 128, b] sum_{i in b} xq[r, i] wq_e[c, i]
- * (+ bias[e * n + c]) for the rows r of each group e; rows of no group: 0.  wq_e is stored n x k.  The products of a
- * block are added in FP32 by the tensor core, the blocks in FP32, and the result is rounded once to y_type. */
+ * (+ bias[e * n + c]) for the rows r of each group e; rows of no group: 0.  wq_e is stored n x k; bias may be NULL.
+ * The products of a block are added in FP32 by the tensor core, the blocks in FP32, and the result is rounded once to y_type. */
 cublasStatus_t cuMpSGEMM_f8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t n, uint64_t k,
                                          uint32_t num_groups, const int32_t *group_ends, const void *xq,
                                          uint64_t ldx, cudaDataType_t x_type, const float *x_scale,
@@ -485,7 +485,9 @@ cublasStatus_t cuMpSGEMM_f8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t row
                                          const float *w_scale, const float *bias, void *y, uint64_t ldy,
                                          cudaDataType_t y_type);
 /* The gated product with such operands, act(x gate_e^T) * (x up_e^T) of unrounded FP32 products, brought to 8 bits
- * again: q (rows x hidden) and its scales.  wq_e is stored 2 hidden x k; hidden is a multiple of 128. */
+ * again: q (rows x hidden) and its scales.  wq_e is stored 2 hidden x k; hidden is a multiple of 128.  For few rows
+ * (those of 32 for each group, or some more) the FP32 products go by way of the handle's workspace where it can have
+ * them. */
 cublasStatus_t cuMpSGEMM_f8_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
                                                uint64_t k, uint32_t num_groups, const int32_t *group_ends,
                                                const void *xq, uint64_t ldx, cudaDataType_t x_type,

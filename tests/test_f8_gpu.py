@@ -381,6 +381,47 @@ def test_slices_of_k_with_and_without_room(handle):
             _holds(torch, *g, act * want[:, n:], far, "float8_e4m3fn")
 
 
+@pytest.mark.parametrize("counts", [[1000], [400, 0, 580]])
+def test_the_larger_kernel_cut_along_k(handle, counts):
+    """Too many rows for the kernel for few of them, and few enough tiles to be cut; without room they stay whole."""
+    torch, api, experts = _setup()
+    rows, hidden, k = sum(counts), 1024, 6000
+    q, s, wq, ws = _operands(torch, experts, handle, rows, 2 * hidden, k, len(counts), 8)
+    want, off = _product(torch, q, s, wq, ws, counts, rows)
+    ends = _ends(torch, counts)
+    act, own = _gate(torch, "silu", want[:, :hidden])
+    far = (1.13 * off[:, :hidden] + own) * (want[:, hidden:].abs() + off[:, hidden:]) + act.abs() * off[:, hidden:]
+    far += 2.0 ** -22 * (act * want[:, hidden:]).abs()
+    for limit in (0, 1 << 20):
+        handle.set_workspace_limit(limit)
+        y = experts.f8_matmul(handle, q, s, wq, ws, ends, out_dtype=torch.float32)
+        assert torch.equal(y, experts.f8_matmul(handle, q, s, wq, ws, ends, out_dtype=torch.float32))
+        _close(torch, y, want, off)
+        _holds(torch, *experts.f8_gated_matmul(handle, q, s, wq, ws, ends), act * want[:, hidden:], far, "float8_e4m3fn")
+    handle.set_workspace_limit(0)
+
+
+@pytest.mark.parametrize("counts", [[200, 3, 0, 0, 0, 0, 37, 0], [0, 0, 256, 0, 0, 0, 0, 0], [31, 32, 33, 64, 65, 7, 0, 24]])
+def test_few_rows_unevenly_spread(handle, counts):
+    """At most 32 rows a group on average, some of them with more; the same numbers as one group after another, and for
+    the gated product with and without room for the FP32 products in between."""
+    torch, api, experts = _setup()
+    rows, hidden, k = sum(counts), 640, 700
+    q, s, wq, ws = _operands(torch, experts, handle, rows, 2 * hidden, k, 8, 6)
+    want, off = _product(torch, q, s, wq, ws, counts, rows)
+    ends = _ends(torch, counts)
+    y = experts.f8_matmul(handle, q, s, wq, ws, ends, out_dtype=torch.float32)
+    _close(torch, y, want, off)
+    act, own = _gate(torch, "gelu", want[:, :hidden])
+    far = (1.13 * off[:, :hidden] + own) * (want[:, hidden:].abs() + off[:, hidden:]) + act.abs() * off[:, hidden:]
+    far += 2.0 ** -22 * (act * want[:, hidden:]).abs()
+    for limit in (0, 4096):
+        handle.set_workspace_limit(limit)
+        _holds(torch, *experts.f8_gated_matmul(handle, q, s, wq, ws, ends, activation="gelu"), act * want[:, hidden:], far,
+               "float8_e4m3fn")
+    handle.set_workspace_limit(0)
+
+
 def test_totals_that_are_wrong(handle):
     torch, api, experts = _setup()
     q, s, wq, ws = _operands(torch, experts, handle, 90, 256, 128, 4, 3)
