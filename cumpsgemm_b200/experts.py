@@ -275,9 +275,10 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
 
 def _dense_rows(t):
     """t, copied where its rows, or its matrices, do not lie one behind the other."""
-    rows, cols = t.shape[-2:]
-    dense = t.stride(-1) == 1 and t.stride(-2) >= cols and (
-        t.dim() < 3 or t.stride(-3) >= (rows - 1) * t.stride(-2) + cols)
+    shape, strides = t.shape, t.stride()
+    rows, cols = shape[-2:]
+    step, ld = strides[-1], strides[-2]
+    dense = step == 1 and ld >= cols and (len(shape) < 3 or strides[-3] >= (rows - 1) * ld + cols)
     return t if dense else t.contiguous()
 
 
@@ -390,21 +391,6 @@ def _gated_rows_grad(handle, pre, dh, act):
     return dpre
 
 
-def _gated_grad(handle, dy, down, group_ends, pre, act, mode):
-    """The gradient of pre from that of the block's result."""
-    groups, width, hidden, ldw, stridew = _matrices_of(down, "down")
-    rows, _, lddy = _rows_of(dy, "the gradient", width)
-    _check(handle, dy.get_device(), (down,), group_ends, groups)
-    if dy.dtype is not pre.dtype:
-        raise ValueError(f"the gradient is {dy.dtype}, the operands are {pre.dtype}")
-    dpre = torch.empty_like(pre)
-    handle.grouped_gemm_gated_grad(api.CUBLAS_OP_N, rows, hidden, width, groups,
-                                   None if group_ends is None else group_ends.data_ptr(), dy.data_ptr(), lddy,
-                                   down.data_ptr(), ldw, stridew, act, pre.data_ptr(), 2 * hidden,
-                                   dpre.data_ptr(), 2 * hidden, _data_type(pre.dtype), mode)
-    return dpre
-
-
 def _composed(handle, x, gate_up, down, group_ends, act, mode):
     """The same made of products that have gradients of any order, for those of gradients."""
     f = torch.nn.functional
@@ -447,12 +433,13 @@ class _GatedMatmul(torch.autograd.Function):
 
 
 class _GatedFeedForward(torch.autograd.Function):
+    # (The checks of `gated_feed_forward` are those of every product in here: a small block's time is the calls'.)
     @staticmethod
     def forward(ctx, x, gate_up, down, group_ends, handle, act, mode, backward_mode):
-        h, pre = _gated(handle, x, gate_up, group_ends, act, mode, keep=True)
+        h, pre, y = _feed_forward(handle, x, gate_up, down, group_ends, act, mode, True)
         ctx.save_for_backward(x, gate_up, down, group_ends, pre, h)
         ctx.how = (handle, act, backward_mode)
-        return grouped_matmul(handle, h, down, group_ends, True, mode=mode)
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -460,17 +447,54 @@ class _GatedFeedForward(torch.autograd.Function):
         handle, act, mode = ctx.how
         if torch.is_grad_enabled():
             return (*_composed_gradients(ctx, dy, (x, gate_up, down), handle, group_ends, act, mode), *(None,) * 5)
+        _check_place(handle, x.get_device())
         dy = _dense_rows(dy)
+        # (strides anew: hooks on saved tensors may have moved them)
+        groups, both, width, ldw, stridew = _matrices_of(gate_up, "gate_up")
+        _, out_width, hidden, ldd, strided = _matrices_of(down, "down")
+        rows, _, ldx = _rows_of(x, "x")
+        _, _, lddy = _rows_of(dy, "the gradient", out_width)
+        ends, data_type = None if group_ends is None else group_ends.data_ptr(), _data_type(x.dtype)
+        need_x, need_gate_up, need_down = ctx.needs_input_grad[:3]
         dx = dgate_up = ddown = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            dpre = _gated_grad(handle, dy, down, group_ends, pre, act, mode)
-        if ctx.needs_input_grad[0]:
-            dx = grouped_matmul(handle, dpre, gate_up, group_ends, mode=mode)
-        if ctx.needs_input_grad[1]:
-            dgate_up = grouped_matmul_wgrad(handle, x, dpre, group_ends, True, mode=mode)
-        if ctx.needs_input_grad[2]:
-            ddown = grouped_matmul_wgrad(handle, h, dy, group_ends, True, mode=mode)
+        if need_x or need_gate_up:
+            dpre = torch.empty_like(pre)
+            dpre_at = dpre.data_ptr()
+            handle.grouped_gemm_gated_grad(api.CUBLAS_OP_N, rows, hidden, out_width, groups, ends, dy.data_ptr(), lddy,
+                                           down.data_ptr(), ldd, strided, act, pre.data_ptr(), both, dpre_at, both,
+                                           data_type, mode)
+        if need_x:
+            dx = x.new_empty((rows, width))
+            handle.grouped_gemm(api.CUBLAS_OP_N, rows, width, both, groups, ends, 1.0, dpre_at, both, gate_up.data_ptr(),
+                                ldw, stridew, 0.0, dx.data_ptr(), width, data_type, mode)
+        if need_gate_up:
+            dgate_up = x.new_empty((groups, both, width))
+            handle.grouped_gemm_wgrad(api.CUBLAS_OP_T, rows, both, width, groups, ends, 1.0, x.data_ptr(), ldx, dpre_at,
+                                      both, 0.0, dgate_up.data_ptr(), width, both * width, data_type, mode)
+        if need_down:
+            ddown = x.new_empty((groups, out_width, hidden))
+            handle.grouped_gemm_wgrad(api.CUBLAS_OP_T, rows, out_width, hidden, groups, ends, 1.0, h.data_ptr(), hidden,
+                                      dy.data_ptr(), lddy, 0.0, ddown.data_ptr(), hidden, out_width * hidden, data_type,
+                                      mode)
         return dx, dgate_up, ddown, None, None, None, None, None
+
+
+def _feed_forward(handle, x, gate_up, down, group_ends, act, mode, keep=False):
+    """(h, what is in front of its activation, the block's result)."""
+    groups, out_width, hidden, ldd, strided = _matrices_of(down, "down")
+    if hidden * 2 != gate_up.shape[1] or groups != gate_up.shape[0]:
+        raise ValueError(f"down {tuple(down.shape)} does not fit gate_up {tuple(gate_up.shape)}")
+    if down.dtype is not x.dtype:
+        raise ValueError(f"x is {x.dtype}, down is {down.dtype}")
+    if down.get_device() != x.get_device():
+        raise ValueError("operands are on different devices")
+    h, pre = _gated(handle, x, gate_up, group_ends, act, mode, keep=keep)
+    rows = h.shape[0]
+    y = x.new_empty((rows, out_width))
+    handle.grouped_gemm(api.CUBLAS_OP_T, rows, out_width, hidden, groups,
+                        None if group_ends is None else group_ends.data_ptr(), 1.0, h.data_ptr(), hidden,
+                        down.data_ptr(), ldd, strided, 0.0, y.data_ptr(), out_width, _data_type(x.dtype), mode)
+    return h, pre, y
 
 
 def gated_matmul(handle: api.Handle, x, gate_up, group_ends=None, *, activation: str = "silu",
@@ -499,15 +523,9 @@ def gated_feed_forward(handle: api.Handle, x, gate_up, down, group_ends=None, *,
     dense block."""
     act = _activation(activation)
     x, gate_up, down = _dense_rows(x), _dense_rows(gate_up), _dense_rows(down)
-    if down.dim() != 3 or gate_up.dim() != 3 or down.shape[2] * 2 != gate_up.shape[1] or down.shape[0] != gate_up.shape[0]:
-        raise ValueError(f"down {tuple(down.shape)} does not fit gate_up {tuple(gate_up.shape)}")
-    if down.dtype is not x.dtype:
-        raise ValueError(f"x is {x.dtype}, down is {down.dtype}")
-    if down.get_device() != x.get_device():
-        raise ValueError("operands are on different devices")
     if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad):
         return _GatedFeedForward.apply(x, gate_up, down, group_ends, handle, act, mode, backward_mode)
-    return grouped_matmul(handle, _gated(handle, x, gate_up, group_ends, act, mode)[0], down, group_ends, True, mode=mode)
+    return _feed_forward(handle, x, gate_up, down, group_ends, act, mode)[2]
 
 
 # ---------------------------------------------------------------- 8-bit floating point
@@ -519,8 +537,8 @@ def _f8_rows(like, rows: int, k: int, dtype):
     """Room for such rows, which start at multiples of 16 bytes, and for their scales, rows side by side."""
     ldq = (k + 15) // 16 * 16
     q = like.new_empty((rows, ldq), dtype=dtype)
-    scale = like.new_empty((_blocks(k), rows), dtype=torch.float32)
-    return (q if ldq == k else q[:, :k]), ldq, scale.t()
+    scale = like.new_empty_strided((rows, _blocks(k)), (1, rows), dtype=torch.float32)
+    return (q if ldq == k else q[:, :k]), ldq, scale
 
 
 def quantize_blocks(handle: api.Handle, x, row_index=None, *, activation: Optional[str] = None,

@@ -385,6 +385,20 @@ def test_gradients_asked_for_one_by_one(handle):
     assert torch.equal(xs.grad, dx) and torch.equal(turned.grad, dw)
 
 
+def test_saved_tensors_that_were_moved(handle):
+    torch, api, experts = _setup()
+    x, gate_up, down, dy = _operands(torch, torch.bfloat16, 50, 64, 72, 2, 5)
+    ends = _ends(torch, [20, 30])
+    dense = [t.detach().requires_grad_() for t in (x, gate_up, down)]
+    want = torch.autograd.grad(experts.gated_feed_forward(handle, *dense, ends), dense, dy)
+    # rows 96 apart when they are saved, 72 or 64 when they come back
+    apart = [_placed(torch, t, 96, 0).requires_grad_() for t in (x, gate_up, down)]
+    with torch.autograd.graph.save_on_cpu():
+        y = experts.gated_feed_forward(handle, *apart, ends)
+    got = torch.autograd.grad(y, apart, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_rows(handle):
     torch, api, experts = _setup()
     for dtype in (torch.bfloat16, torch.float32):
