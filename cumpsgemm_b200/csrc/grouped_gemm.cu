@@ -590,24 +590,51 @@ __device__ __forceinline__ void store_by_rows(uint32_t taddr, bool zero, T *out,
 constexpr int kPlain = static_cast<int>(GatedKind::none), kGated = static_cast<int>(GatedKind::gated),
               kGatedGrad = static_cast<int>(GatedKind::grad);
 
-// 8 elements of a row, of which there are `elems`
-template <class T> __device__ __forceinline__ void store_piece(T *at, const uint4 &v, uint32_t elems, bool vector) {
-  if (vector && elems >= 8) {
-    *reinterpret_cast<uint4 *>(at) = v;
-  } else {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// 8 elements of a row: element by element, `elems` of them, or 16 bytes, all or none, without a branch.
+__device__ __forceinline__ void store_elements(uint16_t *at, const uint4 &v, uint32_t elems) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-      if (i < elems) reinterpret_cast<uint16_t *>(at)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
-  }
+  for (uint32_t i = 0; i < 8; ++i)
+    if (i < elems) at[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
 }
-template <class T> __device__ __forceinline__ uint4 load_piece(const T *at, uint32_t elems, bool vector) {
-  if (vector && elems >= 8) return __ldg(reinterpret_cast<const uint4 *>(at));
+__device__ __forceinline__ uint4 load_elements(const uint16_t *at, uint32_t elems) {
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i)
-    if (i < elems) w[i / 2] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t *>(at) + i)) << (16 * (i & 1));
+    if (i < elems) w[i / 2] |= static_cast<uint32_t>(__ldg(at + i)) << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_if(bool yes, void *at, const uint4 &v) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p st.global.v4.u32 [%0], {%1, %2, %3, %4};\n\t}\n" ::"l"(at),
+               "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(static_cast<uint32_t>(yes))
+               : "memory");
+}
+__device__ __forceinline__ void load_if(bool yes, const void *at, uint4 &v) { // of memory that is not written meanwhile
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+               : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+               : "l"(at), "r"(static_cast<uint32_t>(yes)));
+}
+// Four pieces of a lane, `step` elements from one to the next, of columns first, first + 8, ... below cols.  whole: rows
+// allow 16 bytes, and have a whole number of them.
+__device__ __forceinline__ void store_pieces(uint16_t *at, uint64_t step, const uint4 (&v)[4], uint32_t first, uint32_t cols,
+                                             uint32_t elems, bool whole) {
+  if (whole) {
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) store_if(first + 8 * g < cols && elems == 8, at + g * step, v[g]);
+  } else {
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) store_elements(at + g * step, v[g], first + 8 * g < cols ? elems : 0u);
+  }
+}
+__device__ __forceinline__ void load_pieces(const uint16_t *at, uint64_t step, uint4 (&v)[4], uint32_t first, uint32_t cols,
+                                            uint32_t elems, bool whole) {
+  if (whole) {
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) load_if(first + 8 * g < cols && elems == 8, at + g * step, v[g]);
+  } else {
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) v[g] = load_elements(at + g * step, first + 8 * g < cols ? elems : 0u);
+  }
 }
 template <class T> __device__ __forceinline__ float2 unpack(uint32_t w) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -657,14 +684,12 @@ __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, c
       }
       __syncwarp();
       const uint32_t elems = least(features, 8 * (chunk & 1u), 8);
+      const uint32_t first = c + (lane >> 2);
+      uint4 v[4];
 #pragma unroll
-      for (uint32_t g = 0; g < 4; ++g) {
-        uint4 v;
-        ld_shared_v4(back + g * 512u, v.x, v.y, v.z, v.w);
-        const uint32_t col = c + 8 * g + (lane >> 2);
-        if (col < cols)
-          store_piece(pre + col * p.ldpre + (chunk >> 1) * static_cast<uint64_t>(hidden) + 8 * (chunk & 1u), v, elems, vector_pre);
-      }
+      for (uint32_t g = 0; g < 4; ++g) ld_shared_v4(back + g * 512u, v[g].x, v[g].y, v[g].z, v[g].w);
+      store_pieces(reinterpret_cast<uint16_t *>(pre + first * p.ldpre + (chunk >> 1) * static_cast<uint64_t>(hidden) + 8 * (chunk & 1u)),
+                   8 * p.ldpre, v, first, cols, elems, vector_pre);
     }
     with_activation(p.activation, [&](auto act) {
 #pragma unroll
@@ -689,36 +714,39 @@ __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, c
       uint4 v;
       ld_shared_v4(back_h + j * 512u, v.x, v.y, v.z, v.w);
       const uint32_t col = c + 16 * j + (lane >> 1);
-      if (col < cols) store_piece(out + col * p.ldo + 8 * (lane & 1u), v, elems, vector);
+      uint16_t *to = reinterpret_cast<uint16_t *>(out + col * p.ldo + 8 * (lane & 1u));
+      if (vector) store_if(col < cols && elems == 8, to, v);
+      else store_elements(to, v, col < cols ? elems : 0u);
     }
   }
 }
 
+// pre of 32 features, 16 bytes a lane, of the gate and of what it gates, the way the results leave: columns c on of a warp.
+// from: at the warp's first feature and column.
+__device__ __forceinline__ void fetch_pre(const GroupedParams &p, const uint16_t *from, uint32_t c, uint32_t cols, uint32_t features,
+                                          uint4 (&v)[2][4]) {
+  const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u, first = c + (lane >> 2), elems = least(features, 8 * chunk, 8);
+  const bool whole = (p.vector_out & 2u) != 0;
+  from += first * p.ldpre + 8 * chunk;
+  load_pieces(from, 8 * p.ldpre, v[0], first, cols, elems, whole);
+  load_pieces(from + p.lane_dim, 8 * p.ldpre, v[1], first, cols, elems, whole);
+}
+
 // The gradient of pre, dgate = dh up act'(gate) and dup = dh act(gate), dh being the product, which is not rounded: pre
-// comes the way the results leave, 16 bytes a lane, and through the warp's buffer to the fragments of the sums.
-// pre, out: at the warp's first feature and column; features: of the 32 that there are.
+// goes through the warp's buffer to the fragments of the sums.  v: of pre's first columns, which were fetched while the
+// product was under way; the next are while these are multiplied (without, 4099 rows over 32 experts of 1000 x 1496 took
+// 88 us; with them fetched behind the product, a branch for each access and __expf 67; now 55).  Behind 1000 columns this
+// is what bounds the kernel: dgate and dup leave rounded, as the products behind want them, and cost a fragment 32
+// columns wide some 60 instructions for each of its elements; behind 4096 it hides.  pre, out: at the warp's first feature and column; features: of the 32 that there are.
 template <class T>
 __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *out, const GroupedParams &p, const T *pre,
-                                                 uint32_t buf, uint32_t cols, uint32_t features, uint32_t hidden) {
+                                                 uint4 (&v)[2][4], uint32_t buf, uint32_t cols, uint32_t features,
+                                                 uint32_t hidden) {
   const uint32_t lane = threadIdx.x & 31u, chunk = lane & 3u;
   const uint32_t elems = least(features, 8 * chunk, 8);
-  const bool vector = (p.vector_out & 1u) != 0, vector_pre = (p.vector_out & 2u) != 0;
+  const bool vector = (p.vector_out & 1u) != 0;
   const uint32_t in = buf + (lane & 7u) * 64u + (((lane >> 3) ^ ((lane >> 1) & 3u)) << 4);
   const uint32_t back = buf + (lane >> 2) * 64u + ((chunk ^ ((lane >> 3) & 3u)) << 4);
-  // (of the next columns on its way while these are multiplied: 4099 rows over 32 experts of 1000 x 1496 88 us
-  // without)
-  uint4 v[2][4];
-  auto fetch = [&](uint32_t c) {
-    const uint32_t first = c + (lane >> 2);
-    const T *from = pre + first * p.ldpre + 8 * chunk;
-#pragma unroll
-    for (uint32_t g = 0; g < 4; ++g)
-#pragma unroll
-      for (uint32_t q = 0; q < 2; ++q)
-        v[q][g] = load_piece(from + 8 * g * p.ldpre + q * static_cast<uint64_t>(hidden), first + 8 * g < cols ? elems : 0u,
-                             vector_pre);
-  };
-  if (!zero && cols > 0) fetch(0);
 #pragma unroll 1
   for (uint32_t c = 0; c < cols; c += OUT_COLS) {
     const uint32_t first = c + (lane >> 2);
@@ -738,7 +766,7 @@ __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *o
           ptx::ldmatrix_x4_trans(in + g * 512u, w[q][g][0], w[q][g][1], w[q][g][2], w[q][g][3]);
       }
       ptx::tmem_ld_wait();
-      if (c + OUT_COLS < cols) fetch(c + OUT_COLS);
+      if (c + OUT_COLS < cols) fetch_pre(p, reinterpret_cast<const uint16_t *>(pre), c + OUT_COLS, cols, features, v);
       with_activation(p.activation, [&](auto act) {
 #pragma unroll
         for (uint32_t g = 0; g < 4; ++g)
@@ -764,13 +792,10 @@ __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *o
       for (uint32_t g = 0; g < 4; ++g)
         ptx::stmatrix_x4_trans(in + g * 512u, w[q][g][0], w[q][g][1], w[q][g][2], w[q][g][3]);
       __syncwarp();
+      uint4 r[4];
 #pragma unroll
-      for (uint32_t g = 0; g < 4; ++g) {
-        uint4 v;
-        ld_shared_v4(back + g * 512u, v.x, v.y, v.z, v.w);
-        if (first + 8 * g < cols)
-          store_piece(to + 8 * g * p.ldo + q * static_cast<uint64_t>(hidden), v, elems, vector);
-      }
+      for (uint32_t g = 0; g < 4; ++g) ld_shared_v4(back + g * 512u, r[g].x, r[g].y, r[g].z, r[g].w);
+      store_pieces(reinterpret_cast<uint16_t *>(to + q * static_cast<uint64_t>(hidden)), 8 * p.ldo, r, first, cols, elems, vector);
     }
   }
 }
@@ -1072,6 +1097,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     bool ok = true;
     Tiles<KIND, true> tiles(sbase);
     Tile x;
+    [[maybe_unused]] uint4 before[2][4] = {}; // gradient of a gated product: of what the forward pass left
     // The reads of tensor memory are complete (wait::ld): that is all there is to order.  (As a release
     // it also waited for the results to be written, 1 to 2 us a tile.)
     auto release = [&](uint32_t b) {
@@ -1124,6 +1150,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         tiles.take(x);
         t_sums = t_lanes + second * (x.width() / 2) + COLS;
       } else if (x.blocks != 0) {
+        if constexpr (EPI == kGatedGrad) {
+          const uint32_t l0 = x.lane0 + rank * BM_CTA + quarter * 32u, c0 = second * (x.width() / 2);
+          if (l0 < p.lane_dim && x.cols > c0)
+            fetch_pre(p, static_cast<const uint16_t *>(p.pre) + static_cast<uint64_t>(x.col0 + c0) * p.ldpre + l0, 0,
+                      min(x.width() / 2, x.cols - c0), least(p.lane_dim, l0, 32), before);
+        }
         ok = ptx::warp_agrees(ptx::mbar_wait(sbase + C::ACC_FULL + 8 * acc, f_ph, abort_flag, p.status,
                                              ptx::kErrWaitD0Full));
         if (!ok) break;
@@ -1168,7 +1200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           T *pre = static_cast<T *>(p.pre);
           if (pre != nullptr) pre += row * p.ldpre + f;
           if constexpr (EPI == kGated) store_gated(t_sums, zero, out + row * p.ldo + f, p, pre, buf, cols, features, hidden);
-          else store_gated_grad(t_sums, zero, out + row * p.ldo + f, p, pre, buf, cols, features, hidden);
+          else store_gated_grad(t_sums, zero, out + row * p.ldo + f, p, pre, before, buf, cols, features, hidden);
         };
         if (type == GroupedOut::bf16) go(static_cast<__nv_bfloat16 *>(p.out));
         else go(static_cast<__half *>(p.out));
