@@ -80,8 +80,8 @@ cublasStatus_t stage(cuMpSGEMM_handle *h, const char *where, GroupedArgs &g, int
   const uint64_t parts_at = bytes, parts = grouped_parts_bytes(g, h->num_sms);
   const bool with_parts = parts > 0 && bytes + parts <= workspace_limit(h) && ensure_workspace(h, bytes + parts);
   if (!with_parts && bytes > 0 && (bytes > workspace_limit(h) || !ensure_workspace(h, bytes))) {
-    log_error(std::string(where) + ": no workspace of " + std::to_string(bytes >> 20) +
-              " MB for the operands");
+    if (g.scratch_bytes == 0) // (else the caller has another way)
+      log_error(std::string(where) + ": no workspace of " + std::to_string(bytes >> 20) + " MB for the operands");
     return CUBLAS_STATUS_ALLOC_FAILED;
   }
   char *ws = static_cast<char *>(h->workspace);
