@@ -165,8 +165,14 @@ __device__ __forceinline__ void store_values(float *at, uint32_t n, const float 
   }
 }
 template <class T> __device__ __forceinline__ T rounded(float v) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
   else return __float2half_rn(v);
+}
+template <class T> __device__ __forceinline__ float as_float(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+  else return __half2float(v);
 }
 template <class T> __device__ __forceinline__ void store_values(T *at, uint32_t n, const float (&v)[8]) {
   T x[8];
@@ -186,8 +192,21 @@ template <class T> __device__ __forceinline__ void store_values(T *at, uint32_t 
   }
 }
 
+// One value of a gated product, or of its gradient (g: the first half, u: the second).
+template <Activation ACT, class T, bool GRAD> __device__ __forceinline__ void gated_value(float &g, float &u, float d) {
+  const ActResult act = activate<ACT, sizeof(T) == 2>(g);
+  if constexpr (GRAD) {
+    g = d * u * act.slope;
+    u = d * act.value;
+  } else {
+    g = act.value * u;
+  }
+}
+
 constexpr uint32_t kGatedAtOnce = 2, kGatedSegment = kGatedAtOnce * 32 * 8;
 
+// WHOLE: rows of whole aligned 16 bytes; a lane has eight neighbours.  Otherwise neighbouring lanes have neighbours: eight
+// of a lane, whose stores cannot be 16 bytes, met 32 sectors at each (1999 rows x 1501 in FP32, the gradient: 31 us, and so 18).
 template <class T, bool WHOLE, bool GRAD>
 __global__ void __launch_bounds__(kThreads) gated_rows_kernel(const GatedRowsArgs a) {
   CUMPSGEMM_CHAINED_KERNEL_ENTRY();
@@ -195,40 +214,57 @@ __global__ void __launch_bounds__(kThreads) gated_rows_kernel(const GatedRowsArg
   const uint64_t tasks = static_cast<uint64_t>(a.rows) * segments, step = static_cast<uint64_t>(gridDim.x) * kWarps;
   for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); t < tasks; t += step) {
     const uint32_t r = static_cast<uint32_t>(t / segments), seg = static_cast<uint32_t>(t - static_cast<uint64_t>(r) * segments);
-    const T *pre = static_cast<const T *>(a.pre) + r * a.ldpre;
-    const uint64_t bytes = a.hidden * static_cast<uint64_t>(sizeof(T));
-    const uint32_t first = seg * (kGatedSegment / 8) + lane;
-    Eight<T, WHOLE> gate[kGatedAtOnce], up[kGatedAtOnce], dh[kGatedAtOnce];
-    Eight<T, WHOLE>::load(RowReader(pre, bytes), first, 32, gate);
-    Eight<T, WHOLE>::load(RowReader(pre + a.hidden, bytes), first, 32, up);
-    if constexpr (GRAD)
-      // (dh may be the first half of out: a thread reads its values before it writes there)
-      Eight<T, WHOLE>::template load<false>(RowReader(static_cast<const T *>(a.dh) + r * a.lddh, bytes), first, 32, dh);
+    const T *pre = static_cast<const T *>(a.pre) + r * a.ldpre, *dh = static_cast<const T *>(a.dh) + r * a.lddh;
     T *out = static_cast<T *>(a.out) + r * a.ldo;
-    with_activation(a.activation, [&](auto kind) {
+    if constexpr (WHOLE) {
+      const uint64_t bytes = a.hidden * static_cast<uint64_t>(sizeof(T));
+      const uint32_t first = seg * (kGatedSegment / 8) + lane;
+      Eight<T, true> gate[kGatedAtOnce], up[kGatedAtOnce], back[kGatedAtOnce];
+      Eight<T, true>::load(RowReader(pre, bytes), first, 32, gate);
+      Eight<T, true>::load(RowReader(pre + a.hidden, bytes), first, 32, up);
+      // (dh may be the first half of out: a thread reads its values before it writes there)
+      if constexpr (GRAD) Eight<T, true>::template load<false>(RowReader(dh, bytes), first, 32, back);
+      with_activation(a.activation, [&](auto kind) {
 #pragma unroll
-      for (uint32_t j = 0; j < kGatedAtOnce; ++j) {
-        const uint32_t col = 8 * (first + 32 * j);
-        if (col >= a.hidden) continue;
-        const uint32_t n = min(8u, a.hidden - col);
-        float g[8], u[8], d[8];
-        gate[j].values(g);
-        up[j].values(u);
-        if constexpr (GRAD) dh[j].values(d);
+        for (uint32_t j = 0; j < kGatedAtOnce; ++j) {
+          const uint32_t col = 8 * (first + 32 * j);
+          if (col >= a.hidden) continue;
+          const uint32_t n = min(8u, a.hidden - col);
+          float g[8], u[8], d[8] = {};
+          gate[j].values(g);
+          up[j].values(u);
+          if constexpr (GRAD) back[j].values(d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const ActResult act = activate<kind.value, sizeof(T) == 2>(g[i]);
-          if constexpr (GRAD) {
-            g[i] = d[i] * u[i] * act.slope;
-            u[i] = d[i] * act.value;
-          } else {
-            g[i] = act.value * u[i];
-          }
+          for (int i = 0; i < 8; ++i) gated_value<kind.value, T, GRAD>(g[i], u[i], d[i]);
+          store_values(out + col, n, g);
+          if constexpr (GRAD) store_values(out + a.hidden + col, n, u);
         }
-        store_values(out + col, n, g);
-        if constexpr (GRAD) store_values(out + a.hidden + col, n, u);
+      });
+    } else {
+      constexpr uint32_t N = kGatedSegment / 32;
+      const uint32_t first = seg * kGatedSegment + lane;
+      T gate[N], up[N], back[N];
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        const uint32_t col = first + 32 * j;
+        if (col < a.hidden) {
+          gate[j] = __ldg(pre + col);
+          up[j] = __ldg(pre + a.hidden + col);
+          if constexpr (GRAD) back[j] = dh[col];
+        }
       }
-    });
+      with_activation(a.activation, [&](auto kind) {
+#pragma unroll
+        for (uint32_t j = 0; j < N; ++j) {
+          const uint32_t col = first + 32 * j;
+          if (col >= a.hidden) continue;
+          float g = as_float(gate[j]), u = as_float(up[j]);
+          gated_value<kind.value, T, GRAD>(g, u, GRAD ? as_float(back[j]) : 0.f);
+          out[col] = rounded<T>(g);
+          if constexpr (GRAD) out[a.hidden + col] = rounded<T>(u);
+        }
+      });
+    }
   }
 }
 
