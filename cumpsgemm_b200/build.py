@@ -46,6 +46,7 @@ CUDA_SOURCES = [
     "row_kernels.cu",
     "f8_gemm.cu",
     "f8_few_rows.cu",
+    "gated_few_rows.cu",
     "block_rows.cu",
     "grouped_api.cu",
 ]

@@ -63,6 +63,10 @@ struct GroupedArgs {
 std::size_t grouped_parts_bytes(const GroupedArgs &a, unsigned num_sms);
 cudaError_t launch_grouped_gemm(const GroupedArgs &a, cudaStream_t stream);
 
+// A gated product of 16-bit operands in FP32 arithmetic, for groups of few rows (gated_few_rows.cu).  Rows of x and w
+// are whole 16 bytes at multiples of 16 bytes.
+cudaError_t launch_gated_few_rows(const GroupedArgs &a, cudaStream_t stream);
+
 // What the product of 8-bit floating-point operands has besides: a is w, b is x; lane_dim the features of the
 // result (gated: w has twice as many rows).
 struct F8Args {

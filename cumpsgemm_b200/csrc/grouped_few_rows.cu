@@ -50,51 +50,6 @@ struct FewRowsParams {
   float alpha, beta;
 };
 
-// The rows of one group, at most kMostRows of them, that a block multiplies.
-struct Chunk {
-  uint32_t group, row0, rows; // rows == 0: there is none
-};
-// Chunk `number` (all threads give the same), and how many there are, by all threads.
-__device__ __forceinline__ Chunk find_chunk(const FewRowsParams &p, uint32_t number, uint32_t &all) {
-  __shared__ uint32_t chunks[kWarps];
-  __shared__ Chunk found;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const GroupTotals t(p.ends, p.groups, p.rows);
-  auto chunks_of = [&](uint32_t i) { return (t.end[i] - t.begin_of(i) + kMostRows - 1) / kMostRows; };
-  uint32_t mine = 0;
-#pragma unroll
-  for (uint32_t i = 0; i < GroupTotals::MOST; ++i) mine += chunks_of(i);
-  uint32_t at = mine; // chunks in front of the thread's
-#pragma unroll
-  for (uint32_t d = 1; d < 32; d <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, at, d);
-    if (lane >= d) at += o;
-  }
-  if (lane == 31) chunks[warp] = at;
-  if (threadIdx.x == 0) found.rows = 0;
-  at -= mine;
-  __syncthreads();
-  all = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < kWarps; ++w) {
-    if (w == warp) at += all;
-    all += chunks[w];
-  }
-  if (number >= at && number < at + mine) {
-#pragma unroll
-    for (uint32_t i = 0; i < GroupTotals::MOST; ++i) {
-      const uint32_t n = chunks_of(i);
-      if (number >= at && number < at + n) {
-        const uint32_t row0 = t.begin_of(i) + (number - at) * kMostRows;
-        found = {t.first + i, row0, min(t.end[i] - row0, kMostRows)};
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  return found;
-}
-
 // rows [row0, row0 + R) of x, those behind `have` as 0, values k0 .. k0 + kHeld / R - 1, as far as k goes
 template <int R>
 __device__ __forceinline__ void fetch_x(const FewRowsParams &p, float *xs, uint32_t row0, uint32_t have,
@@ -221,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_rows_kernel(const FewRowsPara
   // more rows than a chunk and others have rows too.
   uint32_t all = ~0u;
   for (uint32_t number = blockIdx.y; number < all; number += gridDim.y) {
-    const Chunk c = find_chunk(p, number, all);
+    const Chunk c = find_chunk<kMostRows>(p.ends, p.groups, p.rows, number, all);
     if (c.rows == 0) return;
     if (c.group == p.groups) { // rows of no group
       constexpr uint32_t COLS = OP_N ? 4 * SHAPE : kWarps * SHAPE;

@@ -40,4 +40,51 @@ struct GroupTotals {
   __device__ __forceinline__ uint32_t begin_of(uint32_t i) const { return i == 0 ? begin : end[i - 1]; }
 };
 
+// The rows of one group, at most MOST_ROWS of them, that a block multiplies.
+struct Chunk {
+  uint32_t group, row0, rows; // rows == 0: there is none
+};
+// Chunk `number` (all threads give the same), and how many there are, by all threads.
+template <uint32_t MOST_ROWS>
+__device__ __forceinline__ Chunk find_chunk(const int32_t *ends, uint32_t groups, uint32_t rows, uint32_t number, uint32_t &all) {
+  constexpr uint32_t WARPS = kTotalsThreads / 32;
+  __shared__ uint32_t chunks[WARPS];
+  __shared__ Chunk found;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const GroupTotals t(ends, groups, rows);
+  auto chunks_of = [&](uint32_t i) { return (t.end[i] - t.begin_of(i) + MOST_ROWS - 1) / MOST_ROWS; };
+  uint32_t mine = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < GroupTotals::MOST; ++i) mine += chunks_of(i);
+  uint32_t at = mine; // chunks in front of the thread's
+#pragma unroll
+  for (uint32_t d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, at, d);
+    if (lane >= d) at += o;
+  }
+  if (lane == 31) chunks[warp] = at;
+  if (threadIdx.x == 0) found.rows = 0;
+  at -= mine;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < WARPS; ++w) {
+    if (w == warp) at += all;
+    all += chunks[w];
+  }
+  if (number >= at && number < at + mine) {
+#pragma unroll
+    for (uint32_t i = 0; i < GroupTotals::MOST; ++i) {
+      const uint32_t n = chunks_of(i);
+      if (number >= at && number < at + n) {
+        const uint32_t row0 = t.begin_of(i) + (number - at) * MOST_ROWS;
+        found = {t.first + i, row0, min(t.end[i] - row0, MOST_ROWS)};
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  return found;
+}
+
 } // namespace cumpsgemm_b200

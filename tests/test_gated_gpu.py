@@ -226,6 +226,47 @@ def test_gated_matmul_and_its_gradients(handle, dtype, name):
         _close(dw[e], _product(torch, dtype, dpre.t(), _Value(x[a:b])).rounded(torch, dtype), "dgate_up")
 
 
+FEW = [  # hidden, width, rows of each expert, rows behind the last: eight rows or fewer
+    (1, 8, [1], 0), (5, 64, [2], 1), (8, 1000, [3, 0, 2], 2), (129, 4096, [8], 0), (72, 200, [1] * 4 + [0] * 60, 0),
+    (520, 72, [0, 0], 4), (33, 2056, [0] * 300 + [1, 0, 5], 1), (64, 1024, [7], 1), (16, 520, [0, 4, 0, 4], 0)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("pad", [0, 8])
+@pytest.mark.parametrize("hidden,width,counts,spare", FEW)
+def test_few_rows(handle, dtype, pad, hidden, width, counts, spare):
+    """A handful of rows, for one expert or for many; nothing outside h and pre is touched."""
+    torch, api, experts = _setup()
+    dtype, rows, n = getattr(torch, dtype), sum(counts) + spare, len(counts)
+    name = ACTIVATIONS[(hidden + width // 8) % 4]
+    x, gate_up, _, _ = _operands(torch, dtype, rows, hidden, width, n, hidden + width)
+    x[sum(counts):] = float("nan")  # rows of no group count for nothing, nor do weights without rows
+    for e in range(n):
+        if counts[e] == 0:
+            gate_up[e] = float("nan")
+    want = _block(torch, dtype, name, x, gate_up, None, None, counts, rows)
+    xs, ws = _placed(torch, x, width + pad, 0), _placed(torch, gate_up, width + pad, 0)
+    hid = _placed(torch, torch.zeros(rows, hidden, dtype=dtype, device="cuda"), hidden + 3, 1)
+    pre = _placed(torch, torch.zeros(rows, 2 * hidden, dtype=dtype, device="cuda"), 2 * hidden + 1, 1)
+    # (totals that fall back or are too large are the one in front and the number of rows)
+    ends = _ends(torch, counts)
+    handle.grouped_gemm_gated(rows, hidden, width, n, ends, xs.data_ptr(), width + pad, ws.data_ptr(), width + pad,
+                              2 * hidden * (width + pad), experts._activation(name), hid.data_ptr(), hidden + 3,
+                              pre.data_ptr(), 2 * hidden + 1, experts._data_type(dtype))
+    _close(hid, want["h"], "h")
+    _close(pre, want["pre"], "pre")
+    for t, cols, ld in ((hid, hidden, hidden + 3), (pre, 2 * hidden, 2 * hidden + 1)):
+        base = t._base.view(-1)
+        assert torch.isnan(base[:1]).all() and torch.isnan(base[1:].view(rows, ld)[:, cols:]).all()
+    assert torch.equal(experts.gated_matmul(handle, xs, ws, ends, activation=name), hid)
+    if spare == 0 and n > 1:
+        wrong = ends.clone()
+        wrong[-1] = rows + 100
+        wrong[1:-1] -= torch.arange(n - 2, device="cuda", dtype=torch.int32) % 2 * (wrong[1:-1] == wrong[:-2]).int()
+        assert torch.equal(experts.gated_matmul(handle, xs, ws, wrong, activation=name), hid)
+    assert handle.kernel_status() == 0
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 @pytest.mark.parametrize("pad,offset", [(0, 0), (8, 8), (3, 1), (5, 0)])
 @pytest.mark.parametrize("hidden", [40, 37])
