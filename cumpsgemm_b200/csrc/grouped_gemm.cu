@@ -3,6 +3,8 @@
 //   product  y[r, :] = alpha * x[r, :] op(w_e) + beta * y[r, :]     for the rows r of group e
 //   wgrad    dw_e    = alpha * x_e^T dy_e + beta * dw_e             over the rows of group e
 //   8 bits   y[r, c] = sx[r] * sw[e][c] * sum_k xq[r, k] wq_e[c, k] (+ bias[e][c])
+//   gated    h[r, f] = act(g) u, g and u being the products of x[r] with rows f and hidden + f of w_e; 16-bit types
+//   its gradient  [dh u act'(g), dh act(g)], dh = dy[r] op(w_e), from the saved g and u
 //
 // The sizes of the groups are known on the device only (`ends`, the running total of rows), so the
 // grid is one persistent CTA pair per SM pair, and every pair walks the tiles of all groups, which it
@@ -644,9 +646,13 @@ __device__ __forceinline__ uint32_t least(uint32_t all, uint32_t from, uint32_t 
   return all > from ? min(all - from, most) : 0u;
 }
 
+// What follows costs nothing where the products take longer: 32768 rows over 16 experts of 4096 x 2 x 4096 in bfloat16 take
+// 1.60 to 1.67 ms, 1.3 PFLOP/s under the power cap, as the plain product does.
+//
 // h = act(gate) * up.  A CTA's lanes are 16 rows of the gate and the same 16 of what it gates in turn (the loads put
 // them there), so of the two fragments that a warp reads of its 32 lanes the one is the gate and the other up, of the
-// same features and columns in the same registers: no exchange.  They are multiplied before they are rounded.
+// same features and columns in the same registers: no exchange.  They are multiplied before they are rounded.  pre, which
+// only a backward pass wants, is rounded to 16 bits: it is the largest tensor that a training step keeps.
 // out, pre: at the warp's first feature and column; features: of the 16 that there are.
 template <class T>
 __device__ __forceinline__ void store_gated(uint32_t taddr, bool zero, T *out, const GroupedParams &p, T *pre, uint32_t buf,
