@@ -61,7 +61,7 @@ constexpr uint32_t WIDTHS = 2;                          // that a launch chooses
 constexpr uint32_t BLOCK = 128;                         // of K, in values and in bytes
 constexpr uint32_t BOX_ROWS = 32;                       // of the smaller boxes
 constexpr uint32_t TILE_BYTES = ROWS_CTA * BLOCK;       // an operand's part of a stage in one CTA
-constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES, STAGES = 6;
+constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t MOST_SLOTS = 4;      // accumulators, of TMEM_COLS / slots columns
 __device__ __forceinline__ uint32_t slots_of(uint32_t width) { return width > 128 ? 2u : MOST_SLOTS; }
@@ -73,7 +73,6 @@ constexpr uint32_t JOIN_AHEAD = 8;  // slices whose sums are fetched together
 constexpr uint32_t AT_ONCE = 4;     // blocks of K whose scales are copied together, into two buffers in turn
 constexpr uint32_t SCALE_WORDS = ROWS_CTA + 4; // of a block: the rows', then two of the weights'
 constexpr uint32_t AHEAD = 3;       // tiles that the roles may be apart
-constexpr uint32_t OUT_BYTES = 32 * 64; // a warp's way out: 64 bytes of each of its rows
 // Two epilogue warps share the 256 columns of 32 lanes.  (With four of 64 columns 8192 x 8192 x 8192 took 598 us where
 // these took 565, and the gated product of 32764 rows x 2048 x 2 x 4096 takes 726 where these take 643: a stage costs a
 // warp what it costs with half as many columns, and twice as many warps want to issue.)  The four warps that
@@ -84,19 +83,25 @@ constexpr int EPI_WARPS = 4 * PARTS, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int REGS_LAUNCH = 168, REGS_REST = 64, REGS_EPI = 216;
 static_assert(128 * REGS_REST + 32 * EPI_WARPS * REGS_EPI <= THREADS * REGS_LAUNCH, "setmaxnreg draws on the launch's registers");
 
-constexpr uint32_t BARS = STAGES * STAGE_BYTES, FULL = BARS, EMPTY = FULL + 8 * STAGES, ACC_FULL = EMPTY + 8 * STAGES,
+constexpr uint32_t MOST_STAGES = 6, FULL = 0, EMPTY = FULL + 8 * MOST_STAGES, ACC_FULL = EMPTY + 8 * MOST_STAGES,
                    ACC_EMPTY = ACC_FULL + 8 * MOST_SLOTS, TILE_FULL = ACC_EMPTY + 8 * MOST_SLOTS, TILE_EMPTY = TILE_FULL + 8 * AHEAD,
                    SC_FULL = TILE_EMPTY + 8 * AHEAD, SC_EMPTY = SC_FULL + 16,
                    PAIR = SC_EMPTY + 16, // gated, for each quarter of the lanes
                    LAST = PAIR + 8 * 4, TMEM_PTR = LAST + 4 * 4, ABORT = TMEM_PTR + 4, WIDTH = ABORT + 4,
-                   TILE = BARS + 320,                // the tiles of the roles
+                   TILE = 320,                       // the tiles of the roles
                    TOPS = TILE + AHEAD * 48,         // gated: largest magnitudes, [tile's parity][part][lane]
                    START = TOPS + 2 * PARTS * ROWS_CTA * 4, FIRST_TILE = START + 4 * (kMaxGroups + 2),
                    SCALE = (FIRST_TILE + 4 * (kMaxGroups + 2) + 127) / 128 * 128,
-                   OUT = SCALE + 2 * AT_ONCE * SCALE_WORDS * 4, BYTES = OUT + EPI_WARPS * OUT_BYTES;
+                   OUT = (SCALE + 2 * AT_ONCE * SCALE_WORDS * 4 + 1023) / 1024 * 1024;
 static_assert(PAIR % 8 == 0 && WIDTH + 4 <= TILE && TILE % 16 == 0 && OUT % 16 == 0, "barriers and flags");
-constexpr uint32_t SMEM = BYTES + 1024; // and what the alignment of the stages takes
-static_assert(SMEM <= 232448, "shared memory of a CTA");
+// What a warp's results take on their way out, 64 bytes of each of its rows (gated) or 256; the stages take the rest.
+constexpr uint32_t OUT_ROW = 256, OUT_BOX = 128, OUT_PITCH = OUT_ROW + 16; // of a row; of it in a box; of rows that leave one by one
+template <bool GATED> struct Shared {
+  static constexpr uint32_t STAGES = GATED ? 6 : 4, OUT_BYTES = GATED ? 32 * 64 : (32 * OUT_PITCH + 1023) / 1024 * 1024,
+                            FIRST = OUT + EPI_WARPS * OUT_BYTES,
+                            BYTES = FIRST + STAGES * STAGE_BYTES + 1024; // and what the alignment takes
+  static_assert(STAGES <= MOST_STAGES && FIRST % 1024 == 0 && BYTES <= 232448, "shared memory of a CTA");
+};
 
 struct F8Params {
   const int32_t *ends;
@@ -374,32 +379,34 @@ __device__ __forceinline__ void join(const float *first, uint32_t slices, uint32
   ptx::tmem_st_wait();
 }
 
-// 64 bytes of each of a warp's rows, which its lanes have in w, to memory by way of the warp's buffer: a lane
-// stores its own as 16-byte chunks (those of two rows side by side XORed, so that neither side meets a bank twice)
-// and four lanes then write a row's together.
+// Results leave the warp's buffer by asynchronous copies, and the next tile's stages go on meanwhile: boxes of 32 rows, or
+// where a group ends in between the rows one by one (gated ones from the lanes).  (All pairs come to the end of a tile
+// together.  Stored by the lanes, their results had to wait for the way to memory, 64 KB from each SM at 3.8 TB/s: 4000
+// cycles a tile.  With all rows one by one 8192 x 8192 x 8192 took 490 us where boxes took 484, and gated ones, of 64
+// bytes, 712 instead of 675.)
+__device__ __forceinline__ void wait_copied() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void wait_written() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_to_copy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_row(void *to, uint32_t from, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_box(const CUtensorMap *map, uint32_t from, uint32_t byte, uint32_t row) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(byte),
+               "r"(row), "r"(0), "r"(from)
+               : "memory");
+}
+
+// 64 bytes of each of a warp's rows, which its lanes have in w, to the warp's buffer: a lane stores its own as 16-byte
+// chunks (those of two rows side by side XORed, so that neither side meets a bank twice).
 __device__ __forceinline__ void to_buffer(uint32_t buf, const uint32_t (&w)[16]) {
   const uint32_t lane = threadIdx.x & 31u;
+  wait_copied();
   __syncwarp(); // the buffer has been read
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i)
     st_shared(buf + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   __syncwarp();
-}
-// Whole 64 bytes of `rows` rows, at 16-byte aligned addresses; out: at the lane's chunk of row lane / 4, `step` bytes
-// from a row to the one 8 further on.  No branches: with one for each store a round took 1000 cycles.
-__device__ __forceinline__ void store_whole(uint32_t buf, const uint32_t (&w)[16], uint8_t *out, uint64_t step, uint32_t rows) {
-  to_buffer(buf, w);
-  const uint32_t lane = threadIdx.x & 31u, row = lane >> 2;
-  const uint32_t from = buf + row * 64u + (((lane & 3u) ^ ((row >> 1) & 3u)) << 4);
-  uint4 v[4];
-#pragma unroll
-  for (uint32_t i = 0; i < 4; ++i) v[i] = ld_shared(from + 512u * i);
-#pragma unroll
-  for (uint32_t i = 0; i < 4; ++i)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %5, %6;\n\t@p st.global.v4.u32 [%0], {%1, %2, %3, %4};\n\t}\n" ::"l"(
-                     out + i * step),
-                 "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w), "r"(row + 8 * i), "r"(rows)
-                 : "memory");
 }
 // `elems` elements of each of `rows` rows, at any address: element by element, neighbours by neighbouring lanes
 template <class E>
@@ -429,37 +436,71 @@ template <uint32_t N> __device__ __forceinline__ void fetch(uint32_t taddr, bool
   }
 }
 
-// `cols` columns of a warp's sums to the result, from `at` on: the one rounding.  full: they are as many as the warp
-// has, a multiple of PER.  E: an element of the result, PER of them 64 bytes.
+// 64 bytes of a lane's row of sums, with the bias added and rounded: the one rounding.  E: an element of the result
 template <class E>
-__device__ __forceinline__ void store_sums(const F8Params &p, uint32_t buf, uint32_t taddr, bool zero, uint64_t at,
-                                           uint32_t rows, uint32_t cols, bool full, const float *bias) {
+__device__ __forceinline__ void results(uint32_t taddr, bool zero, const float *bias, uint32_t cols, bool bf16, uint32_t (&w)[16]) {
   constexpr uint32_t PER = 64 / sizeof(E);
+  uint32_t v[PER];
+  fetch(taddr, zero, v);
+  if (bias != nullptr) {
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + (j < cols ? __ldg(bias + j) : 0.f));
+  }
+  if constexpr (sizeof(E) == 4) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) w[i] = v[i];
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
+      w[i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
+    }
+  }
+}
+// `cols` columns of a warp's sums to the result, from `row` and `col` on.
+template <class E>
+__device__ __forceinline__ void store_sums(const F8Params &p, const CUtensorMap *map, uint32_t buf, uint32_t taddr, bool zero,
+                                           uint32_t row, uint32_t col, uint32_t rows, uint32_t cols, const float *bias) {
+  constexpr uint32_t PER = 64 / sizeof(E), ROW = OUT_ROW / sizeof(E);
   const uint32_t lane = threadIdx.x & 31u;
-  const bool bf16 = static_cast<GroupedOut>(p.out_type) == GroupedOut::bf16, whole = full && p.vector_out != 0;
-  E *out = static_cast<E *>(p.out) + at;
-  uint8_t *mine = reinterpret_cast<uint8_t *>(out + (lane >> 2) * p.ldo) + (lane & 3u) * 16u;
+  const bool bf16 = static_cast<GroupedOut>(p.out_type) == GroupedOut::bf16;
+  E *out = static_cast<E *>(p.out) + static_cast<uint64_t>(row) * p.ldo + col;
+  if (p.vector_out != 0 && cols * sizeof(E) % 16 == 0) {
+    const bool boxes = rows == 32;
 #pragma unroll 1
-  for (uint32_t c = 0; c < cols; c += PER) {
-    uint32_t v[PER], w[16];
-    fetch(taddr + c, zero, v);
-    if (bias != nullptr) {
+    for (uint32_t c0 = 0; c0 < cols; c0 += ROW) {
+      const uint32_t here = min(cols - c0, ROW);
+      wait_copied();
+      __syncwarp();
+#pragma unroll 1
+      for (uint32_t c = 0; c < here; c += PER) {
+        uint32_t w[16];
+        results<E>(taddr + c0 + c, zero, bias == nullptr ? nullptr : bias + c0 + c, here - c, bf16, w);
+        // a box has its 16-byte chunks XORed with the row (modulo 8), as its map says
+        const uint32_t b = c * sizeof(E), to = boxes ? buf + b / OUT_BOX * (32 * OUT_BOX) + lane * OUT_BOX : buf + lane * OUT_PITCH + b,
+                       first = boxes ? b % OUT_BOX / 16 : 0u, flip = boxes ? lane & 7u : 0u;
 #pragma unroll
-      for (uint32_t j = 0; j < PER; ++j)
-        v[j] = __float_as_uint(__uint_as_float(v[j]) + (c + j < cols ? __ldg(bias + c + j) : 0.f));
-    }
-    if constexpr (sizeof(E) == 4) {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) w[i] = v[i];
-    } else {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        const float x = __uint_as_float(v[2 * i]), y = __uint_as_float(v[2 * i + 1]);
-        w[i] = bf16 ? pack_bf16(x, y) : pack_f16(x, y);
+        for (uint32_t i = 0; i < 4; ++i)
+          st_shared(to + (((first + i) ^ flip) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       }
+      fence_to_copy();
+      if (boxes) {
+        __syncwarp();
+        if (lane == 0)
+          for (uint32_t b = 0; b < here * sizeof(E); b += OUT_BOX)
+            copy_box(map, buf + 32 * b, (col + c0) * sizeof(E) + b, row);
+      } else if (lane < rows) {
+        copy_row(out + lane * p.ldo + c0, buf + lane * OUT_PITCH, here * sizeof(E));
+      }
+      commit_copies();
     }
-    if (whole) store_whole(buf, w, mine + c * sizeof(E), 8 * p.ldo * sizeof(E), rows);
-    else store_elements(buf, w, out + c, p.ldo, rows, cols - c);
+  } else {
+#pragma unroll 1
+    for (uint32_t c = 0; c < cols; c += PER) {
+      uint32_t w[16];
+      results<E>(taddr + c, zero, bias == nullptr ? nullptr : bias + c, cols - c, bf16, w);
+      store_elements(buf, w, out + c, p.ldo, rows, cols - c);
+    }
   }
 }
 
@@ -484,7 +525,8 @@ template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     f8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_x_few,
                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_few,
-                   const __grid_constant__ F8Params p) {
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ F8Params p) {
+  using S = Shared<GATED>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *const smem =
       reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -496,7 +538,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t cluster_id = blockIdx.x >> 1, clusters = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < STAGES; ++s) {
+    for (uint32_t s = 0; s < S::STAGES; ++s) {
       ptx::mbar_init(sbase + FULL + 8 * s, 2);
       ptx::mbar_init(sbase + EMPTY + 8 * s, 1);
     }
@@ -519,6 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     ptx::prefetch_tensormap(&map_x_few);
     ptx::prefetch_tensormap(&map_w);
     ptx::prefetch_tensormap(&map_w_few);
+    ptx::prefetch_tensormap(&map_out);
   }
   if (warp == 1) {
     ptx::tmem_alloc_pair(sbase + TMEM_PTR, TMEM_COLS);
@@ -557,7 +600,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           for (uint32_t kb = 0; kb < x.blocks; ++kb) {
             ok = ptx::mbar_wait(sbase + EMPTY + 8 * s, ph, abort_flag, p.status, ptx::kErrWaitEmpty);
             if (!ok) break;
-            const uint32_t x_dst = sbase + s * STAGE_BYTES, w_dst = x_dst + TILE_BYTES;
+            const uint32_t x_dst = sbase + S::FIRST + s * STAGE_BYTES, w_dst = x_dst + TILE_BYTES;
             const uint32_t full = ptx::map_to_cta(sbase + FULL + 8 * s, 0); // the leader's barrier
             if (leader) ptx::mbar_arrive_expect_tx(sbase + FULL + 8 * s, bytes);
             else ptx::mbar_arrive_expect_tx_cluster(full, bytes);
@@ -586,7 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                         c + static_cast<int>(b * BOX_ROWS), e);
               }
             }
-            if (++s == STAGES) {
+            if (++s == S::STAGES) {
               s = 0;
               ph ^= 1u;
             }
@@ -598,7 +641,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (leader && ptx::elect_one()) {
         constexpr uint16_t BOTH = 0x3;
         constexpr uint64_t kStage = STAGE_BYTES >> 4;
-        const uint64_t a0 = ptx::make_kmajor_desc<BLOCK>(sbase), b0 = ptx::make_kmajor_desc<BLOCK>(sbase + TILE_BYTES);
+        const uint64_t a0 = ptx::make_kmajor_desc<BLOCK>(sbase + S::FIRST), b0 = ptx::make_kmajor_desc<BLOCK>(sbase + S::FIRST + TILE_BYTES);
         const uint32_t idesc = p.idesc | ((width >> 3) << 17);
         const uint32_t slots = slots_of(width), slot_cols = TMEM_COLS / slots;
         uint32_t s = 0, ph = 0, acc = 0, e_ph = 1;
@@ -621,7 +664,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               acc = 0;
               e_ph ^= 1u;
             }
-            if (++s == STAGES) {
+            if (++s == S::STAGES) {
               s = 0;
               ph ^= 1u;
             }
@@ -698,7 +741,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t mine = width / PARTS; // columns of the warp, from part * mine on
     const uint32_t t_lanes = tmem_base + ((quarter * 32u) << 16) + part * mine;
     const uint32_t acc_empty = ptx::map_to_cta(sbase + ACC_EMPTY, 0);
-    [[maybe_unused]] const uint32_t buf = sbase + OUT + epi * OUT_BYTES;
+    const uint32_t buf = sbase + OUT + epi * S::OUT_BYTES;
     const uint32_t lane0 = rank * ROWS_CTA + quarter * 32u; // the warp's first row in a tile
     uint32_t turn = 0, group = 0, pair_ph = 0, parity = 0; // accumulators and groups of scales that are behind
     bool ok = true;
@@ -787,16 +830,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         if (!done) {
           float h[MOST / 2];
-          uint32_t top = 0;
+          uint32_t top = 0, gate[2][16], up[2][16]; // the next columns are on their way
+          auto read = [&](uint32_t c, uint32_t i) {
+            if (zero) {
+#pragma unroll
+              for (uint32_t j = 0; j < 16; ++j) gate[i][j] = up[i][j] = 0;
+            } else {
+              read_columns(t_sums + c, gate[i]);
+              read_columns(t_sums + MOST / 2 + c, up[i]);
+            }
+          };
+          read(0, 0);
 #pragma unroll
           for (uint32_t c = 0; c < MOST / 2; c += 16) {
-            uint32_t gate[16], up[16];
-            fetch(t_sums + c, zero, gate);
-            fetch(t_sums + MOST / 2 + c, zero, up);
+            const uint32_t now = (c / 16) & 1u;
+            ptx::tmem_ld_wait();
+            if (c + 16 < MOST / 2) read(c + 16, now ^ 1u);
             with_activation(p.activation, [&](auto act) {
 #pragma unroll
               for (uint32_t i = 0; i < 16; ++i)
-                h[c + i] = activate<act.value, true>(__uint_as_float(gate[i])).value * __uint_as_float(up[i]);
+                h[c + i] = activate<act.value, true>(__uint_as_float(gate[now][i])).value * __uint_as_float(up[now][i]);
             });
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) top = max(top, __float_as_uint(h[c + i]) & 0x7fffffffu);
@@ -815,9 +868,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (type == F8Type::e4m3) quantise<F8Type::e4m3>(s, real, h, w);
           else quantise<F8Type::e5m2>(s, real, h, w);
           const uint64_t row = x.row0 + lane0;
-          // whole sectors of a lane's own row
           uint8_t *out = static_cast<uint8_t *>(p.out) + (row + lane) * p.ldo + x.col0 + part * (MOST / 2);
-          if (real && p.vector_out != 0) {
+          if (p.vector_out != 0 && rows == 32) {
+            wait_copied();
+            __syncwarp();
+#pragma unroll
+            for (uint32_t i = 0; i < MOST / 32; ++i)
+              st_shared(buf + lane * 64u + 16 * i, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            fence_to_copy();
+            __syncwarp();
+            if (lane == 0) copy_box(&map_out, buf, x.col0 + part * (MOST / 2), static_cast<uint32_t>(row));
+            commit_copies();
+          } else if (real && p.vector_out != 0) {
 #pragma unroll
             for (uint32_t i = 0; i < MOST / 32; ++i)
               reinterpret_cast<uint4 *>(out)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
@@ -838,11 +900,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (!done) join(part_of(p, x.slot - x.slice, rank, quarter, part * mine), x.slices, mine, t_sums);
         }
         if (!done) {
-          const uint64_t at = (static_cast<uint64_t>(x.row0) + lane0) * p.ldo + col;
           const float *bias = p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr;
           if (static_cast<GroupedOut>(p.out_type) == GroupedOut::f32)
-            store_sums<uint32_t>(p, buf, t_sums, zero, at, rows, cols, cols == mine, bias);
-          else store_sums<uint16_t>(p, buf, t_sums, zero, at, rows, cols, cols == mine, bias);
+            store_sums<uint32_t>(p, &map_out, buf, t_sums, zero, x.row0 + lane0, col, rows, cols, bias);
+          else store_sums<uint16_t>(p, &map_out, buf, t_sums, zero, x.row0 + lane0, col, rows, cols, bias);
         }
       }
       if (!zero) give_back(true);
@@ -852,6 +913,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       slot = tiles.advance();
       tiles.read(slot, x);
     }
+    wait_written();
   }
 
   // ---------------------------------------------------------------- teardown
@@ -882,14 +944,14 @@ template <bool GATED> cudaError_t set_up(int *clusters_out) {
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   std::call_once(once[dev], [&]() {
     const auto kernel = f8_gemm_kernel<GATED>;
-    setup_error[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    setup_error[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shared<GATED>::BYTES);
     int sms = 0;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     int clusters = sms / 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(2 * clusters));
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM;
+    cfg.dynamicSmemBytes = Shared<GATED>::BYTES;
     int active = 0;
     if (setup_error[dev] == cudaSuccess && cudaOccupancyMaxActiveClusters(&active, kernel, &cfg) == cudaSuccess) {
       if (active > 0 && active < clusters) clusters = active;
@@ -911,7 +973,7 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
   int clusters = 1;
   const cudaError_t se = set_up<GATED>(&clusters);
   if (se != cudaSuccess) return se;
-  CUtensorMap map_x, map_x_few, map_w, map_w_few;
+  CUtensorMap map_x, map_x_few, map_w, map_w_few, map_out;
   if (!operand_map(&map_x_few, a.b, BOX_ROWS) || !operand_map(&map_w_few, a.a, BOX_ROWS))
     return cudaErrorInvalidValue;
   // boxes of 128 rows are for tiles that have as many, and not for gated ones' weights
@@ -944,8 +1006,14 @@ template <bool GATED> cudaError_t launch(const GroupedArgs &a, const F8Args &f, 
   p.activation = static_cast<uint8_t>(f.activation);
   const uint64_t out_bytes = GATED ? 1 : a.out_type == GroupedOut::f32 ? 4 : 2;
   p.vector_out = (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo * out_bytes % 16 == 0;
-  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), THREADS, SMEM, stream, map_x,
-                        map_x_few, map_w, map_w_few, p);
+  // in bytes; used only where rows of the result are whole 16 bytes (and no larger than a map's)
+  const uint64_t row_bytes = p.n * out_bytes, pitch = a.ldo * out_bytes;
+  if (row_bytes >= 1ull << 31 || pitch >= 1ull << 40) p.vector_out = 0;
+  map_out = map_x_few;
+  if (p.vector_out && !make_byte_map(&map_out, 1, a.out, {row_bytes, p.rows, 1}, {pitch, pitch}, {GATED ? MOST / 2 : OUT_BOX, 32, 1}, !GATED))
+    return cudaErrorInvalidValue;
+  return launch_chained(f8_gemm_kernel<GATED>, static_cast<unsigned>(2 * clusters), THREADS, Shared<GATED>::BYTES, stream, map_x,
+                        map_x_few, map_w, map_w_few, map_out, p);
 }
 
 } // namespace
