@@ -10,9 +10,11 @@
 // bounds a long product is the way round: the products of a stage take 512 cycles, their end is known 180 cycles
 // later, an epilogue warp takes 400 to 500 to add 128 columns up (two warps share a scheduler, and 256 of them are
 // multiply-adds), and it is another 200 until the leader knows that both CTAs have, the one's word to the other going
-// through the cluster.  So with two accumulators a stage takes some 820 cycles, which at 8192^3 in a loop, where
-// the power cap leaves 1.55 GHz, is 486 us: 2.26 PFLOP/s.  (As two accumulators of 128 columns each, with products and
-// barriers of their own, the same took 579: products of 128 columns are not twice as fast.)
+// through the cluster.  So with two accumulators a stage takes some 800 cycles, which at 8192^3 in a loop, where
+// the power cap leaves 1.5 to 1.58 GHz, is 483 to 500 us: 2.2 PFLOP/s.  (As two accumulators of 128 columns each, with
+// products and barriers of their own, the same took 579: products of 128 columns are not twice as fast.)  Behind the last
+// stage of a tile come 2500 cycles, gated 5000 (of which 2700 for the activation: two special-function instructions for
+// each of 64 values), in which the tensor core does the next tile's first two stages.
 //
 // Which side is which.  Rows of x are the lanes of tensor memory and output features its columns, the other way
 // round than in grouped_gemm.cu.  So a thread has a row, and a stage has one scale for it, its own times the one of
@@ -457,6 +459,37 @@ __device__ __forceinline__ void results(uint32_t taddr, bool zero, const float *
     }
   }
 }
+// The same for 32 rows of 128 columns of 16 bits from the registers, in two boxes.  (No branches in between: with a test for
+// the bias at every pair the stores took 2200 cycles.)
+template <bool BF16>
+__device__ __forceinline__ void store_whole(const CUtensorMap *map, uint32_t buf, float (&sums)[MOST], uint32_t row, uint32_t col,
+                                            const float *bias) {
+  static_assert(MOST * 2 == OUT_ROW, "a row of the buffer");
+  const uint32_t lane = threadIdx.x & 31u, mine = buf + lane * OUT_BOX;
+  if (bias != nullptr) {
+#pragma unroll
+    for (uint32_t c = 0; c < MOST; ++c) sums[c] += __ldg(bias + c);
+  }
+  wait_copied();
+  __syncwarp();
+#pragma unroll
+  for (uint32_t c = 0; c < MOST; c += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      w[i] = BF16 ? pack_bf16(sums[c + 2 * i], sums[c + 2 * i + 1]) : pack_f16(sums[c + 2 * i], sums[c + 2 * i + 1]);
+    constexpr uint32_t CHUNKS = OUT_BOX / 16;
+    st_shared(mine + c / 8 / CHUNKS * (32 * OUT_BOX) + (((c / 8 % CHUNKS) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
+  }
+  fence_to_copy();
+  __syncwarp();
+  if (lane == 0) {
+    copy_box(map, buf, 2 * col, row);
+    copy_box(map, buf + 32 * OUT_BOX, 2 * col + OUT_BOX, row);
+  }
+  commit_copies();
+}
+
 // `cols` columns of a warp's sums to the result, from `row` and `col` on.
 template <class E>
 __device__ __forceinline__ void store_sums(const F8Params &p, const CUtensorMap *map, uint32_t buf, uint32_t taddr, bool zero,
@@ -797,13 +830,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           all_stages(x.blocks, [&](uint32_t from, float t0, float t1) { drain<GATED, MOST / 2>(from, sums, t0, t1); });
         }
         if (!ok) break;
-        // The sums take the place of the last accumulator: what follows has few registers, and little code.
-        // (From registers it pushed sums to local memory, which came back from L2.)
-        if (x.rows > lane0) put_back(t_lanes + slot_now() * slot_cols, sums, mine);
       }
       // The tile again: kept over the loop it took registers from the sums.
       tiles.read(slot, x);
       const uint32_t rows = x.rows > lane0 ? min(x.rows - lane0, 32u) : 0u;
+      // Whole tiles leave from the registers, and the last accumulator is free at once.  Otherwise the sums take its place:
+      // what follows has few registers then, and little code.
+      const bool whole = x.slices == 1 &&
+                         (GATED || (p.vector_out != 0 && rows == 32 && x.col0 + (part + 1) * MOST <= p.n && mine == MOST &&
+                                    static_cast<GroupedOut>(p.out_type) != GroupedOut::f32));
+      if (!zero) {
+        if (whole) give_back(true);
+        else if (rows > 0) put_back(t_lanes + slot_now() * slot_cols, sums, mine);
+      }
       const bool real = lane < rows;
       const uint32_t t_sums = t_lanes + slot_now() * slot_cols;
       bool done = rows == 0;
@@ -829,27 +868,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (!done) join(part_of(p, x.slot - x.slice, rank, quarter, part * mine), x.slices, mine, t_sums);
         }
         if (!done) {
-          float h[MOST / 2];
-          uint32_t top = 0, gate[2][16], up[2][16]; // the next columns are on their way
-          auto read = [&](uint32_t c, uint32_t i) {
-            if (zero) {
+          if (!whole) {
 #pragma unroll
-              for (uint32_t j = 0; j < 16; ++j) gate[i][j] = up[i][j] = 0;
-            } else {
-              read_columns(t_sums + c, gate[i]);
-              read_columns(t_sums + MOST / 2 + c, up[i]);
+            for (uint32_t c = 0; c < MOST; c += 16) {
+              uint32_t v[16];
+              fetch(t_sums + c, zero, v);
+#pragma unroll
+              for (uint32_t i = 0; i < 16; ++i) sums[c + i] = __uint_as_float(v[i]);
             }
-          };
-          read(0, 0);
+          }
+          float h[MOST / 2];
+          uint32_t top = 0;
 #pragma unroll
-          for (uint32_t c = 0; c < MOST / 2; c += 16) {
-            const uint32_t now = (c / 16) & 1u;
-            ptx::tmem_ld_wait();
-            if (c + 16 < MOST / 2) read(c + 16, now ^ 1u);
+          for (uint32_t c = 0; c < MOST / 2; c += 16) { // (the four activations of all of them at once spilled)
             with_activation(p.activation, [&](auto act) {
 #pragma unroll
-              for (uint32_t i = 0; i < 16; ++i)
-                h[c + i] = activate<act.value, true>(__uint_as_float(gate[now][i])).value * __uint_as_float(up[now][i]);
+              for (uint32_t i = 0; i < 16; ++i) h[c + i] = activate<act.value, true>(sums[c + i]).value * sums[MOST / 2 + c + i];
             });
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) top = max(top, __float_as_uint(h[c + i]) & 0x7fffffffu);
@@ -901,12 +935,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         if (!done) {
           const float *bias = p.bias != nullptr && x.group < p.groups ? p.bias + static_cast<uint64_t>(x.group) * p.n + col : nullptr;
-          if (static_cast<GroupedOut>(p.out_type) == GroupedOut::f32)
+          if (whole && static_cast<GroupedOut>(p.out_type) == GroupedOut::bf16)
+            store_whole<true>(&map_out, buf, sums, x.row0 + lane0, col, bias);
+          else if (whole) store_whole<false>(&map_out, buf, sums, x.row0 + lane0, col, bias);
+          else if (static_cast<GroupedOut>(p.out_type) == GroupedOut::f32)
             store_sums<uint32_t>(p, &map_out, buf, t_sums, zero, x.row0 + lane0, col, rows, cols, bias);
           else store_sums<uint16_t>(p, &map_out, buf, t_sums, zero, x.row0 + lane0, col, rows, cols, bias);
         }
       }
-      if (!zero) give_back(true);
+      if (!zero && !whole) give_back(true);
       tiles.give_back(slot);
       ok = tiles.wait(p.status);
       if (!ok) break;
