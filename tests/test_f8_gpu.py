@@ -401,6 +401,51 @@ def test_the_larger_kernel_cut_along_k(handle, counts):
     handle.set_workspace_limit(0)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("n", [1152, 1160, 1153])
+@pytest.mark.parametrize("pad,offset", [(8, 8), (0, 0), (3, 1)])
+def test_results_of_the_larger_kernel(handle, dtype, n, pad, offset):
+    """Groups that end inside 32 rows, columns that end inside a tile, results in a wider matrix: nothing else is written."""
+    torch, api, experts = _setup()
+    counts, spare, k, dtype = [300, 77, 0, 513, 310], 37, 200, getattr(torch, dtype)
+    rows = sum(counts) + spare
+    q, s, wq, ws = _operands(torch, experts, handle, rows, n, k, len(counts), n + pad)
+    want, off = _product(torch, q, s, wq, ws, counts, rows)
+    bias = torch.randn(len(counts), n, device="cuda")
+    for e, (a, b) in enumerate(_spans(counts)):
+        want[a:b] += bias[e].double()
+        off[a:b] += 2.0 ** -24 * (want[a:b].abs() + off[a:b])
+    buf = torch.full((offset + rows * (n + pad),), 7.0, dtype=dtype, device="cuda")
+    out = buf[offset:].view(rows, n + pad)[:, :n]
+    for _ in range(3):  # one behind the other
+        experts.f8_matmul(handle, q, s, wq, ws, _ends(torch, counts), bias=bias, out=out)
+    _close(torch, out, want, off)
+    assert (buf[:offset] == 7).all() and (buf[offset:].view(rows, -1)[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("pad,offset", [(16, 16), (0, 0), (3, 1)])
+def test_gated_results_of_the_larger_kernel(handle, pad, offset):
+    torch, api, experts = _setup()
+    counts, spare, k, hidden, E4M3 = [300, 77, 0, 513, 310], 37, 200, 1152, api.CUDA_R_8F_E4M3
+    rows = sum(counts) + spare
+    q, s, wq, ws = _operands(torch, experts, handle, rows, 2 * hidden, k, len(counts), 9)
+    ends = _ends(torch, counts)
+    first, first_scale = experts.f8_gated_matmul(handle, q, s, wq, ws, ends)
+    want, off = _product(torch, q, s, wq, ws, counts, rows)
+    act, own = _gate(torch, "silu", want[:, :hidden])
+    far = (1.13 * off[:, :hidden] + own) * (want[:, hidden:].abs() + off[:, hidden:]) + act.abs() * off[:, hidden:]
+    far += 2.0 ** -22 * (act * want[:, hidden:]).abs()
+    _holds(torch, first, first_scale, act * want[:, hidden:], far, "float8_e4m3fn")
+    buf = torch.full((offset + rows * (hidden + pad),), 7, dtype=torch.uint8, device="cuda")
+    out = buf[offset:].view(rows, hidden + pad)[:, :hidden]
+    scale = torch.full((rows, hidden // 128 + 1), 7.0, device="cuda")
+    handle.f8_grouped_gemm_gated(rows, hidden, k, len(counts), ends, q.data_ptr(), q.stride(0), E4M3, s.data_ptr(), *s.stride(),
+                                 wq.data_ptr(), wq.stride(1), wq.stride(0), E4M3, ws.data_ptr(), 0, out.data_ptr(), hidden + pad,
+                                 E4M3, scale.data_ptr(), hidden // 128 + 1, 1)
+    assert torch.equal(out, first.view(torch.uint8)) and torch.equal(scale[:, :-1], first_scale)
+    assert (buf[:offset] == 7).all() and (buf[offset:].view(rows, -1)[:, hidden:] == 7).all() and (scale[:, -1] == 7).all()
+
+
 @pytest.mark.parametrize("counts", [[200, 3, 0, 0, 0, 0, 37, 0], [0, 0, 256, 0, 0, 0, 0, 0], [31, 32, 33, 64, 65, 7, 0, 24]])
 def test_few_rows_unevenly_spread(handle, counts):
     """At most 32 rows a group on average, some of them with more; the same numbers as one group after another, and for
