@@ -575,3 +575,25 @@ def test_refusals(handle):
     empty = experts.f8_matmul(handle, q[:0], s[:0], wq, ws, _ends(torch, [0, 0]))
     assert empty.shape == (0, 256)
     assert experts.quantize_blocks(handle, x[:0])[0].shape == (0, 200)
+
+
+def test_offsets_past_32_bits(handle):
+    """Rows behind 2^32 bytes of operands and results; 128 values of k, so that the sums are the same in any call."""
+    torch, api, experts = _setup()
+    rows, k, n, last = 140000, 128, 32768, 300
+    q, s, wq, ws = _operands(torch, experts, handle, rows, n, k, 1, 4)
+    y = experts.f8_matmul(handle, q, s, wq, ws)
+    few = (q[-last:], s[-last:].t().contiguous().t())
+    assert torch.equal(y[-last:], experts.f8_matmul(handle, *few, wq, ws))
+    part = experts.quantize_blocks(handle, y[-last:])
+    whole = experts.quantize_blocks(handle, y)
+    assert torch.equal(whole[0][-last:].view(torch.uint8), part[0].view(torch.uint8)) and torch.equal(whole[1][-last:], part[1])
+    w, index = torch.randn(1, 128, n, device="cuda"), torch.tensor([rows - 1, 0, rows], dtype=torch.int32, device="cuda")
+    wq, ws = experts.quantize_weight_blocks(handle, w)
+    tail = experts.f8_matmul(handle, *whole, wq, ws, out_dtype=torch.float32)[-last:]
+    want, off = _product(torch, *part, wq, ws, [last], last)
+    _close(torch, tail, want, off)
+    gathered = experts.quantize_blocks(handle, y, row_index=index)[0].view(torch.uint8)
+    assert torch.equal(gathered[0], part[0][-1].view(torch.uint8)) and not gathered[2].any()
+    q, s = experts.f8_gated_matmul(handle, *few, *experts.quantize_weight_blocks(handle, torch.randn(1, 2 * n, k, device="cuda")))
+    assert q.shape == (last, n) and torch.isfinite(s).all()

@@ -533,3 +533,53 @@ def test_refusals(handle):
     out = torch.empty(8, 16, dtype=torch.bfloat16, device="cuda")
     assert experts.gated_matmul(handle, x, gate_up, ends, out=out) is out
     assert torch.equal(out, experts.gated_matmul(handle, x, gate_up, ends))
+
+
+def test_offsets_past_32_bits(handle):
+    """Rows behind 2^32 bytes, and 2^31 elements, of what stands in front of the activation."""
+    torch, api, experts = _setup()
+    rows, hidden, width, last = 70000, 16384, 64, 300
+    x, gate_up, down, dy = _operands(torch, torch.bfloat16, rows, hidden, width, 1, 1)
+
+    def run(x, dy):
+        n = x.shape[0]
+        h, pre = experts._gated(handle, x, gate_up, None, api.Activation.SILU, api.ComputeMode.FP16TCEC, keep=True)
+        dpre = torch.empty_like(pre)
+        handle.grouped_gemm_gated_grad(api.CUBLAS_OP_N, n, hidden, width, 1, None, dy.data_ptr(), width, down.data_ptr(),
+                                       hidden, hidden * width, api.Activation.SILU, pre.data_ptr(), 2 * hidden,
+                                       dpre.data_ptr(), 2 * hidden, api.CUDA_R_16BF)
+        again = torch.empty_like(pre)
+        handle.gated_rows(n, hidden, pre.data_ptr(), 2 * hidden, h.data_ptr(), hidden, api.Activation.SILU, again.data_ptr(),
+                          2 * hidden, api.CUDA_R_16BF)
+        return [t[-last:].clone() for t in (h, pre, dpre, again)]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(x, dy), run(x[-last:], dy[-last:])))
+
+
+def test_two_streams_and_a_graph_at_once(handle):
+    """A handful of rows replayed from a graph while another handle multiplies many on a stream of its own."""
+    torch, api, experts = _setup()
+    x, gate_up, _, _ = _operands(torch, torch.bfloat16, 700, 264, 512, 4, 3)
+    few, ends, few_ends = x[:6].clone(), _ends(torch, [300, 0, 7, 393]), _ends(torch, [1, 0, 3, 2])
+    want_few, want = experts.gated_matmul(handle, few, gate_up, few_ends), experts.gated_matmul(handle, x, gate_up, ends)
+    side, graph, out = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros_like(want_few)
+    with torch.cuda.graph(graph):
+        handle.use_current_torch_stream()
+        experts.gated_matmul(handle, few, gate_up, few_ends, out=out)
+    handle.use_current_torch_stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = api.Handle()
+        other.use_current_torch_stream()
+        results = [experts.gated_matmul(other, x, gate_up, ends) for _ in range(20)]
+    for _ in range(20):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want_few)
+    few.copy_(x[100:106])  # read at each replay
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, experts.gated_matmul(handle, few, gate_up, few_ends))
+    assert all(torch.equal(y, want) for y in results)
+    assert handle.kernel_status() == 0 and other.kernel_status() == 0
+    other.destroy()
