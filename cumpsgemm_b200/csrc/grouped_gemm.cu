@@ -123,7 +123,8 @@ struct GroupedParams {
   float alpha, beta;
   uint8_t out_type;
   uint8_t activation;
-  uint16_t vector_out; // 16-bit results in rows that allow 16-byte accesses, and beta is 0; bit 1: rows of pre do
+  uint16_t vector_out; // 16-bit results in rows that allow 16-byte accesses (gated blocks: that consist of such), and beta is
+                       // 0; bit 1: rows of pre do
   void *pre;           // gated; nullable where it is written
   uint64_t ldpre;
 };
@@ -1341,9 +1342,11 @@ cudaError_t launch(const GroupedArgs &a, cudaStream_t stream) {
   p.vector_out = a.out_type != GroupedOut::f32 && a.beta == 0.f &&
                  (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0 && a.ldo % 8 == 0 &&
                  (!a.wgrad || a.groups == 1 || a.stride_o % 8 == 0);
-  if constexpr (EPI != kPlain) { // pre, and the gradient of it, have their second half `hidden` elements on
+  // The epilogues of gated blocks store 16 bytes of a row, or nothing; the second half of pre, and of its gradient, begins
+  // `hidden` elements on.
+  if constexpr (EPI != kPlain) {
     const bool halves = (EPI == kGated ? a.lane_dim / 2 : a.lane_dim) % 8 == 0;
-    if (EPI == kGatedGrad && !halves) p.vector_out = 0;
+    if (!halves) p.vector_out = 0;
     if (halves && (reinterpret_cast<uintptr_t>(a.pre) & 15u) == 0 && a.ldpre % 8 == 0) p.vector_out |= 2;
   }
   return launch_chained(grouped_gemm_kernel<KIND, A_LANES, WGRAD, EPI>, static_cast<unsigned>(2 * clusters),

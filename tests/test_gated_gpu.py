@@ -583,3 +583,30 @@ def test_two_streams_and_a_graph_at_once(handle):
     assert all(torch.equal(y, want) for y in results)
     assert handle.kernel_status() == 0 and other.kernel_status() == 0
     other.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("hidden", [5, 37, 100, 129])
+@pytest.mark.parametrize("counts,spare", [([130, 0, 61], 9), ([3, 0, 5], 0)])
+def test_results_in_padded_rows(handle, dtype, hidden, counts, spare):
+    """Rows of h that begin at multiples of 16 bytes and end inside the last 16: all of them is written, and nothing else."""
+    torch, api, experts = _setup()
+    dtype, rows, name = getattr(torch, dtype), sum(counts) + spare, "silu"
+    for width, pad in ((72, 0), (72, 16), (70, 0)):  # (of 70 values the kernel for a handful of rows takes none)
+        x, gate_up, _, _ = _operands(torch, dtype, rows, hidden, width, 3, hidden + width)
+        want = _block(torch, dtype, name, x, gate_up, None, None, counts, rows)
+        ld = (hidden + 7) // 8 * 8 + pad
+        out = _placed(torch, torch.full((rows, hidden), float("nan"), dtype=dtype, device="cuda"), ld, 0)
+        ends = _ends(torch, counts)
+        assert experts.gated_matmul(handle, x, gate_up, ends, activation=name, out=out) is out
+        _close(out, want["h"], "h")
+        # the same with what is in front of the activation, in rows of the same kind
+        hid, ldp = torch.full_like(out._base.view(rows, ld), float("nan")), (2 * hidden + 7) // 8 * 8 + pad
+        pre = _placed(torch, torch.full((rows, 2 * hidden), float("nan"), dtype=dtype, device="cuda"), ldp, 0)
+        handle.grouped_gemm_gated(rows, hidden, width, 3, ends, x.data_ptr(), width, gate_up.data_ptr(), width,
+                                  2 * hidden * width, experts._activation(name), hid.data_ptr(), ld, pre.data_ptr(), ldp,
+                                  experts._data_type(dtype))
+        _close(pre, want["pre"], "pre")
+        assert torch.equal(hid[:, :hidden], out)
+        for t, cols in ((out._base.view(rows, ld), hidden), (hid, hidden), (pre._base.view(rows, ldp), 2 * hidden)):
+            assert torch.isnan(t[:, cols:]).all()
