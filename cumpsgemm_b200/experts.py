@@ -275,6 +275,8 @@ def i8_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=None, *, 
 
 def _dense_rows(t):
     """t, copied where its rows, or its matrices, do not lie one behind the other."""
+    if t.is_contiguous():
+        return t
     shape, strides = t.shape, t.stride()
     rows, cols = shape[-2:]
     step, ld = strides[-1], strides[-2]
@@ -380,13 +382,13 @@ def _gated(handle, x, gate_up, group_ends, act, mode, out=None, keep=False):
 
 
 def _gated_rows_grad(handle, pre, dh, act):
-    rows, both = pre.shape
+    rows, both, ldpre = _rows_of(pre, "pre")
     _, _, lddh = _rows_of(dh, "the gradient", both // 2)
     _check_place(handle, dh.get_device())
     if dh.dtype is not pre.dtype:
         raise ValueError(f"the gradient is {dh.dtype}, the operands are {pre.dtype}")
-    dpre = torch.empty_like(pre)
-    handle.gated_rows(rows, both // 2, pre.data_ptr(), both, dh.data_ptr(), lddh, act, dpre.data_ptr(), both,
+    dpre = pre.new_empty((rows, both))
+    handle.gated_rows(rows, both // 2, pre.data_ptr(), ldpre, dh.data_ptr(), lddh, act, dpre.data_ptr(), both,
                       _data_type(pre.dtype))
     return dpre
 
@@ -394,11 +396,12 @@ def _gated_rows_grad(handle, pre, dh, act):
 def _composed(handle, x, gate_up, down, group_ends, act, mode):
     """The same made of products that have gradients of any order, for those of gradients."""
     f = torch.nn.functional
+    x, gate_up = _dense_rows(x), _dense_rows(gate_up)
     gate, up = _linear(x, gate_up, group_ends, handle, True, mode, 1.0).float().chunk(2, -1)
     gate = {api.Activation.SILU: f.silu, api.Activation.GELU: f.gelu, api.Activation.RELU: f.relu,
             api.Activation.GELU_TANH: lambda v: f.gelu(v, approximate="tanh")}[act](gate)
     h = (gate * up).to(x.dtype)
-    return h if down is None else _linear(h, down, group_ends, handle, True, mode, 1.0)
+    return h if down is None else _linear(h, _dense_rows(down), group_ends, handle, True, mode, 1.0)
 
 
 def _composed_gradients(ctx, dy, operands, handle, group_ends, act, mode):
@@ -409,6 +412,7 @@ def _composed_gradients(ctx, dy, operands, handle, group_ends, act, mode):
     return [next(grads) if need else None for _, need in zip(operands, ctx.needs_input_grad)]
 
 
+# Hooks on saved tensors may have moved what the forward pass kept: its order and strides are asked for anew.
 class _GatedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, group_ends, handle, act, mode, backward_mode):
@@ -423,7 +427,8 @@ class _GatedMatmul(torch.autograd.Function):
         handle, act, mode = ctx.how
         if torch.is_grad_enabled():
             return (*_composed_gradients(ctx, dh, (x, gate_up), handle, group_ends, act, mode), *(None,) * 5)
-        dpre = _gated_rows_grad(handle, pre, _dense_rows(dh), act)
+        x, gate_up = _dense_rows(x), _dense_rows(gate_up)
+        dpre = _gated_rows_grad(handle, _dense_rows(pre), _dense_rows(dh), act)
         dx = dgate_up = None
         if ctx.needs_input_grad[0]:
             dx = grouped_matmul(handle, dpre, gate_up, group_ends, mode=mode)
@@ -448,8 +453,8 @@ class _GatedFeedForward(torch.autograd.Function):
         if torch.is_grad_enabled():
             return (*_composed_gradients(ctx, dy, (x, gate_up, down), handle, group_ends, act, mode), *(None,) * 5)
         _check_place(handle, x.get_device())
-        dy = _dense_rows(dy)
-        # (strides anew: hooks on saved tensors may have moved them)
+        x, gate_up, down, dy = _dense_rows(x), _dense_rows(gate_up), _dense_rows(down), _dense_rows(dy)
+        pre, h = pre.contiguous(), h.contiguous()
         groups, both, width, ldw, stridew = _matrices_of(gate_up, "gate_up")
         _, out_width, hidden, ldd, strided = _matrices_of(down, "down")
         rows, _, ldx = _rows_of(x, "x")

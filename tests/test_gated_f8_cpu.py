@@ -59,3 +59,81 @@ def test_shapes_and_names_are_checked():
                  lambda: experts.f8_matmul(None, q, torch.zeros(4, 1), q[:, :7], torch.zeros(1, 1))):
         with pytest.raises(ValueError):
             call()
+
+
+class _Recorder:
+    """Stands for a handle: what the calls would read of the tensors that a backward pass had saved."""
+
+    def __init__(self):
+        self.seen = {}
+
+    def _put(self, what, at, rows, cols, ld):
+        import ctypes
+
+        import torch
+
+        values = (ctypes.c_float * ((rows - 1) * ld + cols)).from_address(at)
+        self.seen[what] = torch.tensor(list(values)).as_strided((rows, cols), (ld, 1)).clone()
+
+    def grouped_gemm_gated_grad(self, op, rows, hidden, k, groups, ends, dy, lddy, w, ldw, stridew, act, pre, ldpre, dpre,
+                                lddpre, kind, mode):
+        self._put("dy", dy, rows, k, lddy)
+        self._put("pre", pre, rows, 2 * hidden, ldpre)
+        self._put("down", w, k, hidden, ldw)
+
+    def grouped_gemm(self, op, rows, n, k, groups, ends, alpha, x, ldx, w, ldw, stridew, beta, y, ldy, kind, mode):
+        self._put("gate_up", w, k, n, ldw)
+
+    def grouped_gemm_wgrad(self, op, rows, n, k, groups, ends, alpha, x, ldx, dy, lddy, beta, dw, lddw, stridedw, kind, mode):
+        self._put("x" if "x" not in self.seen else "h", x, rows, k, ldx)
+
+    def gated_rows(self, rows, hidden, pre, ldpre, dh, lddh, act, out, ldo, kind):
+        self._put("pre", pre, rows, 2 * hidden, ldpre)
+
+
+def _orders(torch, t):
+    """The same values with rows further apart, column after column, and with columns apart."""
+    rows, cols = t.shape[-2:]
+    wide = torch.full((*t.shape[:-1], 2 * cols + 6), float("nan"), dtype=t.dtype, device=t.device)
+    wide[..., 3 : cols + 3] = t
+    yield wide[..., 3 : cols + 3]
+    yield t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    wide[..., 1 : 2 * cols : 2] = t
+    yield wide[..., 1 : 2 * cols : 2]
+
+
+def _saved(torch):
+    g = torch.Generator().manual_seed(3)
+    new = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    ends = torch.tensor([5], dtype=torch.int32)
+    return {"x": new(5, 4), "gate_up": new(1, 6, 4), "down": new(1, 4, 3), "ends": ends, "pre": new(5, 6), "h": new(5, 3)}
+
+
+def test_backward_passes_read_what_was_saved_in_any_order(monkeypatch):
+    from types import SimpleNamespace
+
+    import torch
+
+    from cumpsgemm_b200 import experts
+
+    monkeypatch.setattr(experts, "_check_place", lambda handle, device: None)
+    dy = torch.randn(5, 4)
+    for name in ("x", "gate_up", "down", "pre", "h"):
+        for other in _orders(torch, _saved(torch)[name]):
+            saved, handle = _saved(torch), _Recorder()
+            saved[name] = other
+            ctx = SimpleNamespace(saved_tensors=tuple(saved.values()), how=(handle, 0, 1), needs_input_grad=(True,) * 3)
+            with torch.no_grad():
+                experts._GatedFeedForward.backward(ctx, dy)
+            assert torch.equal(handle.seen["dy"], dy)
+            for key, t in handle.seen.items():
+                assert key == "dy" or torch.equal(t, _saved(torch)[key].view(t.shape)), (name, key)
+            if name not in ("x", "gate_up", "pre"):
+                continue
+            handle = _Recorder()
+            ctx = SimpleNamespace(saved_tensors=(saved["x"], saved["gate_up"], saved["ends"], saved["pre"]),
+                                  how=(handle, 0, 1), needs_input_grad=(True, True))
+            with torch.no_grad():
+                experts._GatedMatmul.backward(ctx, torch.randn(5, 3))
+            for key in ("pre", "gate_up", "x"):
+                assert torch.equal(handle.seen[key], _saved(torch)[key].view(handle.seen[key].shape)), (name, key)

@@ -610,3 +610,32 @@ def test_results_in_padded_rows(handle, dtype, hidden, counts, spare):
         assert torch.equal(hid[:, :hidden], out)
         for t, cols in ((out._base.view(rows, ld), hidden), (hid, hidden), (pre._base.view(rows, ldp), 2 * hidden)):
             assert torch.isnan(t[:, cols:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("order", ["rows apart", "columns first", "columns apart"])
+def test_saved_tensors_in_another_order(handle, dtype, order):
+    """Hooks that give back every tensor that the forward pass kept with other strides: the gradients are the same."""
+    torch, api, experts = _setup()
+    x, gate_up, down, dy = _operands(torch, getattr(torch, dtype), 50, 64, 72, 2, 5)
+    ends, dh = _ends(torch, [20, 30]), torch.randn(50, 64, device="cuda").to(x.dtype)
+
+    def other(t):
+        if t.dim() == 1:
+            return t
+        if order == "columns first":
+            return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+        wide = torch.full((*t.shape[:-1], 2 * t.shape[-1] + 8), float("nan"), dtype=t.dtype, device=t.device)
+        part = wide[..., 8 : t.shape[-1] + 8] if order == "rows apart" else wide[..., 8::2]
+        return part.copy_(t)
+
+    for call, operands, grad in ((experts.gated_feed_forward, (x, gate_up, down), dy), (experts.gated_matmul, (x, gate_up), dh)):
+        leaves = [t.detach().requires_grad_() for t in operands]
+        want = torch.autograd.grad(call(handle, *leaves, ends), leaves, grad)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            y = call(handle, *leaves, ends)
+        got = torch.autograd.grad(y, leaves, grad, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        again = torch.autograd.grad(y, leaves, grad, create_graph=True)
+        plain = torch.autograd.grad(call(handle, *leaves, ends), leaves, grad, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(again, plain))
