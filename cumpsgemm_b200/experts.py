@@ -381,12 +381,18 @@ def _gated(handle, x, gate_up, group_ends, act, mode, out=None, keep=False):
     return out, pre
 
 
+def _as_kept(fits: bool) -> None:
+    if not fits:
+        raise ValueError("a saved tensor has come back on another device, or with another type or size")
+
+
 def _gated_rows_grad(handle, pre, dh, act):
     rows, both, ldpre = _rows_of(pre, "pre")
     _, _, lddh = _rows_of(dh, "the gradient", both // 2)
     _check_place(handle, dh.get_device())
     if dh.dtype is not pre.dtype:
         raise ValueError(f"the gradient is {dh.dtype}, the operands are {pre.dtype}")
+    _as_kept(pre.get_device() == dh.get_device() and rows == dh.shape[0])
     dpre = pre.new_empty((rows, both))
     handle.gated_rows(rows, both // 2, pre.data_ptr(), ldpre, dh.data_ptr(), lddh, act, dpre.data_ptr(), both,
                       _data_type(pre.dtype))
@@ -412,7 +418,8 @@ def _composed_gradients(ctx, dy, operands, handle, group_ends, act, mode):
     return [next(grads) if need else None for _, need in zip(operands, ctx.needs_input_grad)]
 
 
-# Hooks on saved tensors may have moved what the forward pass kept: its order and strides are asked for anew.
+# Hooks on saved tensors may have moved what the forward pass kept, or changed it: order and strides are asked for anew, and
+# what the kernels could not read is refused.
 class _GatedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, group_ends, handle, act, mode, backward_mode):
@@ -428,6 +435,7 @@ class _GatedMatmul(torch.autograd.Function):
         if torch.is_grad_enabled():
             return (*_composed_gradients(ctx, dh, (x, gate_up), handle, group_ends, act, mode), *(None,) * 5)
         x, gate_up = _dense_rows(x), _dense_rows(gate_up)
+        _as_kept(x.shape[1] == gate_up.shape[2])
         dpre = _gated_rows_grad(handle, _dense_rows(pre), _dense_rows(dh), act)
         dx = dgate_up = None
         if ctx.needs_input_grad[0]:
@@ -452,13 +460,15 @@ class _GatedFeedForward(torch.autograd.Function):
         handle, act, mode = ctx.how
         if torch.is_grad_enabled():
             return (*_composed_gradients(ctx, dy, (x, gate_up, down), handle, group_ends, act, mode), *(None,) * 5)
-        _check_place(handle, x.get_device())
         x, gate_up, down, dy = _dense_rows(x), _dense_rows(gate_up), _dense_rows(down), _dense_rows(dy)
         pre, h = pre.contiguous(), h.contiguous()
         groups, both, width, ldw, stridew = _matrices_of(gate_up, "gate_up")
-        _, out_width, hidden, ldd, strided = _matrices_of(down, "down")
-        rows, _, ldx = _rows_of(x, "x")
-        _, _, lddy = _rows_of(dy, "the gradient", out_width)
+        matrices, out_width, hidden, ldd, strided = _matrices_of(down, "down")
+        rows, _, ldx = _rows_of(x, "x", width)
+        dy_rows, _, lddy = _rows_of(dy, "the gradient", out_width)
+        _check(handle, dy.get_device(), (x, gate_up, down, pre, h), group_ends, groups)
+        _as_kept(x.dtype is gate_up.dtype is down.dtype is pre.dtype is h.dtype is dy.dtype and both == 2 * hidden and
+                 matrices == groups and dy_rows == rows and pre.shape == (rows, both) and h.shape == (rows, hidden))
         ends, data_type = None if group_ends is None else group_ends.data_ptr(), _data_type(x.dtype)
         need_x, need_gate_up, need_down = ctx.needs_input_grad[:3]
         dx = dgate_up = ddown = None

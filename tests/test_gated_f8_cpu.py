@@ -137,3 +137,36 @@ def test_backward_passes_read_what_was_saved_in_any_order(monkeypatch):
                 experts._GatedMatmul.backward(ctx, torch.randn(5, 3))
             for key in ("pre", "gate_up", "x"):
                 assert torch.equal(handle.seen[key], _saved(torch)[key].view(handle.seen[key].shape)), (name, key)
+
+
+@pytest.mark.parametrize("name", ["x", "gate_up", "down", "pre", "h", "ends"])
+def test_saved_tensors_that_do_not_fit_are_refused(monkeypatch, name):
+    """On another device (of no memory here), of another type, or of another size."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from cumpsgemm_b200 import experts
+
+    monkeypatch.setattr(experts, "_check_place", lambda handle, device: None)
+
+    class Elsewhere(torch.Tensor):
+        def get_device(self):
+            return 1
+
+    whole = _saved(torch)
+    for changed in (whole[name].as_subclass(Elsewhere), whole[name].double(), whole[name][:0],
+                    torch.cat([whole[name], whole[name]], -1)):
+        saved = dict(whole, **{name: changed})
+        for block in (True, False):
+            if not block and name in ("down", "h"):
+                continue
+            handle = _Recorder()
+            for call in ("grouped_gemm", "grouped_gemm_wgrad", "grouped_gemm_gated_grad", "gated_rows"):
+                monkeypatch.setattr(handle, call, lambda *a: None, raising=False)
+            ctx = SimpleNamespace(how=(handle, 0, 1), needs_input_grad=(True,) * 3 if block else (True, True),
+                                  saved_tensors=tuple(saved.values()) if block else
+                                  (saved["x"], saved["gate_up"], saved["ends"], saved["pre"]))
+            backward = experts._GatedFeedForward.backward if block else experts._GatedMatmul.backward
+            with torch.no_grad(), pytest.raises(ValueError):
+                backward(ctx, torch.randn(5, 4 if block else 3))

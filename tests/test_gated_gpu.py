@@ -639,3 +639,20 @@ def test_saved_tensors_in_another_order(handle, dtype, order):
         again = torch.autograd.grad(y, leaves, grad, create_graph=True)
         plain = torch.autograd.grad(call(handle, *leaves, ends), leaves, grad, create_graph=True)
         assert all(torch.equal(a, b) for a, b in zip(again, plain))
+
+
+def test_saved_tensors_that_do_not_fit(handle):
+    """Hooks that leave a saved tensor in host memory, or give it back with another type: refused before anything runs."""
+    torch, api, experts = _setup()
+    x, gate_up, down, dy = _operands(torch, torch.bfloat16, 50, 64, 72, 2, 5)
+    ends, dh = _ends(torch, [20, 30]), torch.randn(50, 64, device="cuda").bfloat16()
+    pre, h, leaves = (50, 128), (50, 64), [t.detach().requires_grad_() for t in (x, gate_up, down)]
+    kept = [tuple(t.shape) for t in (x, gate_up, ends)] + [pre]
+    for call, count, grad, shapes in ((experts.gated_feed_forward, 3, dy, kept + [tuple(down.shape), h]),
+                                      (experts.gated_matmul, 2, dh, kept)):
+        for changed in shapes:
+            for change in (lambda t: t.cpu(), lambda t: t.to(torch.float16)):
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if tuple(t.shape) == changed else t):
+                    y = call(handle, *leaves[:count], ends)
+                with pytest.raises(ValueError):
+                    torch.autograd.grad(y, leaves[:count], grad)
