@@ -59,6 +59,27 @@ template <Activation ACT, bool FAST> __device__ __forceinline__ ActResult activa
   return r;
 }
 
+// g = dh up act'(gate), u = dh act(gate), of the gradient dh of act(gate) up.  OVERFLOWN (float16): gate and up were rounded,
+// and an infinity stands for a sum past the type's largest value.  Such a one times nothing is nothing, and not NaN: where no
+// gradient comes back (masked rows), where the activation has no slope, and where the gate is far below 0.  Anywhere
+// else the gradient passes the type's largest value as well.
+template <Activation ACT, bool FAST, bool OVERFLOWN>
+__device__ __forceinline__ void gated_gradient(float gate, float up, float dh, float &g, float &u) {
+  if constexpr (OVERFLOWN) { // (NaN stays NaN)
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(gate) : "f"(gate), "f"(-65504.f));
+    const ActResult a = activate<ACT, FAST>(gate);
+    float value;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(value) : "f"(a.value), "f"(3.402823466e38f));
+    const float d = dh * a.slope;
+    g = d == 0.f && fabsf(up) == __uint_as_float(0x7f800000u) ? 0.f : d * up;
+    u = dh * value;
+  } else {
+    const ActResult a = activate<ACT, FAST>(gate);
+    g = dh * up * a.slope;
+    u = dh * a.value;
+  }
+}
+
 // f(ActivationIs<a>{}): a loop asks once, and not for each of its values.
 template <Activation A> struct ActivationIs {
   static constexpr Activation value = A;

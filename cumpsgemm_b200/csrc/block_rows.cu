@@ -195,13 +195,8 @@ template <class T> __device__ __forceinline__ void store_values(T *at, uint32_t 
 
 // One value of a gated product, or of its gradient (g: the first half, u: the second).
 template <Activation ACT, class T, bool GRAD> __device__ __forceinline__ void gated_value(float &g, float &u, float d) {
-  const ActResult act = activate<ACT, sizeof(T) == 2>(g);
-  if constexpr (GRAD) {
-    g = d * u * act.slope;
-    u = d * act.value;
-  } else {
-    g = act.value * u;
-  }
+  if constexpr (GRAD) gated_gradient<ACT, sizeof(T) == 2, std::is_same_v<T, __half>>(g, u, d, g, u);
+  else g = activate<ACT, sizeof(T) == 2>(g).value * u;
 }
 
 constexpr uint32_t kGatedAtOnce = 2, kGatedSegment = kGatedAtOnce * 32 * 8;

@@ -782,9 +782,12 @@ __device__ __forceinline__ void store_gated_grad(uint32_t taddr, bool zero, T *o
             const float x = __uint_as_float(i < 2 ? lo[4 * g + 2 * i] : hi[4 * g + 2 * i - 4]),
                         y = __uint_as_float(i < 2 ? lo[4 * g + 2 * i + 1] : hi[4 * g + 2 * i - 3]);
             const float2 gate = unpack<T>(w[0][g][i]), up = unpack<T>(w[1][g][i]);
-            const ActResult a = activate<act.value, true>(gate.x), b = activate<act.value, true>(gate.y);
-            w[0][g][i] = pack_results<T>(x * up.x * a.slope, y * up.y * b.slope);
-            w[1][g][i] = pack_results<T>(x * a.value, y * b.value);
+            constexpr bool OVERFLOWN = std::is_same_v<T, __half>;
+            float dg[2], du[2];
+            gated_gradient<act.value, true, OVERFLOWN>(gate.x, up.x, x, dg[0], du[0]);
+            gated_gradient<act.value, true, OVERFLOWN>(gate.y, up.y, y, dg[1], du[1]);
+            w[0][g][i] = pack_results<T>(dg[0], dg[1]);
+            w[1][g][i] = pack_results<T>(du[0], du[1]);
           }
       });
     } else {

@@ -441,7 +441,8 @@ cublasStatus_t cuMpSGEMM_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t 
                                             cuMpSGEMM_compute_mode_t mode);
 /* Backwards through the product behind it as well: with dh = dy op(w_e) (dy rows x k, w_e stored k x hidden,
  * CUBLAS_OP_N, or hidden x k, CUBLAS_OP_T), dpre = [dh * up * act'(gate), dh * act(gate)].  pre: as the call above
- * left it.  Rows of no group: 0. */
+ * left it.  Rows of no group: 0.  An infinity in a float16 pre stands for a sum past 65504: times a dh or a slope of 0,
+ * or in a gate far below 0, it counts for nothing. */
 cublasStatus_t cuMpSGEMM_grouped_gemm_gated_grad(cuMpSGEMM_handle_t handle, cublasOperation_t op_W,
                                                  uint64_t rows, uint64_t hidden, uint64_t k,
                                                  uint32_t num_groups, const int32_t *group_ends,

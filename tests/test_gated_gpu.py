@@ -656,3 +656,59 @@ def test_saved_tensors_that_do_not_fit(handle):
                     y = call(handle, *leaves[:count], ends)
                 with pytest.raises(ValueError):
                     torch.autograd.grad(y, leaves[:count], grad)
+
+
+@pytest.mark.parametrize("name", ACTIVATIONS)
+def test_gradients_behind_what_passes_float16(handle, name):
+    """Sums past 65504 are infinities in what the forward pass keeps.  Times nothing they are nothing: where the gradient is 0,
+    where the activation has no slope, or the gate is far below 0; elsewhere the gradient is infinite too."""
+    torch, api, experts = _setup()
+    act, kind, inf = experts._activation(name), api.CUDA_R_16F, float("inf")
+    for hidden, rows in ((64, 70), (37, 70), (64, 5)):
+        pre, dy = torch.randn(rows, 2 * hidden, device="cuda").half(), torch.randn(rows, 48, device="cuda").half()
+        down = torch.randn(1, 48, hidden, device="cuda").half()
+        gate, up = pre[:, :hidden], pre[:, hidden:]
+        dy[::3] = 0  # rows without a gradient, whatever their values
+        gate[:, 3], up[:, 5], gate[:, 7], up[:, 7] = inf, -inf, -inf, inf
+        gate[:, 9], up[:, 9], gate[:, 11] = -300.0, -inf, -inf
+        dh = torch.randn(rows, hidden, device="cuda").half()
+        dh[::3] = 0
+        one, two = (torch.full((rows, 2 * hidden), float("nan"), device="cuda", dtype=torch.float16) for _ in range(2))
+        handle.grouped_gemm_gated_grad(api.CUBLAS_OP_N, rows, hidden, 48, 1, None, dy, 48, down, hidden, 48 * hidden, act,
+                                       pre, 2 * hidden, one, 2 * hidden, kind)
+        handle.gated_rows(rows, hidden, pre, 2 * hidden, dh, hidden, act, two, 2 * hidden, kind)
+        back = _product(torch, torch.float16, _Value(dy), _Value(down[0]))
+        for got, d in ((one, back), (two, _Value(dh))):
+            dgate, dup = got[:, :hidden], got[:, hidden:]
+            assert not got[::3].any()
+            assert not dgate[:, [7, 9, 11]].any() and not dup[:, [7, 9, 11]].any()
+            real = torch.arange(rows, device="cuda") % 3 != 0
+            assert torch.equal(dup[real, 3], (d.v[real, 3].sign() * inf).half())
+            if name != "relu":
+                assert torch.isinf(dgate[real, 5]).all()
+            plain = [i for i in range(hidden) if i not in (3, 5, 7, 9, 11)]
+            a, s = _activated(torch, name, _Value(gate[:, plain]))
+            u, d = _Value(up[:, plain]), d[:, plain]
+            _close(dgate[:, plain], _times(d, u, s).rounded(torch, torch.float16), name)
+            _close(dup[:, plain], _times(d, a).rounded(torch, torch.float16), name)
+
+
+def test_a_block_whose_sums_pass_float16(handle):
+    """From end to end: gates below -65504, and rows that no gradient comes back to."""
+    torch, api, experts = _setup()
+    x, gate_up, down, dy = _operands(torch, torch.float16, 60, 64, 72, 1, 7, scale=2.0 ** -6)
+    gate_up[0, :64:5] = -1000.0 * x.sign()[7]  # times x[7], some -60000 and less
+    x[7] *= 4
+    gate_up[0, 3, :], x[8] = 2000.0, x[8].abs() * 8  # above 65504 in row 8, which no gradient comes back to
+    dy[8] = 0
+    leaves = [t.detach().requires_grad_() for t in (x, gate_up, down)]
+    ends = _ends(torch, [60])
+    raw = x.double() @ gate_up[0].double().t()
+    assert (raw[7, :64:5] < -65520).all() and raw[8, 3] > 65520
+    y = experts.gated_feed_forward(handle, *leaves, ends)
+    dx, dgate_up, _ = torch.autograd.grad(y, leaves, dy)
+    want = _block(torch, torch.float16, "silu", x, gate_up, down, dy, [60], 60)  # (its sums pass nothing)
+    assert want["dx"].v.abs().max() < 60000 and want["dgate_up"].v.abs().max() < 60000
+    assert torch.isfinite(dgate_up).all() and torch.isfinite(dx).all() and not dx[8].any()
+    _close(dx, want["dx"], "dx")
+    _close(dgate_up, want["dgate_up"], "dgate_up")
