@@ -345,16 +345,20 @@ __device__ __forceinline__ void park(float *mine, uint32_t cols, uint32_t taddr)
 #pragma unroll
     for (uint32_t j = 0; j < 16; ++j) __stcg(mine + (c + j) * ROWS_CTA, __uint_as_float(v[j]));
   }
-  __threadfence();
   __syncwarp();
 }
-// by one lane: whether all other slices' sums of these lanes (and columns) have been parked
+// by one lane: whether all other slices' sums of these lanes (and columns) have been parked.  It counts for what other lanes
+// and, gated, another warp have parked as well, of which it has been told inside the CTA: so the fences are its own, in front
+// of its count and behind it, and not those of each lane.
 __device__ __forceinline__ bool is_last(const F8Params &p, const Tile &x, uint32_t rank, uint32_t which) {
-  return atomicInc(p.counters + 2 + (x.number * 2 + rank) * 16 + which, x.slices - 1) == x.slices - 1;
+  __threadfence();
+  const bool last = atomicInc(p.counters + 2 + (x.number * 2 + rank) * 16 + which, x.slices - 1) == x.slices - 1;
+  __threadfence();
+  return last;
 }
 // the sums of all slices, the first of which is at `first`, added in their order, back to tensor memory
 __device__ __forceinline__ void join(const float *first, uint32_t slices, uint32_t cols, uint32_t taddr) {
-  __threadfence();
+  __syncwarp(); // (the lane that counted has been told first)
 #pragma unroll 1
   for (uint32_t c = 0; c < cols; c += 16) {
     float v[16];
