@@ -22,7 +22,7 @@ struct ActResult {
 // FAST: for results of 16 or 8 bits.  exp by the approximation of 2^x, whose relative error is 2^-22 + |v| 2^-23, and
 // the reciprocal to 1 unit in the last place; both are far inside the rounding that follows.  Without the forms for
 // subnormals: an exp(-v) below 2^-126 counts for nothing beside 1, and where it passes 2^126 the quotient is 0 for what
-// is at most 2^-126.  (They are half of the instructions of __expf and __fdividef.)
+// is at most 2^-126.
 template <bool FAST> __device__ __forceinline__ float logistic(float v) {
   if constexpr (FAST) {
     float e, p;

@@ -5,7 +5,7 @@
 // Bound by memory: the weights of each group with rows pass once.  Here features are the lanes of tensor memory, 128
 // for a CTA, whose weights have one scale for each block of K, and up to 64 rows of a group its columns.  A block's
 // products take 64 to 128 cycles instead of 512, eight accumulators of 64 columns are under way, and a CTA needs no
-// word from another: f8_gemm.cu, where a stage of 256 features takes 820 cycles for the way round however few the rows
+// word from another: f8_gemm.cu, where a stage of 256 features takes more than 800 cycles however few the rows
 // are, read the weights of 32 experts of 4096 x 4096 for 8 rows each at 4.1 TB/s; this one takes 83 us, 6.5 TB/s, and
 // 89 with 64 rows each.  One row of 4096 x 4096 takes 8.9 us, most of it in front of the first product and behind the last.
 //

@@ -10,9 +10,12 @@
 // bounds a long product is the way round: the products of a stage take 512 cycles, their end is known 180 cycles
 // later, an epilogue warp takes 400 to 500 to add 128 columns up (two warps share a scheduler, and 256 of them are
 // multiply-adds), and it is another 200 until the leader knows that both CTAs have, the one's word to the other going
-// through the cluster.  So with two accumulators a stage takes some 800 cycles, which at 8192^3 in a loop, where
-// the power cap leaves 1.5 to 1.58 GHz, is 483 to 500 us: 2.2 PFLOP/s.  (As two accumulators of 128 columns each, with
-// products and barriers of their own, the same took 579: products of 128 columns are not twice as fast.)  Behind the last
+// through the cluster.  So with two accumulators a stage takes 855 to 880 cycles.  That is not all of it: with 128 columns,
+// whose products take half as long and whose four accumulators leave time for the way round, a stage still takes 700 to 720,
+// on half of the pairs as on all of them, so some 550 cycles depend on neither width nor accumulators.  Which role's chain they
+// are has not been measured.  8192^3 takes 474 to 530 us over a few dozen calls (2.1 to 2.3 PFLOP/s) and 548 (2.0) where they
+// go on for half a second and the power cap leaves 1.25 GHz.  (As two accumulators of 128 columns each, with products and
+// barriers of their own, it took 579 instead of 485.)  Behind the last
 // stage of a tile come 2500 cycles, gated 5000 (of which 2700 for the activation: two special-function instructions for
 // each of 64 values), in which the tensor core does the next tile's first two stages.
 //
@@ -133,8 +136,9 @@ struct alignas(16) Tile {
 };
 static_assert(sizeof(Tile) == 48, "three times 16 bytes");
 
-// What a launch is expected to take, in cycles: a stage of a tile `width` columns wide (8192 x 8192 x 8192: 820 with 256,
-// 620 with 128), and the join of slices, which passes over the columns of a warp.
+// What a launch is expected to take, in cycles: a stage of a tile `width` columns wide (38 or 72 tiles, operands in L2, by
+// the slope over K: 855 to 880 with 256 columns, 700 to 720 with 128; the line is some 4 % below both, and only which of two
+// launches is the shorter counts), and the join of slices, which passes over the columns of a warp.
 __device__ __forceinline__ float stage_cycles(uint32_t width) { return 560.f + width; }
 __device__ __forceinline__ float join_cycles(uint32_t width, uint32_t slices) {
   return slices > 1 ? 4000.f + width * (30.f + 4.f * slices) : 0.f;

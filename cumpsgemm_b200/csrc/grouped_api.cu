@@ -149,7 +149,9 @@ bool gated_takes_few_rows(const GroupedArgs &g) {
 // group's weights once for every 64 of its rows, and whose tiles are half as high and half as wide.  Up to 32 rows for
 // each group on average, however they are spread: 32 groups of 4096 x 4096 with 32 rows each 85 us against 125; with all
 // of those rows in one group some 50 against 30.  One group with up to 64 rows, and any call whose tiles all have an SM of
-// their own: 256 rows of 4096 x 4096 15 against 21 (512, which are more tiles than that, 25 against 19).
+// their own: 256 rows of 4096 x 4096 15 against 21 (512, which are more tiles than that, 25 against 19).  What it costs where
+// all rows are in one group grows with them, and so does what it saves where they are not: 128 groups of 4096 x 4096
+// with 4096 rows 173 us against 79, evenly spread 332 against 519; 256 of 4096 x 2048 with 8192 rows 183 against 78, and 343 against 568.
 bool f8_takes_few_rows(uint64_t rows, uint64_t n, uint32_t groups, unsigned num_sms) {
   const uint64_t most_tiles = (rows + 63ull * groups) / 64 * ((n + 127) / 128);
   return rows <= (groups == 1 ? 64ull : 32ull * groups) || most_tiles <= num_sms;

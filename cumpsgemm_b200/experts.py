@@ -647,7 +647,8 @@ def f8_gated_matmul(handle: api.Handle, xq, x_scale, wq, w_scale, group_ends=Non
     """(q, scale) of ``act(x[r] @ gate_e^T) * (x[r] @ up_e^T)`` as ``quantize_blocks`` gives them, for ``f8_matmul``
     with the weights behind: operands as there, wq being (experts, 2 * hidden, k) with the rows of the gate
     first.  Products, activation and their product are FP32.  Where hidden is a multiple of 128 and the rows are
-    many nothing else reaches memory; otherwise the products do, in FP32, and a pass over them.  No gradients."""
+    many nothing else reaches memory; otherwise the products do, in FP32, and a pass over them.  Near the middle
+    between two 8-bit values the two ways, and ``quantize_blocks``, may choose either of them.  No gradients."""
     act = _activation(activation)
     if wq.dim() == 2:
         wq = wq.unsqueeze(0)

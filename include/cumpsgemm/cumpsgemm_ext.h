@@ -477,7 +477,8 @@ cublasStatus_t cuMpSGEMM_quantize_blocks_f8(cuMpSGEMM_handle_t handle, uint32_t 
                                             float *scale);
 /* y[r, c] = sum over blocks b of k of x_scale[r, b] w_scale[e, c / 128, b] sum_{i in b} xq[r, i] wq_e[c, i]
  * (+ bias[e * n + c]) for the rows r of each group e; rows of no group: 0.  wq_e is stored n x k; bias may be NULL.
- * The products of a block are added in FP32 by the tensor core, the blocks in FP32, and the result is rounded once to y_type. */
+ * The products of a block are added in FP32 by the tensor core, the blocks in FP32, and the result is rounded once to y_type.
+ * The two scales of a block are multiplied first, in FP32, whose range their product has to keep. */
 cublasStatus_t cuMpSGEMM_f8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t n, uint64_t k,
                                          uint32_t num_groups, const int32_t *group_ends, const void *xq,
                                          uint64_t ldx, cudaDataType_t x_type, const float *x_scale,
@@ -488,7 +489,9 @@ cublasStatus_t cuMpSGEMM_f8_grouped_gemm(cuMpSGEMM_handle_t handle, uint64_t row
 /* The gated product with such operands, act(x gate_e^T) * (x up_e^T) of unrounded FP32 products, brought to 8 bits
  * again: q (rows x hidden) and its scales.  wq_e is stored 2 hidden x k; hidden is a multiple of 128.  For few rows
  * (those of 32 for each group, or some more) the FP32 products go by way of the handle's workspace where it can have
- * them. */
+ * them, and cuMpSGEMM_quantize_rows_f8's rule brings them to 8 bits.  Otherwise each value is multiplied by M / top, rounded to
+ * FP32: q may be the 8-bit value next to the nearest one where a value lies near the middle between the two.  So the two
+ * ways, one of which depends on the workspace, may differ by one step of the 8-bit type, and as the order of FP32 sums does. */
 cublasStatus_t cuMpSGEMM_f8_grouped_gemm_gated(cuMpSGEMM_handle_t handle, uint64_t rows, uint64_t hidden,
                                                uint64_t k, uint32_t num_groups, const int32_t *group_ends,
                                                const void *xq, uint64_t ldx, cudaDataType_t x_type,
